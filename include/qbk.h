@@ -446,6 +446,76 @@ int qbk_sage_blk_quantize_dev(qbk_ctx *ctx, const qbk_attn_shape *shape, const u
                               int8_t *khat, float *kscale, float *kmean, uint16_t *vh,
                               void *stream);
 
+/* ---- 8-bit KV cache and the attention that reads it ------------------------ */
+
+/* No counterpart in the reference (its KvCache is f32, engine/mod.rs:
+ * 1189-1269): n_seqs sequences of up to `capacity` rows, each row's key and
+ * value of every kv head held as head_dim 8-bit codes and one f32 scale.
+ * With A = max(largest |x| of the head's row, 2^-100) and L the format's
+ * largest code (int8 127, e4m3 448):
+ *   scale = A (1 / L),  code = nearest(x (L (1 / A))) (f32 steps; ties to
+ * even; int8: to an integer, fp8: to an OCP e4m3 value), and the row stands
+ * for code * scale.
+ * A head's row that holds a NaN or an infinity reads back as NaN throughout.
+ * head_dim is a multiple of 16 up to 256.  The cache is one device buffer of
+ * qbk_kv_cache_size bytes, 16-byte aligned, that the caller owns; its inner
+ * layout is the attention kernel's, rows enter and leave it through
+ * qbk_kv_cache_write_dev / _read_dev.  A new buffer needs no clearing: rows
+ * never written are never looked at while lengths say so. */
+enum { QBK_KV_INT8 = 0, QBK_KV_FP8 = 1 };
+typedef struct {
+    int format;
+    size_t n_seqs, capacity, n_kv_heads, head_dim;
+} qbk_kv_shape;
+/* Bytes of the buffer; 0 with qbk_last_error for a shape that is refused. */
+size_t qbk_kv_cache_size(const qbk_kv_shape *shape);
+/* Rows of sequences first_seq .. first_seq + n - 1, quantised as they are
+ * written.  k, v: n_rows rows of n_kv_heads * head_dim values each (dtype
+ * QBK_F32 or QBK_BF16), row_stride values from one row to the next (at least
+ * the row; a fused projection's rows are read in place).  Rows row_start[i]
+ * .. row_start[i + 1] - 1 (device uint32, n + 1 entries, ascending) are
+ * sequence first_seq + i's at positions pos[i], pos[i] + 1, ... (device
+ * uint32, n entries); row_start NULL splits the rows evenly (n_rows a
+ * multiple of n: a decode step's one row each, one sequence's prompt).  Both
+ * arrays are read when the call runs, so a captured graph serves every later
+ * position.  A row whose position is at or past the capacity, or that no
+ * sequence claims, is left out; cache rows no position names keep what they
+ * held. */
+int qbk_kv_cache_write_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, void *cache, const void *k, const void *v,
+                           int dtype, size_t row_stride, size_t n_rows, const uint32_t *row_start,
+                           const uint32_t *pos, size_t first_seq, size_t n, void *stream);
+/* The same rows back as values (code * scale in f32, rounded once for
+ * QBK_BF16); a row whose position is at or past the capacity, or that no
+ * sequence claims, is NaN. */
+int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, void *k, void *v, int dtype,
+                          size_t row_stride, size_t n_rows, const uint32_t *row_start, const uint32_t *pos,
+                          size_t first_seq, size_t n, void *stream);
+/* Attention of n sequences' last seq_q positions over the cache, behind a
+ * prefix that all of them share.  q, out: [n][seq_q][n_heads][head_dim] of
+ * dtype (token-major, as the o projection reads them), q unscaled
+ * (1/sqrt(head_dim) applied here), query head h on kv head
+ * h / (n_heads / n_kv_heads).  Sequence i has lens[i] own rows (device
+ * uint32, read when the call runs; counted as at most max_len, a host bound
+ * no larger than the capacity, by which the work is split), the last seq_q
+ * of them the queries' own: query t sees every prefix row and own rows
+ * 0 .. lens[i] - seq_q + t.  The prefix is rows 0 .. prefix_len - 1 of
+ * sequence prefix_seq of `prefix` (a cache of the same format, kv heads and
+ * head_dim; it may be the same buffer) and is read once for the batch, not
+ * once a sequence; prefix_len 0 (prefix and prefix_shape NULL) is plain
+ * batched attention.  A query that sees no row yields zeros.  Softmax
+ * statistics and sums are f32; for QBK_F32 queries and weights are split in
+ * two halves so that the products keep f32's precision.  The result does
+ * not depend on what other calls run.  workspace of at least
+ * qbk_attention_kv_workspace_size bytes, 16-byte aligned; calls that share
+ * one must not overlap. */
+size_t qbk_attention_kv_workspace_size(const qbk_kv_shape *shape, size_t n_heads, size_t n, size_t seq_q,
+                                       size_t max_len, size_t prefix_len);
+int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, size_t first_seq, size_t n,
+                         const uint32_t *lens, size_t max_len, const qbk_kv_shape *prefix_shape,
+                         const void *prefix, size_t prefix_seq, size_t prefix_len, size_t n_heads, size_t seq_q,
+                         const void *q, int dtype, void *out, void *workspace, size_t workspace_size,
+                         void *stream);
+
 /* ---- language-model head (engine/mod.rs:781-800) -------------------------- */
 
 /* Engine::logits: logits[v] = sum_t hidden[t] * head[v][t], one f32 sum per
@@ -466,6 +536,26 @@ int qbk_head_logits(qbk_ctx *ctx, const qbk_head *head, const float *hidden, siz
 /* Device-pointer form, `batch` rows, stream-ordered; allocates nothing. */
 int qbk_head_logits_dev(qbk_ctx *ctx, const qbk_head *head, const float *hidden, size_t batch, float *logits,
                         void *stream);
+
+/* ---- log probabilities ------------------------------------------------------ */
+
+/* What the API's logprobs report and a perplexity sums (no counterpart in the
+ * reference, whose sampler is greedy): for each of `rows` rows of `vocab`
+ * logits (QBK_F32 or QBK_BF16, row_stride values from one row to the next)
+ *   logprobs[r] = x[targets[r]] - lse(x)      (targets: device int32)
+ *   entropy[r]  = lse(x) - sum softmax(x) x   (nats; a logit of -inf adds 0)
+ * and, for top_k > 0 (up to 64 and to vocab), the top_k likeliest tokens in
+ * order, ids in top_ids [rows][top_k] and their log probabilities in
+ * top_logprobs; equal logits go to the lower id and a NaN orders as -inf, as
+ * qbk_argmax_dev has it.  A target outside the vocabulary yields NaN; a row
+ * with a NaN or +inf, or with nothing above -inf, yields NaN (its ids are
+ * still ordered).  targets and logprobs may both be NULL, entropy may be
+ * NULL.  One pass over the logits; sums in f32.  workspace of at least
+ * qbk_logprobs_workspace_size bytes, 16-byte aligned. */
+size_t qbk_logprobs_workspace_size(size_t rows, size_t vocab, size_t top_k);
+int qbk_logprobs_dev(qbk_ctx *ctx, const void *logits, int dtype, size_t rows, size_t vocab, size_t row_stride,
+                     const int32_t *targets, float *logprobs, float *entropy, size_t top_k, int32_t *top_ids,
+                     float *top_logprobs, void *workspace, size_t workspace_size, void *stream);
 
 #ifdef __cplusplus
 }

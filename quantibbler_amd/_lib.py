@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(HERE, "libqbk.so")
 
 QBK_OK, QBK_ERR_VALIDATION, QBK_ERR_DEVICE, QBK_ERR_INIT = 0, 1, 2, 3
 QBK_F64, QBK_F32, QBK_BF16 = 0, 1, 2
+QBK_KV_INT8, QBK_KV_FP8 = 0, 1
 
 
 class KernelError(ValueError):
@@ -32,6 +33,11 @@ class AttnShape(C.Structure):
     """gpu_attention.rs:402-411 AttentionShape."""
     _fields_ = [(n, C.c_size_t) for n in
                 ("batch", "n_heads", "n_kv_heads", "seq_q", "seq_kv", "head_dim", "val_dim")]
+
+
+class KvShape(C.Structure):
+    """qbk_kv_shape: an 8-bit KV cache's format and sizes."""
+    _fields_ = [("format", C.c_int)] + [(n, C.c_size_t) for n in ("n_seqs", "capacity", "n_kv_heads", "head_dim")]
 
 
 _P, _Z, _I = C.c_void_p, C.c_size_t, C.c_int
@@ -109,6 +115,14 @@ _SIGS = {
     "qbk_head_info": (_I, [_P, C.POINTER(_Z), C.POINTER(_Z), C.POINTER(_I)]),
     "qbk_head_logits": (_I, [_P, _P, _P, _Z, _P, _Z]),
     "qbk_head_logits_dev": (_I, [_P, _P, _P, _Z, _P, _P]),
+    "qbk_kv_cache_size": (_Z, [C.POINTER(KvShape)]),
+    "qbk_kv_cache_write_dev": (_I, [_P, C.POINTER(KvShape), _P, _P, _P, _I, _Z, _Z, _P, _P, _Z, _Z, _P]),
+    "qbk_kv_cache_read_dev": (_I, [_P, C.POINTER(KvShape), _P, _P, _P, _I, _Z, _Z, _P, _P, _Z, _Z, _P]),
+    "qbk_attention_kv_workspace_size": (_Z, [C.POINTER(KvShape), _Z, _Z, _Z, _Z, _Z]),
+    "qbk_attention_kv_dev": (_I, [_P, C.POINTER(KvShape), _P, _Z, _Z, _P, _Z, C.POINTER(KvShape), _P, _Z, _Z, _Z,
+                                  _Z, _P, _I, _P, _P, _Z, _P]),
+    "qbk_logprobs_workspace_size": (_Z, [_Z, _Z, _Z]),
+    "qbk_logprobs_dev": (_I, [_P, _P, _I, _Z, _Z, _Z, _P, _P, _P, _Z, _P, _P, _P, _Z, _P]),
     "qbk_sage_blk_workspace_size": (_Z, [C.POINTER(AttnShape)]),
     "qbk_attention_sage_blk_dev": (_I, [_P, C.POINTER(AttnShape), _P, _P, _P, _I, _P, _P, _Z, _P]),
     "qbk_sage_blk_quantize_dev": (_I, [_P, C.POINTER(AttnShape), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),

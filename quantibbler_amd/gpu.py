@@ -18,7 +18,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import AttnShape, check
+from ._lib import AttnShape, KvShape, check
 
 _DTYPES = {"float64": (_lib.QBK_F64, np.float64), "float32": (_lib.QBK_F32, np.float32),
            "bfloat16": (_lib.QBK_BF16, np.uint16)}
@@ -269,6 +269,146 @@ def argmax_dev(ctx: GpuContext, logits, rows: int, vocab: int, out, stream=None)
     """sampler.rs:4-15 greedy, per row (int32 ids into ``out``)."""
     check(_lib.load().qbk_argmax_dev(ctx.handle, _ptr(logits), int(rows), int(vocab), _ptr(out),
                                      _stream(stream)))
+
+
+def logprobs_workspace_size(rows: int, vocab: int, top_k: int = 0) -> int:
+    """Bytes of workspace ``logprobs_dev`` needs."""
+    need = int(_lib.load().qbk_logprobs_workspace_size(int(rows), int(vocab), int(top_k)))
+    if need == 0 and rows > 0:
+        raise _lib.KernelError(_lib.load().qbk_last_error().decode())
+    return need
+
+
+def logprobs_dev(ctx: GpuContext, logits, rows: int, vocab: int, targets, logprobs, entropy, workspace,
+                 workspace_size: int, top_k: int = 0, top_ids=None, top_logprobs=None, dtype: str = "float32",
+                 row_stride: int | None = None, stream=None):
+    """Per row of ``vocab`` logits ("float32" or "bfloat16", ``row_stride``
+    values apart): the log probability of the row's target (device int32)
+    into ``logprobs``, the distribution's entropy in nats into ``entropy``
+    and the ``top_k`` likeliest tokens, ids and log probabilities in order,
+    into ``top_ids`` / ``top_logprobs`` [rows][top_k] (equal logits: the lower
+    id first).  ``targets`` with ``logprobs``, and ``entropy``, may be None."""
+    check(_lib.load().qbk_logprobs_dev(ctx.handle, _ptr(logits), _DTYPES[dtype][0], int(rows), int(vocab),
+                                       int(vocab if row_stride is None else row_stride), _ptr(targets),
+                                       _ptr(logprobs), _ptr(entropy), int(top_k), _ptr(top_ids), _ptr(top_logprobs),
+                                       _ptr(workspace), int(workspace_size), _stream(stream)))
+
+
+class KvCache:
+    """A KV cache in 8 bits for ``n_seqs`` sequences of up to ``capacity``
+    rows: per row and kv head, head_dim codes ("int8" or "fp8", OCP e4m3) and
+    one f32 scale, quantised as rows are written.  ``buffer`` is the caller's
+    device memory of ``size(...)`` bytes.  Positions, lengths and row starts
+    are device uint32 (or int32) read when a call runs, so a captured graph of
+    a step serves every later position."""
+
+    FORMATS = {"int8": _lib.QBK_KV_INT8, "fp8": _lib.QBK_KV_FP8}
+
+    def __init__(self, ctx: GpuContext, fmt: str, n_seqs: int, capacity: int, n_kv_heads: int, head_dim: int, buffer):
+        need = self.size(fmt, n_seqs, capacity, n_kv_heads, head_dim)
+        have = _nbytes(buffer)
+        if have is not None and have < need:
+            raise _lib.KernelError(f"kv cache buffer of {have} bytes is smaller than the {need} it needs")
+        self.ctx, self.format, self.buffer = ctx, fmt, buffer
+        self.n_seqs, self.capacity = int(n_seqs), int(capacity)
+        self.n_kv_heads, self.head_dim = int(n_kv_heads), int(head_dim)
+        self._shape = KvShape(self.FORMATS[fmt], self.n_seqs, self.capacity, self.n_kv_heads, self.head_dim)
+
+    @classmethod
+    def size(cls, fmt: str, n_seqs: int, capacity: int, n_kv_heads: int, head_dim: int) -> int:
+        """Bytes of device memory the cache needs."""
+        if fmt not in cls.FORMATS:
+            raise _lib.KernelError(f"kv cache format must be one of {sorted(cls.FORMATS)}, got {fmt!r}")
+        if min(int(n_seqs), int(capacity), int(n_kv_heads), int(head_dim)) < 0:
+            raise _lib.KernelError("kv cache sizes must not be negative")
+        shape = KvShape(cls.FORMATS[fmt], int(n_seqs), int(capacity), int(n_kv_heads), int(head_dim))
+        need = int(_lib.load().qbk_kv_cache_size(C.byref(shape)))
+        if need == 0:
+            raise _lib.KernelError(_lib.load().qbk_last_error().decode())
+        return need
+
+    def _rows(self, fn, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start, row_stride, stream):
+        if dtype not in ("float32", "bfloat16"):
+            raise _lib.KernelError(f"kv cache rows must be 'float32' or 'bfloat16', got {dtype!r}")
+        n = self.n_seqs - int(first_seq) if n_seqs is None else int(n_seqs)
+        stride = self.n_kv_heads * self.head_dim if row_stride is None else int(row_stride)
+        if min(int(n_rows), int(first_seq), n, stride) < 0:
+            raise _lib.KernelError("kv cache rows, sequences and strides must not be negative")
+        _device_words(pos, n, "positions")
+        if row_start is not None:
+            _device_words(row_start, n + 1, "row starts")
+        check(fn(self.ctx.handle, C.byref(self._shape), _ptr(self.buffer), _ptr(k), _ptr(v), _DTYPES[dtype][0], stride,
+                 int(n_rows), _ptr(row_start), _ptr(pos), int(first_seq), n, _stream(stream)))
+
+    def write_dev(self, k, v, dtype: str, pos, n_rows: int, first_seq: int = 0, n_seqs: int | None = None,
+                  row_start=None, row_stride: int | None = None, stream=None):
+        """Quantises ``n_rows`` rows of [n_kv_heads][head_dim] keys and values
+        (``row_stride`` values apart, so a fused projection's rows are taken
+        in place) into sequences first_seq .. first_seq + n_seqs - 1: rows
+        row_start[i] .. row_start[i + 1] - 1 go to sequence first_seq + i at
+        positions pos[i], pos[i] + 1, ...; ``row_start`` None splits the rows
+        evenly.  Rows past the capacity are left out."""
+        self._rows(_lib.load().qbk_kv_cache_write_dev, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start,
+                   row_stride, stream)
+
+    def read_dev(self, k, v, dtype: str, pos, n_rows: int, first_seq: int = 0, n_seqs: int | None = None,
+                 row_start=None, row_stride: int | None = None, stream=None):
+        """The rows ``write_dev`` of the same arguments put there, as values,
+        into ``k`` and ``v``; a row past the capacity is NaN."""
+        self._rows(_lib.load().qbk_kv_cache_read_dev, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start,
+                   row_stride, stream)
+
+    def _bounds(self, n_seqs, first_seq, max_len):
+        n = self.n_seqs - int(first_seq) if n_seqs is None else int(n_seqs)
+        most = self.capacity if max_len is None else int(max_len)
+        return n, most
+
+    def attention_workspace_size(self, n_heads: int, n_seqs: int | None = None, seq_q: int = 1,
+                                 max_len: int | None = None, prefix_len: int = 0) -> int:
+        """Bytes of workspace ``attention_dev`` of the same sizes needs."""
+        n, most = self._bounds(n_seqs, 0, max_len)
+        if min(n, most, int(n_heads), int(seq_q), int(prefix_len)) < 0:
+            raise _lib.KernelError("kv attention sizes must not be negative")
+        lib = _lib.load()
+        need = int(lib.qbk_attention_kv_workspace_size(C.byref(self._shape), int(n_heads), n, int(seq_q), most,
+                                                       int(prefix_len)))
+        return need
+
+    def attention_dev(self, q, dtype: str, n_heads: int, lens, out, workspace, workspace_size: int,
+                      first_seq: int = 0, n_seqs: int | None = None, seq_q: int = 1, max_len: int | None = None,
+                      prefix: "KvCache | None" = None, prefix_seq: int = 0, prefix_len: int = 0, stream=None):
+        """Attention of the last ``seq_q`` positions of n_seqs sequences:
+        ``q`` and ``out`` [n_seqs][seq_q][n_heads][head_dim] ("float32" or
+        "bfloat16"), ``lens`` each sequence's own rows (the queries' rows
+        among them), at most ``max_len`` (the capacity if None).  Every query
+        also sees rows 0 .. prefix_len - 1 of ``prefix``'s sequence
+        ``prefix_seq``, read once for the whole batch."""
+        if dtype not in ("float32", "bfloat16"):
+            raise _lib.KernelError(f"kv attention takes 'float32' or 'bfloat16' queries, got {dtype!r}")
+        n, most = self._bounds(n_seqs, first_seq, max_len)
+        if min(n, most, int(first_seq), int(n_heads), int(seq_q), int(prefix_seq), int(prefix_len)) < 0:
+            raise _lib.KernelError("kv attention sizes must not be negative")
+        if prefix_len and prefix is None:
+            raise _lib.KernelError("a prefix_len needs the cache that holds the prefix")
+        _device_words(lens, n, "lengths")
+        p = prefix if prefix_len else None
+        check(_lib.load().qbk_attention_kv_dev(
+            self.ctx.handle, C.byref(self._shape), _ptr(self.buffer), int(first_seq), n, _ptr(lens), most,
+            None if p is None else C.byref(p._shape), None if p is None else _ptr(p.buffer), int(prefix_seq),
+            int(prefix_len), int(n_heads), int(seq_q), _ptr(q), _DTYPES[dtype][0], _ptr(out), _ptr(workspace),
+            int(workspace_size), _stream(stream)))
+
+
+def _device_words(x, n: int, what: str):
+    """``x`` a contiguous 32-bit device tensor of at least n entries, or a raw
+    device address the caller vouches for."""
+    if hasattr(x, "is_cuda"):
+        if not x.is_cuda or str(x.dtype) not in ("torch.int32", "torch.uint32") or not x.is_contiguous() \
+                or x.numel() < n:
+            raise _lib.KernelError(f"{what} must be a contiguous 32-bit device tensor of at least {n} entries; got "
+                                   f"{x.dtype} of {x.numel()} on {x.device}")
+    elif not isinstance(x, int):
+        raise _lib.KernelError(f"{what} must be a device tensor or a device address")
 
 
 class SageDecodeState:

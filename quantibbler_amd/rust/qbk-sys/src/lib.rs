@@ -29,6 +29,8 @@ pub const QBK_F32: c_int = 1;
 pub const QBK_BF16: c_int = 2;
 pub const QBK_ATTN_SAGE: c_int = 0;
 pub const QBK_ATTN_EXACT: c_int = 1;
+pub const QBK_KV_INT8: c_int = 0;
+pub const QBK_KV_FP8: c_int = 1;
 
 #[repr(C)]
 pub struct QbkCtx {
@@ -62,6 +64,17 @@ pub struct AttentionShape {
     pub seq_kv: usize,
     pub head_dim: usize,
     pub val_dim: usize,
+}
+
+/// qbk_kv_shape: an 8-bit KV cache's format and sizes.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub struct KvShape {
+    pub format: c_int,
+    pub n_seqs: usize,
+    pub capacity: usize,
+    pub n_kv_heads: usize,
+    pub head_dim: usize,
 }
 
 extern "C" {
@@ -207,6 +220,27 @@ extern "C" {
     pub fn qbk_head_info(head: *const QbkHead, vocab: *mut usize, d_model: *mut usize, bf16: *mut c_int) -> c_int;
     pub fn qbk_head_logits_dev(ctx: *mut QbkCtx, head: *const QbkHead, hidden: *const f32, batch: usize,
                                logits: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn qbk_kv_cache_size(shape: *const KvShape) -> usize;
+    pub fn qbk_kv_cache_write_dev(ctx: *mut QbkCtx, shape: *const KvShape, cache: *mut c_void, k: *const c_void,
+                                  v: *const c_void, dtype: c_int, row_stride: usize, n_rows: usize,
+                                  row_start: *const u32, pos: *const u32, first_seq: usize, n: usize,
+                                  stream: *mut c_void) -> c_int;
+    pub fn qbk_kv_cache_read_dev(ctx: *mut QbkCtx, shape: *const KvShape, cache: *const c_void, k: *mut c_void,
+                                 v: *mut c_void, dtype: c_int, row_stride: usize, n_rows: usize,
+                                 row_start: *const u32, pos: *const u32, first_seq: usize, n: usize,
+                                 stream: *mut c_void) -> c_int;
+    pub fn qbk_attention_kv_workspace_size(shape: *const KvShape, n_heads: usize, n: usize, seq_q: usize,
+                                           max_len: usize, prefix_len: usize) -> usize;
+    pub fn qbk_attention_kv_dev(ctx: *mut QbkCtx, shape: *const KvShape, cache: *const c_void, first_seq: usize,
+                                n: usize, lens: *const u32, max_len: usize, prefix_shape: *const KvShape,
+                                prefix: *const c_void, prefix_seq: usize, prefix_len: usize, n_heads: usize,
+                                seq_q: usize, q: *const c_void, dtype: c_int, out: *mut c_void,
+                                workspace: *mut c_void, workspace_size: usize, stream: *mut c_void) -> c_int;
+    pub fn qbk_logprobs_workspace_size(rows: usize, vocab: usize, top_k: usize) -> usize;
+    pub fn qbk_logprobs_dev(ctx: *mut QbkCtx, logits: *const c_void, dtype: c_int, rows: usize, vocab: usize,
+                            row_stride: usize, targets: *const i32, logprobs: *mut f32, entropy: *mut f32,
+                            top_k: usize, top_ids: *mut i32, top_logprobs: *mut f32, workspace: *mut c_void,
+                            workspace_size: usize, stream: *mut c_void) -> c_int;
 }
 
 /// core.rs:31 KernelError: the reference's message text.
