@@ -21,6 +21,8 @@
 // that a weight keeps its bits down to 2^-26 of the largest.  Sums are f32.
 #include <math.h>
 
+#include <atomic>
+
 #include "kvcache.h"
 
 #pragma clang fp contract(off)
@@ -122,24 +124,16 @@ struct KvaLds {
     static constexpr int BYTES = BODY + NQ * 16 * 4 * (1 + 2 * KVA_WAVES);
 };
 
-// Rows row0 .. row0 + n_rows - 1 (at most 16 NQ) of kv head hk over key tiles
-// tile0 .. tile1 - 1 of the slab k, v, ks, vs.  Row r of the body sees keys
-// below limit(r), none of them at or past `written`.
-template <int FMT, int DC, int NQ, typename T, class Limit>
-__device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows, uint32_t hk,
-                                         const uint8_t *kcode, const uint8_t *vcode, const float *ksc,
-                                         const float *vsc, uint32_t tile0, uint32_t tile1, uint32_t written,
-                                         Limit limit, uint32_t split, bool last) {
-    constexpr bool HI = sizeof(T) == 4;
-    using L = KvaLds<DC, NQ, HI>;
-    constexpr int STEPS = L::STEPS;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-    const int hd = (int)a.own.hd, nc = hd / 16;
-    char *qs = smem;
-    float *cqs = (float *)(smem + L::BODY), *refs = cqs + NQ * 16, *sums = refs + KVA_WAVES * NQ * 16;
-
-    // queries: a wave a row, four channels a lane
-    for (int r = wave; r < 16 * NQ; r += KVA_WAVES) {
+// Queries row0 .. row0 + n_rows - 1 (at most 16 NT) of kv head hk into LDS as
+// the B operands of K q^T, [tile][step][lane][16 bytes], for f32 queries the
+// low halves behind them; cqs[r]: the factor that scores of row r still need.
+template <int DC, int NT, typename T>
+__device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float *cqs, uint32_t row0, uint32_t n_rows,
+                                            uint32_t hk) {
+    constexpr int STEPS = 2 * DC;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = (int)a.own.hd;
+    // a wave a row, four channels a lane
+    for (int r = wave; r < 16 * NT; r += KVA_WAVES) {
         float x[4] = {0, 0, 0, 0};
         uint32_t top = 0;
         const int c = 4 * lane;
@@ -176,12 +170,133 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
             const int chunk = c >> 4, step = 2 * (chunk >> 2) + ((c >> 3) & 1);
             const size_t at = (size_t)(((r >> 4) * STEPS + step) * 64 + (chunk & 3) * 16 + (r & 15)) * 16 + (c & 7) * 2;
             *(uint2 *)(qs + at) = uint2{__builtin_bit_cast(uint32_t, hi[0]), __builtin_bit_cast(uint32_t, hi[1])};
-            if constexpr (HI)
-                *(uint2 *)(qs + NQ * STEPS * 1024 + at) =
+            if constexpr (sizeof(T) == 4)
+                *(uint2 *)(qs + NT * STEPS * 1024 + at) =
                     uint2{__builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1])};
         }
         if (lane == 0) cqs[r] = whole ? a.scale * __uint_as_float((ex - 3) << 23) : __builtin_nanf("");
     }
+}
+
+// Value scales to 2^12 over a power of two at or above every one so far
+// (vref; the outputs follow when it moves).
+template <int NQ, int CT>
+__device__ __forceinline__ void kva_value_scales(kva_f4_t (&vs)[4], float &vref, float &vinv, kva_f4_t (&o)[NQ][CT]) {
+    float vm = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) vm = fmaxf(fmaxf(fmaxf(vm, vs[i][0]), fmaxf(vs[i][1], vs[i][2])), vs[i][3]);
+    if (__ballot(vm > vref)) {
+        vm = kva_max4(vm);
+        const uint32_t e = (__float_as_uint(vm) >> 23) + 1;  // scales are 2^-107 .. 2^122
+        const float to = __uint_as_float(e << 23);
+        vinv = __uint_as_float((266 - e) << 23);
+        const float f = vref * __uint_as_float((254 - e) << 23);
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) o[q][ct] *= f;
+        vref = to;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) vs[i] *= vinv;
+}
+
+// One query tile's scores (16 keys a lane: 16 i + j past key) to weights: the
+// reference moves when a score passes it eightfold, sum and outputs with it;
+// p times the value scales as operands ph (and pl, the halves' rests).
+template <int CT, bool HI>
+__device__ __forceinline__ void kva_softmax(const kva_f4_t (&s)[4], const kva_f4_t (&vs)[4], float cq, bool masked,
+                                            uint32_t key, uint32_t lim, float &ref, float &sum, kva_f4_t (&o)[CT],
+                                            kva_h8_t (&ph)[2], kva_h8_t (&pl)[2]) {
+    float t[4][4], tm = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            t[i][j] = s[i][j];
+            if (masked && key + 16 * i + j >= lim) t[i][j] = -INFINITY;
+            tm = fmaxf(tm, t[i][j]);
+        }
+    if (__ballot(tm * cq > ref + 3.0f)) {
+        const float to = fmaxf(ref, ceilf(kva_max4(tm) * cq));
+        const float f = kva_rescale(ref, to);
+        sum *= f;
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) o[ct] *= f;
+        ref = to;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const bool out = masked && key + 16 * i + j >= lim;
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j], cq, -ref));
+            if (out) p = 0.0f;
+            sum += p;
+            w[j] = p * vs[i][j];
+            if (out) w[j] = 0.0f;  // whatever the scale holds
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const _Float16 h = (_Float16)w[j];
+            ph[i >> 1][4 * (i & 1) + j] = h;
+            if constexpr (HI) pl[i >> 1][4 * (i & 1) + j] = (_Float16)(w[j] - (float)h);
+        }
+    }
+}
+
+// Rows row0 .. row0 + n_rows - 1 (at most 16 NQ) of kv head hk over key tiles
+// tile0 .. tile1 - 1 of the slab k, v, ks, vs.  Row r of the body sees keys
+// below limit(r), none of them at or past `written`.
+template <int FMT, int DC, int NQ, typename T, class Limit>
+__device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows, uint32_t hk,
+                                         const uint8_t *kcode, const uint8_t *vcode, const float *ksc,
+                                         const float *vsc, uint32_t tile0, uint32_t tile1, uint32_t written,
+                                         Limit limit, uint32_t split, bool last) {
+    constexpr bool HI = sizeof(T) == 4;
+    using L = KvaLds<DC, NQ, HI>;
+    constexpr int STEPS = L::STEPS;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int hd = (int)a.own.hd, nc = hd / 16;
+    char *qs = smem;
+    float *cqs = (float *)(smem + L::BODY), *refs = cqs + NQ * 16, *sums = refs + KVA_WAVES * NQ * 16;
+
+    // A tile's codes and scales travel while the one before is worked on: keys
+    // and their scales are asked for again as soon as the scores are formed,
+    // values once they are added, the first of both before the queries are read.
+    kva_u4_t kc[DC][4], vc[4 * DC];
+    kva_f4_t ks[4], vs[4];
+    const int spread = col * 16;
+    auto load_k = [&](uint32_t tt) {
+        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + spread;
+        const float *st = ksc + (size_t)tt * 64 + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) ks[i] = *(const kva_f4_t *)(st + 16 * i);
+#pragma unroll
+        for (int c = 0; c < DC; c++) {
+            if (4 * c >= nc) continue;
+            const int chunk = 4 * c + g < nc ? 4 * c + g : nc - 1;  // past the last chunk q is zero
+#pragma unroll
+            for (int i = 0; i < 4; i++) kc[c][i] = *(const kva_u4_t *)(kt + (i * nc + chunk) * 256);
+        }
+    };
+    auto load_v = [&](uint32_t tt) {
+        const uint8_t *vt = vcode + (size_t)tt * 64 * hd + col * 64 + g * 16;
+        const float *st = vsc + (size_t)tt * 64 + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) vs[i] = *(const kva_f4_t *)(st + 16 * i);
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++)
+            if (ct < nc) vc[ct] = *(const kva_u4_t *)(vt + ct * 1024);
+    };
+    const uint32_t first = tile0 + wave;
+    if (first < tile1) {
+        load_k(first);
+        load_v(first);
+    }
+
+    kva_queries<DC, NQ, T>(a, qs, cqs, row0, n_rows, hk);
     __syncthreads();
 
     kva_f4_t o[NQ][4 * DC];
@@ -201,16 +316,9 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     least = limit(0);
     float vref = 0.0f, vinv = 0.0f;  // a power of two at or above every value scale so far, and 2^12 over it
 
-    for (uint32_t tt = tile0 + wave; tt < tile1; tt += KVA_WAVES) {
+    for (uint32_t tt = first; tt < tile1; tt += KVA_WAVES) {
         const uint32_t key0 = tt * 64;
-        const bool masked = key0 + 64 > least;
-        const uint8_t *kt = kcode + (size_t)tt * 64 * hd, *vt = vcode + (size_t)tt * 64 * hd;
-        kva_f4_t ks[4], vs[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            ks[i] = *(const kva_f4_t *)(ksc + key0 + 16 * i + 4 * g);
-            vs[i] = *(const kva_f4_t *)(vsc + key0 + 16 * i + 4 * g);
-        }
+        const bool masked = key0 + 64 > least, more = tt + KVA_WAVES < tile1;
         if (masked) {  // what was never written takes no part, whatever it holds
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -226,15 +334,11 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
 #pragma unroll
         for (int c = 0; c < DC; c++) {
             if (4 * c >= nc) continue;
-            const int chunk = 4 * c + g < nc ? 4 * c + g : nc - 1;  // past the last chunk q is zero
-            kva_u4_t kc[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) kc[i] = *(const kva_u4_t *)(kt + (size_t)(i * nc + chunk) * 256 + col * 16);
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 kva_h8_t kf[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) kf[i] = kva_wide<FMT>(kc[i][2 * u], kc[i][2 * u + 1]);
+                for (int i = 0; i < 4; i++) kf[i] = kva_wide<FMT>(kc[c][i][2 * u], kc[c][i][2 * u + 1]);
 #pragma unroll
                 for (int q = 0; q < NQ; q++) {
                     const kva_h8_t qf = *(const kva_h8_t *)(qs + (size_t)((q * STEPS + 2 * c + u) * 64 + lane) * 16);
@@ -251,64 +355,18 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
                 }
             }
         }
-        // value scales: a common power of two for the wave's outputs
-        float vm = 0.0f;
+        // scores in units of 1 / cq; the key registers are free again
 #pragma unroll
-        for (int i = 0; i < 4; i++) vm = fmaxf(fmaxf(fmaxf(vm, vs[i][0]), fmaxf(vs[i][1], vs[i][2])), vs[i][3]);
-        if (__ballot(vm > vref)) {
-            vm = kva_max4(vm);
-            const uint32_t e = (__float_as_uint(vm) >> 23) + 1;  // scales are 2^-107 .. 2^122
-            const float to = __uint_as_float(e << 23);
-            vinv = __uint_as_float((266 - e) << 23);
-            const float f = vref * __uint_as_float((254 - e) << 23);
+        for (int q = 0; q < NQ; q++)
 #pragma unroll
-            for (int q = 0; q < NQ; q++)
-#pragma unroll
-                for (int ct = 0; ct < 4 * DC; ct++) o[q][ct] *= f;
-            vref = to;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) vs[i] *= vinv;
+            for (int i = 0; i < 4; i++) s[q][i] *= ks[i];
+        if (more) load_k(tt + KVA_WAVES);
+        kva_value_scales<NQ, 4 * DC>(vs, vref, vinv, o);
 
         kva_h8_t ph[NQ][2], pl[NQ][2];
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
-            float t[4][4], tm = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    t[i][j] = s[q][i][j] * ks[i][j];
-                    if (masked && key0 + 16 * i + 4 * g + j >= lim[q]) t[i][j] = -INFINITY;
-                    tm = fmaxf(tm, t[i][j]);
-                }
-            // weights may pass the reference eightfold before it moves
-            if (__ballot(tm * cq[q] > ref[q] + 3.0f)) {
-                const float to = fmaxf(ref[q], ceilf(kva_max4(tm) * cq[q]));
-                const float f = kva_rescale(ref[q], to);
-                sum[q] *= f;
-#pragma unroll
-                for (int ct = 0; ct < 4 * DC; ct++) o[q][ct] *= f;
-                ref[q] = to;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float w[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j], cq[q], -ref[q]));
-                    if (masked && key0 + 16 * i + 4 * g + j >= lim[q]) p = 0.0f;
-                    sum[q] += p;
-                    w[j] = p * vs[i][j];
-                    if (masked && key0 + 16 * i + 4 * g + j >= lim[q]) w[j] = 0.0f;
-                }
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const _Float16 h = (_Float16)w[j];
-                    ph[q][i >> 1][4 * (i & 1) + j] = h;
-                    if constexpr (HI) pl[q][i >> 1][4 * (i & 1) + j] = (_Float16)(w[j] - (float)h);
-                }
-            }
+            kva_softmax<4 * DC, HI>(s[q], vs, cq[q], masked, key0 + 4 * g, lim[q], ref[q], sum[q], o[q], ph[q], pl[q]);
         }
         // fp8 rows that were never written may hold NaN codes
         uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
@@ -322,14 +380,14 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++) {
             if (ct >= nc) continue;
-            kva_u4_t vc = *(const kva_u4_t *)(vt + (size_t)(ct * 16 + col) * 64 + g * 16);
+            kva_u4_t w = vc[ct];
             if (FMT == QBK_KV_FP8) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) vc[i] &= keep[i];
+                for (int i = 0; i < 4; i++) w[i] &= keep[i];
             }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const kva_h8_t vf = kva_wide<FMT>(vc[2 * u], vc[2 * u + 1]);
+                const kva_h8_t vf = kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
 #pragma unroll
                 for (int q = 0; q < NQ; q++) {
                     o[q][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[q][u], o[q][ct], 0, 0, 0);
@@ -338,6 +396,7 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
                 }
             }
         }
+        if (more) load_v(tt + KVA_WAVES);
     }
 
     // join the waves on each row's largest reference
@@ -401,20 +460,205 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     }
 }
 
+// The body of many rows: a wave 16 NQ rows of the 64 NQ, every wave every key
+// tile.  A tile is widened once for the four of them, a quarter by each wave,
+// into LDS in operand order (each 16-byte access of a wave is 1 KiB in a row),
+// while the next tile's codes travel; two buffers and one barrier a tile (256
+// channels: one buffer, two barriers).
+template <int DC>
+struct KvaStage {
+    static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 512, BUFS = DC < 4 ? 2 : 1;
+};
+template <int DC, int NQ, bool HI>
+struct KvaWideLds {
+    static constexpr int Q = 4 * NQ * 2 * DC * 1024 * (HI ? 2 : 1);  // under the stages, read into registers first
+    static constexpr int S = KvaStage<DC>::BYTES * KvaStage<DC>::BUFS;
+    static constexpr int BODY = Q > S ? Q : S;
+    static constexpr int BYTES = BODY + 64 * NQ * 4;
+};
+
+template <int FMT, int DC, int NQ, typename T, class Limit>
+__device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows,
+                                              uint32_t hk, const uint8_t *kcode, const uint8_t *vcode,
+                                              const float *ksc, const float *vsc, uint32_t tile0, uint32_t tile1,
+                                              uint32_t written, Limit limit, uint32_t split, bool last) {
+    constexpr bool HI = sizeof(T) == 4;
+    constexpr int STEPS = 2 * DC, BUFS = KvaStage<DC>::BUFS;
+    using L = KvaWideLds<DC, NQ, HI>;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int hd = (int)a.own.hd, nc = hd / 16;
+    float *cqs = (float *)(smem + L::BODY);
+
+    kva_u4_t kc[DC], vc[DC];  // this wave's quarter: keys of block `wave`, channel tiles wave, wave + 4, ..
+    float sc = 0.0f;          // threads 0 .. 63 a key's scale, 64 .. 127 a value's
+    auto load = [&](uint32_t tt) {
+        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + (size_t)wave * 16 * hd + col * 16;
+        const uint8_t *vt = vcode + (size_t)tt * 64 * hd + col * 64 + g * 16;
+#pragma unroll
+        for (int c = 0; c < DC; c++) {
+            const int chunk = 4 * c + g < nc ? 4 * c + g : nc - 1;  // past the last chunk q is zero
+            kc[c] = *(const kva_u4_t *)(kt + chunk * 256);
+            if (wave + 4 * c < nc) vc[c] = *(const kva_u4_t *)(vt + (wave + 4 * c) * 1024);
+        }
+        if (wave < 2) sc = (wave ? vsc : ksc)[(size_t)tt * 64 + lane];
+    };
+    auto stage = [&](uint32_t tt, char *buf) {
+        const uint32_t key0 = tt * 64;
+        kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
+        const bool tail = key0 + 64 > written;  // rows that were never written take no part, whatever they hold
+        if (FMT == QBK_KV_FP8 && tail) {        // NaN codes
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t k0 = key0 + 16 * i + 4 * g, left = written > k0 ? written - k0 : 0;
+                keep[i] = left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < DC; c++) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                *(kva_h8_t *)(buf + ((wave * STEPS + 2 * c + u) * 64 + lane) * 16) =
+                    kva_wide<FMT>(kc[c][2 * u], kc[c][2 * u + 1]);
+            if (wave + 4 * c < nc) {
+                const kva_u4_t w = vc[c] & keep;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+                    *(kva_h8_t *)(buf + KvaStage<DC>::KEYS + ((2 * (wave + 4 * c) + u) * 64 + lane) * 16) =
+                        kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
+            }
+        }
+        if (wave < 2)
+            *(float *)(buf + 2 * KvaStage<DC>::KEYS + wave * 256 + lane * 4) = tail && key0 + lane >= written ? 0.0f : sc;
+    };
+    if (tile0 < tile1) load(tile0);
+    kva_queries<DC, 4 * NQ, T>(a, smem, cqs, row0, n_rows, hk);
+    __syncthreads();
+    kva_h8_t qh[NQ][STEPS], ql[NQ][STEPS];
+    kva_f4_t o[NQ][4 * DC];
+    float ref[NQ], sum[NQ], cq[NQ], vref = 0.0f, vinv = 0.0f;
+    uint32_t lim[NQ];
+    const uint32_t my0 = wave * 16 * NQ;  // this wave's first row
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            const char *at = smem + (((wave * NQ + q) * STEPS + st) * 64 + lane) * 16;
+            qh[q][st] = *(const kva_h8_t *)at;
+            if constexpr (HI) ql[q][st] = *(const kva_h8_t *)(at + 4 * NQ * STEPS * 1024);
+        }
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++) o[q][ct] = kva_f4_t{0, 0, 0, 0};
+        ref[q] = -INFINITY;
+        sum[q] = 0.0f;
+        cq[q] = cqs[my0 + 16 * q + col];
+        const uint32_t r = my0 + 16 * q + col;
+        lim[q] = limit(r < n_rows ? r : n_rows - 1);
+    }
+    const bool rows = my0 < n_rows;
+    const uint32_t least = limit(rows ? my0 : 0), end = my0 + 16 * NQ < n_rows ? my0 + 16 * NQ : n_rows;
+    const uint32_t most = rows ? limit(end - 1) : 0;  // no row of the wave sees keys from here on
+    __syncthreads();  // the queries are read
+
+    for (uint32_t tt = tile0; tt < tile1; tt++) {
+        char *buf = smem + (BUFS == 2 ? ((tt - tile0) & 1) * KvaStage<DC>::BYTES : 0);
+        if (BUFS == 1 && tt > tile0) __syncthreads();
+        stage(tt, buf);
+        __syncthreads();
+        if (tt + 1 < tile1) load(tt + 1);
+        const uint32_t key0 = tt * 64;
+        if (key0 >= most) continue;
+        const bool masked = key0 + 64 > least;
+        kva_f4_t ks[4], vs[4], s[NQ][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            ks[i] = *(const kva_f4_t *)(buf + 2 * KvaStage<DC>::KEYS + (16 * i + 4 * g) * 4);
+            vs[i] = *(const kva_f4_t *)(buf + 2 * KvaStage<DC>::KEYS + 256 + (16 * i + 4 * g) * 4);
+#pragma unroll
+            for (int q = 0; q < NQ; q++) s[q][i] = kva_f4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+            if (4 * (st / 2) >= nc) continue;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const kva_h8_t kf = *(const kva_h8_t *)(buf + ((i * STEPS + st) * 64 + lane) * 16);
+#pragma unroll
+                for (int q = 0; q < NQ; q++) {
+                    s[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[q][st], s[q][i], 0, 0, 0);
+                    if constexpr (HI) s[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[q][st], s[q][i], 0, 0, 0);
+                }
+            }
+        }
+        kva_value_scales<NQ, 4 * DC>(vs, vref, vinv, o);
+        kva_h8_t ph[NQ][2], pl[NQ][2];
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[q][i] *= ks[i];
+            kva_softmax<4 * DC, HI>(s[q], vs, cq[q], masked, key0 + 4 * g, lim[q], ref[q], sum[q], o[q], ph[q], pl[q]);
+        }
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++) {
+            if (ct >= nc) continue;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const kva_h8_t vf =
+                    *(const kva_h8_t *)(buf + KvaStage<DC>::KEYS + ((2 * ct + u) * 64 + lane) * 16);
+#pragma unroll
+                for (int q = 0; q < NQ; q++) {
+                    o[q][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[q][u], o[q][ct], 0, 0, 0);
+                    if constexpr (HI) o[q][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[q][u], o[q][ct], 0, 0, 0);
+                }
+            }
+        }
+    }
+    const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0;
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        const uint32_t r = my0 + 16 * q + col;
+        const float l = kva_sum4(sum[q]), f = vref * 0x1p-12f;
+        if (r >= n_rows) continue;
+        if (last) {
+            const uint32_t rho = row0 + r;
+            T *dst = (T *)a.out + ((size_t)(rho / a.G) * a.H + (size_t)hk * a.G + rho % a.G) * hd + 4 * g;
+#pragma unroll
+            for (int ct = 0; ct < 4 * DC; ct++) {
+                if (ct >= nc) continue;
+#pragma unroll
+                for (int j = 0; j < 4; j++) dst[16 * ct + j] = kva_out<T>(l == 0.0f ? 0.0f : o[q][ct][j] * f / l);
+            }
+        } else {
+            float *dst = a.po + (part + r) * hd + 4 * g;
+#pragma unroll
+            for (int ct = 0; ct < 4 * DC; ct++)
+                if (ct < nc) *(kva_f4_t *)(dst + 16 * ct) = o[q][ct] * f;
+            if (g == 0) a.ml[part + r] = float2{ref[q], l};
+        }
+    }
+}
+
+// W 0: a body of up to 16 rows, each wave every fourth key tile; else one of 64 W.
+template <int FMT, int DC, int W, typename T, class... ARGS>
+__device__ __forceinline__ void kva_any(ARGS &&...args) {
+    if constexpr (W == 0) kva_body<FMT, DC, 1, T>(args...);
+    else kva_wide_body<FMT, DC, W, T>(args...);
+}
+
 template <int FMT, int DC, int NQP, int NQS, typename T>
-__global__ void __launch_bounds__(64 * KVA_WAVES) kva_items(KvAttArgs a) {
+__global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAttArgs a) {
     extern __shared__ char smem[];
     const uint32_t Hk = a.own.Hk;
     const bool last = a.sp + a.ss == 1;
     if (blockIdx.x < a.n_pre) {
         // kv heads next to each other: with eight of them each stays on one XCD, whose L2 serves its row tiles
         const uint32_t hk = blockIdx.x % Hk, x = blockIdx.x / Hk, rt = x % a.rtp, split = x / a.rtp;
-        const uint32_t row0 = rt * 16 * NQP, n_rows = a.rows - row0 < 16 * NQP ? a.rows - row0 : 16 * NQP;
+        constexpr uint32_t R = NQP ? 64 * NQP : 16;
+        const uint32_t row0 = rt * R, n_rows = a.rows - row0 < R ? a.rows - row0 : R;
         const uint32_t tiles = (a.prefix_len + 63) / 64, run = (tiles + a.sp - 1) / a.sp;
         const uint32_t t0 = split * run < tiles ? split * run : tiles, t1 = t0 + run < tiles ? t0 + run : tiles;
         const size_t slab = a.pre.slab(a.prefix_seq, hk);
         const uint32_t len = a.prefix_len;
-        kva_body<FMT, DC, NQP, T>(a, smem, row0, n_rows, hk, a.pre.k + slab * a.pre.hd, a.pre.v + slab * a.pre.hd,
+        kva_any<FMT, DC, NQP, T>(a, smem, row0, n_rows, hk, a.pre.k + slab * a.pre.hd, a.pre.v + slab * a.pre.hd,
                                   a.pre.ks + slab, a.pre.vs + slab, t0, t1, len, [&](uint32_t) { return len; }, split,
                                   last);
         return;
@@ -423,7 +667,8 @@ __global__ void __launch_bounds__(64 * KVA_WAVES) kva_items(KvAttArgs a) {
     const uint32_t hk = item % Hk, x = item / Hk, rt = x % a.rts, y = x / a.rts, b = y % a.n, split = y / a.n;
     const uint32_t len = kva_len(a, b), tiles = (len + 63) / 64, run = kva_run(len, a.ss);
     if (split * run >= tiles && split > 0) return;  // split 0 is there for a sequence with no rows
-    const uint32_t per = a.sq * a.G, r0 = rt * 16 * NQS, n_rows = per - r0 < 16 * NQS ? per - r0 : 16 * NQS;
+    constexpr uint32_t R = NQS ? 64 * NQS : 16;
+    const uint32_t per = a.sq * a.G, r0 = rt * R, n_rows = per - r0 < R ? per - r0 : R;
     const uint32_t sq = a.sq, G = a.G;
     auto limit = [&](uint32_t r) {  // own rows seen by row r of the body: len - sq + t + 1, none where that is negative
         const uint32_t up = len + (r0 + r) / G + 1;
@@ -433,7 +678,7 @@ __global__ void __launch_bounds__(64 * KVA_WAVES) kva_items(KvAttArgs a) {
     uint32_t t1 = split * run + run;
     t1 = t1 < most ? t1 : most;
     const size_t slab = a.own.slab(a.first_seq + b, hk);
-    kva_body<FMT, DC, NQS, T>(a, smem, b * per + r0, n_rows, hk, a.own.k + slab * a.own.hd, a.own.v + slab * a.own.hd,
+    kva_any<FMT, DC, NQS, T>(a, smem, b * per + r0, n_rows, hk, a.own.k + slab * a.own.hd, a.own.v + slab * a.own.hd,
                               a.own.ks + slab, a.own.vs + slab, split * run, t1, len, limit, a.sp + split, last);
 }
 
@@ -463,18 +708,33 @@ __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
     float lf = lane < splits ? l * f : 0.0f;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) lf += __shfl_xor(lf, o, 64);
-    float v[4] = {0, 0, 0, 0};
-    for (uint32_t s = 0; s < splits; s++) {
-        const float fs = __shfl(f, (int)s, 64);
-        const float *src = a.po + (((size_t)s * Hk + hk) * a.rows + rho) * hd;
+    // four channels a lane, 64 / (hd / 4) splits at a time, the loads of four such steps in flight
+    const uint32_t lanes = hd <= 64 ? 16 : hd <= 128 ? 32 : 64, c = 4 * (lane % lanes), step = 64 / lanes;
+    kva_f4_t v = {0, 0, 0, 0};
+    const float *src = a.po + ((size_t)hk * a.rows + rho) * hd + (c < hd ? c : 0);
+    const size_t apart = (size_t)Hk * a.rows * hd;
+    for (uint32_t s0 = 0; s0 < splits; s0 += 4 * step) {
+        kva_f4_t x[4];
+        float fs[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (lane + 64 * k < hd) v[k] += fs * src[lane + 64 * k];
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint32_t s = s0 + k * step + lane / lanes, at = s < splits ? s : splits - 1;
+            x[k] = *(const kva_f4_t *)(src + at * apart);
+            fs[k] = __shfl(f, (int)at, 64);
+            if (s >= splits) x[k] = kva_f4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) v += x[k] * fs[k];
     }
-    T *dst = (T *)a.out + ((size_t)(rho / a.G) * a.H + (size_t)hk * a.G + rho % a.G) * hd;
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (lane + 64 * k < hd) dst[lane + 64 * k] = kva_out<T>(lf == 0.0f ? 0.0f : v[k] / lf);
+    for (int o = 32; o >= 16; o >>= 1)
+        if (lanes <= (uint32_t)o)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], o, 64);
+    if (lane >= lanes || c >= hd) return;
+    T *dst = (T *)a.out + ((size_t)(rho / a.G) * a.H + (size_t)hk * a.G + rho % a.G) * hd + c;
+#pragma unroll
+    for (int e = 0; e < 4; e++) dst[e] = kva_out<T>(lf == 0.0f ? 0.0f : v[e] / lf);
 }
 
 // How a call is cut: row tiles (16 NQ rows) and splits of the prefix and of
@@ -488,46 +748,60 @@ struct KvaPlan {
 static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq, size_t max_len, size_t prefix_len) {
     KvaPlan p{};
     const size_t Hk = s->n_kv_heads, G = n_heads / Hk, rows = n * sq * G, per = sq * G;
-    const uint32_t wide = s->head_dim > 128 ? 2 : 4;  // accumulators of four row tiles of 256 channels do not fit
-    p.nqs = per > 16 && max_len ? wide : 1;
-    p.nqp = rows > 16 || p.nqs > 1 ? wide : 1;
-    p.rtp = (uint32_t)div_ceil(rows, 16 * p.nqp);
-    p.rts = (uint32_t)div_ceil(per, 16 * p.nqs);
+    const uint32_t most = s->head_dim > 128 ? 1 : 2;
+    auto rows_of = [](uint32_t w) { return w ? 64 * w : 16; };
+    p.nqs = per > 16 && max_len ? most : 0;
+    p.nqp = p.nqs ? most : rows > 16 && prefix_len ? (rows > 64 ? most : 1) : 0;
+    p.rtp = (uint32_t)div_ceil(rows, rows_of(p.nqp));
+    p.rts = (uint32_t)div_ceil(per, rows_of(p.nqs));
     auto splits = [](size_t tiles, uint64_t others, uint64_t target) -> uint32_t {
         uint64_t most = div_ceil(tiles, KVA_WAVES), want = div_ceil(target, others ? others : 1);
         want = want < most ? want : most;
         return (uint32_t)(want < 1 ? 1 : want > KVA_MAX_SPLITS ? KVA_MAX_SPLITS : want);
     };
     if (prefix_len) p.sp = splits(div_ceil(prefix_len, 64), (uint64_t)Hk * p.rtp, 512);
-    if (max_len) p.ss = splits(div_ceil(max_len, 64), (uint64_t)n * Hk * p.rts, 4096);
+    if (max_len) p.ss = splits(div_ceil(max_len, 64), (uint64_t)n * Hk * p.rts, 1024);
     p.items = (uint64_t)Hk * p.rtp * p.sp + (uint64_t)n * Hk * p.rts * p.ss;
     p.bytes = p.sp + p.ss > 1 ? round_up((size_t)(p.sp + p.ss) * Hk * rows * (s->head_dim * 4 + 8), 256) : 0;
     return p;
 }
 
 template <int FMT, int DC, int NQP, int NQS, typename T>
-static int kva_launch(const KvAttArgs &a, uint64_t items, hipStream_t st) {
+static int kva_launch(const KvAttArgs &a, uint64_t items, int device, hipStream_t st) {
     constexpr bool HI = sizeof(T) == 4;
-    constexpr int A = KvaLds<DC, NQP, HI>::BYTES, B = KvaLds<DC, NQS, HI>::BYTES, lds = A > B ? A : B;
-    static_assert(lds <= 64 * 1024, "LDS past what a launch gets unasked");
-    hipLaunchKernelGGL((kva_items<FMT, DC, NQP, NQS, T>), dim3((unsigned)items), dim3(64 * KVA_WAVES), lds, st, a);
+    constexpr int N = KvaLds<DC, 1, HI>::BYTES, W = KvaWideLds<DC, NQP ? NQP : 1, HI>::BYTES;
+    constexpr int lds = NQP == 0 ? N : W > N ? W : N;
+    void (*k)(KvAttArgs) = kva_items<FMT, DC, NQP, NQS, T>;
+    if (lds > 64 * 1024) {  // once a device
+        static std::atomic<uint64_t> asked{0};
+        const uint64_t bit = device < 64 ? 1ull << device : 0;
+        if (!bit || !(asked.load(std::memory_order_acquire) & bit)) {
+            QBK_HIP(hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+            asked.fetch_or(bit, std::memory_order_release);
+        }
+    }
+    hipLaunchKernelGGL(k, dim3((unsigned)items), dim3(64 * KVA_WAVES), lds, st, a);
     QBK_HIP(hipGetLastError());
     return QBK_OK;
 }
 
+template <int FMT, int DC, typename T>
+static int kva_dispatch_dc(const KvAttArgs &a, const KvaPlan &p, int device, hipStream_t st) {
+    if constexpr (DC < 4) {
+        if (p.nqs == 2) return kva_launch<FMT, DC, 2, 2, T>(a, p.items, device, st);
+        if (p.nqp == 2) return kva_launch<FMT, DC, 2, 0, T>(a, p.items, device, st);
+    } else {
+        if (p.nqs == 1) return kva_launch<FMT, DC, 1, 1, T>(a, p.items, device, st);
+    }
+    if (p.nqp == 1) return kva_launch<FMT, DC, 1, 0, T>(a, p.items, device, st);
+    return kva_launch<FMT, DC, 0, 0, T>(a, p.items, device, st);
+}
+
 template <int FMT, typename T>
-static int kva_dispatch(const KvAttArgs &a, const KvaPlan &p, hipStream_t st) {
-    const int dc = a.own.hd > 128 ? 4 : a.own.hd > 64 ? 2 : 1;
-    if (dc == 4) {
-        if (p.nqs > 1) return kva_launch<FMT, 4, 2, 2, T>(a, p.items, st);
-        return p.nqp > 1 ? kva_launch<FMT, 4, 2, 1, T>(a, p.items, st) : kva_launch<FMT, 4, 1, 1, T>(a, p.items, st);
-    }
-    if (dc == 2) {
-        if (p.nqs > 1) return kva_launch<FMT, 2, 4, 4, T>(a, p.items, st);
-        return p.nqp > 1 ? kva_launch<FMT, 2, 4, 1, T>(a, p.items, st) : kva_launch<FMT, 2, 1, 1, T>(a, p.items, st);
-    }
-    if (p.nqs > 1) return kva_launch<FMT, 1, 4, 4, T>(a, p.items, st);
-    return p.nqp > 1 ? kva_launch<FMT, 1, 4, 1, T>(a, p.items, st) : kva_launch<FMT, 1, 1, 1, T>(a, p.items, st);
+static int kva_dispatch(const KvAttArgs &a, const KvaPlan &p, int device, hipStream_t st) {
+    if (a.own.hd > 128) return kva_dispatch_dc<FMT, 4, T>(a, p, device, st);
+    if (a.own.hd > 64) return kva_dispatch_dc<FMT, 2, T>(a, p, device, st);
+    return kva_dispatch_dc<FMT, 1, T>(a, p, device, st);
 }
 
 // The checks that need no buffers, in one place for the size and the call.
@@ -624,11 +898,11 @@ int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *ca
     hipStream_t st = (hipStream_t)stream;
     if (p.items) {
         if (shape->format == QBK_KV_INT8)
-            rc = dtype == QBK_F32 ? kva_dispatch<QBK_KV_INT8, float>(a, p, st)
-                                  : kva_dispatch<QBK_KV_INT8, uint16_t>(a, p, st);
+            rc = dtype == QBK_F32 ? kva_dispatch<QBK_KV_INT8, float>(a, p, ctx->device, st)
+                                  : kva_dispatch<QBK_KV_INT8, uint16_t>(a, p, ctx->device, st);
         else
-            rc = dtype == QBK_F32 ? kva_dispatch<QBK_KV_FP8, float>(a, p, st)
-                                  : kva_dispatch<QBK_KV_FP8, uint16_t>(a, p, st);
+            rc = dtype == QBK_F32 ? kva_dispatch<QBK_KV_FP8, float>(a, p, ctx->device, st)
+                                  : kva_dispatch<QBK_KV_FP8, uint16_t>(a, p, ctx->device, st);
         if (rc) return rc;
     }
     if (p.sp + p.ss == 1) return QBK_OK;  // the items wrote the output
