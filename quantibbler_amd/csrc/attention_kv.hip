@@ -124,31 +124,60 @@ struct KvaLds {
     static constexpr int BYTES = BODY + NQ * 16 * 4 * (1 + 2 * KVA_WAVES);
 };
 
+// Rows of a body from row0 on: row r is query (b, t) = base + r's quotient by
+// G, head the remainder.  The float quotient is exact: x + 1/2 is half a unit
+// from every multiple of G and below 2^21 (G at most 2^20, checked on the host).
+struct KvaRow {
+    uint32_t base, rem, G;
+    float inv;
+    __device__ __forceinline__ KvaRow(const KvAttArgs &a, uint32_t row0)
+        : base(row0 / a.G), rem(row0 % a.G), G(a.G), inv(1.0f / (float)a.G) {}
+    __device__ __forceinline__ void at(uint32_t r, uint32_t &query, uint32_t &head) const {
+        const uint32_t x = rem + r, d = (uint32_t)(((float)x + 0.5f) * inv);
+        query = base + d;
+        head = x - d * G;
+    }
+};
+
+// Four values of a row at any alignment (one load on this machine).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Kva4 {
+    T v[4];
+};
+
 // Queries row0 .. row0 + n_rows - 1 (at most 16 NT) of kv head hk into LDS as
 // the B operands of K q^T, [tile][step][lane][16 bytes], for f32 queries the
 // low halves behind them; cqs[r]: the factor that scores of row r still need.
+// 16 DC lanes a row, four channels a lane, every row's load before the first
+// is used (a row at a time, the 128 rows of the widest body took 25 us).
 template <int DC, int NT, typename T>
 __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float *cqs, uint32_t row0, uint32_t n_rows,
                                             uint32_t hk) {
-    constexpr int STEPS = 2 * DC;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = (int)a.own.hd;
-    // a wave a row, four channels a lane
-    for (int r = wave; r < 16 * NT; r += KVA_WAVES) {
-        float x[4] = {0, 0, 0, 0};
-        uint32_t top = 0;
-        const int c = 4 * lane;
-        if (r < (int)n_rows && c < hd) {
-            const uint32_t rho = row0 + r;
-            const T *src = (const T *)a.q + ((size_t)(rho / a.G) * a.H + (size_t)hk * a.G + rho % a.G) * hd + c;
+    constexpr int STEPS = 2 * DC, LANES = 16 * DC, AT_ONCE = KVA_WAVES * 64 / LANES, N = 16 * NT / AT_ONCE;
+    const int tid = threadIdx.x, hd = (int)a.own.hd, c = 4 * (tid % LANES), r0 = tid / LANES;
+    const KvaRow rows(a, row0);
+    Kva4<T> raw[N];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[e] = kva_in<T>(src[e]);
-                const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
-                top = b > top ? b : top;
-            }
+    for (int k = 0; k < N; k++) {
+        const uint32_t r = r0 + k * AT_ONCE;
+        uint32_t query, head;
+        rows.at(r < n_rows ? r : 0, query, head);
+        const T *src = (const T *)a.q + ((size_t)query * a.H + (size_t)hk * a.G + head) * hd;
+        raw[k] = *(const Kva4<T> *)(src + (c < hd ? c : 0));
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int r = r0 + k * AT_ONCE;
+        float x[4];
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[e] = r < (int)n_rows && c < hd ? kva_in<T>(raw[k].v[e]) : 0.0f;
+            const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
+            top = b > top ? b : top;
         }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
+        for (int o = LANES / 2; o >= 1; o >>= 1) {
             const uint32_t b = (uint32_t)__shfl_xor((int)top, o, 64);
             top = b > top ? b : top;
         }
@@ -157,24 +186,22 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
         uint32_t ex = top >> 23;
         ex = ex < 30 ? 30 : ex > 254 ? 254 : ex;
         const float f = __uint_as_float((257 - ex) << 23);
-        if (c < 64 * DC) {
-            kva_h2_t hi[2], lo[2];
+        kva_h2_t hi[2], lo[2];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float y = whole ? x[e] * f : 0.0f;
-                const _Float16 h = (_Float16)y;
-                hi[e >> 1][e & 1] = h;
-                lo[e >> 1][e & 1] = (_Float16)(y - (float)h);
-            }
-            // channel c: chunk c / 16 -> step 2 (chunk / 4) + (c % 16) / 8, operand lane (chunk % 4, column r % 16)
-            const int chunk = c >> 4, step = 2 * (chunk >> 2) + ((c >> 3) & 1);
-            const size_t at = (size_t)(((r >> 4) * STEPS + step) * 64 + (chunk & 3) * 16 + (r & 15)) * 16 + (c & 7) * 2;
-            *(uint2 *)(qs + at) = uint2{__builtin_bit_cast(uint32_t, hi[0]), __builtin_bit_cast(uint32_t, hi[1])};
-            if constexpr (sizeof(T) == 4)
-                *(uint2 *)(qs + NT * STEPS * 1024 + at) =
-                    uint2{__builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1])};
+        for (int e = 0; e < 4; e++) {
+            const float y = whole ? x[e] * f : 0.0f;
+            const _Float16 h = (_Float16)y;
+            hi[e >> 1][e & 1] = h;
+            lo[e >> 1][e & 1] = (_Float16)(y - (float)h);
         }
-        if (lane == 0) cqs[r] = whole ? a.scale * __uint_as_float((ex - 3) << 23) : __builtin_nanf("");
+        // channel c: chunk c / 16 -> step 2 (chunk / 4) + (c % 16) / 8, operand lane (chunk % 4, column r % 16)
+        const int chunk = c >> 4, step = 2 * (chunk >> 2) + ((c >> 3) & 1);
+        const size_t at = (size_t)(((r >> 4) * STEPS + step) * 64 + (chunk & 3) * 16 + (r & 15)) * 16 + (c & 7) * 2;
+        *(uint2 *)(qs + at) = uint2{__builtin_bit_cast(uint32_t, hi[0]), __builtin_bit_cast(uint32_t, hi[1])};
+        if constexpr (sizeof(T) == 4)
+            *(uint2 *)(qs + NT * STEPS * 1024 + at) =
+                uint2{__builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1])};
+        if (c == 0) cqs[r] = whole ? a.scale * __uint_as_float((ex - 3) << 23) : __builtin_nanf("");
     }
 }
 
@@ -669,9 +696,12 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
     if (split * run >= tiles && split > 0) return;  // split 0 is there for a sequence with no rows
     constexpr uint32_t R = NQS ? 64 * NQS : 16;
     const uint32_t per = a.sq * a.G, r0 = rt * R, n_rows = per - r0 < R ? per - r0 : R;
-    const uint32_t sq = a.sq, G = a.G;
+    const uint32_t sq = a.sq;
+    const KvaRow rows(a, r0);
     auto limit = [&](uint32_t r) {  // own rows seen by row r of the body: len - sq + t + 1, none where that is negative
-        const uint32_t up = len + (r0 + r) / G + 1;
+        uint32_t t, head;
+        rows.at(r, t, head);
+        const uint32_t up = len + t + 1;
         return up > sq ? up - sq : 0;
     };
     const uint32_t most = (limit(n_rows - 1) + 63) / 64;
@@ -812,6 +842,7 @@ static int kva_check(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq,
     if (n_heads == 0 || n_heads % s->n_kv_heads != 0)
         return fail(QBK_ERR_VALIDATION, fmt("n_kv_heads must divide n_heads: n_heads=%zu, n_kv_heads=%zu", n_heads,
                                             s->n_kv_heads));
+    if (n_heads > (1u << 20)) return fail(QBK_ERR_VALIDATION, "kv attention takes up to 2^20 heads");
     if (sq == 0) return fail(QBK_ERR_VALIDATION, "kv attention requires at least one query a sequence");
     if (max_len > s->capacity)
         return fail(QBK_ERR_VALIDATION, fmt("max_len %zu is past the kv cache's capacity of %zu", max_len, s->capacity));
