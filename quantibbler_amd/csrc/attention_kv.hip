@@ -2,12 +2,13 @@
 // prefix that every sequence shares.
 //
 // Rows: query row rho = (b sq + t) G + hg of kv head hk is sequence b's query
-// t, head hk G + hg.  Every row sees the prefix, so the prefix's items take 16
-// NQP rows of all sequences together and read its codes once; a sequence's own
-// rows are seen by its sq G rows alone.  Both kinds are items of one launch:
-//   item = (kv head, tile of 16 NQ rows, run of 64-row key tiles)
+// t, head hk G + hg.  Every row sees the prefix, so the prefix's items take
+// rows of all sequences together and read its codes once for them; a
+// sequence's own rows are seen by its sq G rows alone.  Both kinds are items of
+// one launch:
+//   item = (kv head, 16 or 64 rows, run of 64-row key tiles)
 // and leave a partial result (sum of weights, weighted values, reference) per
-// row; a second launch joins them.  A wave takes every fourth key tile:
+// row; a second launch joins them.  A key tile and 16 rows, a wave:
 //   S^T = K q^T      v_mfma_f32_16x16x32_f16, codes widened to fp16 (exact)
 //   p = exp2(s - M)  online, per query column; M is a whole number, so moving
 //                    to another M and joining partials scale by powers of two
@@ -31,11 +32,29 @@ namespace qbk {
 
 typedef _Float16 kva_h8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 kva_h2_t __attribute__((ext_vector_type(2)));
+typedef float kva_f2_t __attribute__((ext_vector_type(2)));
 typedef float kva_f4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t kva_u4_t __attribute__((ext_vector_type(4)));
 
 #define KVA_WAVES 4
 #define KVA_MAX_SPLITS 32  // of the prefix, and of a sequence's own rows
+
+// x / d and x % d for x below 2^31 by a multiplication (a division costs some
+// 25 dependent instructions, and an item begins with five).
+struct KvaDiv {
+    uint32_t d, mul, shift;
+    void set(uint32_t by) {
+        d = by;
+        shift = 0;
+        while ((1ull << shift) < by) shift++;
+        mul = (uint32_t)((((1ull << shift) - by) << 32) / by + 1);
+    }
+    __device__ __forceinline__ uint32_t split(uint32_t x, uint32_t &rest) const {
+        const uint32_t q = (__umulhi(x, mul) + x) >> shift;
+        rest = x - q * d;
+        return q;
+    }
+};
 
 struct KvAttArgs {
     KvView own, pre;
@@ -48,6 +67,7 @@ struct KvAttArgs {
     uint32_t n, sq, H, G, rows;      // rows = n sq G
     uint32_t sp, ss, rtp, rts;       // splits and row tiles of prefix and own items
     uint32_t n_pre;                  // prefix items
+    KvaDiv by_hk, by_rtp, by_rts, by_n, by_g, by_sp, by_ss, by_sq, by_rows;
     float scale;                     // log2(e) / sqrt(hd)
 };
 
@@ -57,8 +77,9 @@ __device__ __forceinline__ uint32_t kva_len(const KvAttArgs &a, uint32_t b) {
     const uint32_t l = a.lens[b];
     return l < a.max_len ? l : a.max_len;
 }
-__device__ __forceinline__ uint32_t kva_run(uint32_t len, uint32_t splits) {
-    const uint32_t t = (len + 63) / 64, c = (t + splits - 1) / splits;
+__device__ __forceinline__ uint32_t kva_run(const KvAttArgs &a, uint32_t len) {
+    uint32_t rest;
+    const uint32_t c = a.by_ss.split((len + 63) / 64 + a.ss - 1, rest);
     return c > KVA_WAVES ? c : KVA_WAVES;
 }
 
@@ -95,6 +116,10 @@ __device__ __forceinline__ float kva_sum4(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// A value that every lane holds, as a scalar.
+__device__ __forceinline__ uint32_t kva_scalar(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ float kva_scalar(float v) { return __uint_as_float(kva_scalar(__float_as_uint(v))); }
+
 // exp2 of a difference of references: a power of two, 1 where both are equal
 // (two empty ones included).
 __device__ __forceinline__ float kva_rescale(float from, float to) {
@@ -112,32 +137,53 @@ __device__ __forceinline__ T kva_out(float x) {
     else return f32_to_bf16(x);
 }
 
-// LDS of a body: queries as operands, then (over them) the waves' outputs, and
-// the rows' scale, references and sums.
-template <int DC, int NQ, bool HI>
+// LDS of a body of up to 16 rows: queries as operands, then (over them) the
+// waves' outputs; the rows' factors, references and sums.
+template <int DC, bool HI>
 struct KvaLds {
-    static constexpr int STEPS = 2 * DC;
-    static constexpr int Q = NQ * STEPS * 1024 * (HI ? 2 : 1);
-    static constexpr int OC = DC < 2 ? 64 : 128;                  // channels joined at a time
+    static constexpr int Q = 2 * DC * 1024 * (HI ? 2 : 1);
+    static constexpr int OC = DC < 2 ? 64 : 128;  // channels joined at a time
     static constexpr int O = KVA_WAVES * 16 * (OC + 4) * 4;
     static constexpr int BODY = Q > O ? Q : O;
-    static constexpr int BYTES = BODY + NQ * 16 * 4 * (1 + 2 * KVA_WAVES);
+    static constexpr int BYTES = BODY + 16 * 4 * (1 + 2 * KVA_WAVES);
 };
 
 // Rows of a body from row0 on: row r is query (b, t) = base + r's quotient by
 // G, head the remainder.  The float quotient is exact: x + 1/2 is half a unit
-// from every multiple of G and below 2^21 (G at most 2^20, checked on the host).
+// from every multiple of G and below 2^14 (G at most 2^13, checked on the
+// host), rounding and reciprocal are within 2^-22 together.
 struct KvaRow {
     uint32_t base, rem, G;
     float inv;
     __device__ __forceinline__ KvaRow(const KvAttArgs &a, uint32_t row0)
-        : base(row0 / a.G), rem(row0 % a.G), G(a.G), inv(1.0f / (float)a.G) {}
+        : G(a.G), inv(__builtin_amdgcn_rcpf((float)a.G)) {
+        base = a.by_g.split(row0, rem);
+    }
     __device__ __forceinline__ void at(uint32_t r, uint32_t &query, uint32_t &head) const {
         const uint32_t x = rem + r, d = (uint32_t)(((float)x + 0.5f) * inv);
         query = base + d;
         head = x - d * G;
     }
 };
+
+// The largest over aligned runs of LANES (16, 32 or 64) lanes.
+template <int LANES>
+__device__ __forceinline__ uint32_t kva_row_max(uint32_t v) {
+    auto up = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));  // row_ror 8, 4, 2, 1
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
+    if constexpr (LANES >= 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = up(a[0], a[1]);
+    }
+    if constexpr (LANES >= 64) {
+        const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = up(b[0], b[1]);
+    }
+    return v;
+}
 
 // Four values of a row at any alignment (one load on this machine).
 template <typename T>
@@ -149,101 +195,95 @@ struct __attribute__((packed, aligned(sizeof(T)))) Kva4 {
 // the B operands of K q^T, [tile][step][lane][16 bytes], for f32 queries the
 // low halves behind them; cqs[r]: the factor that scores of row r still need.
 // 16 DC lanes a row, four channels a lane, every row's load before the first
-// is used (a row at a time, the 128 rows of the widest body took 25 us).
+// is used (a row at a time, 128 rows took 25 us).
 template <int DC, int NT, typename T>
 __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float *cqs, uint32_t row0, uint32_t n_rows,
                                             uint32_t hk) {
     constexpr int STEPS = 2 * DC, LANES = 16 * DC, AT_ONCE = KVA_WAVES * 64 / LANES, N = 16 * NT / AT_ONCE;
     const int tid = threadIdx.x, hd = (int)a.own.hd, c = 4 * (tid % LANES), r0 = tid / LANES;
     const KvaRow rows(a, row0);
+    // from the first row's query on; rows of a body span less than 2^32 bytes (kva_check)
+    const T *q0 = (const T *)a.q + ((size_t)rows.base * a.H + (size_t)hk * a.G) * hd;
     Kva4<T> raw[N];
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const uint32_t r = r0 + k * AT_ONCE;
         uint32_t query, head;
         rows.at(r < n_rows ? r : 0, query, head);
-        const T *src = (const T *)a.q + ((size_t)query * a.H + (size_t)hk * a.G + head) * hd;
-        raw[k] = *(const Kva4<T> *)(src + (c < hd ? c : 0));
+        raw[k] = *(const Kva4<T> *)(q0 + (((query - rows.base) * a.H + head) * hd + (c < hd ? c : 0)));
     }
+    uint32_t top[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const bool in = r0 + k * AT_ONCE < (int)n_rows && c < hd;
+        top[k] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            raw[k].v[e] = in ? raw[k].v[e] : (T)0;
+            const uint32_t b = __float_as_uint(kva_in<T>(raw[k].v[e])) & 0x7fffffffu;
+            top[k] = b > top[k] ? b : top[k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) top[k] = kva_row_max<LANES>(top[k]);
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const int r = r0 + k * AT_ONCE;
-        float x[4];
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[e] = r < (int)n_rows && c < hd ? kva_in<T>(raw[k].v[e]) : 0.0f;
-            const uint32_t b = __float_as_uint(x[e]) & 0x7fffffffu;
-            top = b > top ? b : top;
-        }
-#pragma unroll
-        for (int o = LANES / 2; o >= 1; o >>= 1) {
-            const uint32_t b = (uint32_t)__shfl_xor((int)top, o, 64);
-            top = b > top ? b : top;
-        }
         // the largest channel to [8, 16): both halves of every channel within fp16
-        const bool whole = top < 0x7f800000u;
-        uint32_t ex = top >> 23;
-        ex = ex < 30 ? 30 : ex > 254 ? 254 : ex;
-        const float f = __uint_as_float((257 - ex) << 23);
+        const bool whole = top[k] < 0x7f800000u;
+        uint32_t ex = top[k] >> 23;
+        ex = ex < 30 ? 30 : ex;
+        const float f = __uint_as_float((257 - ex) << 23);  // NaN rows: the scores become NaN by cqs
         kva_h2_t hi[2], lo[2];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float y = whole ? x[e] * f : 0.0f;
-            const _Float16 h = (_Float16)y;
-            hi[e >> 1][e & 1] = h;
-            lo[e >> 1][e & 1] = (_Float16)(y - (float)h);
+        for (int e = 0; e < 4; e += 2) {
+            const kva_f2_t y = {kva_in<T>(raw[k].v[e]) * f, kva_in<T>(raw[k].v[e + 1]) * f};
+            hi[e >> 1] = __builtin_convertvector(y, kva_h2_t);
+            if constexpr (sizeof(T) == 4)
+                lo[e >> 1] = __builtin_convertvector(y - __builtin_convertvector(hi[e >> 1], kva_f2_t), kva_h2_t);
         }
         // channel c: chunk c / 16 -> step 2 (chunk / 4) + (c % 16) / 8, operand lane (chunk % 4, column r % 16)
         const int chunk = c >> 4, step = 2 * (chunk >> 2) + ((c >> 3) & 1);
-        const size_t at = (size_t)(((r >> 4) * STEPS + step) * 64 + (chunk & 3) * 16 + (r & 15)) * 16 + (c & 7) * 2;
+        const int at = (((r >> 4) * STEPS + step) * 64 + (chunk & 3) * 16 + (r & 15)) * 16 + (c & 7) * 2;
         *(uint2 *)(qs + at) = uint2{__builtin_bit_cast(uint32_t, hi[0]), __builtin_bit_cast(uint32_t, hi[1])};
         if constexpr (sizeof(T) == 4)
             *(uint2 *)(qs + NT * STEPS * 1024 + at) =
                 uint2{__builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1])};
-        if (c == 0) cqs[r] = whole ? a.scale * __uint_as_float((ex - 3) << 23) : __builtin_nanf("");
+        top[k] = whole ? __float_as_uint(a.scale * __uint_as_float((ex - 3) << 23)) : 0x7fc00000u;
     }
+    if (c == 0)
+#pragma unroll
+        for (int k = 0; k < N; k++) cqs[r0 + k * AT_ONCE] = __uint_as_float(top[k]);
 }
 
-// Value scales to 2^12 over a power of two at or above every one so far
-// (vref; the outputs follow when it moves).
-template <int NQ, int CT>
-__device__ __forceinline__ void kva_value_scales(kva_f4_t (&vs)[4], float &vref, float &vinv, kva_f4_t (&o)[NQ][CT]) {
-    float vm = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) vm = fmaxf(fmaxf(fmaxf(vm, vs[i][0]), fmaxf(vs[i][1], vs[i][2])), vs[i][3]);
-    if (__ballot(vm > vref)) {
-        vm = kva_max4(vm);
+// The largest value scale vm of a tile against vref, a power of two at or above
+// every one so far: the outputs follow when it moves, vinv = 2^12 / vref.
+template <int CT>
+__device__ __forceinline__ void kva_value_scales(float vm, float &vref, float &vinv, kva_f4_t (&o)[CT]) {
+    if (vm > vref) {  // the same in every lane
         const uint32_t e = (__float_as_uint(vm) >> 23) + 1;  // scales are 2^-107 .. 2^122
         const float to = __uint_as_float(e << 23);
         vinv = __uint_as_float((266 - e) << 23);
         const float f = vref * __uint_as_float((254 - e) << 23);
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++) o[q][ct] *= f;
+        for (int ct = 0; ct < CT; ct++) o[ct] *= f;
         vref = to;
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) vs[i] *= vinv;
 }
 
 // One query tile's scores (16 keys a lane: 16 i + j past key) to weights: the
 // reference moves when a score passes it eightfold, sum and outputs with it;
 // p times the value scales as operands ph (and pl, the halves' rests).
-template <int CT, bool HI>
-__device__ __forceinline__ void kva_softmax(const kva_f4_t (&s)[4], const kva_f4_t (&vs)[4], float cq, bool masked,
-                                            uint32_t key, uint32_t lim, float &ref, float &sum, kva_f4_t (&o)[CT],
+template <bool MASKED, int CT, bool HI>
+__device__ __forceinline__ void kva_softmax(const kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float cq, uint32_t key,
+                                            uint32_t lim, float &ref, float &sum, kva_f4_t (&o)[CT],
                                             kva_h8_t (&ph)[2], kva_h8_t (&pl)[2]) {
-    float t[4][4], tm = -INFINITY;
+    auto out = [&](int i, int j) { return MASKED && key + 16 * i + j >= lim; };
+    float tm = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            t[i][j] = s[i][j];
-            if (masked && key + 16 * i + j >= lim) t[i][j] = -INFINITY;
-            tm = fmaxf(tm, t[i][j]);
-        }
+        for (int j = 0; j < 4; j++) tm = fmaxf(tm, out(i, j) ? -INFINITY : t[i][j]);
     if (__ballot(tm * cq > ref + 3.0f)) {
         const float to = fmaxf(ref, ceilf(kva_max4(tm) * cq));
         const float f = kva_rescale(ref, to);
@@ -252,57 +292,95 @@ __device__ __forceinline__ void kva_softmax(const kva_f4_t (&s)[4], const kva_f4
         for (int ct = 0; ct < CT; ct++) o[ct] *= f;
         ref = to;
     }
+    float l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float w[4];
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bool out = masked && key + 16 * i + j >= lim;
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j], cq, -ref));
-            if (out) p = 0.0f;
-            sum += p;
-            w[j] = p * vs[i][j];
-            if (out) w[j] = 0.0f;  // whatever the scale holds
+        for (int j = 0; j < 4; j += 2) {
+            kva_f2_t w;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j + e], cq, -ref));
+                l += out(i, j + e) ? 0.0f : p;
+                w[e] = out(i, j + e) ? 0.0f : p * vs[i][j + e];  // whatever the scale holds
+            }
+            const kva_h2_t h = __builtin_convertvector(w, kva_h2_t);
+            ph[i >> 1][4 * (i & 1) + j] = h[0];
+            ph[i >> 1][4 * (i & 1) + j + 1] = h[1];
+            if constexpr (HI) {
+                const kva_h2_t r = __builtin_convertvector(w - __builtin_convertvector(h, kva_f2_t), kva_h2_t);
+                pl[i >> 1][4 * (i & 1) + j] = r[0];
+                pl[i >> 1][4 * (i & 1) + j + 1] = r[1];
+            }
         }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const _Float16 h = (_Float16)w[j];
-            ph[i >> 1][4 * (i & 1) + j] = h;
-            if constexpr (HI) pl[i >> 1][4 * (i & 1) + j] = (_Float16)(w[j] - (float)h);
-        }
-    }
+    sum += l;
 }
 
-// Rows row0 .. row0 + n_rows - 1 (at most 16 NQ) of kv head hk over key tiles
-// tile0 .. tile1 - 1 of the slab k, v, ks, vs.  Row r of the body sees keys
-// below limit(r), none of them at or past `written`.
-template <int FMT, int DC, int NQ, typename T, class Limit>
+// A wave's running state for its 16 rows: reference, sum of weights and
+// weighted values (O^T, channel 16 ct + 4 g + j of row col) over vref's 2^12.
+template <int DC>
+struct KvaState {
+    kva_f4_t o[4 * DC];
+    float ref, sum, cq, vref, vinv;
+    uint32_t lim;
+    __device__ __forceinline__ KvaState(float cq, uint32_t lim)
+        : ref(-INFINITY), sum(0.0f), cq(cq), vref(0.0f), vinv(0.0f), lim(lim) {
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++) o[ct] = kva_f4_t{0, 0, 0, 0};
+    }
+};
+
+// Codes of rows at or past `written` as zero: 32 bits a 16-row block for the
+// lane's four rows 4 g .. of it.
+__device__ __forceinline__ kva_u4_t kva_keep(uint32_t key0, uint32_t written, int g) {
+    kva_u4_t keep;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t k0 = key0 + 16 * i + 4 * g, left = written > k0 ? written - k0 : 0;
+        keep[i] = left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
+    }
+    return keep;
+}
+
+// Where row rho's output goes.
+template <typename T>
+__device__ __forceinline__ T *kva_out_row(const KvAttArgs &a, uint32_t rho, uint32_t hk) {
+    uint32_t head;
+    const uint32_t query = a.by_g.split(rho, head);
+    return (T *)a.out + ((size_t)query * a.H + (size_t)hk * a.G + head) * a.own.hd;
+}
+
+// Up to 16 rows, row0 .. row0 + n_rows - 1 of kv head hk, over key tiles tile0
+// .. tile1 - 1 of the slab k, v, ks, vs: a wave every fourth tile, in registers
+// alone (few rows are bound by the cache's bytes; 32 sequences of up to 2085
+// rows, 32/8 heads of 128: 107 MB in 23.6 us, 4.5 TB/s).  Row r of the body sees
+// keys below limit(r), none of them at or past `written`.
+template <int FMT, int DC, typename T, class Limit>
 __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows, uint32_t hk,
                                          const uint8_t *kcode, const uint8_t *vcode, const float *ksc,
                                          const float *vsc, uint32_t tile0, uint32_t tile1, uint32_t written,
                                          Limit limit, uint32_t split, bool last) {
     constexpr bool HI = sizeof(T) == 4;
-    using L = KvaLds<DC, NQ, HI>;
-    constexpr int STEPS = L::STEPS;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    using L = KvaLds<DC, HI>;
+    constexpr int STEPS = 2 * DC;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: loops and addresses by it are too
     const int hd = (int)a.own.hd, nc = hd / 16;
     char *qs = smem;
-    float *cqs = (float *)(smem + L::BODY), *refs = cqs + NQ * 16, *sums = refs + KVA_WAVES * NQ * 16;
+    float *cqs = (float *)(smem + L::BODY), *refs = cqs + 16, *sums = refs + KVA_WAVES * 16;
 
     // A tile's codes and scales travel while the one before is worked on: keys
     // and their scales are asked for again as soon as the scores are formed,
     // values once they are added, the first of both before the queries are read.
     kva_u4_t kc[DC][4], vc[4 * DC];
     kva_f4_t ks[4], vs[4];
-    const int spread = col * 16;
     auto load_k = [&](uint32_t tt) {
-        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + spread;
+        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + col * 16;
         const float *st = ksc + (size_t)tt * 64 + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; i++) ks[i] = *(const kva_f4_t *)(st + 16 * i);
 #pragma unroll
         for (int c = 0; c < DC; c++) {
-            if (4 * c >= nc) continue;
             const int chunk = 4 * c + g < nc ? 4 * c + g : nc - 1;  // past the last chunk q is zero
 #pragma unroll
             for (int i = 0; i < 4; i++) kc[c][i] = *(const kva_u4_t *)(kt + (i * nc + chunk) * 256);
@@ -315,33 +393,17 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
         for (int i = 0; i < 4; i++) vs[i] = *(const kva_f4_t *)(st + 16 * i);
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++)
-            if (ct < nc) vc[ct] = *(const kva_u4_t *)(vt + ct * 1024);
+            vc[ct] = *(const kva_u4_t *)(vt + (ct < nc ? ct : nc - 1) * 1024);  // past the last tile: not stored
     };
     const uint32_t first = tile0 + wave;
     if (first < tile1) {
         load_k(first);
         load_v(first);
     }
-
-    kva_queries<DC, NQ, T>(a, qs, cqs, row0, n_rows, hk);
+    kva_queries<DC, 1, T>(a, qs, cqs, row0, n_rows, hk);
     __syncthreads();
-
-    kva_f4_t o[NQ][4 * DC];
-    float ref[NQ], sum[NQ], cq[NQ];
-    uint32_t lim[NQ];
-    uint32_t least = 0xFFFFFFFFu;  // keys below it are seen by every row
-#pragma unroll
-    for (int q = 0; q < NQ; q++) {
-#pragma unroll
-        for (int ct = 0; ct < 4 * DC; ct++) o[q][ct] = kva_f4_t{0, 0, 0, 0};
-        ref[q] = -INFINITY;
-        sum[q] = 0.0f;
-        cq[q] = cqs[16 * q + col];
-        const uint32_t r = 16 * q + col;
-        lim[q] = limit(r < n_rows ? r : n_rows - 1);
-    }
-    least = limit(0);
-    float vref = 0.0f, vinv = 0.0f;  // a power of two at or above every value scale so far, and 2^12 over it
+    KvaState<DC> st(cqs[col], limit((uint32_t)col < n_rows ? col : n_rows - 1));
+    const uint32_t least = kva_scalar(limit(0));  // keys below it are seen by every row
 
     for (uint32_t tt = first; tt < tile1; tt += KVA_WAVES) {
         const uint32_t key0 = tt * 64;
@@ -353,348 +415,296 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
                 for (int j = 0; j < 4; j++)
                     if (key0 + 16 * i + 4 * g + j >= written) vs[i][j] = 0.0f;
         }
-        kva_f4_t s[NQ][4];
+        asm volatile("" ::: "memory");  // the queries are read from LDS again, not kept in registers that spill
+        kva_f4_t s[4];
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
+        for (int i = 0; i < 4; i++) s[i] = kva_f4_t{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[q][i] = kva_f4_t{0, 0, 0, 0};
+        for (int x = 0; x < STEPS; x++) {
+            const kva_h8_t qf = *(const kva_h8_t *)(qs + (x * 64 + lane) * 16);
+            kva_h8_t kf[4];
 #pragma unroll
-        for (int c = 0; c < DC; c++) {
-            if (4 * c >= nc) continue;
+            for (int i = 0; i < 4; i++) {
+                kf[i] = kva_wide<FMT>(kc[x / 2][i][2 * (x & 1)], kc[x / 2][i][2 * (x & 1) + 1]);
+                s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qf, s[i], 0, 0, 0);
+            }
+            if constexpr (HI) {
+                const kva_h8_t ql = *(const kva_h8_t *)(qs + STEPS * 1024 + (x * 64 + lane) * 16);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                kva_h8_t kf[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) kf[i] = kva_wide<FMT>(kc[c][i][2 * u], kc[c][i][2 * u + 1]);
-#pragma unroll
-                for (int q = 0; q < NQ; q++) {
-                    const kva_h8_t qf = *(const kva_h8_t *)(qs + (size_t)((q * STEPS + 2 * c + u) * 64 + lane) * 16);
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        s[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qf, s[q][i], 0, 0, 0);
-                    if constexpr (HI) {
-                        const kva_h8_t ql = *(const kva_h8_t *)(qs + NQ * STEPS * 1024 +
-                                                                (size_t)((q * STEPS + 2 * c + u) * 64 + lane) * 16);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            s[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], ql, s[q][i], 0, 0, 0);
-                    }
-                }
+                for (int i = 0; i < 4; i++) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], ql, s[i], 0, 0, 0);
             }
         }
         // scores in units of 1 / cq; the key registers are free again
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[q][i] *= ks[i];
+        for (int i = 0; i < 4; i++) s[i] *= ks[i];
         if (more) load_k(tt + KVA_WAVES);
-        kva_value_scales<NQ, 4 * DC>(vs, vref, vinv, o);
-
-        kva_h8_t ph[NQ][2], pl[NQ][2];
+        float vm = 0.0f;
 #pragma unroll
-        for (int q = 0; q < NQ; q++) {
-            kva_softmax<4 * DC, HI>(s[q], vs, cq[q], masked, key0 + 4 * g, lim[q], ref[q], sum[q], o[q], ph[q], pl[q]);
-        }
+        for (int i = 0; i < 4; i++) vm = fmaxf(fmaxf(fmaxf(vm, vs[i][0]), fmaxf(vs[i][1], vs[i][2])), vs[i][3]);
+        if (__ballot(vm > st.vref)) kva_value_scales(kva_scalar(kva_max4(vm)), st.vref, st.vinv, st.o);
+#pragma unroll
+        for (int i = 0; i < 4; i++) vs[i] *= st.vinv;
+        kva_h8_t ph[2], pl[2];
+        if (masked)
+            kva_softmax<true, 4 * DC, HI>(s, vs, st.cq, key0 + 4 * g, st.lim, st.ref, st.sum, st.o, ph, pl);
+        else
+            kva_softmax<false, 4 * DC, HI>(s, vs, st.cq, 0, 0, st.ref, st.sum, st.o, ph, pl);
         // fp8 rows that were never written may hold NaN codes
-        uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-        if (FMT == QBK_KV_FP8 && masked) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t k0 = key0 + 16 * i + 4 * g, left = written > k0 ? written - k0 : 0;
-                keep[i] = left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
-            }
-        }
+        kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
+        if (FMT == QBK_KV_FP8 && masked) keep = kva_keep(key0, written, g);
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++) {
-            if (ct >= nc) continue;
-            kva_u4_t w = vc[ct];
-            if (FMT == QBK_KV_FP8) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] &= keep[i];
-            }
+            const kva_u4_t w = FMT == QBK_KV_FP8 ? vc[ct] & keep : vc[ct];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const kva_h8_t vf = kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
-#pragma unroll
-                for (int q = 0; q < NQ; q++) {
-                    o[q][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[q][u], o[q][ct], 0, 0, 0);
-                    if constexpr (HI)
-                        o[q][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[q][u], o[q][ct], 0, 0, 0);
-                }
+                st.o[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[u], st.o[ct], 0, 0, 0);
+                if constexpr (HI) st.o[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[u], st.o[ct], 0, 0, 0);
             }
         }
         if (more) load_v(tt + KVA_WAVES);
     }
 
     // join the waves on each row's largest reference
-#pragma unroll
-    for (int q = 0; q < NQ; q++) {
-        const float l = kva_sum4(sum[q]);
-        if (g == 0) {
-            refs[(wave * NQ + q) * 16 + col] = ref[q];
-            sums[(wave * NQ + q) * 16 + col] = l;
-        }
+    const float l = kva_sum4(st.sum);
+    if (g == 0) {
+        refs[wave * 16 + col] = st.ref;
+        sums[wave * 16 + col] = l;
     }
     __syncthreads();
-    auto largest = [&](int r) {  // row r of the body
+    auto largest = [&](int r) {
         float m = refs[r];
 #pragma unroll
-        for (int w = 1; w < KVA_WAVES; w++) m = fmaxf(m, refs[w * NQ * 16 + r]);
+        for (int w = 1; w < KVA_WAVES; w++) m = fmaxf(m, refs[w * 16 + r]);
         return m;
+    };
+    auto total = [&](int r, float m) {
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KVA_WAVES; w++) l += sums[w * 16 + r] * kva_rescale(refs[w * 16 + r], m);
+        return l;
     };
     constexpr int OC = L::OC, LD = OC + 4;
     float *ob = (float *)smem;  // [wave][16 rows][LD]
     const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0;
+    const float f = kva_rescale(st.ref, largest(col)) * st.vref * 0x1p-12f;
 #pragma unroll
-    for (int q = 0; q < NQ; q++) {
-        const float f = kva_rescale(ref[q], largest(16 * q + col)) * vref * 0x1p-12f;
+    for (int c0 = 0; c0 < 64 * DC; c0 += OC) {
+        if (c0 >= hd) continue;
+        if (c0) __syncthreads();  // what the region held has been read
 #pragma unroll
-        for (int c0 = 0; c0 < 64 * DC; c0 += OC) {
-            if (c0 >= hd) continue;
-            __syncthreads();  // what the region held has been read
+        for (int k = 0; k < OC / 16; k++)
+            *(kva_f4_t *)(ob + (wave * 16 + col) * LD + 16 * k + 4 * g) = st.o[c0 / 16 + k] * f;
+        __syncthreads();
+        for (int x = tid; x < 16 * OC; x += 64 * KVA_WAVES) {
+            const int r = x / OC, c = x % OC;
+            if (r >= (int)n_rows || c0 + c >= hd) continue;
+            float v = 0.0f;
 #pragma unroll
-            for (int k = 0; k < OC / 16; k++)
-                *(kva_f4_t *)(ob + (wave * 16 + col) * LD + 16 * k + 4 * g) = o[q][c0 / 16 + k] * f;
-            __syncthreads();
-            for (int x = tid; x < 16 * OC; x += 64 * KVA_WAVES) {
-                const int r = x / OC, c = x % OC;
-                if (16 * q + r >= (int)n_rows || c0 + c >= hd) continue;
-                float v = 0.0f;
-#pragma unroll
-                for (int w = 0; w < KVA_WAVES; w++) v += ob[(w * 16 + r) * LD + c];
-                if (last) {
-                    float l = 0.0f;
-                    const float m = largest(16 * q + r);
-#pragma unroll
-                    for (int w = 0; w < KVA_WAVES; w++)
-                        l += sums[(w * NQ + q) * 16 + r] * kva_rescale(refs[(w * NQ + q) * 16 + r], m);
-                    const uint32_t rho = row0 + 16 * q + r;
-                    T *dst = (T *)a.out + ((size_t)(rho / a.G) * a.H + (size_t)hk * a.G + rho % a.G) * hd;
-                    dst[c0 + c] = kva_out<T>(l == 0.0f ? 0.0f : v / l);
-                } else {
-                    a.po[(part + 16 * q + r) * hd + c0 + c] = v;
-                }
+            for (int w = 0; w < KVA_WAVES; w++) v += ob[(w * 16 + r) * LD + c];
+            if (last) {
+                const float l = total(r, largest(r));
+                kva_out_row<T>(a, row0 + r, hk)[c0 + c] = kva_out<T>(l == 0.0f ? 0.0f : v / l);
+            } else {
+                a.po[(part + r) * hd + c0 + c] = v;
             }
         }
-        if (!last && tid < 16 && 16 * q + tid < (int)n_rows) {
-            const float m = largest(16 * q + tid);
-            float l = 0.0f;
-#pragma unroll
-            for (int w = 0; w < KVA_WAVES; w++)
-                l += sums[(w * NQ + q) * 16 + tid] * kva_rescale(refs[(w * NQ + q) * 16 + tid], m);
-            a.ml[part + 16 * q + tid] = float2{m, l};
-        }
+    }
+    if (!last && tid < (int)n_rows) {
+        const float m = largest(tid);
+        a.ml[part + tid] = float2{m, total(tid, m)};
     }
 }
 
-// The body of many rows: a wave 16 NQ rows of the 64 NQ, every wave every key
-// tile.  A tile is widened once for the four of them, a quarter by each wave,
-// into LDS in operand order (each 16-byte access of a wave is 1 KiB in a row),
-// while the next tile's codes travel; two buffers and one barrier a tile (256
-// channels: one buffer, two barriers).
+// The body of many rows: four waves of 16 rows, every wave every key tile.  A
+// tile is widened once for the four of them, a quarter by each, into LDS in
+// operand order (each 16-byte access of a wave is 1 KiB in a row) while the
+// codes of the two tiles behind it travel; two buffers, one barrier a tile (256
+// channels: one buffer, so that a CU still holds two workgroups, two barriers
+// and one tile behind).  Two workgroups a CU, so that every SIMD has two waves
+// at unlike places (one alone issues a vector operation every four cycles, two
+// of one workgroup stand at its barriers together); 32 rows a wave halve the
+// widening but spill (64 behind 16384: 67 us and 56).
 template <int DC>
 struct KvaStage {
-    static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 512, BUFS = DC < 4 ? 2 : 1;
+    static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 528, BUFS = DC < 4 ? 2 : 1;
 };
-template <int DC, int NQ, bool HI>
+template <int DC, bool HI>
 struct KvaWideLds {
-    static constexpr int Q = 4 * NQ * 2 * DC * 1024 * (HI ? 2 : 1);  // under the stages, read into registers first
+    static constexpr int Q = KVA_WAVES * 2 * DC * 1024 * (HI ? 2 : 1);  // under the stages, read into registers first
     static constexpr int S = KvaStage<DC>::BYTES * KvaStage<DC>::BUFS;
     static constexpr int BODY = Q > S ? Q : S;
-    static constexpr int BYTES = BODY + 64 * NQ * 4;
+    static constexpr int BYTES = BODY + 16 * KVA_WAVES * 4;
 };
 
-template <int FMT, int DC, int NQ, typename T, class Limit>
+template <int FMT, int DC, typename T, class Limit>
 __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows,
                                               uint32_t hk, const uint8_t *kcode, const uint8_t *vcode,
                                               const float *ksc, const float *vsc, uint32_t tile0, uint32_t tile1,
                                               uint32_t written, Limit limit, uint32_t split, bool last) {
     constexpr bool HI = sizeof(T) == 4;
-    constexpr int STEPS = 2 * DC, BUFS = KvaStage<DC>::BUFS;
-    using L = KvaWideLds<DC, NQ, HI>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    constexpr int STEPS = 2 * DC, KEYS = KvaStage<DC>::KEYS, BUFS = KvaStage<DC>::BUFS;
+    using L = KvaWideLds<DC, HI>;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: loops and addresses by it are too
     const int hd = (int)a.own.hd, nc = hd / 16;
     float *cqs = (float *)(smem + L::BODY);
 
-    kva_u4_t kc[DC], vc[DC];  // this wave's quarter: keys of block `wave`, channel tiles wave, wave + 4, ..
-    float sc = 0.0f;          // threads 0 .. 63 a key's scale, 64 .. 127 a value's
-    auto load = [&](uint32_t tt) {
-        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + (size_t)wave * 16 * hd + col * 16;
+    // This wave's part of a tile: the keys of block `wave` and every fourth
+    // channel tile of the values.
+    kva_u4_t kc[BUFS][DC], vc[BUFS][DC];
+    float sc[BUFS];  // waves 0 and 1: a key's and a value's scale a lane
+    auto load = [&](uint32_t tt, int at) {
+        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + (wave * nc) * 256 + col * 16;
         const uint8_t *vt = vcode + (size_t)tt * 64 * hd + col * 64 + g * 16;
 #pragma unroll
         for (int c = 0; c < DC; c++) {
-            const int chunk = 4 * c + g < nc ? 4 * c + g : nc - 1;  // past the last chunk q is zero
-            kc[c] = *(const kva_u4_t *)(kt + chunk * 256);
-            if (wave + 4 * c < nc) vc[c] = *(const kva_u4_t *)(vt + (wave + 4 * c) * 1024);
+            const int chunk = 4 * c + g, ct = 4 * c + wave;
+            kc[at][c] = *(const kva_u4_t *)(kt + (chunk < nc ? chunk : nc - 1) * 256);  // past the last chunk q is zero
+            vc[at][c] = *(const kva_u4_t *)(vt + (ct < nc ? ct : nc - 1) * 1024);       // past the last tile: not stored
         }
-        if (wave < 2) sc = (wave ? vsc : ksc)[(size_t)tt * 64 + lane];
+        if (wave < 2) sc[at] = (wave ? vsc : ksc)[(size_t)tt * 64 + lane];
     };
-    auto stage = [&](uint32_t tt, char *buf) {
+    auto stage = [&](uint32_t tt, int at, char *buf) {
         const uint32_t key0 = tt * 64;
-        kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
         const bool tail = key0 + 64 > written;  // rows that were never written take no part, whatever they hold
-        if (FMT == QBK_KV_FP8 && tail) {        // NaN codes
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t k0 = key0 + 16 * i + 4 * g, left = written > k0 ? written - k0 : 0;
-                keep[i] = left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
-            }
-        }
+        kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
+        if (FMT == QBK_KV_FP8 && tail) keep = kva_keep(key0, written, g);  // NaN codes
 #pragma unroll
         for (int c = 0; c < DC; c++) {
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                *(kva_h8_t *)(buf + ((wave * STEPS + 2 * c + u) * 64 + lane) * 16) =
-                    kva_wide<FMT>(kc[c][2 * u], kc[c][2 * u + 1]);
-            if (wave + 4 * c < nc) {
-                const kva_u4_t w = vc[c] & keep;
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-                    *(kva_h8_t *)(buf + KvaStage<DC>::KEYS + ((2 * (wave + 4 * c) + u) * 64 + lane) * 16) =
-                        kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
-            }
-        }
-        if (wave < 2)
-            *(float *)(buf + 2 * KvaStage<DC>::KEYS + wave * 256 + lane * 4) = tail && key0 + lane >= written ? 0.0f : sc;
-    };
-    if (tile0 < tile1) load(tile0);
-    kva_queries<DC, 4 * NQ, T>(a, smem, cqs, row0, n_rows, hk);
-    __syncthreads();
-    kva_h8_t qh[NQ][STEPS], ql[NQ][STEPS];
-    kva_f4_t o[NQ][4 * DC];
-    float ref[NQ], sum[NQ], cq[NQ], vref = 0.0f, vinv = 0.0f;
-    uint32_t lim[NQ];
-    const uint32_t my0 = wave * 16 * NQ;  // this wave's first row
-#pragma unroll
-    for (int q = 0; q < NQ; q++) {
-#pragma unroll
-        for (int st = 0; st < STEPS; st++) {
-            const char *at = smem + (((wave * NQ + q) * STEPS + st) * 64 + lane) * 16;
-            qh[q][st] = *(const kva_h8_t *)at;
-            if constexpr (HI) ql[q][st] = *(const kva_h8_t *)(at + 4 * NQ * STEPS * 1024);
-        }
-#pragma unroll
-        for (int ct = 0; ct < 4 * DC; ct++) o[q][ct] = kva_f4_t{0, 0, 0, 0};
-        ref[q] = -INFINITY;
-        sum[q] = 0.0f;
-        cq[q] = cqs[my0 + 16 * q + col];
-        const uint32_t r = my0 + 16 * q + col;
-        lim[q] = limit(r < n_rows ? r : n_rows - 1);
-    }
-    const bool rows = my0 < n_rows;
-    const uint32_t least = limit(rows ? my0 : 0), end = my0 + 16 * NQ < n_rows ? my0 + 16 * NQ : n_rows;
-    const uint32_t most = rows ? limit(end - 1) : 0;  // no row of the wave sees keys from here on
-    __syncthreads();  // the queries are read
-
-    for (uint32_t tt = tile0; tt < tile1; tt++) {
-        char *buf = smem + (BUFS == 2 ? ((tt - tile0) & 1) * KvaStage<DC>::BYTES : 0);
-        if (BUFS == 1 && tt > tile0) __syncthreads();
-        stage(tt, buf);
-        __syncthreads();
-        if (tt + 1 < tile1) load(tt + 1);
-        const uint32_t key0 = tt * 64;
-        if (key0 >= most) continue;
-        const bool masked = key0 + 64 > least;
-        kva_f4_t ks[4], vs[4], s[NQ][4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            ks[i] = *(const kva_f4_t *)(buf + 2 * KvaStage<DC>::KEYS + (16 * i + 4 * g) * 4);
-            vs[i] = *(const kva_f4_t *)(buf + 2 * KvaStage<DC>::KEYS + 256 + (16 * i + 4 * g) * 4);
-#pragma unroll
-            for (int q = 0; q < NQ; q++) s[q][i] = kva_f4_t{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int st = 0; st < STEPS; st++) {
-            if (4 * (st / 2) >= nc) continue;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const kva_h8_t kf = *(const kva_h8_t *)(buf + ((i * STEPS + st) * 64 + lane) * 16);
-#pragma unroll
-                for (int q = 0; q < NQ; q++) {
-                    s[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[q][st], s[q][i], 0, 0, 0);
-                    if constexpr (HI) s[q][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[q][st], s[q][i], 0, 0, 0);
-                }
-            }
-        }
-        kva_value_scales<NQ, 4 * DC>(vs, vref, vinv, o);
-        kva_h8_t ph[NQ][2], pl[NQ][2];
-#pragma unroll
-        for (int q = 0; q < NQ; q++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[q][i] *= ks[i];
-            kva_softmax<4 * DC, HI>(s[q], vs, cq[q], masked, key0 + 4 * g, lim[q], ref[q], sum[q], o[q], ph[q], pl[q]);
-        }
-#pragma unroll
-        for (int ct = 0; ct < 4 * DC; ct++) {
-            if (ct >= nc) continue;
+            const kva_u4_t w = FMT == QBK_KV_FP8 ? vc[at][c] & keep : vc[at][c];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const kva_h8_t vf =
-                    *(const kva_h8_t *)(buf + KvaStage<DC>::KEYS + ((2 * ct + u) * 64 + lane) * 16);
-#pragma unroll
-                for (int q = 0; q < NQ; q++) {
-                    o[q][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[q][u], o[q][ct], 0, 0, 0);
-                    if constexpr (HI) o[q][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[q][u], o[q][ct], 0, 0, 0);
-                }
+                *(kva_h8_t *)(buf + ((wave * STEPS + 2 * c + u) * 64 + lane) * 16) =
+                    kva_wide<FMT>(kc[at][c][2 * u], kc[at][c][2 * u + 1]);
+                *(kva_h8_t *)(buf + KEYS + ((2 * (4 * c + wave) + u) * 64 + lane) * 16) =
+                    kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
             }
         }
+        if (wave < 2) {
+            const float x = tail && key0 + lane >= written ? 0.0f : sc[at];
+            *(float *)(buf + 2 * KEYS + wave * 256 + lane * 4) = x;
+            // the largest value scale, NaN aside: no scale is negative
+            const uint32_t most = kva_row_max<64>(x == x ? __float_as_uint(x) : 0u);
+            if (tid == 64) *(uint32_t *)(buf + 2 * KEYS + 512) = most;
+        }
+    };
+    if (tile0 < tile1) load(tile0, 0);
+    if (BUFS > 1 && tile0 + 1 < tile1) load(tile0 + 1, BUFS - 1);
+    kva_queries<DC, KVA_WAVES, T>(a, smem, cqs, row0, n_rows, hk);
+    __syncthreads();
+    kva_h8_t qh[STEPS], ql[STEPS];
+#pragma unroll
+    for (int x = 0; x < STEPS; x++) {
+        const char *at = smem + ((wave * STEPS + x) * 64 + lane) * 16;
+        qh[x] = *(const kva_h8_t *)at;
+        if constexpr (HI) ql[x] = *(const kva_h8_t *)(at + KVA_WAVES * STEPS * 1024);
     }
-    const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0;
+    const uint32_t my0 = wave * 16, r = my0 + col;  // this wave's first row, this lane's
+    const bool rows = my0 < n_rows;
+    KvaState<DC> st(cqs[r], limit(r < n_rows ? r : n_rows - 1));
+    const uint32_t least = kva_scalar(limit(rows ? my0 : 0)), end = my0 + 16 < n_rows ? my0 + 16 : n_rows;
+    const uint32_t most = rows ? kva_scalar(limit(end - 1)) : 0;  // no row of the wave sees keys from here on
+    __syncthreads();  // the queries are read
+
+    auto work = [&](uint32_t tt, const char *buf) {
+        const uint32_t key0 = tt * 64;
+        if (key0 >= most) return;
+        kva_f4_t ks[4], vs[4], s[4];
 #pragma unroll
-    for (int q = 0; q < NQ; q++) {
-        const uint32_t r = my0 + 16 * q + col;
-        const float l = kva_sum4(sum[q]), f = vref * 0x1p-12f;
-        if (r >= n_rows) continue;
-        if (last) {
-            const uint32_t rho = row0 + r;
-            T *dst = (T *)a.out + ((size_t)(rho / a.G) * a.H + (size_t)hk * a.G + rho % a.G) * hd + 4 * g;
+        for (int i = 0; i < 4; i++) s[i] = kva_f4_t{0, 0, 0, 0};
 #pragma unroll
-            for (int ct = 0; ct < 4 * DC; ct++) {
-                if (ct >= nc) continue;
+        for (int x = 0; x < STEPS; x++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) dst[16 * ct + j] = kva_out<T>(l == 0.0f ? 0.0f : o[q][ct][j] * f / l);
+            for (int i = 0; i < 4; i++) {
+                const kva_h8_t kf = *(const kva_h8_t *)(buf + ((i * STEPS + x) * 64 + lane) * 16);
+                s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[x], s[i], 0, 0, 0);
+                if constexpr (HI) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[x], s[i], 0, 0, 0);
             }
-        } else {
-            float *dst = a.po + (part + r) * hd + 4 * g;
+        kva_value_scales(kva_scalar(*(const float *)(buf + 2 * KEYS + 512)), st.vref, st.vinv, st.o);
 #pragma unroll
-            for (int ct = 0; ct < 4 * DC; ct++)
-                if (ct < nc) *(kva_f4_t *)(dst + 16 * ct) = o[q][ct] * f;
-            if (g == 0) a.ml[part + r] = float2{ref[q], l};
+        for (int i = 0; i < 4; i++) {
+            ks[i] = *(const kva_f4_t *)(buf + 2 * KEYS + (16 * i + 4 * g) * 4);
+            vs[i] = *(const kva_f4_t *)(buf + 2 * KEYS + 256 + (16 * i + 4 * g) * 4) * st.vinv;
+            s[i] *= ks[i];
         }
+        kva_h8_t ph[2], pl[2];
+        if (key0 + 64 > least)
+            kva_softmax<true, 4 * DC, HI>(s, vs, st.cq, key0 + 4 * g, st.lim, st.ref, st.sum, st.o, ph, pl);
+        else
+            kva_softmax<false, 4 * DC, HI>(s, vs, st.cq, 0, 0, st.ref, st.sum, st.o, ph, pl);
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const kva_h8_t vf = *(const kva_h8_t *)(buf + KEYS + ((2 * ct + u) * 64 + lane) * 16);
+                st.o[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[u], st.o[ct], 0, 0, 0);
+                if constexpr (HI) st.o[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[u], st.o[ct], 0, 0, 0);
+            }
+    };
+    for (uint32_t t = tile0; t < tile1; t += BUFS)
+#pragma unroll
+        for (int p = 0; p < BUFS; p++) {
+            const uint32_t tt = t + p;
+            if (tt >= tile1) continue;
+            char *buf = smem + p * KvaStage<DC>::BYTES;
+            if (BUFS == 1 && tt > tile0) __syncthreads();
+            stage(tt, p, buf);
+            __syncthreads();  // every wave is past the tile before, so the other buffer is free as well
+            if (tt + BUFS < tile1) load(tt + BUFS, p);
+            work(tt, buf);
+        }
+    const float l = kva_sum4(st.sum), f = st.vref * 0x1p-12f;
+    if (r >= n_rows) return;
+    if (last) {
+        T *dst = kva_out_row<T>(a, row0 + r, hk) + 4 * g;
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++)
+            if (ct < nc)
+#pragma unroll
+                for (int j = 0; j < 4; j++) dst[16 * ct + j] = kva_out<T>(l == 0.0f ? 0.0f : st.o[ct][j] * f / l);
+    } else {
+        const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0 + r;
+        float *dst = a.po + part * hd + 4 * g;
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++)
+            if (ct < nc) *(kva_f4_t *)(dst + 16 * ct) = st.o[ct] * f;
+        if (g == 0) a.ml[part] = float2{st.ref, l};
     }
 }
 
-// W 0: a body of up to 16 rows, each wave every fourth key tile; else one of 64 W.
-template <int FMT, int DC, int W, typename T, class... ARGS>
+template <int FMT, int DC, bool WIDE, typename T, class... ARGS>
 __device__ __forceinline__ void kva_any(ARGS &&...args) {
-    if constexpr (W == 0) kva_body<FMT, DC, 1, T>(args...);
-    else kva_wide_body<FMT, DC, W, T>(args...);
+    if constexpr (WIDE) kva_wide_body<FMT, DC, T>(args...);
+    else kva_body<FMT, DC, T>(args...);
 }
 
-template <int FMT, int DC, int NQP, int NQS, typename T>
+template <int FMT, int DC, bool WIDEP, bool WIDES, typename T>
 __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAttArgs a) {
     extern __shared__ char smem[];
     const uint32_t Hk = a.own.Hk;
     const bool last = a.sp + a.ss == 1;
     if (blockIdx.x < a.n_pre) {
         // kv heads next to each other: with eight of them each stays on one XCD, whose L2 serves its row tiles
-        const uint32_t hk = blockIdx.x % Hk, x = blockIdx.x / Hk, rt = x % a.rtp, split = x / a.rtp;
-        constexpr uint32_t R = NQP ? 64 * NQP : 16;
+        uint32_t hk, rt, rest;
+        const uint32_t split = a.by_rtp.split(a.by_hk.split(blockIdx.x, hk), rt);
+        constexpr uint32_t R = WIDEP ? 64 : 16;
         const uint32_t row0 = rt * R, n_rows = a.rows - row0 < R ? a.rows - row0 : R;
-        const uint32_t tiles = (a.prefix_len + 63) / 64, run = (tiles + a.sp - 1) / a.sp;
+        const uint32_t tiles = (a.prefix_len + 63) / 64, run = a.by_sp.split(tiles + a.sp - 1, rest);
         const uint32_t t0 = split * run < tiles ? split * run : tiles, t1 = t0 + run < tiles ? t0 + run : tiles;
         const size_t slab = a.pre.slab(a.prefix_seq, hk);
         const uint32_t len = a.prefix_len;
-        kva_any<FMT, DC, NQP, T>(a, smem, row0, n_rows, hk, a.pre.k + slab * a.pre.hd, a.pre.v + slab * a.pre.hd,
+        kva_any<FMT, DC, WIDEP, T>(a, smem, row0, n_rows, hk, a.pre.k + slab * a.pre.hd, a.pre.v + slab * a.pre.hd,
                                   a.pre.ks + slab, a.pre.vs + slab, t0, t1, len, [&](uint32_t) { return len; }, split,
                                   last);
         return;
     }
     const uint32_t item = blockIdx.x - a.n_pre;
-    const uint32_t hk = item % Hk, x = item / Hk, rt = x % a.rts, y = x / a.rts, b = y % a.n, split = y / a.n;
-    const uint32_t len = kva_len(a, b), tiles = (len + 63) / 64, run = kva_run(len, a.ss);
+    uint32_t hk, rt, b;
+    const uint32_t split = a.by_n.split(a.by_rts.split(a.by_hk.split(item, hk), rt), b);
+    const uint32_t len = kva_len(a, b), tiles = (len + 63) / 64, run = kva_run(a, len);
     if (split * run >= tiles && split > 0) return;  // split 0 is there for a sequence with no rows
-    constexpr uint32_t R = NQS ? 64 * NQS : 16;
+    constexpr uint32_t R = WIDES ? 64 : 16;
     const uint32_t per = a.sq * a.G, r0 = rt * R, n_rows = per - r0 < R ? per - r0 : R;
     const uint32_t sq = a.sq;
     const KvaRow rows(a, r0);
@@ -704,73 +714,83 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
         const uint32_t up = len + t + 1;
         return up > sq ? up - sq : 0;
     };
-    const uint32_t most = (limit(n_rows - 1) + 63) / 64;
+    const uint32_t most = (kva_scalar(limit(n_rows - 1)) + 63) / 64;
     uint32_t t1 = split * run + run;
     t1 = t1 < most ? t1 : most;
     const size_t slab = a.own.slab(a.first_seq + b, hk);
-    kva_any<FMT, DC, NQS, T>(a, smem, b * per + r0, n_rows, hk, a.own.k + slab * a.own.hd, a.own.v + slab * a.own.hd,
+    kva_any<FMT, DC, WIDES, T>(a, smem, b * per + r0, n_rows, hk, a.own.k + slab * a.own.hd, a.own.v + slab * a.own.hd,
                               a.own.ks + slab, a.own.vs + slab, split * run, t1, len, limit, a.sp + split, last);
 }
 
 // A wave a row and kv head: the partial results of its splits on their largest
-// reference.
-template <typename T>
+// reference.  Four channels a lane and, up to 128 channels, two or four splits
+// at a time; everything is asked for before anything is used (references
+// first, 20 splits of 1024 rows took twice as long).
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
-    const size_t item = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int STEP = 64 / LANES, N = (2 * KVA_MAX_SPLITS + STEP - 1) / STEP, BATCH = N < 16 ? N : 16;
+    const uint32_t item = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t lane = threadIdx.x & 63, Hk = a.own.Hk, hd = a.own.hd;
-    if (item >= (size_t)a.rows * Hk) return;
-    const uint32_t hk = (uint32_t)(item / a.rows), rho = (uint32_t)(item % a.rows);
+    if (item >= a.rows * Hk) return;
+    uint32_t rho, head, rest;
+    const uint32_t hk = a.by_rows.split(item, rho), query = a.by_g.split(rho, head);
     uint32_t splits = a.sp;
     if (a.ss) {
-        const uint32_t len = kva_len(a, rho / (a.sq * a.G)), run = kva_run(len, a.ss), k = ((len + 63) / 64 + run - 1) / run;
-        splits += k ? k : 1;
+        const uint32_t len = kva_len(a, a.by_sq.split(query, rest)), run = kva_run(a, len);
+        for (uint32_t at = 0; at == 0 || (at < len && splits < a.sp + a.ss); at += 64 * run) splits++;
     }
+    splits = kva_scalar(splits);
     float m = -INFINITY, l = 0.0f;
     if (lane < splits) {
         const float2 v = a.ml[((size_t)lane * Hk + hk) * a.rows + rho];
         m = v.x;
         l = v.y;
     }
-    float M = m;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    const float f = kva_rescale(m, M);
-    float lf = lane < splits ? l * f : 0.0f;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) lf += __shfl_xor(lf, o, 64);
-    // four channels a lane, 64 / (hd / 4) splits at a time, the loads of four such steps in flight
-    const uint32_t lanes = hd <= 64 ? 16 : hd <= 128 ? 32 : 64, c = 4 * (lane % lanes), step = 64 / lanes;
-    kva_f4_t v = {0, 0, 0, 0};
+    const uint32_t c = 4 * (lane % LANES), sub = lane / LANES;
     const float *src = a.po + ((size_t)hk * a.rows + rho) * hd + (c < hd ? c : 0);
     const size_t apart = (size_t)Hk * a.rows * hd;
-    for (uint32_t s0 = 0; s0 < splits; s0 += 4 * step) {
-        kva_f4_t x[4];
-        float fs[4];
+    float M = -INFINITY, f = 0.0f, lf = 0.0f;
+    kva_f4_t v = {0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++) {
-            const uint32_t s = s0 + k * step + lane / lanes, at = s < splits ? s : splits - 1;
-            x[k] = *(const kva_f4_t *)(src + at * apart);
-            fs[k] = __shfl(f, (int)at, 64);
-            if (s >= splits) x[k] = kva_f4_t{0, 0, 0, 0};
+    for (int b = 0; b < N; b += BATCH) {
+        if (b * STEP >= (int)splits) continue;
+        kva_f4_t x[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+            const uint32_t s = (b + k) * STEP + sub;
+            if ((b + k) * STEP < (int)splits) x[k] = *(const kva_f4_t *)(src + (s < splits ? s : splits - 1) * apart);
+        }
+        if (b == 0) {
+            M = m;
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+            f = lane < splits ? kva_rescale(m, M) : 0.0f;
+            lf = lane < splits ? l * f : 0.0f;
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) lf += __shfl_xor(lf, o, 64);
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) v += x[k] * fs[k];
+        for (int k = 0; k < BATCH; k++) {
+            const uint32_t s = (b + k) * STEP + sub;
+            const float fs = __shfl(f, (int)(s < 64 ? s : 63), 64);
+            if (s < splits) v += x[k] * fs;
+        }
     }
 #pragma unroll
-    for (int o = 32; o >= 16; o >>= 1)
-        if (lanes <= (uint32_t)o)
+    for (int o = LANES; o < 64; o <<= 1)
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], o, 64);
-    if (lane >= lanes || c >= hd) return;
-    T *dst = (T *)a.out + ((size_t)(rho / a.G) * a.H + (size_t)hk * a.G + rho % a.G) * hd + c;
+        for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], o, 64);
+    if (lane >= LANES || c >= hd) return;
+    T *dst = kva_out_row<T>(a, rho, hk) + c;
 #pragma unroll
     for (int e = 0; e < 4; e++) dst[e] = kva_out<T>(lf == 0.0f ? 0.0f : v[e] / lf);
 }
 
-// How a call is cut: row tiles (16 NQ rows) and splits of the prefix and of
+// How a call is cut: row tiles (16 or 64 rows) and splits of the prefix and of
 // the sequences' own rows.
 struct KvaPlan {
-    uint32_t nqp, nqs, rtp, rts, sp, ss;
+    bool widep, wides;  // bodies of 64 rows
+    uint32_t rtp, rts, sp, ss;
     uint64_t items;
     size_t bytes;
 };
@@ -778,30 +798,35 @@ struct KvaPlan {
 static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq, size_t max_len, size_t prefix_len) {
     KvaPlan p{};
     const size_t Hk = s->n_kv_heads, G = n_heads / Hk, rows = n * sq * G, per = sq * G;
-    const uint32_t most = s->head_dim > 128 ? 1 : 2;
-    auto rows_of = [](uint32_t w) { return w ? 64 * w : 16; };
-    p.nqs = per > 16 && max_len ? most : 0;
-    p.nqp = p.nqs ? most : rows > 16 && prefix_len ? (rows > 64 ? most : 1) : 0;
-    p.rtp = (uint32_t)div_ceil(rows, rows_of(p.nqp));
-    p.rts = (uint32_t)div_ceil(per, rows_of(p.nqs));
-    auto splits = [](size_t tiles, uint64_t others, uint64_t target) -> uint32_t {
-        uint64_t most = div_ceil(tiles, KVA_WAVES), want = div_ceil(target, others ? others : 1);
+    p.wides = per > 16 && max_len;
+    p.widep = p.wides || (rows > 16 && prefix_len);
+    p.rtp = (uint32_t)div_ceil(rows, p.widep ? 64 : 16);
+    p.rts = (uint32_t)div_ceil(per, p.wides ? 64 : 16);
+    const uint64_t op = (uint64_t)Hk * p.rtp, os = (uint64_t)n * Hk * p.rts;
+    // Splits: a workgroup a CU for the prefix, of four key tiles at least, and two for own rows where the sequences
+    // alone leave CUs idle; past that a run of at most 64 tiles, so that no workgroup outlasts the rest on one long
+    // sequence.  More of them write and join more partial rows (us, prefix of 8192 behind 32 sequences of 32/8 heads:
+    // 8 splits 32, 16 24.6, 32 24.7; own rows of 32 sequences up to 2085: one split 23.6, two 25.5).
+    auto splits = [](uint64_t want, size_t tiles) -> uint32_t {
+        const uint64_t most = div_ceil(tiles, KVA_WAVES);
         want = want < most ? want : most;
         return (uint32_t)(want < 1 ? 1 : want > KVA_MAX_SPLITS ? KVA_MAX_SPLITS : want);
     };
-    if (prefix_len) p.sp = splits(div_ceil(prefix_len, 64), (uint64_t)Hk * p.rtp, 512);
-    if (max_len) p.ss = splits(div_ceil(max_len, 64), (uint64_t)n * Hk * p.rts, 1024);
-    p.items = (uint64_t)Hk * p.rtp * p.sp + (uint64_t)n * Hk * p.rts * p.ss;
+    const size_t tp = div_ceil(prefix_len, 64), ts = div_ceil(max_len, 64);
+    if (prefix_len) p.sp = splits(div_ceil(256, op), tp);
+    if (max_len) p.ss = splits(os >= 256 ? div_ceil(ts, 64) : div_ceil(512, os), ts);
+    p.items = op * p.sp + os * p.ss;
     p.bytes = p.sp + p.ss > 1 ? round_up((size_t)(p.sp + p.ss) * Hk * rows * (s->head_dim * 4 + 8), 256) : 0;
     return p;
 }
 
-template <int FMT, int DC, int NQP, int NQS, typename T>
+template <int FMT, int DC, bool WIDEP, bool WIDES, typename T>
 static int kva_launch(const KvAttArgs &a, uint64_t items, int device, hipStream_t st) {
     constexpr bool HI = sizeof(T) == 4;
-    constexpr int N = KvaLds<DC, 1, HI>::BYTES, W = KvaWideLds<DC, NQP ? NQP : 1, HI>::BYTES;
-    constexpr int lds = NQP == 0 ? N : W > N ? W : N;
-    void (*k)(KvAttArgs) = kva_items<FMT, DC, NQP, NQS, T>;
+    constexpr int N = KvaLds<DC, HI>::BYTES, W = KvaWideLds<DC, HI>::BYTES;
+    constexpr int lds = !WIDEP ? N : WIDES || W > N ? W : N;
+    static_assert(!WIDES || WIDEP, "own rows are no more than the prefix's");
+    void (*k)(KvAttArgs) = kva_items<FMT, DC, WIDEP, WIDES, T>;
     if (lds > 64 * 1024) {  // once a device
         static std::atomic<uint64_t> asked{0};
         const uint64_t bit = device < 64 ? 1ull << device : 0;
@@ -817,14 +842,9 @@ static int kva_launch(const KvAttArgs &a, uint64_t items, int device, hipStream_
 
 template <int FMT, int DC, typename T>
 static int kva_dispatch_dc(const KvAttArgs &a, const KvaPlan &p, int device, hipStream_t st) {
-    if constexpr (DC < 4) {
-        if (p.nqs == 2) return kva_launch<FMT, DC, 2, 2, T>(a, p.items, device, st);
-        if (p.nqp == 2) return kva_launch<FMT, DC, 2, 0, T>(a, p.items, device, st);
-    } else {
-        if (p.nqs == 1) return kva_launch<FMT, DC, 1, 1, T>(a, p.items, device, st);
-    }
-    if (p.nqp == 1) return kva_launch<FMT, DC, 1, 0, T>(a, p.items, device, st);
-    return kva_launch<FMT, DC, 0, 0, T>(a, p.items, device, st);
+    if (p.wides) return kva_launch<FMT, DC, true, true, T>(a, p.items, device, st);
+    if (p.widep) return kva_launch<FMT, DC, true, false, T>(a, p.items, device, st);
+    return kva_launch<FMT, DC, false, false, T>(a, p.items, device, st);
 }
 
 template <int FMT, typename T>
@@ -842,7 +862,7 @@ static int kva_check(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq,
     if (n_heads == 0 || n_heads % s->n_kv_heads != 0)
         return fail(QBK_ERR_VALIDATION, fmt("n_kv_heads must divide n_heads: n_heads=%zu, n_kv_heads=%zu", n_heads,
                                             s->n_kv_heads));
-    if (n_heads > (1u << 20)) return fail(QBK_ERR_VALIDATION, "kv attention takes up to 2^20 heads");
+    if (n_heads > (1u << 13)) return fail(QBK_ERR_VALIDATION, "kv attention takes up to 8192 heads");
     if (sq == 0) return fail(QBK_ERR_VALIDATION, "kv attention requires at least one query a sequence");
     if (max_len > s->capacity)
         return fail(QBK_ERR_VALIDATION, fmt("max_len %zu is past the kv cache's capacity of %zu", max_len, s->capacity));
@@ -850,7 +870,7 @@ static int kva_check(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq,
         (n && (unsigned __int128)n * sq * (n_heads / s->n_kv_heads) > 0x7FFFFFFFull))
         return fail(QBK_ERR_VALIDATION, "kv attention: too many query rows for one launch");
     const KvaPlan p = n ? kva_plan(s, n_heads, n, sq, max_len, prefix_len) : KvaPlan{};
-    if (p.items > 0x7FFFFFFFull || (unsigned __int128)n * sq * n_heads > 0x1FFFFFFFCull)
+    if (p.items > 0x7FFFFFFFull || (unsigned __int128)n * sq * n_heads > 0x7FFFFFFFull)
         return fail(QBK_ERR_VALIDATION, "kv attention: too many query rows for one launch");
     return QBK_OK;
 }
@@ -922,6 +942,15 @@ int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *ca
     a.rtp = p.rtp;
     a.rts = p.rts;
     a.n_pre = (uint32_t)(shape->n_kv_heads * p.rtp * p.sp);
+    a.by_hk.set((uint32_t)shape->n_kv_heads);
+    a.by_rtp.set(p.rtp);
+    a.by_rts.set(p.rts);
+    a.by_n.set(a.n);
+    a.by_g.set(a.G);
+    a.by_sq.set(a.sq);
+    a.by_rows.set(a.rows);
+    a.by_sp.set(p.sp ? p.sp : 1);
+    a.by_ss.set(p.ss ? p.ss : 1);
     a.scale = (float)(1.4426950408889634 / sqrt((double)shape->head_dim));
     const size_t parts = (size_t)(p.sp + p.ss) * shape->n_kv_heads * a.rows;
     a.po = (float *)workspace;
@@ -938,10 +967,12 @@ int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *ca
     }
     if (p.sp + p.ss == 1) return QBK_OK;  // the items wrote the output
     const dim3 grid((unsigned)div_ceil((size_t)a.rows * shape->n_kv_heads, 4));
-    if (dtype == QBK_F32)
-        hipLaunchKernelGGL((kva_join<float>), grid, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((kva_join<uint16_t>), grid, dim3(256), 0, st, a);
+    void (*join)(KvAttArgs) =
+        dtype == QBK_F32 ? (a.own.hd <= 64 ? kva_join<float, 16> : a.own.hd <= 128 ? kva_join<float, 32> : kva_join<float, 64>)
+                         : (a.own.hd <= 64    ? kva_join<uint16_t, 16>
+                            : a.own.hd <= 128 ? kva_join<uint16_t, 32>
+                                              : kva_join<uint16_t, 64>);
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, st, a);
     QBK_HIP(hipGetLastError());
     return QBK_OK;
 }
