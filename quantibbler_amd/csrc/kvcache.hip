@@ -188,6 +188,264 @@ __global__ void __launch_bounds__(256) kv_read(KvRows a, T *k, T *v) {
     }
 }
 
+// Four values at any alignment (one access on this machine).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Kv4 {
+    T v[4];
+};
+
+// ---- many rows a sequence: a workgroup a 64-row tile of one kv head ----------
+
+// The workgroup's tile: input rows row .. row + hi - lo - 1 stand at rows lo ..
+// hi - 1 of the tile that begins at position first of sequence seq; seq -1:
+// rows that no sequence claims (lo 0).  Sequences' tiles are counted in order,
+// then those of the unclaimed rows behind the last one and before the first.
+struct KvTile {
+    int32_t seq;
+    uint32_t row, lo, hi;
+    uint64_t first;
+};
+__device__ __forceinline__ bool kv_tile(const KvRows &a, uint32_t tile, KvTile *t) {
+    __shared__ uint32_t sums[4];
+    __shared__ KvTile found;
+    __shared__ uint32_t have;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) have = 0;
+    uint32_t base = 0;
+    for (uint32_t s0 = 0; s0 < a.n + 2; s0 += 256) {
+        const uint32_t s = s0 + tid;
+        uint32_t from = 0, to = 0, at = 0;
+        if (s < a.n) {
+            from = a.row_start ? a.row_start[s] : s * a.per;
+            to = a.row_start ? a.row_start[s + 1] : from + a.per;
+            at = a.pos[s];
+        } else if (a.row_start && s == a.n) {
+            from = a.row_start[a.n];
+            to = a.n_rows;
+        } else if (a.row_start && s == a.n + 1) {
+            to = a.row_start[0];
+        }
+        to = to < a.n_rows ? to : a.n_rows;
+        const uint32_t count = to > from ? (uint32_t)(((uint64_t)(at & 63) + (to - from) + 63) / 64) : 0;
+        uint32_t up = count;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t x = (uint32_t)__shfl_up((int)up, o, 64);
+            if ((int)lane >= o) up += x;
+        }
+        __syncthreads();  // sums of the round before are read
+        if (lane == 63) sums[wave] = up;
+        __syncthreads();
+        uint32_t before = base + up - count;
+        for (uint32_t w = 0; w < wave; w++) before += sums[w];
+        if (tile >= before && tile - before < count) {
+            const uint32_t k = tile - before, skip = at & 63;
+            KvTile f;
+            f.seq = s < a.n ? (int32_t)s : -1;
+            f.lo = k == 0 ? skip : 0;
+            f.row = from + (k == 0 ? 0 : 64 * k - skip);
+            f.hi = to - f.row < 64 - f.lo ? f.lo + (to - f.row) : 64;
+            f.first = (uint64_t)(at - skip) + 64ull * k;
+            found = f;
+            have = 1;
+        }
+        __syncthreads();
+        base += sums[0] + sums[1] + sums[2] + sums[3];
+        if (have) break;
+    }
+    *t = found;
+    return have != 0;
+}
+
+// 4 x 4 bytes: out[i] = bytes i of in[0 .. 3].
+__device__ __forceinline__ void kv_transpose4(const uint32_t (&in)[4], uint32_t (&out)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(in[1], in[0], 0x05010400u), b = __builtin_amdgcn_perm(in[3], in[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(in[1], in[0], 0x07030602u), d = __builtin_amdgcn_perm(in[3], in[2], 0x07030602u);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+// Largest over 16 lanes.
+__device__ __forceinline__ uint32_t kv_max16(uint32_t v) {
+    auto up = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));  // row_ror 8, 4, 2, 1
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
+    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
+    return up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t kv_codes(const float (&x)[4], float inv) {
+    uint32_t w = 0;
+    if constexpr (FMT == QBK_KV_INT8) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) w |= (uint32_t)((int)rintf(x[e] * inv) + 128) << (8 * e);
+    } else {
+        w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+        w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, (int)w, true);
+    }
+    return w;
+}
+
+// Sixteen lanes a row, four channels a lane and P times 64 channels, sixteen
+// rows at a time and every row's loads before the first is used; the values'
+// codes go through LDS, from where 4 x 4 bytes turn round and leave as a
+// channel's 16 bytes.  PADW: dwords of an LDS row.
+template <int FMT, int P, typename T>
+__global__ void __launch_bounds__(256) kv_write_tiles(KvRows a, const T *k, const T *v) {
+    constexpr int PADW = 16 * P + 1;
+    __shared__ uint32_t codes[64 * PADW];
+    const uint32_t h = blockIdx.x % a.c.Hk, tid = threadIdx.x, hd = a.c.hd;
+    KvTile t;
+    if (!kv_tile(a, blockIdx.x / a.c.Hk, &t) || t.seq < 0 || t.first >= a.c.cap) return;
+    const size_t slab = a.c.slab(a.first + t.seq, h);
+    uint32_t hi = t.hi;
+    if (t.first + hi > a.c.cap) hi = (uint32_t)(a.c.cap - t.first);
+    const uint32_t c0 = 4 * (tid & 15);
+    constexpr float L = FMT == QBK_KV_INT8 ? 127.0f : 448.0f;
+#pragma unroll
+    for (int val = 0; val < 2; val++) {
+        Kv4<T> raw[4][P];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t r = 16 * q + (tid >> 4);
+            const bool in = r >= t.lo && r < hi;
+            const T *src = (val ? v : k) + (size_t)(t.row + (in ? r - t.lo : 0)) * a.stride + (size_t)h * hd;
+#pragma unroll
+            for (int p = 0; p < P; p++) raw[q][p] = *(const Kv4<T> *)(src + (c0 + 64 * p < hd ? c0 + 64 * p : 0));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t r = 16 * q + (tid >> 4);
+            float x[P][4];
+            uint32_t top = 0;
+#pragma unroll
+            for (int p = 0; p < P; p++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[p][e] = kv_in<T>(raw[q][p].v[e]);  // channels past the last repeat the first four
+                    const uint32_t b = __float_as_uint(x[p][e]) & 0x7fffffffu;
+                    top = b > top ? b : top;
+                }
+            top = kv_max16(top);
+            const bool whole = top < 0x7f800000u, in = r >= t.lo && r < hi;
+            const float A = fmaxf(__uint_as_float(whole ? top : 0u), 0x1p-100f), inv = L * (1.0f / A);
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                if (c0 + 64 * p >= hd) continue;
+                if (!whole)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[p][e] = 0.0f;
+                const uint32_t w = kv_codes<FMT>(x[p], inv);
+                if (val) codes[r * PADW + c0 / 4 + 16 * p] = w;
+                else if (in) *(uint32_t *)(a.c.k + slab * hd + kv_key_at(t.first + r, c0 + 64 * p, hd)) = w;
+            }
+            if (in && (tid & 15) == 0)
+                (val ? a.c.vs : a.c.ks)[slab + t.first + r] = whole ? A * (1.0f / L) : __builtin_nanf("");
+        }
+    }
+    __syncthreads();
+    uint8_t *dst = a.c.v + slab * hd + t.first * hd;
+    for (uint32_t x = tid; x < hd; x += 256) {  // four channels, rows 16 i + 4 g + j of one g
+        const uint32_t c4 = x >> 2, g = x & 3;
+        uint32_t out[4][4];  // [i][channel]
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t in[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) in[j] = codes[(16 * i + 4 * g + j) * PADW + c4];
+            kv_transpose4(in, out[i]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            uint8_t *d = dst + (size_t)(4 * c4 + e) * 64 + 16 * g;
+            if (t.lo == 0 && hi == 64) {
+                *(uint4 *)d = uint4{out[0][e], out[1][e], out[2][e], out[3][e]};
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t r = 16 * i + 4 * g;
+                if (r >= t.lo && r + 4 <= hi) {
+                    *(uint32_t *)(d + 4 * i) = out[i][e];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (r + j >= t.lo && r + j < hi) d[4 * i + j] = (uint8_t)(out[i][e] >> (8 * j));
+                }
+            }
+        }
+    }
+}
+
+// The other way: a lane takes 16 channels of a row, keys straight from their
+// 16-byte pieces, values from LDS, where 4 x 4 bytes have been turned.
+template <int FMT, typename T>
+__global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
+    __shared__ uint32_t codes[64 * 68];
+    __shared__ float scale[2][64];
+    const uint32_t h = blockIdx.x % a.c.Hk, tid = threadIdx.x, hd = a.c.hd, nc = hd / 16;
+    KvTile t;
+    if (!kv_tile(a, blockIdx.x / a.c.Hk, &t)) return;
+    const bool held = t.seq >= 0 && t.first < a.c.cap;
+    const size_t slab = a.c.slab(a.first + (held ? t.seq : 0), h);
+    const uint64_t first = held ? t.first : 0;
+    const uint32_t padw = hd / 4 + 4;  // 16-byte rows
+    const uint8_t *src = a.c.v + slab * hd + first * hd;
+    if (tid < 128) {
+        const uint32_t r = tid & 63;
+        const bool in = held && r >= t.lo && first + r < a.c.cap;
+        scale[tid >> 6][r] = in ? (tid < 64 ? a.c.ks : a.c.vs)[slab + first + r] : __builtin_nanf("");
+    }
+    for (uint32_t x = tid; x < hd; x += 256) {
+        const uint32_t c4 = x >> 2, g = x & 3;
+        uint4 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = *(const uint4 *)(src + (size_t)(4 * c4 + e) * 64 + 16 * g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t in[4] = {(&w[0].x)[i], (&w[1].x)[i], (&w[2].x)[i], (&w[3].x)[i]};
+            uint32_t out[4];
+            kv_transpose4(in, out);
+#pragma unroll
+            for (int j = 0; j < 4; j++) codes[(16 * i + 4 * g + j) * padw + c4] = out[j];
+        }
+    }
+    __syncthreads();
+    const uint32_t units = (t.hi - t.lo) * nc;
+    for (uint32_t x = tid; x < units; x += 256) {
+        const uint32_t r = t.lo + x / nc, chunk = x % nc;
+        const bool in = held && first + r < a.c.cap;
+        const uint4 kw = in ? *(const uint4 *)(a.c.k + slab * hd + kv_key_at(first + r, 16 * chunk, hd))
+                            : uint4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+        const uint4 vw = in ? *(const uint4 *)(codes + r * padw + 4 * chunk)
+                            : uint4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+        const size_t at = (size_t)(t.row + r - t.lo) * a.stride + (size_t)h * hd + 16 * chunk;
+        const float ks = scale[0][r], vs = scale[1][r];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            Kv4<T> y, z;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                y.v[e] = kv_out<T>(kv_value<FMT>((&kw.x)[i] >> (8 * e) & 255u, ks));
+                z.v[e] = kv_out<T>(kv_value<FMT>((&vw.x)[i] >> (8 * e) & 255u, vs));
+            }
+            *(Kv4<T> *)(k + at + 4 * i) = y;
+            *(Kv4<T> *)(v + at + 4 * i) = z;
+        }
+    }
+}
+
+// Whether a call goes by tiles: a tile's fixed work is that of some sixteen
+// rows by themselves.
+static bool kv_by_tiles(size_t n_rows, size_t n) { return n_rows >= 16 * n; }
+
+// Tiles that a call can have: a sequence's rows touch one more than they fill,
+// or two where they fill none, and the unclaimed ones make two runs of their own.
+static size_t kv_tiles(size_t n_rows, size_t n) { return n_rows / 64 + 2 * (n + 2); }
+
 // Checks shared by the write and the read; *a filled for a launch, n_rows 0
 // where there is nothing to do.
 static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void *k, const void *v, int dtype,
@@ -223,6 +481,29 @@ static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void
     return QBK_OK;
 }
 
+template <int FMT, typename T>
+static void kv_write_go(const KvRows &a, const T *k, const T *v, hipStream_t s) {
+    if (kv_by_tiles(a.n_rows, a.n)) {
+        void (*kern)(KvRows, const T *, const T *) = a.c.hd <= 64    ? kv_write_tiles<FMT, 1, T>
+                                                     : a.c.hd <= 128 ? kv_write_tiles<FMT, 2, T>
+                                                                     : kv_write_tiles<FMT, 4, T>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk)), dim3(256), 0, s, a, k, v);
+    } else {
+        hipLaunchKernelGGL((kv_write<FMT, T>), dim3((unsigned)div_ceil((size_t)a.n_rows * a.c.Hk, 4)), dim3(256), 0, s,
+                           a, k, v);
+    }
+}
+
+template <int FMT, typename T>
+static void kv_read_go(const KvRows &a, T *k, T *v, hipStream_t s) {
+    if (kv_by_tiles(a.n_rows, a.n))
+        hipLaunchKernelGGL((kv_read_tiles<FMT, T>), dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk)), dim3(256), 0, s,
+                           a, k, v);
+    else
+        hipLaunchKernelGGL((kv_read<FMT, T>), dim3((unsigned)div_ceil((size_t)a.n_rows * a.c.Hk, 4)), dim3(256), 0, s,
+                           a, k, v);
+}
+
 }  // namespace qbk
 
 using namespace qbk;
@@ -243,20 +524,13 @@ int qbk_kv_cache_write_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, void *cache,
         return rc;
     if (a.n_rows == 0) return QBK_OK;
     if ((rc = bind(ctx))) return rc;
-    const dim3 grid((unsigned)div_ceil(n_rows * shape->n_kv_heads, 4));
     hipStream_t s = (hipStream_t)stream;
-#define KV_GO(FMT)                                                                                                \
-    if (dtype == QBK_F32)                                                                                         \
-        hipLaunchKernelGGL((kv_write<FMT, float>), grid, dim3(256), 0, s, a, (const float *)k, (const float *)v); \
-    else                                                                                                          \
-        hipLaunchKernelGGL((kv_write<FMT, uint16_t>), grid, dim3(256), 0, s, a, (const uint16_t *)k,              \
-                           (const uint16_t *)v);
-    if (shape->format == QBK_KV_INT8) {
-        KV_GO(QBK_KV_INT8)
-    } else {
-        KV_GO(QBK_KV_FP8)
-    }
-#undef KV_GO
+    if (dtype == QBK_F32)
+        shape->format == QBK_KV_INT8 ? kv_write_go<QBK_KV_INT8>(a, (const float *)k, (const float *)v, s)
+                                     : kv_write_go<QBK_KV_FP8>(a, (const float *)k, (const float *)v, s);
+    else
+        shape->format == QBK_KV_INT8 ? kv_write_go<QBK_KV_INT8>(a, (const uint16_t *)k, (const uint16_t *)v, s)
+                                     : kv_write_go<QBK_KV_FP8>(a, (const uint16_t *)k, (const uint16_t *)v, s);
     QBK_HIP(hipGetLastError());
     return QBK_OK;
 }
@@ -270,19 +544,13 @@ int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *c
         return rc;
     if (a.n_rows == 0) return QBK_OK;
     if ((rc = bind(ctx))) return rc;
-    const dim3 grid((unsigned)div_ceil(n_rows * shape->n_kv_heads, 4));
     hipStream_t s = (hipStream_t)stream;
-#define KV_GO(FMT)                                                                                          \
-    if (dtype == QBK_F32)                                                                                   \
-        hipLaunchKernelGGL((kv_read<FMT, float>), grid, dim3(256), 0, s, a, (float *)k, (float *)v);        \
-    else                                                                                                    \
-        hipLaunchKernelGGL((kv_read<FMT, uint16_t>), grid, dim3(256), 0, s, a, (uint16_t *)k, (uint16_t *)v);
-    if (shape->format == QBK_KV_INT8) {
-        KV_GO(QBK_KV_INT8)
-    } else {
-        KV_GO(QBK_KV_FP8)
-    }
-#undef KV_GO
+    if (dtype == QBK_F32)
+        shape->format == QBK_KV_INT8 ? kv_read_go<QBK_KV_INT8>(a, (float *)k, (float *)v, s)
+                                     : kv_read_go<QBK_KV_FP8>(a, (float *)k, (float *)v, s);
+    else
+        shape->format == QBK_KV_INT8 ? kv_read_go<QBK_KV_INT8>(a, (uint16_t *)k, (uint16_t *)v, s)
+                                     : kv_read_go<QBK_KV_FP8>(a, (uint16_t *)k, (uint16_t *)v, s);
     QBK_HIP(hipGetLastError());
     return QBK_OK;
 }
