@@ -24,7 +24,8 @@ int kv_check_shape(const qbk_kv_shape *s, size_t *bytes) {
     if (s->head_dim == 0 || s->head_dim % 16 != 0 || s->head_dim > 256)
         return fail(QBK_ERR_VALIDATION, fmt("kv cache head_dim must be a multiple of 16 up to 256, got %zu",
                                             s->head_dim));
-    if (s->capacity > 0x7FFFFF00u || s->n_seqs > 0x7FFFFFFFu || s->n_kv_heads > 0x7FFFFFFFu)
+    if (s->n_kv_heads > 65536) return fail(QBK_ERR_VALIDATION, "kv cache heads must be at most 65536");
+    if (s->capacity > 0x7FFFFF00u || s->n_seqs > 0x7FFFFFFFu)
         return fail(QBK_ERR_VALIDATION, "kv cache sizes must be below 2^31");
     // 64-bit throughout: at most 2^31 * 2^31 slabs before the check below
     const unsigned __int128 rows = (unsigned __int128)s->n_seqs * s->n_kv_heads * round_up(s->capacity, 64);
@@ -380,6 +381,29 @@ __global__ void __launch_bounds__(256) kv_write_tiles(KvRows a, const T *k, cons
     }
 }
 
+// Sixteen codes as values at any alignment, 16 bytes a store.
+template <int FMT, typename T>
+__device__ __forceinline__ void kv_store16(T *dst, const uint4 &w, float scale) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Out {
+        uint32_t v[4];
+    };
+#pragma unroll
+    for (int i = 0; i < 4; i += sizeof(T) == 4 ? 1 : 2) {
+        Out y;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) y.v[e] = __float_as_uint(kv_value<FMT>((&w.x)[i] >> (8 * e) & 255u, scale));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t b = (&w.x)[i + e / 2] >> (16 * (e & 1));
+                y.v[e] = f32x2_to_bf16x2(kv_value<FMT>(b & 255u, scale), kv_value<FMT>(b >> 8 & 255u, scale));
+            }
+        }
+        *(Out *)(dst + 4 * i) = y;
+    }
+}
+
 // The other way: a lane takes 16 channels of a row, keys straight from their
 // 16-byte pieces, values from LDS, where 4 x 4 bytes have been turned.
 template <int FMT, typename T>
@@ -424,17 +448,8 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
                             : uint4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
         const size_t at = (size_t)(t.row + r - t.lo) * a.stride + (size_t)h * hd + 16 * chunk;
         const float ks = scale[0][r], vs = scale[1][r];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            Kv4<T> y, z;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                y.v[e] = kv_out<T>(kv_value<FMT>((&kw.x)[i] >> (8 * e) & 255u, ks));
-                z.v[e] = kv_out<T>(kv_value<FMT>((&vw.x)[i] >> (8 * e) & 255u, vs));
-            }
-            *(Kv4<T> *)(k + at + 4 * i) = y;
-            *(Kv4<T> *)(v + at + 4 * i) = z;
-        }
+        kv_store16<FMT>(k + at, kw, ks);
+        kv_store16<FMT>(v + at, vw, vs);
     }
 }
 

@@ -313,6 +313,7 @@ class KvCache:
         self.n_seqs, self.capacity = int(n_seqs), int(capacity)
         self.n_kv_heads, self.head_dim = int(n_kv_heads), int(head_dim)
         self._shape = KvShape(self.FORMATS[fmt], self.n_seqs, self.capacity, self.n_kv_heads, self.head_dim)
+        self._shape_ref, self._base = C.byref(self._shape), _ptr(buffer)
 
     @classmethod
     def size(cls, fmt: str, n_seqs: int, capacity: int, n_kv_heads: int, head_dim: int) -> int:
@@ -328,17 +329,17 @@ class KvCache:
         return need
 
     def _rows(self, fn, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start, row_stride, stream):
-        if dtype not in ("float32", "bfloat16"):
+        code = _KV_DTYPES.get(dtype)
+        if code is None:
             raise _lib.KernelError(f"kv cache rows must be 'float32' or 'bfloat16', got {dtype!r}")
-        n = self.n_seqs - int(first_seq) if n_seqs is None else int(n_seqs)
-        stride = self.n_kv_heads * self.head_dim if row_stride is None else int(row_stride)
-        if min(int(n_rows), int(first_seq), n, stride) < 0:
+        n = self.n_seqs - first_seq if n_seqs is None else n_seqs
+        stride = self.n_kv_heads * self.head_dim if row_stride is None else row_stride
+        if n_rows < 0 or first_seq < 0 or n < 0 or stride < 0:
             raise _lib.KernelError("kv cache rows, sequences and strides must not be negative")
-        _device_words(pos, n, "positions")
-        if row_start is not None:
-            _device_words(row_start, n + 1, "row starts")
-        check(fn(self.ctx.handle, C.byref(self._shape), _ptr(self.buffer), _ptr(k), _ptr(v), _DTYPES[dtype][0], stride,
-                 int(n_rows), _ptr(row_start), _ptr(pos), int(first_seq), n, _stream(stream)))
+        at = _device_words(pos, n, "positions")
+        starts = None if row_start is None else _device_words(row_start, n + 1, "row starts")
+        check(fn(self.ctx.handle, self._shape_ref, self._base, _ptr(k), _ptr(v), code, stride, n_rows, starts, at,
+                 first_seq, n, _stream(stream)))
 
     def write_dev(self, k, v, dtype: str, pos, n_rows: int, first_seq: int = 0, n_seqs: int | None = None,
                   row_start=None, row_stride: int | None = None, stream=None):
@@ -358,21 +359,14 @@ class KvCache:
         self._rows(_lib.load().qbk_kv_cache_read_dev, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start,
                    row_stride, stream)
 
-    def _bounds(self, n_seqs, first_seq, max_len):
-        n = self.n_seqs - int(first_seq) if n_seqs is None else int(n_seqs)
-        most = self.capacity if max_len is None else int(max_len)
-        return n, most
-
     def attention_workspace_size(self, n_heads: int, n_seqs: int | None = None, seq_q: int = 1,
                                  max_len: int | None = None, prefix_len: int = 0) -> int:
         """Bytes of workspace ``attention_dev`` of the same sizes needs."""
-        n, most = self._bounds(n_seqs, 0, max_len)
-        if min(n, most, int(n_heads), int(seq_q), int(prefix_len)) < 0:
+        n = self.n_seqs if n_seqs is None else n_seqs
+        most = self.capacity if max_len is None else max_len
+        if min(n, most, n_heads, seq_q, prefix_len) < 0:
             raise _lib.KernelError("kv attention sizes must not be negative")
-        lib = _lib.load()
-        need = int(lib.qbk_attention_kv_workspace_size(C.byref(self._shape), int(n_heads), n, int(seq_q), most,
-                                                       int(prefix_len)))
-        return need
+        return int(_lib.load().qbk_attention_kv_workspace_size(self._shape_ref, n_heads, n, seq_q, most, prefix_len))
 
     def attention_dev(self, q, dtype: str, n_heads: int, lens, out, workspace, workspace_size: int,
                       first_seq: int = 0, n_seqs: int | None = None, seq_q: int = 1, max_len: int | None = None,
@@ -383,32 +377,36 @@ class KvCache:
         among them), at most ``max_len`` (the capacity if None).  Every query
         also sees rows 0 .. prefix_len - 1 of ``prefix``'s sequence
         ``prefix_seq``, read once for the whole batch."""
-        if dtype not in ("float32", "bfloat16"):
+        code = _KV_DTYPES.get(dtype)
+        if code is None:
             raise _lib.KernelError(f"kv attention takes 'float32' or 'bfloat16' queries, got {dtype!r}")
-        n, most = self._bounds(n_seqs, first_seq, max_len)
-        if min(n, most, int(first_seq), int(n_heads), int(seq_q), int(prefix_seq), int(prefix_len)) < 0:
+        n = self.n_seqs - first_seq if n_seqs is None else n_seqs
+        most = self.capacity if max_len is None else max_len
+        if min(n, most, first_seq, n_heads, seq_q, prefix_seq, prefix_len) < 0:
             raise _lib.KernelError("kv attention sizes must not be negative")
         if prefix_len and prefix is None:
             raise _lib.KernelError("a prefix_len needs the cache that holds the prefix")
-        _device_words(lens, n, "lengths")
-        p = prefix if prefix_len else None
+        words = _device_words(lens, n, "lengths")
+        shared, base = (prefix._shape_ref, prefix._base) if prefix_len else (None, None)
         check(_lib.load().qbk_attention_kv_dev(
-            self.ctx.handle, C.byref(self._shape), _ptr(self.buffer), int(first_seq), n, _ptr(lens), most,
-            None if p is None else C.byref(p._shape), None if p is None else _ptr(p.buffer), int(prefix_seq),
-            int(prefix_len), int(n_heads), int(seq_q), _ptr(q), _DTYPES[dtype][0], _ptr(out), _ptr(workspace),
-            int(workspace_size), _stream(stream)))
+            self.ctx.handle, self._shape_ref, self._base, first_seq, n, words, most, shared, base, prefix_seq,
+            prefix_len, n_heads, seq_q, _ptr(q), code, _ptr(out), _ptr(workspace), workspace_size, _stream(stream)))
 
 
-def _device_words(x, n: int, what: str):
-    """``x`` a contiguous 32-bit device tensor of at least n entries, or a raw
-    device address the caller vouches for."""
-    if hasattr(x, "is_cuda"):
-        if not x.is_cuda or str(x.dtype) not in ("torch.int32", "torch.uint32") or not x.is_contiguous() \
-                or x.numel() < n:
-            raise _lib.KernelError(f"{what} must be a contiguous 32-bit device tensor of at least {n} entries; got "
-                                   f"{x.dtype} of {x.numel()} on {x.device}")
-    elif not isinstance(x, int):
+_KV_DTYPES = {"float32": _lib.QBK_F32, "bfloat16": _lib.QBK_BF16}
+
+
+def _device_words(x, n: int, what: str) -> int:
+    """The address of ``x``, a contiguous 32-bit integer device tensor of at
+    least n entries, or a raw device address the caller vouches for."""
+    if isinstance(x, int):
+        return x
+    if not hasattr(x, "is_cuda"):
         raise _lib.KernelError(f"{what} must be a device tensor or a device address")
+    if not x.is_cuda or x.element_size() != 4 or x.is_floating_point() or not x.is_contiguous() or x.numel() < n:
+        raise _lib.KernelError(f"{what} must be a contiguous 32-bit device tensor of at least {n} entries; got "
+                               f"{x.dtype} of {x.numel()} on {x.device}")
+    return x.data_ptr()
 
 
 class SageDecodeState:

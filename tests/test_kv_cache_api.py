@@ -34,6 +34,7 @@ def test_sizes():
     (("int8", 1, 8, 1, 272), "multiple of 16 up to 256, got 272"),
     (("int8", 1, 8, 1, 0), "multiple of 16 up to 256, got 0"),
     (("int8", 1, 1 << 31, 1, 64), "below 2\\^31"),
+    (("int8", 1, 8, (1 << 16) + 1, 64), "heads must be at most 65536"),
     (("int8", 1 << 20, 1 << 20, 64, 64), "2\\^48"),
     (("int8", -1, 8, 1, 64), "negative"),
 ])
@@ -121,6 +122,7 @@ def test_attention_words_need_not_be_on_the_host():
     cache = KvCache.__new__(KvCache)
     cache.n_seqs, cache.capacity, cache.n_kv_heads, cache.head_dim = 2, 8, 1, 16
     cache.buffer, cache._shape = BUF, KvShape(0, 2, 8, 1, 16)
+    cache._shape_ref, cache._base, cache.ctx = C.byref(cache._shape), BUF, None
     host = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(KernelError, match="lengths must be a contiguous 32-bit device tensor"):
         cache.attention_dev(BUF, "float32", 1, host, BUF, BUF, 1 << 20)
