@@ -8,9 +8,12 @@
 //   log p = (x - M) - log l,   entropy = log l - t / l
 // (t moves from m to M as t' = f (t + (m - M) l), f = exp(m - M)).
 //
-// The top_k of a chunk: the k-th largest of the 256 threads' own largest keys
-// is no larger than the chunk's k-th, and only k threads hold anything above
-// it, so what is left to order is at most 32 k keys and mostly little past k.
+// The top_k of a chunk: of the 64 threads of a wave, k hold a value at or above
+// the k-th largest of their own largest values, so the largest such bound of
+// the four waves is no more than the chunk's k-th largest value, and what is
+// left to order is mostly little past k.  Where ties leave more than fit (a row
+// of few different values) the same is done once more on keys of value and id,
+// which all differ: only k threads hold keys above the k-th largest of theirs.
 #include <math.h>
 
 #include "qbk_internal.h"
@@ -23,6 +26,7 @@ namespace qbk {
 #define LP_PER 32
 #define LP_CHUNK (LP_THREADS * LP_PER)
 #define LP_MAX_TOP 64
+#define LP_CAND (LP_MAX_TOP * LP_PER)  // keys that fit in LDS
 
 struct LpArgs {
     const void *x;
@@ -36,18 +40,30 @@ struct LpArgs {
     uint64_t *keys;   // [row][chunk][top]
 };
 
-// A key that orders as (value, lower id first); above 0 for every logit.
-__device__ __forceinline__ uint64_t lp_key(float x, uint32_t id) {
-    x = x != x ? -INFINITY : x + 0.0f;  // -0 ties with 0
+// A float's bits as an unsigned number of the same order, and back.
+__device__ __forceinline__ uint32_t lp_rank(float x) {
     const uint32_t b = __float_as_uint(x);
-    return (uint64_t)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32 | (uint32_t)~id;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float lp_key_value(uint64_t key) {
-    const uint32_t b = (uint32_t)(key >> 32);
+__device__ __forceinline__ float lp_unrank(uint32_t b) {
     return __uint_as_float(b ^ (b >> 31 ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-__device__ __forceinline__ float lp_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.4426950408889634f); }
+// A key that orders as (value, lower id first); above 0 for every logit.
+__device__ __forceinline__ uint64_t lp_key(float x, uint32_t id) {
+    x = x != x ? -INFINITY : x + 0.0f;  // -0 ties with 0
+    return (uint64_t)lp_rank(x) << 32 | (uint32_t)~id;
+}
+
+// exp(d), d <= 0 or NaN: d log2(e) in two parts, the second as a factor, so
+// that far terms keep their last places (one rounded product is off by |d| of
+// them).  Below -1000 the result is 0 and e d is 0 as well, -inf included.
+__device__ __forceinline__ float lp_exp(float &d) {
+    d = d < -1000.0f ? -1000.0f : d;
+    const float p = d * 1.44269502f, r = __builtin_fmaf(d, 1.92596303e-8f, __builtin_fmaf(d, 1.44269502f, -p));
+    const float e = __builtin_amdgcn_exp2f(p);
+    return __builtin_fmaf(e, r * 0.693147182f, e);
+}
 
 template <typename T>
 struct LpVec {
@@ -73,23 +89,42 @@ __device__ __forceinline__ float lp_reduce(float v, float *red, OP op) {
 }
 
 // The `top` largest of n distinct keys in LDS, in order, into out (0 where
-// there are fewer).
-__device__ __forceinline__ void lp_order(const uint64_t *key, uint32_t n, uint32_t top, uint64_t *out) {
+// there are fewer).  The keys are followed by room for seven more.
+__device__ __forceinline__ void lp_order(uint64_t *key, uint32_t n, uint32_t top, uint64_t *out) {
+    if (threadIdx.x < 7) key[n + threadIdx.x] = 0;
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += LP_THREADS) {
         const uint64_t mine = key[i];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; j++) rank += key[j] > mine;
+        for (uint32_t j = 0; j < n; j += 8) {
+            uint64_t k[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) k[e] = key[j + e];
+#pragma unroll
+            for (int e = 0; e < 8; e++) rank += k[e] > mine;
+        }
         if (rank < top) out[rank] = mine;
     }
     for (uint32_t i = n + threadIdx.x; i < top; i += LP_THREADS) out[i] = 0;
+}
+
+// The k-th largest of a wave's 64 values (k <= 64), bit by bit.
+__device__ __forceinline__ uint32_t lp_kth(uint32_t v, uint32_t k) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int b = 31; b >= 0; b--) {
+        const uint32_t up = t | 1u << b;
+        t = (uint32_t)__popcll(__ballot(v >= up)) >= k ? up : t;
+    }
+    return t;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
     __shared__ float red[LP_THREADS / 64];
     __shared__ uint64_t best[LP_THREADS];
-    __shared__ uint64_t cand[LP_MAX_TOP * LP_PER];
-    __shared__ uint32_t count;
+    __shared__ uint64_t cand[LP_CAND + 8];
+    __shared__ uint32_t count, bounds[LP_THREADS / 64];
     __shared__ uint64_t bar;
     constexpr int V = 16 / sizeof(T), LOADS = LP_PER / V;
     const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
@@ -108,50 +143,76 @@ __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
             for (int e = 0; e < V; e++) v[j * V + e] = i + e < a.vocab ? lp_in(x[i + e]) : -INFINITY;
         }
     }
-    float m = -INFINITY;
+    float most = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < LP_PER; j++) m = fmaxf(m, v[j]);
-    m = lp_reduce(m, red, [](float p, float q) { return fmaxf(p, q); });
+    for (int j = 0; j < LP_PER; j++) most = fmaxf(most, v[j]);
+    if (a.top > 1) {
+        const uint32_t bound = lp_kth(lp_rank(most + 0.0f), a.top);
+        if ((tid & 63) == 0) bounds[tid >> 6] = bound;
+    }
+    if (tid == 0) count = 0;
+    const float m = lp_reduce(most, red, [](float p, float q) { return fmaxf(p, q); });
     const float from = m == -INFINITY ? 0.0f : m;  // a chunk of nothing but -inf adds nothing (a NaN stays one)
-    float l = 0.0f, t = 0.0f;
+    float l[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < LP_PER; j++) {
-        const float d = v[j] - from, e = lp_exp(d);
-        l += e;
-        t += d == -INFINITY ? 0.0f : e * d;
+        float d = v[j] - from;
+        const float e = lp_exp(d);
+        l[j & 1] += e;
+        t[j & 1] = __builtin_fmaf(e, d, t[j & 1]);
     }
-    l = lp_reduce(l, red, [](float p, float q) { return p + q; });
-    t = lp_reduce(t, red, [](float p, float q) { return p + q; });
-    if (tid == 0) a.part[blockIdx.x] = float4{m, l, t, 0.0f};
+    const float ls = lp_reduce(l[0] + l[1], red, [](float p, float q) { return p + q; });
+    const float ts = lp_reduce(t[0] + t[1], red, [](float p, float q) { return p + q; });
+    if (tid == 0) a.part[blockIdx.x] = float4{m, ls, ts, 0.0f};
     if (a.top == 0) return;
 
     auto id = [&](int j) { return base + ((j / V) * LP_THREADS + tid) * V + j % V; };
-    uint64_t mine = 0;
+    auto take = [&](uint64_t k) {
+        const uint32_t at = atomicAdd(&count, 1u);
+        if (at < LP_CAND) cand[at] = k;
+    };
+    float least = m;
+    if (a.top > 1) {
+        uint32_t b = bounds[0];
 #pragma unroll
-    for (int j = 0; j < LP_PER; j++)
-        if (id(j) < a.vocab) {
-            const uint64_t k = lp_key(v[j], id(j));
-            mine = k > mine ? k : mine;
+        for (int w = 1; w < LP_THREADS / 64; w++) b = bounds[w] > b ? bounds[w] : b;
+        least = lp_unrank(b);
+    }
+    // NaN counts as -inf, which is only asked for where nothing above it is left
+    if (most >= least)
+#pragma unroll
+        for (int j = 0; j < LP_PER; j++)
+            if ((v[j] >= least || least == -INFINITY) && id(j) < a.vocab) take(lp_key(v[j], id(j)));
+    __syncthreads();
+    if (count > LP_CAND) {
+        __syncthreads();
+        if (tid == 0) {
+            count = 0;
+            bar = 1;  // fewer threads with a logit than top: everything is above it
         }
-    best[tid] = mine;
-    if (tid == 0) count = 0;
-    __syncthreads();
-    uint32_t rank = 0;
-    for (int j = 0; j < LP_THREADS; j++) rank += best[j] > mine;
-    if (tid == 0) bar = 1;  // fewer threads with a logit than top: everything is above it
-    __syncthreads();
-    if (mine && rank == a.top - 1) bar = mine;
-    __syncthreads();
-    if (mine >= bar) {
-        const uint64_t least = bar;
+        uint64_t mine = 0;
 #pragma unroll
         for (int j = 0; j < LP_PER; j++)
             if (id(j) < a.vocab) {
                 const uint64_t k = lp_key(v[j], id(j));
-                if (k >= least) cand[atomicAdd(&count, 1u)] = k;
+                mine = k > mine ? k : mine;
             }
+        best[tid] = mine;
+        __syncthreads();
+        uint32_t rank = 0;
+        for (int j = 0; j < LP_THREADS; j++) rank += best[j] > mine;
+        if (mine && rank == a.top - 1) bar = mine;
+        __syncthreads();
+        const uint64_t floor = bar;
+        if (mine >= floor)
+#pragma unroll
+            for (int j = 0; j < LP_PER; j++)
+                if (id(j) < a.vocab) {
+                    const uint64_t k = lp_key(v[j], id(j));
+                    if (k >= floor) take(k);
+                }
+        __syncthreads();
     }
-    __syncthreads();
     lp_order(cand, count, a.top, a.keys + (size_t)blockIdx.x * a.top);
 }
 
@@ -159,8 +220,10 @@ __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
     __shared__ float red[LP_THREADS / 64];
-    __shared__ uint64_t cand[LP_MAX_TOP * LP_PER];
+    __shared__ uint64_t cand[LP_CAND + 8];
     __shared__ uint64_t first[LP_MAX_TOP];
+    __shared__ uint64_t floors[LP_THREADS / 64];
+    __shared__ uint32_t count;
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const float4 *part = a.part + (size_t)row * a.chunks;
     float M = -INFINITY;
@@ -170,7 +233,8 @@ __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
     for (uint32_t c = tid; c < a.chunks; c += LP_THREADS) {
         const float4 p = part[c];
         if (p.x == -INFINITY && p.y == 0.0f) continue;
-        const float d = p.x - M, f = lp_exp(d);
+        float d = p.x - M;
+        const float f = lp_exp(d);
         l += p.y * f;
         t += f == 0.0f ? 0.0f : f * (p.z + d * p.y);  // d l may pass f32 where f is 0
     }
@@ -188,31 +252,47 @@ __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
         }
     }
     if (a.top == 0) return;
-    // batches of keys that fit, the best so far among them
+    // The largest last key of a chunk's list is no more than the row's last: what lies at or above it is ordered, in
+    // batches where it does not fit, the best so far among them.
     const uint64_t *keys = a.keys + (size_t)row * a.chunks * a.top;
+    uint64_t floor = 1;  // above the zeros of a chunk short of logits
+    for (uint32_t c = tid; c < a.chunks; c += LP_THREADS) {
+        const uint64_t k = keys[(size_t)c * a.top + a.top - 1];
+        floor = k > floor ? k : floor;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const uint64_t k = (uint64_t)__shfl_xor((unsigned long long)floor, o, 64);
+        floor = k > floor ? k : floor;
+    }
+    if ((tid & 63) == 0) floors[tid >> 6] = floor;
+    if (tid == 0) count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < LP_THREADS / 64; w++) floor = floors[w] > floor ? floors[w] : floor;
     const uint64_t all = (uint64_t)a.chunks * a.top;
-    uint32_t kept = 0;
-    for (uint64_t at = 0; at < all;) {
-        const uint32_t room = LP_MAX_TOP * LP_PER - kept, take = all - at < room ? (uint32_t)(all - at) : room;
-        // the last chunk may be short of logits and leave zeros: the first batch holds a whole chunk's (or, of one
-        // chunk, the row's) keys, so every zero ranks past `top`
-        for (uint32_t i = tid; i < take; i += LP_THREADS) cand[kept + i] = keys[at + i];
-        __syncthreads();
-        lp_order(cand, kept + take, a.top, first);
-        __syncthreads();
-        at += take;
-        kept = 0;
-        if (at < all) {
-            for (uint32_t i = tid; i < a.top; i += LP_THREADS) cand[i] = first[i];
-            kept = a.top;
+    constexpr uint32_t BATCH = LP_CAND - LP_MAX_TOP;
+    for (uint64_t at = 0; at < all; at += BATCH) {
+        for (uint64_t i = at + tid; i < all && i < at + BATCH; i += LP_THREADS) {
+            const uint64_t k = keys[i];
+            if (k >= floor) cand[atomicAdd(&count, 1u)] = k;
         }
         __syncthreads();
+        lp_order(cand, count, a.top, first);
+        __syncthreads();
+        if (at + BATCH < all) {  // the next batch begins with the best so far
+            uint32_t kept = count < a.top ? count : a.top;
+            __syncthreads();
+            for (uint32_t i = tid; i < kept; i += LP_THREADS) cand[i] = first[i];
+            if (tid == 0) count = kept;
+            __syncthreads();
+        }
     }
     for (uint32_t i = tid; i < a.top; i += LP_THREADS) {
         const uint64_t k = first[i];
         const uint32_t id = ~(uint32_t)k;
         a.top_ids[(size_t)row * a.top + i] = (int32_t)id;
-        a.top_logprobs[(size_t)row * a.top + i] = ok ? (lp_key_value(k) - M) - lse : nan;
+        a.top_logprobs[(size_t)row * a.top + i] = ok ? (lp_unrank((uint32_t)(k >> 32)) - M) - lse : nan;
     }
 }
 
