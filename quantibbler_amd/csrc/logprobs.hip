@@ -16,6 +16,8 @@
 // which all differ: only k threads hold keys above the k-th largest of theirs.
 #include <math.h>
 
+#include <type_traits>
+
 #include "qbk_internal.h"
 
 #pragma clang fp contract(off)
@@ -74,18 +76,43 @@ struct LpVec {
 __device__ __forceinline__ float lp_in(float x) { return x; }
 __device__ __forceinline__ float lp_in(uint16_t x) { return bf16_to_f32(x); }
 
-// Sum / largest over the workgroup; every thread gets it.  red: a float a wave.
+// Over a wave, every lane gets it: rotations within 16 lanes, then swaps of 16
+// and 32 (a dozen cycles each where a permute through LDS takes a hundred).
 template <class OP>
-__device__ __forceinline__ float lp_reduce(float v, float *red, OP op) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
-    __syncthreads();
+__device__ __forceinline__ float lp_wave(float v, OP op) {
+    auto turn = [](float x, auto ctrl) {
+        return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value,
+                                                                     0xf, 0xf, true));
+    };
+    v = op(v, turn(v, std::integral_constant<int, 0x128>{}));  // row_ror 8, 4, 2, 1
+    v = op(v, turn(v, std::integral_constant<int, 0x124>{}));
+    v = op(v, turn(v, std::integral_constant<int, 0x122>{}));
+    v = op(v, turn(v, std::integral_constant<int, 0x121>{}));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// Over the workgroup; red: a float a wave, not in use by a reduction before.
+__device__ __forceinline__ float lp_max(float v, float *red) {
+    v = lp_wave(v, [](float p, float q) { return fmaxf(p, q); });
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int w = 1; w < LP_THREADS / 64; w++) v = op(v, red[w]);
+    for (int w = 1; w < LP_THREADS / 64; w++) v = fmaxf(v, red[w]);
     return v;
+}
+__device__ __forceinline__ float2 lp_sum(float x, float y, float2 *red) {
+    auto add = [](float p, float q) { return p + q; };
+    x = lp_wave(x, add);
+    y = lp_wave(y, add);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = float2{x, y};
+    __syncthreads();
+    float2 s = red[0];
+#pragma unroll
+    for (int w = 1; w < LP_THREADS / 64; w++) s = float2{s.x + red[w].x, s.y + red[w].y};
+    return s;
 }
 
 // The `top` largest of n distinct keys in LDS, in order, into out (0 where
@@ -122,6 +149,7 @@ __device__ __forceinline__ uint32_t lp_kth(uint32_t v, uint32_t k) {
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
     __shared__ float red[LP_THREADS / 64];
+    __shared__ float2 red2[LP_THREADS / 64];
     __shared__ uint64_t best[LP_THREADS];
     __shared__ uint64_t cand[LP_CAND + 8];
     __shared__ uint32_t count, bounds[LP_THREADS / 64];
@@ -151,7 +179,7 @@ __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
         if ((tid & 63) == 0) bounds[tid >> 6] = bound;
     }
     if (tid == 0) count = 0;
-    const float m = lp_reduce(most, red, [](float p, float q) { return fmaxf(p, q); });
+    const float m = lp_max(most, red);
     const float from = m == -INFINITY ? 0.0f : m;  // a chunk of nothing but -inf adds nothing (a NaN stays one)
     float l[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -161,9 +189,8 @@ __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
         l[j & 1] += e;
         t[j & 1] = __builtin_fmaf(e, d, t[j & 1]);
     }
-    const float ls = lp_reduce(l[0] + l[1], red, [](float p, float q) { return p + q; });
-    const float ts = lp_reduce(t[0] + t[1], red, [](float p, float q) { return p + q; });
-    if (tid == 0) a.part[blockIdx.x] = float4{m, ls, ts, 0.0f};
+    const float2 sum = lp_sum(l[0] + l[1], t[0] + t[1], red2);
+    if (tid == 0) a.part[blockIdx.x] = float4{m, sum.x, sum.y, 0.0f};
     if (a.top == 0) return;
 
     auto id = [&](int j) { return base + ((j / V) * LP_THREADS + tid) * V + j % V; };
@@ -220,15 +247,31 @@ __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
     __shared__ float red[LP_THREADS / 64];
+    __shared__ float2 red2[LP_THREADS / 64];
     __shared__ uint64_t cand[LP_CAND + 8];
     __shared__ uint64_t first[LP_MAX_TOP];
     __shared__ uint64_t floors[LP_THREADS / 64];
     __shared__ uint32_t count;
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const float4 *part = a.part + (size_t)row * a.chunks;
+    // asked for first: the chunks' last keys, the first four keys of every thread and the target's logit
+    const uint64_t *keys = a.keys + (size_t)row * a.chunks * a.top;
+    uint64_t floor = 1;  // above the zeros of a chunk short of logits
+    if (a.top)
+        for (uint32_t c = tid; c < a.chunks; c += LP_THREADS) {
+            const uint64_t k = keys[(size_t)c * a.top + a.top - 1];
+            floor = k > floor ? k : floor;
+        }
+    const uint64_t all = (uint64_t)a.chunks * a.top;
+    uint64_t early[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) early[e] = tid + LP_THREADS * e < all ? keys[tid + LP_THREADS * e] : 0;
+    const int32_t id = a.logprobs ? a.targets[row] : -1;
+    const bool in = id >= 0 && (uint32_t)id < a.vocab;
+    const float target = lp_in(((const T *)a.x)[(size_t)row * a.stride + (in ? id : 0)]);
     float M = -INFINITY;
     for (uint32_t c = tid; c < a.chunks; c += LP_THREADS) M = fmaxf(M, part[c].x);
-    M = lp_reduce(M, red, [](float p, float q) { return fmaxf(p, q); });
+    M = lp_max(M, red);
     float l = 0.0f, t = 0.0f;
     for (uint32_t c = tid; c < a.chunks; c += LP_THREADS) {
         const float4 p = part[c];
@@ -238,28 +281,19 @@ __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
         l += p.y * f;
         t += f == 0.0f ? 0.0f : f * (p.z + d * p.y);  // d l may pass f32 where f is 0
     }
-    l = lp_reduce(l, red, [](float p, float q) { return p + q; });
-    t = lp_reduce(t, red, [](float p, float q) { return p + q; });
+    const float2 sum = lp_sum(l, t, red2);
+    l = sum.x;
+    t = sum.y;
     const float lse = logf(l);  // on M
     const float nan = __builtin_nanf("");
     const bool ok = l > 0.0f && l < INFINITY;
     if (tid == 0) {
         if (a.entropy) a.entropy[row] = ok ? lse - t / l : nan;
-        if (a.logprobs) {
-            const int32_t id = a.targets[row];
-            const bool in = id >= 0 && (uint32_t)id < a.vocab;
-            a.logprobs[row] = ok && in ? (lp_in(((const T *)a.x)[(size_t)row * a.stride + id]) - M) - lse : nan;
-        }
+        if (a.logprobs) a.logprobs[row] = ok && in ? (target - M) - lse : nan;
     }
     if (a.top == 0) return;
     // The largest last key of a chunk's list is no more than the row's last: what lies at or above it is ordered, in
     // batches where it does not fit, the best so far among them.
-    const uint64_t *keys = a.keys + (size_t)row * a.chunks * a.top;
-    uint64_t floor = 1;  // above the zeros of a chunk short of logits
-    for (uint32_t c = tid; c < a.chunks; c += LP_THREADS) {
-        const uint64_t k = keys[(size_t)c * a.top + a.top - 1];
-        floor = k > floor ? k : floor;
-    }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
         const uint64_t k = (uint64_t)__shfl_xor((unsigned long long)floor, o, 64);
@@ -270,10 +304,13 @@ __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < LP_THREADS / 64; w++) floor = floors[w] > floor ? floors[w] : floor;
-    const uint64_t all = (uint64_t)a.chunks * a.top;
     constexpr uint32_t BATCH = LP_CAND - LP_MAX_TOP;
+    static_assert(BATCH >= 4 * LP_THREADS, "the early keys are of the first batch");
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (early[e] >= floor) cand[atomicAdd(&count, 1u)] = early[e];
     for (uint64_t at = 0; at < all; at += BATCH) {
-        for (uint64_t i = at + tid; i < all && i < at + BATCH; i += LP_THREADS) {
+        for (uint64_t i = at + tid + (at ? 0 : 4 * LP_THREADS); i < all && i < at + BATCH; i += LP_THREADS) {
             const uint64_t k = keys[i];
             if (k >= floor) cand[atomicAdd(&count, 1u)] = k;
         }

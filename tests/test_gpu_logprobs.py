@@ -39,7 +39,8 @@ def call(ctx, x, targets, top, stride=None, rows=None, vocab=None, ws=None):
 
 def close(got, want, tol, label):
     got = got.astype(np.float64)
-    same = (np.abs(got - want) <= tol) | (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        same = (np.abs(got - want) <= tol) | (got == want) | (np.isnan(got) & np.isnan(want))
     assert same.all(), f"{label}: {np.count_nonzero(~same)} off, {got[~same][:3]} for {want[~same][:3]}"
 
 
