@@ -551,7 +551,8 @@ int qbk_head_logits_dev(qbk_ctx *ctx, const qbk_head *head, const float *hidden,
  * with a NaN or +inf, or with nothing above -inf, yields NaN (its ids are
  * still ordered).  targets and logprobs may both be NULL, entropy may be
  * NULL.  One pass over the logits; sums in f32.  workspace of at least
- * qbk_logprobs_workspace_size bytes, 16-byte aligned. */
+ * qbk_logprobs_workspace_size bytes, 16-byte aligned (0 bytes, and NULL, for
+ * rows of up to 8192 logits). */
 size_t qbk_logprobs_workspace_size(size_t rows, size_t vocab, size_t top_k);
 int qbk_logprobs_dev(qbk_ctx *ctx, const void *logits, int dtype, size_t rows, size_t vocab, size_t row_stride,
                      const int32_t *targets, float *logprobs, float *entropy, size_t top_k, int32_t *top_ids,

@@ -815,6 +815,8 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
     const size_t tp = div_ceil(prefix_len, 64), ts = div_ceil(max_len, 64);
     if (prefix_len) p.sp = splits(div_ceil(256, op), tp);
     if (max_len) p.ss = splits(os >= 256 ? div_ceil(ts, 64) : div_ceil(512, os), ts);
+    // a second launch takes longer than one more tile a wave
+    if (!prefix_len && ts <= 2 * KVA_WAVES) p.ss = 1;
     p.items = op * p.sp + os * p.ss;
     p.bytes = p.sp + p.ss > 1 ? round_up((size_t)(p.sp + p.ss) * Hk * rows * (s->head_dim * 4 + 8), 256) : 0;
     return p;

@@ -4,7 +4,7 @@
 // A row is cut into chunks of 8192 logits, a workgroup each, held in
 // registers: m = max x, l = sum exp(x - m), t = sum exp(x - m) (x - m), and the
 // chunk's top_k as 64-bit keys (value, then lower id first).  A second launch
-// joins a row's chunks:
+// joins a row's chunks (a row of one chunk is finished by the first):
 //   log p = (x - M) - log l,   entropy = log l - t / l
 // (t moves from m to M as t' = f (t + (m - M) l), f = exp(m - M)).
 //
@@ -146,6 +146,30 @@ __device__ __forceinline__ uint32_t lp_kth(uint32_t v, uint32_t k) {
     return t;
 }
 
+// The rest of a row, of its statistics (sums l and t on M), target and ordered keys; a whole workgroup.
+template <typename T>
+__device__ __forceinline__ void lp_finish(const LpArgs &a, uint32_t row, float M, float l, float t, bool in,
+                                          float target, const uint64_t *first) {
+    const float lse = logf(l), nan = __builtin_nanf("");
+    const bool ok = l > 0.0f && l < INFINITY;
+    if (threadIdx.x == 0) {
+        if (a.entropy) a.entropy[row] = ok ? lse - t / l : nan;
+        if (a.logprobs) a.logprobs[row] = ok && in ? (target - M) - lse : nan;
+    }
+    for (uint32_t i = threadIdx.x; i < a.top; i += LP_THREADS) {
+        const uint64_t k = first[i];
+        a.top_ids[(size_t)row * a.top + i] = (int32_t)~(uint32_t)k;
+        a.top_logprobs[(size_t)row * a.top + i] = ok ? (lp_unrank((uint32_t)(k >> 32)) - M) - lse : nan;
+    }
+}
+// Whether the row has a target, and its logit.
+template <typename T>
+__device__ __forceinline__ float lp_target(const LpArgs &a, uint32_t row, bool &in) {
+    const int32_t id = a.logprobs ? a.targets[row] : -1;
+    in = id >= 0 && (uint32_t)id < a.vocab;
+    return lp_in(((const T *)a.x)[(size_t)row * a.stride + (in ? id : 0)]);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
     __shared__ float red[LP_THREADS / 64];
@@ -190,8 +214,15 @@ __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
         t[j & 1] = __builtin_fmaf(e, d, t[j & 1]);
     }
     const float2 sum = lp_sum(l[0] + l[1], t[0] + t[1], red2);
-    if (tid == 0) a.part[blockIdx.x] = float4{m, sum.x, sum.y, 0.0f};
-    if (a.top == 0) return;
+    const bool whole = a.chunks == 1;  // the row is this chunk: no second launch
+    bool in = false;
+    float target = 0.0f;
+    if (whole) target = lp_target<T>(a, row, in);
+    else if (tid == 0) a.part[blockIdx.x] = float4{m, sum.x, sum.y, 0.0f};
+    if (a.top == 0) {
+        if (whole) lp_finish<T>(a, row, m, sum.x, sum.y, in, target, nullptr);
+        return;
+    }
 
     auto id = [&](int j) { return base + ((j / V) * LP_THREADS + tid) * V + j % V; };
     auto take = [&](uint64_t k) {
@@ -240,7 +271,10 @@ __global__ void __launch_bounds__(LP_THREADS) lp_chunk(LpArgs a) {
                 }
         __syncthreads();
     }
-    lp_order(cand, count, a.top, a.keys + (size_t)blockIdx.x * a.top);
+    lp_order(cand, count, a.top, whole ? best : a.keys + (size_t)blockIdx.x * a.top);
+    if (!whole) return;
+    __syncthreads();
+    lp_finish<T>(a, row, m, sum.x, sum.y, in, target, best);
 }
 
 // A workgroup a row: the chunks' statistics and keys.
@@ -266,9 +300,8 @@ __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
     uint64_t early[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) early[e] = tid + LP_THREADS * e < all ? keys[tid + LP_THREADS * e] : 0;
-    const int32_t id = a.logprobs ? a.targets[row] : -1;
-    const bool in = id >= 0 && (uint32_t)id < a.vocab;
-    const float target = lp_in(((const T *)a.x)[(size_t)row * a.stride + (in ? id : 0)]);
+    bool in;
+    const float target = lp_target<T>(a, row, in);
     float M = -INFINITY;
     for (uint32_t c = tid; c < a.chunks; c += LP_THREADS) M = fmaxf(M, part[c].x);
     M = lp_max(M, red);
@@ -284,14 +317,10 @@ __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
     const float2 sum = lp_sum(l, t, red2);
     l = sum.x;
     t = sum.y;
-    const float lse = logf(l);  // on M
-    const float nan = __builtin_nanf("");
-    const bool ok = l > 0.0f && l < INFINITY;
-    if (tid == 0) {
-        if (a.entropy) a.entropy[row] = ok ? lse - t / l : nan;
-        if (a.logprobs) a.logprobs[row] = ok && in ? (target - M) - lse : nan;
+    if (a.top == 0) {
+        lp_finish<T>(a, row, M, l, t, in, target, first);
+        return;
     }
-    if (a.top == 0) return;
     // The largest last key of a chunk's list is no more than the row's last: what lies at or above it is ordered, in
     // batches where it does not fit, the best so far among them.
 #pragma unroll
@@ -325,15 +354,11 @@ __global__ void __launch_bounds__(LP_THREADS) lp_join(LpArgs a) {
             __syncthreads();
         }
     }
-    for (uint32_t i = tid; i < a.top; i += LP_THREADS) {
-        const uint64_t k = first[i];
-        const uint32_t id = ~(uint32_t)k;
-        a.top_ids[(size_t)row * a.top + i] = (int32_t)id;
-        a.top_logprobs[(size_t)row * a.top + i] = ok ? (lp_unrank((uint32_t)(k >> 32)) - M) - lse : nan;
-    }
+    lp_finish<T>(a, row, M, l, t, in, target, first);
 }
 
 static size_t lp_bytes(size_t rows, size_t vocab, size_t top) {
+    if (vocab <= LP_CHUNK) return 0;  // a row is one chunk, done in one launch
     return round_up(rows * div_ceil(vocab, LP_CHUNK) * (sizeof(float4) + 8 * top), 256);
 }
 
@@ -372,7 +397,7 @@ int qbk_logprobs_dev(qbk_ctx *ctx, const void *logits, int dtype, size_t rows, s
     if (rows == 0) return QBK_OK;
     if (!logits) return fail(QBK_ERR_VALIDATION, "null argument");
     const size_t need = lp_bytes(rows, vocab, top_k);
-    if (!workspace || workspace_size < need)
+    if (need && (!workspace || workspace_size < need))
         return fail(QBK_ERR_VALIDATION, fmt("logprobs workspace of %zu bytes is smaller than the %zu needed",
                                             workspace ? workspace_size : (size_t)0, need));
     if ((uintptr_t)workspace & 15) return fail(QBK_ERR_VALIDATION, "logprobs workspace must be 16-byte aligned");
@@ -392,13 +417,8 @@ int qbk_logprobs_dev(qbk_ctx *ctx, const void *logits, int dtype, size_t rows, s
     a.keys = (uint64_t *)(a.part + rows * a.chunks);
     const dim3 grid((unsigned)(rows * a.chunks)), rgrid((unsigned)rows), block(LP_THREADS);
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == QBK_F32) {
-        hipLaunchKernelGGL((lp_chunk<float>), grid, block, 0, s, a);
-        hipLaunchKernelGGL((lp_join<float>), rgrid, block, 0, s, a);
-    } else {
-        hipLaunchKernelGGL((lp_chunk<uint16_t>), grid, block, 0, s, a);
-        hipLaunchKernelGGL((lp_join<uint16_t>), rgrid, block, 0, s, a);
-    }
+    hipLaunchKernelGGL(dtype == QBK_F32 ? lp_chunk<float> : lp_chunk<uint16_t>, grid, block, 0, s, a);
+    if (a.chunks > 1) hipLaunchKernelGGL(dtype == QBK_F32 ? lp_join<float> : lp_join<uint16_t>, rgrid, block, 0, s, a);
     QBK_HIP(hipGetLastError());
     return QBK_OK;
 }

@@ -273,10 +273,7 @@ def argmax_dev(ctx: GpuContext, logits, rows: int, vocab: int, out, stream=None)
 
 def logprobs_workspace_size(rows: int, vocab: int, top_k: int = 0) -> int:
     """Bytes of workspace ``logprobs_dev`` needs."""
-    need = int(_lib.load().qbk_logprobs_workspace_size(int(rows), int(vocab), int(top_k)))
-    if need == 0 and rows > 0:
-        raise _lib.KernelError(_lib.load().qbk_last_error().decode())
-    return need
+    return int(_lib.load().qbk_logprobs_workspace_size(int(rows), int(vocab), int(top_k)))
 
 
 def logprobs_dev(ctx: GpuContext, logits, rows: int, vocab: int, targets, logprobs, entropy, workspace,

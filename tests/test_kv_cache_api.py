@@ -158,11 +158,11 @@ def test_logprobs_refusals():
     _err(call(ids=None), "needs top_ids and top_logprobs")
     _err(call(tops=None), "needs top_ids and top_logprobs")
     _err(call(x=None), "null argument")
-    need = lib.qbk_logprobs_workspace_size(2, 100, 3)
-    _err(call(size=need - 1), f"smaller than the {need} needed")
-    _err(call(ws=None), "workspace of 0 bytes")
-    _err(call(ws=BUF + 8), "16-byte aligned")
+    need = lib.qbk_logprobs_workspace_size(2, 10000, 3)
+    wide = dict(vocab=10000, stride=10000)
+    _err(call(size=need - 1, **wide), f"smaller than the {need} needed")
+    _err(call(ws=None, **wide), "workspace of 0 bytes")
+    _err(call(ws=BUF + 8, **wide), "16-byte aligned")
+    assert lib.qbk_logprobs_workspace_size(2, 100, 3) == 0  # short rows need none
     _err(call(), "null qbk_ctx")
     assert call(rows=0, x=None, ws=None, size=0) == 0
-    with pytest.raises(KernelError, match="top_k must be at most 64"):
-        logprobs_workspace_size(1, 1000, 65)
