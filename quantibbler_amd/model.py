@@ -283,9 +283,21 @@ class DeviceModel:
         last position -- the logits a token-at-a-time prefill ends with.
         Returns them (a device tensor, overwritten by the next call);
         decoding continues with step() (sequence 0) or step_batch()."""
+        from .gpu import rms_norm_dev
+
+        md = self.md
+        h, n, _ = self._prefill_rows(tokens, stream, seq)
+        rms_norm_dev(self.ctx, h[n - 1], 1, md.d_model, self.final_norm, md.rms_norm_eps, self.hn, stream,
+                     self.serving)
+        self.head.logits_dev(self.hn, 1, self.logits, stream)
+        return self.logits
+
+    def _prefill_rows(self, tokens, stream, seq):
+        """A new sequence's tokens through every block: the rows that leave
+        the last one, their number, and the workspace (kept while it is read)."""
         import torch
 
-        from .gpu import embed, rms_norm_dev
+        from .gpu import embed
 
         md = self.md
         ids = [int(t) for t in tokens]
@@ -296,13 +308,49 @@ class DeviceModel:
         ws = torch.empty(need, dtype=torch.uint8, device="cuda")
         for b in self.blocks:
             b.prefill_seq_dev(int(seq), h, n, ws, need, stream)
-        rms_norm_dev(self.ctx, h[n - 1], 1, md.d_model, self.final_norm, md.rms_norm_eps, self.hn, stream,
-                     self.serving)
-        self.head.logits_dev(self.hn, 1, self.logits, stream)
         self.positions[int(seq)] = n
         if int(seq) == 0:
             self.pos = n
-        return self.logits
+        return h, n, ws
+
+    SCORE_ROWS = 256  # rows of logits held at a time
+
+    def score(self, tokens, stream=None, seq: int = 0, top_k: int = 0):
+        """How likely each token of a new sequence is after those before it
+        (held as sequence ``seq``, as prefill leaves it): device tensors
+        logprobs and entropy [len(tokens) - 1], in nats, row i of token
+        i + 1, and with top_k the likeliest tokens there, ids and log
+        probabilities [len(tokens) - 1][top_k].  The mean of -logprobs is
+        the log of the sequence's perplexity.  Returns once they are written."""
+        import torch
+
+        from .gpu import logprobs_dev, logprobs_workspace_size, rms_norm_dev
+
+        md, k = self.md, int(top_k)
+        ids = [int(t) for t in tokens]
+        if len(ids) < 2:
+            raise ValueError(f"a score needs at least two tokens, got {len(ids)}")
+        h, n, ws = self._prefill_rows(ids, stream, seq)
+        targets = torch.tensor(ids[1:], dtype=torch.int32, device="cuda")
+        torch.cuda.current_stream().synchronize()  # the targets are there, whatever stream reads them
+        step = min(n - 1, self.SCORE_ROWS)
+        hn = torch.empty((step, md.d_model), dtype=torch.float32, device="cuda")
+        logits = torch.empty((step, md.vocab_size), dtype=torch.float32, device="cuda")
+        logp, ent = (torch.empty(n - 1, dtype=torch.float32, device="cuda") for _ in range(2))
+        top_ids = torch.empty((n - 1, k), dtype=torch.int32, device="cuda") if k else None
+        tops = torch.empty((n - 1, k), dtype=torch.float32, device="cuda") if k else None
+        need = logprobs_workspace_size(step, md.vocab_size, k)
+        lws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+        for r in range(0, n - 1, step):
+            m = min(step, n - 1 - r)
+            rms_norm_dev(self.ctx, h[r:r + m], m, md.d_model, self.final_norm, md.rms_norm_eps, hn, stream,
+                         self.serving)
+            self.head.logits_dev(hn, m, logits, stream)
+            logprobs_dev(self.ctx, logits, m, md.vocab_size, targets[r:r + m], logp[r:r + m], ent[r:r + m], lws, need,
+                         top_k=k, top_ids=top_ids[r:r + m] if k else None, top_logprobs=tops[r:r + m] if k else None,
+                         stream=stream)
+        torch.cuda.synchronize()  # what was allocated here is free again for any stream
+        return (logp, ent, top_ids, tops) if k else (logp, ent)
 
     def step_batch(self, tokens, stream=None):
         """One position of each of sequences 0 .. n - 1 (the batched decode of
