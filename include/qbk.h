@@ -537,6 +537,27 @@ int qbk_head_logits(qbk_ctx *ctx, const qbk_head *head, const float *hidden, siz
 int qbk_head_logits_dev(qbk_ctx *ctx, const qbk_head *head, const float *hidden, size_t batch, float *logits,
                         void *stream);
 
+/* One decode position of n sequences (1 .. 64) through a block whose rows
+ * stand in an 8-bit cache in place of the block's own f32 cache (which, with
+ * its attention state, is left as it is): the batched step of
+ * qbk_block_decode_batch_dev with its attention over `cache` behind the
+ * shared prefix.  h f32 [n][d_model], replaced by the block's outputs; pos:
+ * device uint32, read when the step runs, the own rows that sequence
+ * first_seq + i holds before the step (its new row's place in the cache); the
+ * token's position is prefix_len + pos[i], which RoPE turns by, so prefix_len
+ * + max_len is at most the block's capacity.  max_len: a host bound on pos[i]
+ * + 1, at most the cache's capacity; a step at a position past it has no
+ * meaning (and writes nothing past the capacity).  bf16 serving, either
+ * attention face setting.  pos is advanced by the caller
+ * (qbk_positions_advance_dev) once every block has made the step; a captured
+ * step serves every later position. */
+size_t qbk_block_decode_kv_workspace_size(const qbk_block *block, const qbk_kv_shape *shape, size_t n,
+                                          size_t max_len, size_t prefix_len);
+int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *block, float *h, const uint32_t *pos, size_t n,
+                            const qbk_kv_shape *shape, void *cache, size_t first_seq, size_t max_len,
+                            const qbk_kv_shape *prefix_shape, const void *prefix, size_t prefix_seq,
+                            size_t prefix_len, void *workspace, size_t workspace_size, void *stream);
+
 /* ---- log probabilities ------------------------------------------------------ */
 
 /* What the API's logprobs report and a perplexity sums (no counterpart in the

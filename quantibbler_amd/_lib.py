@@ -121,6 +121,9 @@ _SIGS = {
     "qbk_attention_kv_workspace_size": (_Z, [C.POINTER(KvShape), _Z, _Z, _Z, _Z, _Z]),
     "qbk_attention_kv_dev": (_I, [_P, C.POINTER(KvShape), _P, _Z, _Z, _P, _Z, C.POINTER(KvShape), _P, _Z, _Z, _Z,
                                   _Z, _P, _I, _P, _P, _Z, _P]),
+    "qbk_block_decode_kv_workspace_size": (_Z, [_P, C.POINTER(KvShape), _Z, _Z, _Z]),
+    "qbk_block_decode_kv_dev": (_I, [_P, _P, _P, _P, _Z, C.POINTER(KvShape), _P, _Z, _Z, C.POINTER(KvShape), _P, _Z,
+                                     _Z, _P, _Z, _P]),
     "qbk_logprobs_workspace_size": (_Z, [_Z, _Z, _Z]),
     "qbk_logprobs_dev": (_I, [_P, _P, _I, _Z, _Z, _Z, _P, _P, _P, _Z, _P, _P, _P, _Z, _P]),
     "qbk_sage_blk_workspace_size": (_Z, [C.POINTER(AttnShape)]),

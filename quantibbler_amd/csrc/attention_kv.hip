@@ -64,6 +64,7 @@ struct KvAttArgs {
     float *po;    // [split][hk][rho][hd] weighted values
     float2 *ml;   // [split][hk][rho] reference, sum of weights
     uint32_t first_seq, prefix_seq, prefix_len, max_len;
+    uint32_t plus;                   // 1: lens are positions, the rows before the one just written
     uint32_t n, sq, H, G, rows;      // rows = n sq G
     uint32_t sp, ss, rtp, rts;       // splits and row tiles of prefix and own items
     uint32_t n_pre;                  // prefix items
@@ -75,7 +76,7 @@ struct KvAttArgs {
 // at least one a wave, so that short sequences use few splits.
 __device__ __forceinline__ uint32_t kva_len(const KvAttArgs &a, uint32_t b) {
     const uint32_t l = a.lens[b];
-    return l < a.max_len ? l : a.max_len;
+    return l < a.max_len ? l + a.plus : a.max_len;
 }
 __device__ __forceinline__ uint32_t kva_run(const KvAttArgs &a, uint32_t len) {
     uint32_t rest;
@@ -877,22 +878,12 @@ static int kva_check(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq,
     return QBK_OK;
 }
 
-}  // namespace qbk
-
-using namespace qbk;
-
-extern "C" {
-
-size_t qbk_attention_kv_workspace_size(const qbk_kv_shape *shape, size_t n_heads, size_t n, size_t seq_q,
-                                       size_t max_len, size_t prefix_len) {
-    if (kva_check(shape, n_heads, n, seq_q, max_len, prefix_len) || n == 0) return 0;
-    return kva_plan(shape, n_heads, n, seq_q, max_len, prefix_len).bytes;
-}
-
-int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, size_t first_seq, size_t n,
-                         const uint32_t *lens, size_t max_len, const qbk_kv_shape *prefix_shape,
-                         const void *prefix, size_t prefix_seq, size_t prefix_len, size_t n_heads, size_t seq_q,
-                         const void *q, int dtype, void *out, void *workspace, size_t workspace_size, void *stream) {
+// qbk_attention_kv_dev; plus 1: lens[i] counts the rows before the queries'
+// last one.
+int attention_kv_run(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, size_t first_seq, size_t n,
+                     const uint32_t *lens, uint32_t plus, size_t max_len, const qbk_kv_shape *prefix_shape,
+                     const void *prefix, size_t prefix_seq, size_t prefix_len, size_t n_heads, size_t seq_q,
+                     const void *q, int dtype, void *out, void *workspace, size_t workspace_size, void *stream) {
     int rc;
     if ((rc = kva_check(shape, n_heads, n, seq_q, max_len, prefix_len))) return rc;
     if (dtype != QBK_F32 && dtype != QBK_BF16)
@@ -934,6 +925,7 @@ int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *ca
     a.prefix_seq = (uint32_t)prefix_seq;
     a.prefix_len = (uint32_t)prefix_len;
     a.max_len = (uint32_t)max_len;
+    a.plus = plus;
     a.n = (uint32_t)n;
     a.sq = (uint32_t)seq_q;
     a.H = (uint32_t)n_heads;
@@ -977,6 +969,26 @@ int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *ca
     hipLaunchKernelGGL(join, grid, dim3(256), 0, st, a);
     QBK_HIP(hipGetLastError());
     return QBK_OK;
+}
+
+}  // namespace qbk
+
+using namespace qbk;
+
+extern "C" {
+
+size_t qbk_attention_kv_workspace_size(const qbk_kv_shape *shape, size_t n_heads, size_t n, size_t seq_q,
+                                       size_t max_len, size_t prefix_len) {
+    if (kva_check(shape, n_heads, n, seq_q, max_len, prefix_len) || n == 0) return 0;
+    return kva_plan(shape, n_heads, n, seq_q, max_len, prefix_len).bytes;
+}
+
+int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, size_t first_seq, size_t n,
+                         const uint32_t *lens, size_t max_len, const qbk_kv_shape *prefix_shape,
+                         const void *prefix, size_t prefix_seq, size_t prefix_len, size_t n_heads, size_t seq_q,
+                         const void *q, int dtype, void *out, void *workspace, size_t workspace_size, void *stream) {
+    return attention_kv_run(ctx, shape, cache, first_seq, n, lens, 0, max_len, prefix_shape, prefix, prefix_seq,
+                            prefix_len, n_heads, seq_q, q, dtype, out, workspace, workspace_size, stream);
 }
 
 }  // extern "C"

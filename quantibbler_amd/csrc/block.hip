@@ -758,6 +758,26 @@ __global__ void __launch_bounds__(64) blkb_qk_rope(const float *q, const float *
     }
 }
 
+// The same for a step over an 8-bit cache: row t at position before + pos[t],
+// q to qr [n][H hd], k to kr [n][Hk hd] (the cache takes k from there and v
+// from the projection); zeros past the block's positions.
+__global__ void __launch_bounds__(64) blkb_qk_rope_rows(const float *q, const float *k, const float2 *rope,
+                                                        const uint32_t *pos, uint32_t before, size_t cap,
+                                                        const float *wq, const float *wk, float eps, float *qr,
+                                                        float *kr, int H, int Hk, int hd) {
+    const int head = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
+    const size_t p = (size_t)pos[t] + before;
+    const bool is_q = head < H;
+    const size_t at = is_q ? ((size_t)t * H + head) * hd : ((size_t)t * Hk + head - H) * hd;
+    float *dst = (is_q ? qr : kr) + at;
+    if (p >= cap) {
+        for (int j = lane; j < hd; j += 64) dst[j] = 0.0f;
+        return;
+    }
+    rope_head((is_q ? q : k) + at, is_q ? wq : wk, eps, rope + p * (size_t)(hd / 2), hd, lane,
+              [&](int j, float x) { dst[j] = x; });
+}
+
 // Up to Q4_MAXB sequences the projections run on the fp4 decode GEMV, q/k/v
 // and gate/up as the block's layer sets (one launch per stage for each set,
 // x written once per layer of the set); beyond, layer by layer on the
@@ -1328,17 +1348,37 @@ size_t qbk_block_decode_batch_workspace_size(const qbk_block *B, size_t n) {
 // attention stepping every sequence's kept state.
 }  // extern "C"
 
+// A batched step over an 8-bit cache in place of the block's own (qbk.h,
+// qbk_block_decode_kv_dev).
+struct BlkKv {
+    const qbk_kv_shape *shape, *prefix_shape;
+    void *cache;
+    const void *prefix;
+    size_t first_seq, max_len, prefix_seq, prefix_len;
+};
+// Its workspace: the batched step's, the rotated keys, the attention's.
+static size_t blkkv_workspace(const qbk_block *B, const qbk_kv_shape *shape, size_t n, size_t max_len,
+                              size_t prefix_len, size_t *o_kr, size_t *o_att, size_t *att) {
+    *o_kr = blkb_plan(B, n).bytes;
+    *o_att = *o_kr + round_up(n * B->Hk * B->hd * 4, 256);
+    *att = qbk_attention_kv_workspace_size(shape, B->H, n, 1, max_len, prefix_len);
+    return *o_att + *att;
+}
+
 // With pos_dev (device, n entries) in place of pos: each sequence at the
 // position its word holds when the step runs; the host record of cached
-// positions is then left to the caller.
+// positions is then left to the caller.  With kv (pos_dev given): rows and
+// attention on that cache.
 static int block_decode_batch(qbk_ctx *ctx, qbk_block *B, float *h, const size_t *pos, const uint32_t *pos_dev,
-                              size_t n, void *workspace, size_t workspace_size, void *stream) {
+                              size_t n, void *workspace, size_t workspace_size, void *stream,
+                              const BlkKv *kv = nullptr) {
     int rc;
     if (!B || !h || (!pos && !pos_dev)) return fail(QBK_ERR_VALIDATION, "null argument");
-    if (B->face == QBK_ATTN_EXACT) return fail(QBK_ERR_VALIDATION, kExactFaceOnly);
+    if (B->face == QBK_ATTN_EXACT && !kv) return fail(QBK_ERR_VALIDATION, kExactFaceOnly);
     if (B->serving == QBK_F32) return fail(QBK_ERR_VALIDATION, kF32Only);
-    if (n == 0 || n > B->nseq)
-        return fail(QBK_ERR_VALIDATION, fmt("batch of %zu sequences on a block holding %zu", n, B->nseq));
+    if (n == 0 || n > (kv ? BLKB_MAXSEQ : B->nseq))
+        return fail(QBK_ERR_VALIDATION, kv ? fmt("a step over a kv cache takes 1 .. %d sequences, got %zu", BLKB_MAXSEQ, n)
+                                           : fmt("batch of %zu sequences on a block holding %zu", n, B->nseq));
     for (size_t i = 0; !pos_dev && i < n; i++) {
         if (pos[i] >= B->cap)
             return fail(QBK_ERR_VALIDATION,
@@ -1348,9 +1388,11 @@ static int block_decode_batch(qbk_ctx *ctx, qbk_block *B, float *h, const size_t
                                                 "positions", i, pos[i], B->filled[i]));
     }
     const BlkbPlan P = blkb_plan(B, n);
-    if (!workspace || workspace_size < P.bytes)
+    size_t o_kr = 0, o_att = 0, att = 0;
+    const size_t need = kv ? blkkv_workspace(B, kv->shape, n, kv->max_len, kv->prefix_len, &o_kr, &o_att, &att) : P.bytes;
+    if (!workspace || workspace_size < need)
         return fail(QBK_ERR_VALIDATION,
-                    fmt("workspace of %zu bytes is smaller than the %zu this step needs", workspace_size, P.bytes));
+                    fmt("workspace of %zu bytes is smaller than the %zu this step needs", workspace_size, need));
     if ((rc = bind(ctx))) return rc;
     if (B->device != ctx->device) return fail(QBK_ERR_VALIDATION, "block lives on another device than the context");
     hipStream_t s = (hipStream_t)stream;
@@ -1390,36 +1432,49 @@ static int block_decode_batch(qbk_ctx *ctx, qbk_block *B, float *h, const size_t
     }
     BlkbPos bp{};
     for (size_t i = 0; !pos_dev && i < n; i++) bp.p[i] = (uint32_t)pos[i];
-    hipLaunchKernelGGL(blkb_qk_rope, dim3(H + Hk, (unsigned)n), dim3(64), 0, s, q, k, v, B->rope, bp, pos_dev,
-                       B->cap, B->w_q, B->w_k, B->eps, B->kc, B->vc, kvs, qr, H, Hk, hd);
-    QBK_HIP(hipGetLastError());
-    const qbk_attn_shape one{1, B->H, B->Hk, 1, B->cap, B->hd, B->hd};
-    const size_t qs = B->H * B->hd;
-    if (pos_dev) {
-        if ((rc = sage_decode_batch(&one, qr, qs, B->kc, B->vc, kvs, B->block, at, qs, B->state, B->state_bytes,
-                                    B->cap, nullptr, nullptr, n, s, pos_dev)))
-            return rc;
-    } else if (sage_decode_batchable(&one, B->block, B->cap, B->kc, B->vc, kvs)) {
-        size_t skv[BLKB_MAXSEQ], kept[BLKB_MAXSEQ];
-        for (size_t i = 0; i < n; i++) {
-            skv[i] = pos[i] + 1;
-            kept[i] = B->tokens[i] <= pos[i] ? B->tokens[i] : 0;
-        }
-        if ((rc = sage_decode_batch(&one, qr, qs, B->kc, B->vc, kvs, B->block, at, qs, B->state, B->state_bytes,
-                                    B->cap, skv, kept, n, s)))
+    if (kv) {
+        float *kr = (float *)(w + o_kr);
+        hipLaunchKernelGGL(blkb_qk_rope_rows, dim3(H + Hk, (unsigned)n), dim3(64), 0, s, q, k, B->rope, pos_dev,
+                           (uint32_t)kv->prefix_len, B->cap, B->w_q, B->w_k, B->eps, qr, kr, H, Hk, hd);
+        QBK_HIP(hipGetLastError());
+        if ((rc = qbk_kv_cache_write_dev(ctx, kv->shape, kv->cache, kr, v, QBK_F32, kd, n, nullptr, pos_dev,
+                                         kv->first_seq, n, stream)) ||
+            (rc = attention_kv_run(ctx, kv->shape, kv->cache, kv->first_seq, n, pos_dev, 1, kv->max_len,
+                                   kv->prefix_shape, kv->prefix, kv->prefix_seq, kv->prefix_len, B->H, 1, qr, QBK_F32,
+                                   at, w + o_att, att, stream)))
             return rc;
     } else {
-        for (size_t i = 0; i < n; i++) {
-            const qbk_attn_shape sh{1, B->H, B->Hk, 1, pos[i] + 1, B->hd, B->hd};
-            const size_t cached = B->tokens[i] <= pos[i] ? B->tokens[i] : 0;
-            if ((rc = qbk_attention_sage_decode_step_dev(ctx, &sh, qr + i * qs, B->kc + i * kvs, B->vc + i * kvs,
-                                                         B->block, at + i * qs,
-                                                         (char *)B->state + i * B->state_bytes, B->state_bytes,
-                                                         B->cap, cached, stream)))
+        hipLaunchKernelGGL(blkb_qk_rope, dim3(H + Hk, (unsigned)n), dim3(64), 0, s, q, k, v, B->rope, bp, pos_dev,
+                           B->cap, B->w_q, B->w_k, B->eps, B->kc, B->vc, kvs, qr, H, Hk, hd);
+        QBK_HIP(hipGetLastError());
+        const qbk_attn_shape one{1, B->H, B->Hk, 1, B->cap, B->hd, B->hd};
+        const size_t qs = B->H * B->hd;
+        if (pos_dev) {
+            if ((rc = sage_decode_batch(&one, qr, qs, B->kc, B->vc, kvs, B->block, at, qs, B->state, B->state_bytes,
+                                        B->cap, nullptr, nullptr, n, s, pos_dev)))
                 return rc;
+        } else if (sage_decode_batchable(&one, B->block, B->cap, B->kc, B->vc, kvs)) {
+            size_t skv[BLKB_MAXSEQ], kept[BLKB_MAXSEQ];
+            for (size_t i = 0; i < n; i++) {
+                skv[i] = pos[i] + 1;
+                kept[i] = B->tokens[i] <= pos[i] ? B->tokens[i] : 0;
+            }
+            if ((rc = sage_decode_batch(&one, qr, qs, B->kc, B->vc, kvs, B->block, at, qs, B->state, B->state_bytes,
+                                        B->cap, skv, kept, n, s)))
+                return rc;
+        } else {
+            for (size_t i = 0; i < n; i++) {
+                const qbk_attn_shape sh{1, B->H, B->Hk, 1, pos[i] + 1, B->hd, B->hd};
+                const size_t cached = B->tokens[i] <= pos[i] ? B->tokens[i] : 0;
+                if ((rc = qbk_attention_sage_decode_step_dev(ctx, &sh, qr + i * qs, B->kc + i * kvs, B->vc + i * kvs,
+                                                             B->block, at + i * qs,
+                                                             (char *)B->state + i * B->state_bytes, B->state_bytes,
+                                                             B->cap, cached, stream)))
+                    return rc;
+            }
         }
+        for (size_t i = 0; !pos_dev && i < n; i++) B->tokens[i] = B->filled[i] = pos[i] + 1;
     }
-    for (size_t i = 0; !pos_dev && i < n; i++) B->tokens[i] = B->filled[i] = pos[i] + 1;
     if ((rc = P.sets ? q4_run(B->o, n, at, true, oo, false, ws, s) : blkp_proj(B->o, n, at, true, oo, ws, s)))
         return rc;
     const bool gu_op = fits && q4_set_flat_operand_batch(B->gu, n, ws, &op, &sc, &s2c);
@@ -1477,6 +1532,45 @@ int qbk_block_decode_batch_pos_dev(qbk_ctx *ctx, qbk_block *B, float *h, const u
                                             "to 64 tokens)");
     }
     return block_decode_batch(ctx, B, h, nullptr, pos, n, workspace, workspace_size, stream);
+}
+
+size_t qbk_block_decode_kv_workspace_size(const qbk_block *B, const qbk_kv_shape *shape, size_t n, size_t max_len,
+                                          size_t prefix_len) {
+    if (!B || n == 0 || n > BLKB_MAXSEQ || !shape || qbk_kv_cache_size(shape) == 0) return 0;
+    size_t o_kr, o_att, att;
+    return blkkv_workspace(B, shape, n, max_len, prefix_len, &o_kr, &o_att, &att);
+}
+
+int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *B, float *h, const uint32_t *pos, size_t n,
+                            const qbk_kv_shape *shape, void *cache, size_t first_seq, size_t max_len,
+                            const qbk_kv_shape *prefix_shape, const void *prefix, size_t prefix_seq, size_t prefix_len,
+                            void *workspace, size_t workspace_size, void *stream) {
+    if (!B || !h || !pos || !shape || !cache || (prefix_len && (!prefix_shape || !prefix)))
+        return fail(QBK_ERR_VALIDATION, "null argument");
+    if (qbk_kv_cache_size(shape) == 0) return QBK_ERR_VALIDATION;
+    if (shape->n_kv_heads != B->Hk || shape->head_dim != B->hd)
+        return fail(QBK_ERR_VALIDATION, fmt("a kv cache of %zu heads of %zu for a block of %zu heads of %zu",
+                                            shape->n_kv_heads, shape->head_dim, B->Hk, B->hd));
+    if (max_len == 0 || max_len > shape->capacity)
+        return fail(QBK_ERR_VALIDATION,
+                    fmt("max_len %zu is not within the kv cache's capacity of %zu", max_len, shape->capacity));
+    if (prefix_len > B->cap || max_len > B->cap - prefix_len)
+        return fail(QBK_ERR_VALIDATION, fmt("a prefix of %zu rows and %zu own positions exceed the block's capacity of "
+                                            "%zu positions", prefix_len, max_len, B->cap));
+    if (prefix_len) {  // before anything is launched: what the attention would refuse
+        if (qbk_kv_cache_size(prefix_shape) == 0) return QBK_ERR_VALIDATION;
+        if (prefix_shape->format != shape->format || prefix_shape->n_kv_heads != shape->n_kv_heads ||
+            prefix_shape->head_dim != shape->head_dim || prefix_seq >= prefix_shape->n_seqs ||
+            prefix_len > prefix_shape->capacity)
+            return fail(QBK_ERR_VALIDATION, "the prefix does not fit its cache, or its cache the sequences'");
+    }
+    if (first_seq > shape->n_seqs || n > shape->n_seqs - first_seq)
+        return fail(QBK_ERR_VALIDATION, fmt("sequences %zu .. %zu of a kv cache holding %zu", first_seq, first_seq + n,
+                                            shape->n_seqs));
+    if (((uintptr_t)cache | (uintptr_t)(prefix_len ? prefix : nullptr) | (uintptr_t)workspace) & 15)
+        return fail(QBK_ERR_VALIDATION, "kv cache buffers and the workspace must be 16-byte aligned");
+    const BlkKv kv{shape, prefix_shape, cache, prefix, first_seq, max_len, prefix_seq, prefix_len};
+    return block_decode_batch(ctx, B, h, nullptr, pos, n, workspace, workspace_size, stream, &kv);
 }
 
 }  // extern "C"

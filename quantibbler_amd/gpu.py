@@ -560,6 +560,33 @@ class DecoderBlock:
         check(_lib.load().qbk_block_decode_batch_pos_dev(self.ctx.handle, self._h, _ptr(h), _ptr(pos), int(n),
                                                          _ptr(workspace), int(workspace_size), _stream(stream)))
 
+    def decode_kv_workspace_size(self, cache: KvCache, n: int, max_len: int | None = None, prefix_len: int = 0) -> int:
+        most = cache.capacity if max_len is None else max_len
+        if min(n, most, prefix_len) < 0:
+            raise _lib.KernelError("kv decode sizes must not be negative")
+        return int(_lib.load().qbk_block_decode_kv_workspace_size(self._h, cache._shape_ref, n, most, prefix_len))
+
+    def decode_kv_dev(self, h, pos, n: int, cache: KvCache, workspace, workspace_size: int, first_seq: int = 0,
+                      max_len: int | None = None, prefix: KvCache | None = None, prefix_seq: int = 0,
+                      prefix_len: int = 0, stream=None):
+        """decode_batch_pos_dev with the rows in an 8-bit ``cache`` (which the
+        caller keeps) in place of the block's own: h device f32 [n][d_model];
+        pos device uint32, sequence first_seq + i's own rows before the step,
+        its token standing at position prefix_len + pos[i] behind rows 0 ..
+        prefix_len - 1 of ``prefix``'s sequence ``prefix_seq``, shared by
+        all.  ``pos`` is left for the caller to advance."""
+        self._check_rows(h, int(n), "batched decode input")
+        most = cache.capacity if max_len is None else max_len
+        if min(n, most, first_seq, prefix_seq, prefix_len) < 0:
+            raise _lib.KernelError("kv decode sizes must not be negative")
+        if prefix_len and prefix is None:
+            raise _lib.KernelError("a prefix_len needs the cache that holds the prefix")
+        words = _device_words(pos, n, "positions")
+        shared, base = (prefix._shape_ref, prefix._base) if prefix_len else (None, None)
+        check(_lib.load().qbk_block_decode_kv_dev(
+            self.ctx.handle, self._h, _ptr(h), words, n, cache._shape_ref, cache._base, first_seq, most, shared, base,
+            prefix_seq, prefix_len, _ptr(workspace), int(workspace_size), _stream(stream)))
+
     def set_positions(self, positions):
         """The host record after device-position steps: sequence i holds
         positions[i] positions, its attention state stepped through them."""

@@ -267,6 +267,7 @@ class DeviceModel:
         self.logits = torch.empty(md.vocab_size, dtype=torch.float32, device=dev)
         self.pos = 0                        # sequence 0's, the one step() serves
         self.positions = [0] * self.n_seqs  # every sequence's
+        self._shared = None                 # share_prefix's caches and buffers
         self._batch = {}                    # n -> (h, hn, logits, workspace) of step_batch
 
     def reset(self):
@@ -274,6 +275,7 @@ class DeviceModel:
             b.reset()
         self.pos = 0
         self.positions = [0] * self.n_seqs
+        self._shared = None
 
     def prefill(self, tokens, stream=None, seq: int = 0):
         """forward_prefill (engine/mod.rs:811-822) of a new sequence (held as
@@ -387,6 +389,75 @@ class DeviceModel:
             self.positions[i] += 1
         self.pos = self.positions[0]
         return logits
+
+    def share_prefix(self, tokens, n_seqs: int, capacity: int, fmt: str = "int8", stream=None):
+        """Serves ``n_seqs`` (up to 64) requests behind one prompt: the tokens
+        are prefilled once (as sequence 0), their cache rows quantised into an
+        8-bit cache per block, and every request gets room for ``capacity``
+        rows of its own there; step_shared() then steps them together, each
+        block reading the prompt's rows once for all of them.  bf16 serving;
+        prompt and capacity together within the model's capacity.  Returns the
+        prompt's last logits, as prefill."""
+        import torch
+
+        from .gpu import KvCache
+
+        md, n, kd = self.md, len(tokens), self.md.n_kv_heads * self.md.head_dim
+        if self.serving != "bf16":
+            raise ValueError("a shared prefix is served in bf16")
+        if not 1 <= int(n_seqs) <= 64 or n + int(capacity) > self.capacity:
+            raise ValueError(f"{n_seqs} requests of {capacity} rows behind {n} on a model of {self.capacity} positions")
+        logits = self.prefill(tokens, stream)
+
+        def cache(seqs, rows):
+            need = KvCache.size(fmt, seqs, rows, md.n_kv_heads, md.head_dim)
+            return KvCache(self.ctx, fmt, seqs, rows, md.n_kv_heads, md.head_dim,
+                           torch.empty(need, dtype=torch.uint8, device="cuda"))
+
+        pos = torch.zeros(int(n_seqs), dtype=torch.int32, device="cuda")
+        torch.cuda.current_stream().synchronize()  # the positions are there, whatever stream reads them
+        prefixes, caches = [], []
+        for b in self.blocks:
+            k, v = b.cache_ptrs()
+            prefixes.append(cache(1, n))
+            prefixes[-1].write_dev(k, v, "float32", pos, n, row_stride=kd, stream=stream)
+            caches.append(cache(int(n_seqs), int(capacity)))
+        need = max(b.decode_kv_workspace_size(c, int(n_seqs), prefix_len=n) for b, c in zip(self.blocks, caches))
+        d = md.d_model
+        self._shared = {"n": int(n_seqs), "prefix": prefixes, "len": n, "own": caches, "pos": pos, "steps": 0,
+                        "h": torch.empty((int(n_seqs), d), dtype=torch.float32, device="cuda"),
+                        "hn": torch.empty((int(n_seqs), d), dtype=torch.float32, device="cuda"),
+                        "logits": torch.empty((int(n_seqs), md.vocab_size), dtype=torch.float32, device="cuda"),
+                        "ws": torch.empty(need, dtype=torch.uint8, device="cuda"), "need": need}
+        return logits
+
+    def step_shared(self, tokens, stream=None):
+        """The next position of every request of share_prefix(): ``tokens`` as
+        step_batch's, one a request.  Returns the logits [n][vocab] (a device
+        tensor, overwritten by the next call)."""
+        from .gpu import advance_positions_dev, embed, embed_dev, rms_norm_dev
+
+        md, s = self.md, self._shared
+        if s is None:
+            raise ValueError("step_shared needs share_prefix first")
+        dev_ids = hasattr(tokens, "is_cuda")
+        n = int(tokens.numel()) if dev_ids else len(tokens)
+        if n != s["n"]:
+            raise ValueError(f"{n} tokens for {s['n']} requests")
+        if s["steps"] >= s["own"][0].capacity:
+            raise ValueError(f"the requests hold their {s['steps']} rows already")
+        if dev_ids:
+            embed_dev(self.ctx, self.embedding, md.vocab_size, md.d_model, tokens, n, s["h"], stream)
+        else:
+            embed(self.ctx, self.embedding, md.vocab_size, md.d_model, [int(t) for t in tokens], s["h"], stream)
+        for b, own, prefix in zip(self.blocks, s["own"], s["prefix"]):
+            b.decode_kv_dev(s["h"], s["pos"], n, own, s["ws"], s["need"], prefix=prefix, prefix_len=s["len"],
+                            stream=stream)
+        advance_positions_dev(self.ctx, s["pos"], n, stream)
+        rms_norm_dev(self.ctx, s["h"], n, md.d_model, self.final_norm, md.rms_norm_eps, s["hn"], stream)
+        self.head.logits_dev(s["hn"], n, s["logits"], stream)
+        s["steps"] += 1
+        return s["logits"]
 
     def step(self, token: int, stream=None):
         """The next position's logits (a device tensor, overwritten by the

@@ -236,6 +236,13 @@ extern "C" {
                                 prefix: *const c_void, prefix_seq: usize, prefix_len: usize, n_heads: usize,
                                 seq_q: usize, q: *const c_void, dtype: c_int, out: *mut c_void,
                                 workspace: *mut c_void, workspace_size: usize, stream: *mut c_void) -> c_int;
+    pub fn qbk_block_decode_kv_workspace_size(block: *const QbkBlock, shape: *const KvShape, n: usize,
+                                              max_len: usize, prefix_len: usize) -> usize;
+    pub fn qbk_block_decode_kv_dev(ctx: *mut QbkCtx, block: *mut QbkBlock, h: *mut f32, pos: *const u32, n: usize,
+                                   shape: *const KvShape, cache: *mut c_void, first_seq: usize, max_len: usize,
+                                   prefix_shape: *const KvShape, prefix: *const c_void, prefix_seq: usize,
+                                   prefix_len: usize, workspace: *mut c_void, workspace_size: usize,
+                                   stream: *mut c_void) -> c_int;
     pub fn qbk_logprobs_workspace_size(rows: usize, vocab: usize, top_k: usize) -> usize;
     pub fn qbk_logprobs_dev(ctx: *mut QbkCtx, logits: *const c_void, dtype: c_int, rows: usize, vocab: usize,
                             row_stride: usize, targets: *const i32, logprobs: *mut f32, entropy: *mut f32,
