@@ -272,19 +272,28 @@ __device__ __forceinline__ void kva_value_scales(float vm, float &vref, float &v
     }
 }
 
-// One query tile's scores (16 keys a lane: 16 i + j past key) to weights: the
-// reference moves when a score passes it eightfold, sum and outputs with it;
-// p times the value scales as operands ph (and pl, the halves' rests).
-template <bool MASKED, int CT, bool HI>
-__device__ __forceinline__ void kva_softmax(const kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float cq, uint32_t key,
-                                            uint32_t lim, float &ref, float &sum, kva_f4_t (&o)[CT],
-                                            kva_h8_t (&ph)[2], kva_h8_t (&pl)[2]) {
-    auto out = [&](int i, int j) { return MASKED && key + 16 * i + j >= lim; };
-    float tm = -INFINITY;
+// Scores t and value scales vs of a lane's 16 keys (16 i + j past key) that its
+// row does not see: no score and no scale, whatever the cache holds there.
+__device__ __forceinline__ void kva_mask(kva_f4_t (&t)[4], kva_f4_t (&vs)[4], uint32_t key, uint32_t lim) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) tm = fmaxf(tm, out(i, j) ? -INFINITY : t[i][j]);
+        for (int j = 0; j < 4; j++) {
+            const bool out = key + 16 * i + j >= lim;
+            t[i][j] = out ? -INFINITY : t[i][j];
+            vs[i][j] = out ? 0.0f : vs[i][j];
+        }
+}
+
+// The row's reference moves when a score passes it eightfold, its sum and
+// outputs with it.
+template <int CT>
+__device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float cq, float &ref, float &sum,
+                                              kva_f4_t (&o)[CT]) {
+    float m[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) m[i] = fmaxf(fmaxf(t[i][0], t[i][1]), fmaxf(t[i][2], t[i][3]));
+    const float tm = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     if (__ballot(tm * cq > ref + 3.0f)) {
         const float to = fmaxf(ref, ceilf(kva_max4(tm) * cq));
         const float f = kva_rescale(ref, to);
@@ -293,7 +302,15 @@ __device__ __forceinline__ void kva_softmax(const kva_f4_t (&t)[4], const kva_f4
         for (int ct = 0; ct < CT; ct++) o[ct] *= f;
         ref = to;
     }
-    float l = 0.0f;
+}
+
+// Scores to weights: p = exp2(t cq - ref) into sum, p times the value scales
+// as operands ph (and pl, what the first half leaves).
+template <bool HI>
+__device__ __forceinline__ void kva_weights(const kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float cq, float ref,
+                                            float &sum, kva_h8_t (&ph)[2], kva_h8_t (&pl)[2]) {
+    const float base = ref == -INFINITY ? 0.0f : ref;  // a row that has seen nothing: every p is 0
+    float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -301,9 +318,9 @@ __device__ __forceinline__ void kva_softmax(const kva_f4_t (&t)[4], const kva_f4
             kva_f2_t w;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j + e], cq, -ref));
-                l += out(i, j + e) ? 0.0f : p;
-                w[e] = out(i, j + e) ? 0.0f : p * vs[i][j + e];  // whatever the scale holds
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j + e], cq, -base));
+                l[i] += p;
+                w[e] = p * vs[i][j + e];
             }
             const kva_h2_t h = __builtin_convertvector(w, kva_h2_t);
             ph[i >> 1][4 * (i & 1) + j] = h[0];
@@ -314,7 +331,7 @@ __device__ __forceinline__ void kva_softmax(const kva_f4_t (&t)[4], const kva_f4
                 pl[i >> 1][4 * (i & 1) + j + 1] = r[1];
             }
         }
-    sum += l;
+    sum += (l[0] + l[1]) + (l[2] + l[3]);
 }
 
 // A wave's running state for its 16 rows: reference, sum of weights and
@@ -446,10 +463,9 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
 #pragma unroll
         for (int i = 0; i < 4; i++) vs[i] *= st.vinv;
         kva_h8_t ph[2], pl[2];
-        if (masked)
-            kva_softmax<true, 4 * DC, HI>(s, vs, st.cq, key0 + 4 * g, st.lim, st.ref, st.sum, st.o, ph, pl);
-        else
-            kva_softmax<false, 4 * DC, HI>(s, vs, st.cq, 0, 0, st.ref, st.sum, st.o, ph, pl);
+        if (masked) kva_mask(s, vs, key0 + 4 * g, st.lim);
+        kva_reference(s, st.cq, st.ref, st.sum, st.o);
+        kva_weights<HI>(s, vs, st.cq, st.ref, st.sum, ph, pl);
         // fp8 rows that were never written may hold NaN codes
         kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
         if (FMT == QBK_KV_FP8 && masked) keep = kva_keep(key0, written, g);
@@ -612,8 +628,13 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
         const uint32_t key0 = tt * 64;
         if (key0 >= most) return;
         kva_f4_t ks[4], vs[4], s[4];
+        const float vm = kva_scalar(*(const float *)(buf + 2 * KEYS + 512));
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = kva_f4_t{0, 0, 0, 0};
+        for (int i = 0; i < 4; i++) {
+            ks[i] = *(const kva_f4_t *)(buf + 2 * KEYS + (16 * i + 4 * g) * 4);
+            vs[i] = *(const kva_f4_t *)(buf + 2 * KEYS + 256 + (16 * i + 4 * g) * 4);
+            s[i] = kva_f4_t{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int x = 0; x < STEPS; x++)
 #pragma unroll
@@ -622,18 +643,16 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
                 s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[x], s[i], 0, 0, 0);
                 if constexpr (HI) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[x], s[i], 0, 0, 0);
             }
-        kva_value_scales(kva_scalar(*(const float *)(buf + 2 * KEYS + 512)), st.vref, st.vinv, st.o);
+        kva_value_scales(vm, st.vref, st.vinv, st.o);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            ks[i] = *(const kva_f4_t *)(buf + 2 * KEYS + (16 * i + 4 * g) * 4);
-            vs[i] = *(const kva_f4_t *)(buf + 2 * KEYS + 256 + (16 * i + 4 * g) * 4) * st.vinv;
+            vs[i] *= st.vinv;
             s[i] *= ks[i];
         }
+        if (key0 + 64 > least) kva_mask(s, vs, key0 + 4 * g, st.lim);
+        kva_reference(s, st.cq, st.ref, st.sum, st.o);
         kva_h8_t ph[2], pl[2];
-        if (key0 + 64 > least)
-            kva_softmax<true, 4 * DC, HI>(s, vs, st.cq, key0 + 4 * g, st.lim, st.ref, st.sum, st.o, ph, pl);
-        else
-            kva_softmax<false, 4 * DC, HI>(s, vs, st.cq, 0, 0, st.ref, st.sum, st.o, ph, pl);
+        kva_weights<HI>(s, vs, st.cq, st.ref, st.sum, ph, pl);
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++)
 #pragma unroll
