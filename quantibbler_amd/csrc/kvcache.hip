@@ -418,6 +418,16 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
     const uint64_t first = held ? t.first : 0;
     const uint32_t padw = hd / 4 + 4;  // 16-byte rows
     const uint8_t *src = a.c.v + slab * hd + first * hd;
+    const uint4 none = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};  // numbers in either format
+    const uint32_t units = (t.hi - t.lo) * nc;  // at most 64 * 16
+    uint4 keys[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {  // asked for before the values are turned
+        const uint32_t x = tid + 256 * i, r = t.lo + x / nc, chunk = x % nc;
+        keys[i] = none;
+        if (x < units && held && first + r < a.c.cap)
+            keys[i] = *(const uint4 *)(a.c.k + slab * hd + kv_key_at(first + r, 16 * chunk, hd));
+    }
     if (tid < 128) {
         const uint32_t r = tid & 63;
         const bool in = held && r >= t.lo && first + r < a.c.cap;
@@ -438,18 +448,14 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
         }
     }
     __syncthreads();
-    const uint32_t units = (t.hi - t.lo) * nc;
-    for (uint32_t x = tid; x < units; x += 256) {
-        const uint32_t r = t.lo + x / nc, chunk = x % nc;
-        const bool in = held && first + r < a.c.cap;
-        const uint4 kw = in ? *(const uint4 *)(a.c.k + slab * hd + kv_key_at(first + r, 16 * chunk, hd))
-                            : uint4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
-        const uint4 vw = in ? *(const uint4 *)(codes + r * padw + 4 * chunk)
-                            : uint4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t x = tid + 256 * i, r = t.lo + x / nc, chunk = x % nc;
+        if (x >= units) continue;
+        const uint4 vw = held && first + r < a.c.cap ? *(const uint4 *)(codes + r * padw + 4 * chunk) : none;
         const size_t at = (size_t)(t.row + r - t.lo) * a.stride + (size_t)h * hd + 16 * chunk;
-        const float ks = scale[0][r], vs = scale[1][r];
-        kv_store16<FMT>(k + at, kw, ks);
-        kv_store16<FMT>(v + at, vw, vs);
+        kv_store16<FMT>(k + at, keys[i], scale[0][r]);
+        kv_store16<FMT>(v + at, vw, scale[1][r]);
     }
 }
 
