@@ -1569,6 +1569,7 @@ int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *B, float *h, const uint32_t
                                             shape->n_seqs));
     if (((uintptr_t)cache | (uintptr_t)(prefix_len ? prefix : nullptr) | (uintptr_t)workspace) & 15)
         return fail(QBK_ERR_VALIDATION, "kv cache buffers and the workspace must be 16-byte aligned");
+    if (B->H > 8192) return fail(QBK_ERR_VALIDATION, "kv attention takes up to 8192 heads");
     const BlkKv kv{shape, prefix_shape, cache, prefix, first_seq, max_len, prefix_seq, prefix_len};
     return block_decode_batch(ctx, B, h, nullptr, pos, n, workspace, workspace_size, stream, &kv);
 }

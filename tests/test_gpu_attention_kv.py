@@ -310,6 +310,19 @@ def test_a_sequence_alone_or_in_the_batch(ctx):
               tol[i:i + 1])
 
 
+@pytest.mark.parametrize("n,heads,kv,d", [(1, 2, 2, 64), (9, 4, 1, 128)])
+def test_a_long_prefix(ctx, n, heads, kv, d):
+    """More key tiles than there are splits, by far: one row tile of 16 and one of 64."""
+    plen = 100003
+    shared, cache = make(ctx, "fp8", 1, plen, kv, d), make(ctx, "fp8", n, 70, kv, d)
+    p = fill(shared, 150, [plen])[0]
+    rows = [70 - i for i in range(n)]
+    own = fill(cache, 151, rows)
+    q = normal(152, (n, 1, heads, d))
+    want, tol = reference(q, p, own, rows)
+    check(attend(cache, q, words(rows), "float32", shared, plen), want, tol)
+
+
 def test_offsets_past_32_bits(ctx):
     """The last sequence of a cache of eleven gigabytes."""
     n, cap, kv, d, heads, rows = 40, 131072, 8, 128, 16, 500

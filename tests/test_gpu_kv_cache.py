@@ -57,7 +57,8 @@ def check(got, want, label):
     assert same.all(), f"{label}: {np.count_nonzero(~same)} values differ, first at {np.argwhere(~same)[:3].tolist()}"
 
 
-CASES = [(1, 1, 16, [1], [0], 1), (1, 1, 16, [3], [61], 64), (3, 2, 64, [5, 0, 70], [7, 3, 60], 131),
+CASES = [(4, 2, 64, [15, 9, 0, 14], [0, 50, 3, 60], 80), (20, 3, 128, [i % 13 for i in range(20)], [5 * i for i in range(20)], 110),
+         (300, 1, 32, [17 + i % 3 for i in range(300)], [i for i in range(300)], 330), (1, 1, 16, [1], [0], 1), (1, 1, 16, [3], [61], 64), (3, 2, 64, [5, 0, 70], [7, 3, 60], 131),
          (2, 5, 80, [130, 1], [1, 63], 140), (4, 8, 128, [1, 1, 1, 1], [0, 15, 64, 1000], 1025),
          (2, 1, 256, [65, 64], [15, 0], 128), (1, 3, 240, [17], [0], 17), (2, 8, 128, [300, 211], [0, 5], 320)]
 
@@ -185,6 +186,23 @@ def test_rows_left_alone(ctx, fmt):
     out[2:22], out[32:34] = w[2:22], w[32:34]
     check(ko, out, "key")
     check(vo, out, "value")
+
+
+def test_rows_written_one_step_at_a_time(ctx):
+    """Decode steps beside each other in one 64-row tile, eight sequences a call: what earlier steps wrote stays."""
+    rng = np.random.default_rng(8)
+    n, kv, d, steps = 8, 3, 48, 70
+    cache = make(ctx, "int8", n, steps, kv, d)
+    x = torch.from_numpy(rows_of(rng, steps * n, kv, d)).cuda().view(steps, n, kv, d)
+    at = words([0] * n)
+    for t in range(steps):
+        cache.write_dev(x[t], x[t], "float32", at, n)
+        at += 1
+    ko, vo = torch.empty((n * steps, kv, d), device="cuda"), torch.empty((n * steps, kv, d), device="cuda")
+    cache.read_dev(ko, vo, "float32", words([0] * n), n * steps)
+    want = stored(x.permute(1, 0, 2, 3).contiguous().cpu().numpy().reshape(n * steps, kv, d), "int8")
+    check(ko, want, "key")
+    check(vo, want, "value")
 
 
 def test_row_starts_that_say_nothing_sensible(ctx):
