@@ -381,34 +381,43 @@ __global__ void __launch_bounds__(256) kv_write_tiles(KvRows a, const T *k, cons
     }
 }
 
-// Sixteen codes as values at any alignment, 16 bytes a store.
-template <int FMT, typename T>
-__device__ __forceinline__ void kv_store16(T *dst, const uint4 &w, float scale) {
-    struct __attribute__((packed, aligned(sizeof(T)))) Out {
+// Sixteen codes as bf16 at any alignment, 16 bytes a store.
+template <int FMT>
+__device__ __forceinline__ void kv_store16(uint16_t *dst, const uint4 &w, float scale) {
+    struct __attribute__((packed, aligned(2))) Out {
         uint32_t v[4];
     };
 #pragma unroll
-    for (int i = 0; i < 4; i += sizeof(T) == 4 ? 1 : 2) {
+    for (int i = 0; i < 4; i += 2) {
         Out y;
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) y.v[e] = __float_as_uint(kv_value<FMT>((&w.x)[i] >> (8 * e) & 255u, scale));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t b = (&w.x)[i + e / 2] >> (16 * (e & 1));
-                y.v[e] = f32x2_to_bf16x2(kv_value<FMT>(b & 255u, scale), kv_value<FMT>(b >> 8 & 255u, scale));
-            }
+        for (int e = 0; e < 4; e++) {
+            const uint32_t b = (&w.x)[i + e / 2] >> (16 * (e & 1));
+            y.v[e] = f32x2_to_bf16x2(kv_value<FMT>(b & 255u, scale), kv_value<FMT>(b >> 8 & 255u, scale));
         }
         *(Out *)(dst + 4 * i) = y;
     }
 }
 
+// Four codes as f32, 16 bytes a store.
+template <int FMT>
+__device__ __forceinline__ void kv_store4(float *dst, uint32_t w, float scale) {
+    struct __attribute__((packed, aligned(4))) Out {
+        float v[4];
+    } y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y.v[e] = kv_value<FMT>(w >> (8 * e) & 255u, scale);
+    *(Out *)dst = y;
+}
+
 // The other way: a lane takes 16 channels of a row, keys straight from their
-// 16-byte pieces, values from LDS, where 4 x 4 bytes have been turned.
+// 16-byte pieces, values from LDS, where 4 x 4 bytes have been turned.  f32 has
+// the keys in LDS as well and a lane four channels, so that a wave's stores lie
+// behind one another.
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
-    __shared__ uint32_t codes[64 * 68];
+    __shared__ __attribute__((aligned(16))) uint32_t codes[64 * 68];
+    __shared__ __attribute__((aligned(16))) uint32_t kcodes[sizeof(T) == 4 ? 64 * 68 : 4];
     __shared__ float scale[2][64];
     const uint32_t h = blockIdx.x % a.c.Hk, tid = threadIdx.x, hd = a.c.hd, nc = hd / 16;
     KvTile t;
@@ -447,15 +456,32 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
             for (int j = 0; j < 4; j++) codes[(16 * i + 4 * g + j) * padw + c4] = out[j];
         }
     }
-    __syncthreads();
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t x = tid + 256 * i, r = t.lo + x / nc, chunk = x % nc;
-        if (x >= units) continue;
-        const uint4 vw = held && first + r < a.c.cap ? *(const uint4 *)(codes + r * padw + 4 * chunk) : none;
-        const size_t at = (size_t)(t.row + r - t.lo) * a.stride + (size_t)h * hd + 16 * chunk;
-        kv_store16<FMT>(k + at, keys[i], scale[0][r]);
-        kv_store16<FMT>(v + at, vw, scale[1][r]);
+        for (int i = 0; i < 4; i++) {
+            const uint32_t x = tid + 256 * i, r = t.lo + x / nc, chunk = x % nc;
+            if (x < units) *(uint4 *)(kcodes + r * padw + 4 * chunk) = keys[i];
+        }
+        __syncthreads();
+        // x / words by a multiplication: x < 2^12, words <= 2^6, so that x times the factor's excess is below 2^20
+        const uint32_t words = hd / 4, by = ((1u << 20) + words - 1) / words, all = (t.hi - t.lo) * words;
+        for (uint32_t x = tid; x < all; x += 256) {
+            const uint32_t row = x * by >> 20, c4 = x - row * words, r = t.lo + row;
+            const size_t at = (size_t)(t.row + row) * a.stride + (size_t)h * hd + 4 * c4;
+            kv_store4<FMT>(k + at, kcodes[r * padw + c4], scale[0][r]);  // rows not held: codes times NaN
+            kv_store4<FMT>(v + at, codes[r * padw + c4], scale[1][r]);
+        }
+    } else {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t x = tid + 256 * i, r = t.lo + x / nc, chunk = x % nc;
+            if (x >= units) continue;
+            const uint4 vw = held && first + r < a.c.cap ? *(const uint4 *)(codes + r * padw + 4 * chunk) : none;
+            const size_t at = (size_t)(t.row + r - t.lo) * a.stride + (size_t)h * hd + 16 * chunk;
+            kv_store16<FMT>(k + at, keys[i], scale[0][r]);
+            kv_store16<FMT>(v + at, vw, scale[1][r]);
+        }
     }
 }
 
