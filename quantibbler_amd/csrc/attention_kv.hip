@@ -371,7 +371,7 @@ __device__ __forceinline__ T *kva_out_row(const KvAttArgs &a, uint32_t rho, uint
 // Up to 16 rows, row0 .. row0 + n_rows - 1 of kv head hk, over key tiles tile0
 // .. tile1 - 1 of the slab k, v, ks, vs: a wave every fourth tile, in registers
 // alone (few rows are bound by the cache's bytes; 32 sequences of up to 2085
-// rows, 32/8 heads of 128: 107 MB in 23.6 us, 4.5 TB/s).  Row r of the body sees
+// rows, 32/8 heads of 128: 107 MB in 23.3 us, 4.6 TB/s).  Row r of the body sees
 // keys below limit(r), none of them at or past `written`.
 template <int FMT, int DC, typename T, class Limit>
 __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows, uint32_t hk,
@@ -540,8 +540,9 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
 // channels: one buffer, so that a CU still holds two workgroups, two barriers
 // and one tile behind).  Two workgroups a CU, so that every SIMD has two waves
 // at unlike places (one alone issues a vector operation every four cycles, two
-// of one workgroup stand at its barriers together); 32 rows a wave halve the
-// widening but spill (64 behind 16384: 67 us and 56).
+// of one workgroup stand at its barriers together); 32 rows a wave would halve
+// the widening but do not fit 256 registers.  64 requests of up to 2048 rows
+// behind 16384, 32/8 heads of 128: 244 MB in 54.4 us, 4.5 TB/s.
 template <int DC>
 struct KvaStage {
     static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 528, BUFS = DC < 4 ? 2 : 1;
@@ -744,8 +745,8 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
 
 // A wave a row and kv head: the partial results of its splits on their largest
 // reference.  Four channels a lane and, up to 128 channels, two or four splits
-// at a time; everything is asked for before anything is used (references
-// first, 20 splits of 1024 rows took twice as long).
+// at a time; everything is asked for before anything is used, so that the
+// partial rows and their references take one latency (1024 rows: 4.9 us).
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
     constexpr int STEP = 64 / LANES, N = (2 * KVA_MAX_SPLITS + STEP - 1) / STEP, BATCH = N < 16 ? N : 16;
@@ -818,15 +819,27 @@ struct KvaPlan {
 static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq, size_t max_len, size_t prefix_len) {
     KvaPlan p{};
     const size_t Hk = s->n_kv_heads, G = n_heads / Hk, rows = n * sq * G, per = sq * G;
-    p.wides = per > 16 && max_len;
-    p.widep = p.wides || (rows > 16 && prefix_len);
+    const size_t dc = s->head_dim > 128 ? 4 : s->head_dim > 64 ? 2 : 1;
+    // The body of 64 rows reads and widens a tile once for four of 16 rows, that of 16 rows splits a sequence's tiles
+    // over its waves and is done sooner.  Own rows take the first once there are more items of 16 rows than the card
+    // holds at once (us by 64 / 16 rows, 32/8 heads of 128, sequences up to 300: 512 items 13.3 / 11.3, 1024 13.8 /
+    // 19.4, 2048 21 / 35; up to 1500: 27.8 / 21.1, 36.2 / 36.4, 45 / 66; heads of 64, 1024 items 9.5 / 11.7 and 24.8 /
+    // 21.8; heads of 256, 256 items 24.5 / 17.6 and 41.5 / 31.3, 512 24.9 / 29.3 and 53.8 / 51.9).
+    p.wides = per > 16 && max_len && (uint64_t)n * Hk * div_ceil(per, 16) > 1024 / dc;
+    // The prefix, split over the card by either, from the row tiles on whose reading of the same codes shows (8 kv heads
+    // of 128 behind 500, 8192 and 16384: 64 tiles 13.9 / 11.5, 23.7 / 20.7, 31.2 / 32.5; 128 tiles 14.9 / 15.8, 32.4 /
+    // 31.4, 49.2 / 53.9; heads of 64 behind 500 and 2048: 128 tiles 12.1 / 10.3, 14.2 / 12.6, 512 24.3 / 24.8, 29.6 /
+    // 32.4; heads of 256: 32 tiles 19.8 / 14.2, 21.6 / 23.2, 64 tiles 20.8 / 21.0, 24.0 / 26.8).
+    p.widep = p.wides || (prefix_len && (uint64_t)Hk * div_ceil(rows, 16) >= (dc == 1 ? 512 : 256 / dc));
     p.rtp = (uint32_t)div_ceil(rows, p.widep ? 64 : 16);
     p.rts = (uint32_t)div_ceil(per, p.wides ? 64 : 16);
     const uint64_t op = (uint64_t)Hk * p.rtp, os = (uint64_t)n * Hk * p.rts;
     // Splits: a workgroup a CU for the prefix, of four key tiles at least, and two for own rows where the sequences
     // alone leave CUs idle; past that a run of at most 64 tiles, so that no workgroup outlasts the rest on one long
-    // sequence.  More of them write and join more partial rows (us, prefix of 8192 behind 32 sequences of 32/8 heads:
-    // 8 splits 32, 16 24.6, 32 24.7; own rows of 32 sequences up to 2085: one split 23.6, two 25.5).
+    // sequence.  More of them write and join more partial rows (us for 128, 256 and 512 workgroups of the prefix: 32
+    // requests behind 8192 30.0, 21.9, 22.8, 64 behind 16384 86.8, 54.6, 70.9; own rows of 32 sequences up to 2085: one
+    // split 23.5, two 25.1, of 8 sequences for 128, 256, 512 workgroups 15.8, 13.1, 13.2; 32 sequences up to 16384,
+    // runs of 16, 64 and 512 tiles: 159.8, 154.1, 161.9).
     auto splits = [](uint64_t want, size_t tiles) -> uint32_t {
         const uint64_t most = div_ceil(tiles, KVA_WAVES);
         want = want < most ? want : most;
@@ -835,7 +848,8 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
     const size_t tp = div_ceil(prefix_len, 64), ts = div_ceil(max_len, 64);
     if (prefix_len) p.sp = splits(div_ceil(256, op), tp);
     if (max_len) p.ss = splits(os >= 256 ? div_ceil(ts, 64) : div_ceil(512, os), ts);
-    // a second launch takes longer than one more tile a wave
+    // a second launch takes longer than one more tile a wave (one sequence of 512 rows in one launch 7.9 us, split 9.2;
+    // of 768 9.6 and 9.4, of 1024 11.1 and 9.4)
     if (!prefix_len && ts <= 2 * KVA_WAVES) p.ss = 1;
     p.items = op * p.sp + os * p.ss;
     p.bytes = p.sp + p.ss > 1 ? round_up((size_t)(p.sp + p.ss) * Hk * rows * (s->head_dim * 4 + 8), 256) : 0;

@@ -5,8 +5,10 @@
 //   scale = A (1 / L),  code = nearest(x (L (1 / A))),  value = code * scale
 //
 // each product and reciprocal rounded to f32.  The floor on A keeps L / A and
-// every scale a normal number.  Both kernels
-// are one pass over rows and codes, bound by memory (a few rows: by the launch).
+// every scale a normal number.  One pass over
+// rows and codes either way, bound by memory (16384 rows of 8 heads of 128 read
+// as f32 28.4 us, 5.9 TB/s, as bf16 19.3, 5.2; 50584 f32 rows written 117, 4.5;
+// a few rows are bound by the launch, 3 us).
 #include <math.h>
 
 #include "kvcache.h"
@@ -485,9 +487,16 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
     }
 }
 
-// Whether a call goes by tiles: a tile's fixed work is that of some sixteen
-// rows by themselves.
-static bool kv_by_tiles(size_t n_rows, size_t n) { return n_rows >= 16 * n; }
+// Whether a call goes by tiles.  A tile takes its search, transposes and
+// barriers however few rows it has; rows by themselves store bytes 64 apart and
+// pay only once they fill the chip.  us by rows / by tiles, heads of 128:
+//   written (f32): 2048 rows x heads 4.5 / 6.7, 4096 6.6 / 6.8, 8192 10.1 / 7.0, 32768 29.0 / 10.6
+//   read (bf16):   2048 3.4 / 4.8, 4096 4.2 / 4.9, 8192 6.2 / 5.3, 32768 18.3 / 8.5
+//   256 sequences: two rows each written 10.1 / 16.8, four 17.4 / 17.3, eight 21.8 / 17.6
+// Heads of 64 and 256 cross within a factor of two of it.
+static bool kv_by_tiles(size_t n_rows, size_t n, size_t n_kv_heads) {
+    return (unsigned __int128)n_rows * n_kv_heads > 4096 && n_rows / 4 >= n;
+}
 
 // Tiles that a call can have: a sequence's rows touch one more than they fill,
 // or two where they fill none, and the unclaimed ones make two runs of their own.
@@ -530,7 +539,7 @@ static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void
 
 template <int FMT, typename T>
 static void kv_write_go(const KvRows &a, const T *k, const T *v, hipStream_t s) {
-    if (kv_by_tiles(a.n_rows, a.n)) {
+    if (kv_by_tiles(a.n_rows, a.n, a.c.Hk)) {
         void (*kern)(KvRows, const T *, const T *) = a.c.hd <= 64    ? kv_write_tiles<FMT, 1, T>
                                                      : a.c.hd <= 128 ? kv_write_tiles<FMT, 2, T>
                                                                      : kv_write_tiles<FMT, 4, T>;
@@ -543,7 +552,7 @@ static void kv_write_go(const KvRows &a, const T *k, const T *v, hipStream_t s) 
 
 template <int FMT, typename T>
 static void kv_read_go(const KvRows &a, T *k, T *v, hipStream_t s) {
-    if (kv_by_tiles(a.n_rows, a.n))
+    if (kv_by_tiles(a.n_rows, a.n, a.c.Hk))
         hipLaunchKernelGGL((kv_read_tiles<FMT, T>), dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk)), dim3(256), 0, s,
                            a, k, v);
     else

@@ -4,7 +4,8 @@
 // A row is cut into chunks of 8192 logits, a workgroup each, held in
 // registers: m = max x, l = sum exp(x - m), t = sum exp(x - m) (x - m), and the
 // chunk's top_k as 64-bit keys (value, then lower id first).  A second launch
-// joins a row's chunks (a row of one chunk is finished by the first):
+// joins a row's chunks; a row of one chunk is finished by the first (32 x 8192
+// 6.6 us, joined all the same 10.0; 2048 x 1000 14.2 and 19.1):
 //   log p = (x - M) - log l,   entropy = log l - t / l
 // (t moves from m to M as t' = f (t + (m - M) l), f = exp(m - M)).
 //
@@ -14,6 +15,9 @@
 // left to order is mostly little past k.  Where ties leave more than fit (a row
 // of few different values) the same is done once more on keys of value and id,
 // which all differ: only k threads hold keys above the k-th largest of theirs.
+//
+// Many rows are bound by memory: 2048 x 128256 f32, 1.05 GB in 179 us, 5.9 TB/s.
+// One row is bound by two dependent launches, 9.4 and 5.9 us.
 #include <math.h>
 
 #include <type_traits>
