@@ -500,8 +500,8 @@ int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *c
  * of them the queries' own: query t sees every prefix row and own rows
  * 0 .. lens[i] - seq_q + t.  The prefix is rows 0 .. prefix_len - 1 of
  * sequence prefix_seq of `prefix` (a cache of the same format, kv heads and
- * head_dim; it may be the same buffer) and is read once for the batch, not
- * once a sequence; prefix_len 0 (prefix and prefix_shape NULL) is plain
+ * head_dim; it may be the same buffer) and is read for 16 or 64 query rows
+ * of any sequences at a time, not once a sequence; prefix_len 0 (prefix and prefix_shape NULL) is plain
  * batched attention.  A query that sees no row yields zeros.  Softmax
  * statistics and sums are f32; for QBK_F32 queries and weights are split in
  * two halves so that the products keep f32's precision.  The result does

@@ -3,7 +3,7 @@
 //
 // Rows: query row rho = (b sq + t) G + hg of kv head hk is sequence b's query
 // t, head hk G + hg.  Every row sees the prefix, so the prefix's items take
-// rows of all sequences together and read its codes once for them; a
+// rows of all sequences together and read its codes for 16 or 64 of them; a
 // sequence's own rows are seen by its sq G rows alone.  Both kinds are items of
 // one launch:
 //   item = (kv head, 16 or 64 rows, run of 64-row key tiles)

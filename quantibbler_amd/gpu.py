@@ -373,7 +373,7 @@ class KvCache:
         "bfloat16"), ``lens`` each sequence's own rows (the queries' rows
         among them), at most ``max_len`` (the capacity if None).  Every query
         also sees rows 0 .. prefix_len - 1 of ``prefix``'s sequence
-        ``prefix_seq``, read once for the whole batch."""
+        ``prefix_seq``, read for 16 or 64 query rows of the batch at a time."""
         code = _KV_DTYPES.get(dtype)
         if code is None:
             raise _lib.KernelError(f"kv attention takes 'float32' or 'bfloat16' queries, got {dtype!r}")

@@ -395,7 +395,7 @@ class DeviceModel:
         are prefilled once (as sequence 0), their cache rows quantised into an
         8-bit cache per block, and every request gets room for ``capacity``
         rows of its own there; step_shared() then steps them together, each
-        block reading the prompt's rows once for all of them.  bf16 serving;
+        block reading the prompt's rows for many of them at a time.  bf16 serving;
         prompt and capacity together within the model's capacity.  Returns the
         prompt's last logits, as prefill."""
         import torch
