@@ -407,10 +407,15 @@ class DeviceModel:
             raise ValueError("a shared prefix is served in bf16")
         if not 1 <= int(n_seqs) <= 64 or n + int(capacity) > self.capacity:
             raise ValueError(f"{n_seqs} requests of {capacity} rows behind {n} on a model of {self.capacity} positions")
+
+        def size(seqs, rows):
+            return KvCache.size(fmt, seqs, rows, md.n_kv_heads, md.head_dim)
+
+        size(1, n), size(int(n_seqs), int(capacity))  # refusals come before sequence 0 is replaced
         logits = self.prefill(tokens, stream)
 
         def cache(seqs, rows):
-            need = KvCache.size(fmt, seqs, rows, md.n_kv_heads, md.head_dim)
+            need = size(seqs, rows)
             return KvCache(self.ctx, fmt, seqs, rows, md.n_kv_heads, md.head_dim,
                            torch.empty(need, dtype=torch.uint8, device="cuda"))
 

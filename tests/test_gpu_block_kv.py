@@ -291,3 +291,21 @@ def test_model_behind_a_shared_prefix(ctx, orc):
     with pytest.raises(ValueError, match="needs share_prefix"):
         m.step_shared([1, 2, 3])
     m.close()
+
+
+def test_a_refused_prefix_leaves_the_model_as_it_was(ctx, orc):
+    from test_gpu_trunk import synthetic_model
+
+    from quantibbler_amd.model import DeviceModel
+
+    m = DeviceModel(ctx, synthetic_model(orc, 808), capacity=70)
+    m.prefill([5, 6, 7])
+    want = m.step(9).clone()
+    m.reset()
+    m.prefill([5, 6, 7])
+    for args, kw in ((([1, 2], 3, 6), {"fmt": "int4"}), (([1, 2], 3, 0), {}), (([1, 2], 0, 6), {}), (([], 3, 6), {})):
+        with pytest.raises((ValueError, KernelError)):
+            m.share_prefix(*args, **kw)
+        assert m.pos == 3 and m._shared is None
+    assert torch.equal(m.step(9), want)
+    m.close()
