@@ -57,6 +57,7 @@ struct KvRows {
     const uint32_t *row_start, *pos;  // row_start null: `per` rows a sequence
     size_t stride;                    // values from one row to the next
     uint32_t n_rows, n, per, first;
+    bool tiles;  // by 64-row tiles
 };
 
 // The sequence (0 .. n - 1) and position of row r; false for a row that no
@@ -201,63 +202,47 @@ struct __attribute__((packed, aligned(sizeof(T)))) Kv4 {
 
 // The workgroup's tile: input rows row .. row + hi - lo - 1 stand at rows lo ..
 // hi - 1 of the tile that begins at position first of sequence seq; seq -1:
-// rows that no sequence claims (lo 0).  Sequences' tiles are counted in order,
-// then those of the unclaimed rows behind the last one and before the first.
+// rows that no sequence claims (lo 0).
 struct KvTile {
     int32_t seq;
     uint32_t row, lo, hi;
     uint64_t first;
 };
+// Segments of the rows: 0 those before the first sequence's, 1 .. n the
+// sequences', n + 1 those behind the last one's.  Segment i's tiles are numbered
+// from (its first row) / 64 + 2 i on, which leaves room for the two that its
+// rows touch past those they fill, so that a tile finds its segment among 64 in
+// one load and one ballot, without the other segments' counts (a running sum
+// over them took 6.6 ms for 16384 sequences of four rows).
 __device__ __forceinline__ bool kv_tile(const KvRows &a, uint32_t tile, KvTile *t) {
-    __shared__ uint32_t sums[4];
-    __shared__ KvTile found;
-    __shared__ uint32_t have;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid == 0) have = 0;
-    uint32_t base = 0;
-    for (uint32_t s0 = 0; s0 < a.n + 2; s0 += 256) {
-        const uint32_t s = s0 + tid;
-        uint32_t from = 0, to = 0, at = 0;
-        if (s < a.n) {
-            from = a.row_start ? a.row_start[s] : s * a.per;
-            to = a.row_start ? a.row_start[s + 1] : from + a.per;
-            at = a.pos[s];
-        } else if (a.row_start && s == a.n) {
-            from = a.row_start[a.n];
-            to = a.n_rows;
-        } else if (a.row_start && s == a.n + 1) {
-            to = a.row_start[0];
-        }
-        to = to < a.n_rows ? to : a.n_rows;
-        const uint32_t count = to > from ? (uint32_t)(((uint64_t)(at & 63) + (to - from) + 63) / 64) : 0;
-        uint32_t up = count;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t x = (uint32_t)__shfl_up((int)up, o, 64);
-            if ((int)lane >= o) up += x;
-        }
-        __syncthreads();  // sums of the round before are read
-        if (lane == 63) sums[wave] = up;
-        __syncthreads();
-        uint32_t before = base + up - count;
-        for (uint32_t w = 0; w < wave; w++) before += sums[w];
-        if (tile >= before && tile - before < count) {
-            const uint32_t k = tile - before, skip = at & 63;
-            KvTile f;
-            f.seq = s < a.n ? (int32_t)s : -1;
-            f.lo = k == 0 ? skip : 0;
-            f.row = from + (k == 0 ? 0 : 64 * k - skip);
-            f.hi = to - f.row < 64 - f.lo ? f.lo + (to - f.row) : 64;
-            f.first = (uint64_t)(at - skip) + 64ull * k;
-            found = f;
-            have = 1;
-        }
-        __syncthreads();
-        base += sums[0] + sums[1] + sums[2] + sums[3];
-        if (have) break;
+    const uint32_t lane = threadIdx.x & 63;
+    auto bound = [&](uint32_t i) -> uint32_t {  // first row of segment i, 0 .. n + 2
+        if (i == 0) return 0;
+        if (i == a.n + 2) return a.n_rows;
+        const uint32_t r = a.row_start ? a.row_start[i - 1] : (i - 1) * a.per;
+        return r < a.n_rows ? r : a.n_rows;
+    };
+    uint32_t seg = 0, len = a.n + 2;  // seg .. seg + len - 1 hold it; the first of them begins at or before tile
+    while (len > 1) {
+        const uint32_t step = (len + 63) / 64, off = lane * step;
+        bool below = false;
+        if (off < len) below = bound(seg + off) / 64 + 2 * (seg + off) <= tile;
+        const uint64_t above = ~__ballot(below);
+        const uint32_t at = (above ? (uint32_t)__builtin_ctzll(above) : 64u) - 1;
+        const uint32_t skip = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at * step));
+        seg += skip;
+        len = len - skip < step ? len - skip : step;
     }
-    *t = found;
-    return have != 0;
+    const bool claimed = seg >= 1 && seg <= a.n;
+    const uint32_t from = bound(seg), to = bound(seg + 1), k = tile - (from / 64 + 2 * seg);
+    const uint32_t at = claimed ? a.pos[seg - 1] : 0, skip = at & 63;
+    if (to <= from || k >= (skip + (uint64_t)(to - from) + 63) / 64) return false;
+    t->seq = claimed ? (int32_t)(seg - 1) : -1;
+    t->lo = k == 0 ? skip : 0;
+    t->row = from + (k == 0 ? 0 : 64 * k - skip);
+    t->hi = to - t->row < 64 - t->lo ? t->lo + (to - t->row) : 64;
+    t->first = (uint64_t)(at - skip) + 64ull * k;
+    return true;
 }
 
 // 4 x 4 bytes: out[i] = bytes i of in[0 .. 3].
@@ -487,19 +472,19 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
     }
 }
 
-// Whether a call goes by tiles.  A tile takes its search, transposes and
-// barriers however few rows it has; rows by themselves store bytes 64 apart and
-// pay only once they fill the chip.  us by rows / by tiles, heads of 128:
-//   written (f32): 2048 rows x heads 4.5 / 6.7, 4096 6.6 / 6.8, 8192 10.1 / 7.0, 32768 29.0 / 10.6
-//   read (bf16):   2048 3.4 / 4.8, 4096 4.2 / 4.9, 8192 6.2 / 5.3, 32768 18.3 / 8.5
-//   256 sequences: two rows each written 10.1 / 16.8, four 17.4 / 17.3, eight 21.8 / 17.6
-// Heads of 64 and 256 cross within a factor of two of it.
-static bool kv_by_tiles(size_t n_rows, size_t n, size_t n_kv_heads) {
-    return (unsigned __int128)n_rows * n_kv_heads > 4096 && n_rows / 4 >= n;
+// Whether a call goes by tiles.  A tile takes its transposes and barriers
+// however few rows it has; rows by themselves store bytes 64 apart.  Tiles pay
+// once the rows fill the chip and a sequence's are some 512 channels of a head
+// (us by rows / by tiles, f32, 8 heads of 128 unless said):
+//   one sequence, written: 256 rows 4.5 / 6.3, 512 6.6 / 6.3, 1024 10.1 / 6.5
+//   the same read: 512 rows 4.3 / 5.1, 1024 6.2 / 5.6, 2048 9.9 / 6.8
+//   1024 sequences, written: two rows each 31 / 47, four 57 / 49, sixteen 135 / 57; read 26 / 34, 49 / 35, 71 / 42
+//   4096 sequences, 2 heads of 64, written: four rows 20.5 / 37, eight 37.5 / 38, sixteen 69 / 39
+static bool kv_by_tiles(size_t n_rows, size_t n, const qbk_kv_shape *s) {
+    return (unsigned __int128)n_rows * s->n_kv_heads > 4096 && n_rows * s->head_dim / 512 >= n;
 }
 
-// Tiles that a call can have: a sequence's rows touch one more than they fill,
-// or two where they fill none, and the unclaimed ones make two runs of their own.
+// Tile numbers of a call (kv_tile): at most two a segment past the tiles that the rows fill.
 static size_t kv_tiles(size_t n_rows, size_t n) { return n_rows / 64 + 2 * (n + 2); }
 
 // Checks shared by the write and the read; *a filled for a launch, n_rows 0
@@ -518,11 +503,16 @@ static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void
     const size_t width = shape->n_kv_heads * shape->head_dim;
     if (n_rows > 1 && row_stride < width)
         return fail(QBK_ERR_VALIDATION, fmt("row_stride %zu is smaller than a row of %zu values", row_stride, width));
-    if (n_rows > 0x7FFFFFFFull || n_rows * shape->n_kv_heads > 0x1FFFFFFFFull || row_stride > ((size_t)1 << 40))
+    if (n_rows > 0x7FFFFFFFull || row_stride > ((size_t)1 << 40))
         return fail(QBK_ERR_VALIDATION, "kv cache: too many rows for one call");
     if (n_rows != 0 && n == 0) return fail(QBK_ERR_VALIDATION, "kv cache rows for no sequence");
     if (n_rows != 0 && !row_start && n_rows % n != 0)
         return fail(QBK_ERR_VALIDATION, fmt("%zu rows do not split evenly over %zu sequences", n_rows, n));
+    // a launch is below 2^32 threads
+    a->tiles = kv_by_tiles(n_rows, n, shape);
+    const size_t groups = a->tiles ? kv_tiles(n_rows, n) * shape->n_kv_heads
+                                   : div_ceil(n_rows * shape->n_kv_heads, 4);
+    if (groups > 0xFFFFFF) return fail(QBK_ERR_VALIDATION, "kv cache: too many rows for one call");
     if (n_rows != 0 && (!cache || !k || !v || !pos)) return fail(QBK_ERR_VALIDATION, "null argument");
     if ((uintptr_t)cache & 15) return fail(QBK_ERR_VALIDATION, "kv cache buffer must be 16-byte aligned");
     a->n_rows = (uint32_t)n_rows;
@@ -539,7 +529,7 @@ static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void
 
 template <int FMT, typename T>
 static void kv_write_go(const KvRows &a, const T *k, const T *v, hipStream_t s) {
-    if (kv_by_tiles(a.n_rows, a.n, a.c.Hk)) {
+    if (a.tiles) {
         void (*kern)(KvRows, const T *, const T *) = a.c.hd <= 64    ? kv_write_tiles<FMT, 1, T>
                                                      : a.c.hd <= 128 ? kv_write_tiles<FMT, 2, T>
                                                                      : kv_write_tiles<FMT, 4, T>;
@@ -552,7 +542,7 @@ static void kv_write_go(const KvRows &a, const T *k, const T *v, hipStream_t s) 
 
 template <int FMT, typename T>
 static void kv_read_go(const KvRows &a, T *k, T *v, hipStream_t s) {
-    if (kv_by_tiles(a.n_rows, a.n, a.c.Hk))
+    if (a.tiles)
         hipLaunchKernelGGL((kv_read_tiles<FMT, T>), dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk)), dim3(256), 0, s,
                            a, k, v);
     else

@@ -371,7 +371,7 @@ static int lp_check(size_t rows, size_t vocab, size_t top) {
     if (top > LP_MAX_TOP || top > vocab)
         return fail(QBK_ERR_VALIDATION, fmt("logprobs top_k must be at most %d and the vocabulary of %zu, got %zu",
                                             LP_MAX_TOP, vocab, top));
-    if (rows > 0x7FFFFFFFull || rows * div_ceil(vocab, LP_CHUNK) > 0x7FFFFFFFull)
+    if (rows > 0xFFFFFF || rows * div_ceil(vocab, LP_CHUNK) > 0xFFFFFF)  // a launch is below 2^32 threads
         return fail(QBK_ERR_VALIDATION, "logprobs: too many rows for one launch");
     return QBK_OK;
 }

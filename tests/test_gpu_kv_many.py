@@ -13,7 +13,11 @@ import test_gpu_kv_cache as kvc
 from quantibbler_amd import GpuContext
 
 words, normal = kvc.words, att.normal
-BY_TILES = 4096  # rows times kv heads past which rows go by tiles
+
+
+def by_tiles(total, kv, n, d):
+    """Past 4096 rows and heads, of 512 channels a sequence and head, rows go by tiles."""
+    return total * kv > 4096 and total * d // 512 >= n
 
 
 @pytest.fixture(scope="module")
@@ -23,12 +27,13 @@ def ctx():
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("n,kv,d,rows,at,cap", [c for c in kvc.CASES if sum(c[3]) >= 4 * c[0]] +
+@pytest.mark.parametrize("n,kv,d,rows,at,cap", [c for c in kvc.CASES if by_tiles(sum(c[3]), 4097, c[0], c[2])] +
                          [(1, 1, 208, [64], [0], 64), (1, 1, 48, [65], [63], 128), (2, 1, 144, [4, 4], [62, 0], 66)])
 def test_rows_by_tiles(ctx, fmt, dtype, n, kv, d, rows, at, cap):
     rng = np.random.default_rng(d + cap)
     total = sum(rows)
-    kv = max(kv, BY_TILES // total + 1)
+    kv = max(kv, 4096 // total + 1)
+    assert by_tiles(total, kv, n, d)
     k, v = kvc.rows_of(rng, total, kv, d), kvc.rows_of(rng, total, kv, d)
     k[rng.random(k.shape) < 0.05] = 0.0
     k[1, 0] = 0.0
@@ -100,8 +105,33 @@ def test_rows_left_alone_by_tiles(ctx, fmt, dtype):
     kvc.check(vo, cast(out), "value")
 
 
+@pytest.mark.parametrize("n", [61, 62, 63, 126, 127, 5000])
+@pytest.mark.parametrize("even", [False, True])
+def test_many_sequences_by_tiles(ctx, n, even):
+    """A tile finds its sequence among few and many, empty ones between them, rows of none before and behind."""
+    rng = np.random.default_rng(n)
+    kv, d, cap = 1 if n > 1000 else 64, 128, 90
+    lens = np.full(n, 9) if even else np.where(rng.random(n) < 0.2, 0, rng.integers(1, 17, n))
+    lens[n // 2] = 9 if even else 80
+    pre, post = (0, 0) if even else (70, 3)
+    total = int(lens.sum()) + pre + post
+    assert by_tiles(total, kv, n, d)
+    x = torch.from_numpy(kvc.rows_of(rng, total, kv, d)).cuda()
+    at = rng.integers(0, cap, n)
+    starts = None if even else words(pre + np.concatenate([[0], np.cumsum(lens)]))
+    cache = kvc.make(ctx, "int8", n, cap, kv, d)
+    cache.write_dev(x, x, "float32", words(at), total, row_start=starts)
+    ko, vo = torch.zeros_like(x), torch.zeros_like(x)
+    cache.read_dev(ko, vo, "float32", words(at), total, row_start=starts)
+    want = kvc.stored(x.cpu().numpy(), "int8")
+    where = np.concatenate([np.full(pre, cap)] + [a + np.arange(r) for a, r in zip(at, lens)] + [np.full(post, cap)])
+    want[where >= cap] = np.nan
+    kvc.check(ko, want, "key")
+    kvc.check(vo, want, "value")
+
+
 def test_row_starts_that_say_nothing_sensible_by_tiles(ctx):
-    kv, d, cap = 150, 16, 40
+    kv, d, cap = 150, 64, 40
     size = kvc.KvCache.size("int8", 2, cap, kv, d)
     buf = torch.zeros(size + 4096, dtype=torch.uint8, device="cuda")
     cache = kvc.KvCache(ctx, "int8", 2, cap, kv, d, buf)
