@@ -233,7 +233,7 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
         // the largest channel to [8, 16): both halves of every channel within fp16
         const bool whole = top[k] < 0x7f800000u;
         uint32_t ex = top[k] >> 23;
-        ex = ex < 30 ? 30 : ex;
+        ex = ex < 8 ? 8 : ex;  // rows below 2^-119 stay below 8: the factor below is a normal number down to here
         const float f = __uint_as_float((257 - ex) << 23);  // NaN rows: the scores become NaN by cqs
         kva_h2_t hi[2], lo[2];
 #pragma unroll

@@ -1,0 +1,89 @@
+"""GPU: attention over the 8-bit KV cache where keys, values and queries are of
+very unlike size, in every body (16 and 64 query rows, own rows and prefix),
+against float64 on the values the cache stands for.
+
+Tolerance as test_gpu_attention_kv's, with everything taken over the rows a
+query sees alone: a weight below 2^-26 of the query's largest weight times
+value scale is a step of fp16's subnormals, and is off by at most 2^-36 of it
+(half a step, 2^-25, where that largest stands between 2^11 and 2^12, or
+higher)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+import test_gpu_attention_kv as att
+from quantibbler_amd import GpuContext
+
+EPS = att.EPS
+words, normal = att.words, att.normal
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return GpuContext(0)
+
+
+def reference(q, prefix, own, lens):
+    """float64 outputs and their tolerances (without the output's rounding)."""
+    n, sq, heads, d = q.shape
+    f32 = q.dtype == torch.float32
+    q64, scale = q.double(), d ** -0.5
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    for b in range(n):
+        k = torch.cat([prefix[0], own[b][0][:lens[b]]])
+        v = torch.cat([prefix[1], own[b][1][:lens[b]]])
+        p, kv, m = prefix[0].shape[0], k.shape[1], k.shape[0]
+        last = p + lens[b] - sq + 1 + torch.arange(sq, device="cuda")[:, None]
+        index = torch.arange(m, device="cuda")[None]
+        seen = (index < p) | (index < last)
+        none = ~seen.any(-1)
+        for h in range(heads):
+            j = h // (heads // kv)
+            kk, vv, qq = k[:, j], v[:, j], q64[b, :, h]
+            s = torch.where(seen, (qq @ kk.t().contiguous()) * scale, torch.full_like(seen, -torch.inf, dtype=torch.float64))
+            w = s.softmax(-1)
+            w[none] = 0.0
+            out[b, :, h] = w @ vv
+            mass = torch.where(seen, qq.abs() @ kk.abs().t().contiguous(), 0.0).amax(-1, keepdim=True)
+            low = torch.where(seen, kk.abs().sum(-1)[None], 0.0).amax(-1, keepdim=True)
+            bound = scale * (((d + 8) * EPS + (2.0 ** -23 if f32 else 0)) * mass +
+                             2.0 ** -28 * qq.abs().amax(-1, keepdim=True) * low)
+            rel = 2 * bound + (2.0 ** -22 if f32 else 2.0 ** -11) + (2 * m + 70) * EPS
+            most = (w * vv.abs().amax(-1)[None]).amax(-1, keepdim=True)
+            tol[b, :, h] = rel * (w @ vv.abs()) + m * 2.0 ** -36 * most
+    return out, tol
+
+
+# n, heads, kv heads, d, queries, own rows, prefix: own rows by 16 and by 64, the prefix by 16 and by 64
+SHAPES = [(1, 4, 2, 64, 5, [90], 0), (2, 4, 2, 128, 5, [90, 300], 150), (1, 4, 1, 256, 3, [70], 40),
+          (1, 8, 2, 80, 1, [2000], 0), (1, 256, 256, 64, 70, [200], 0), (1, 128, 128, 128, 70, [90], 100),
+          (1, 64, 64, 256, 70, [90], 30), (17, 64, 16, 128, 1, [9 + i for i in range(17)], 500)]
+
+
+def both(ctx, fmt, shape, poke=None, poke_prefix=None):
+    n, heads, kv, d, sq, rows, plen = shape
+    cache = att.make(ctx, fmt, n, max(rows), kv, d)
+    own = att.fill(cache, 10, rows, poke=poke)
+    shared, p = None, att.empty_prefix(kv, d)
+    if plen:
+        shared = att.make(ctx, fmt, 1, plen, kv, d)
+        p = att.fill(shared, 30, [plen], poke=poke_prefix or poke)[0]
+    return cache, own, shared, p
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_queries_near_the_bottom_of_the_range(ctx, fmt, dtype, shape):
+    """Queries of 1e-36 against keys of 2e34: the scores are ordinary numbers, and a query keeps its bits."""
+    n, heads, kv, d, sq, rows, plen = shape
+
+    def poke(k, v):
+        k *= 2e34
+    cache, own, shared, p = both(ctx, fmt, shape, poke)
+    q = (1e-36 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
+    want, tol = reference(q, p, own, rows)
+    att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol)
