@@ -503,9 +503,11 @@ int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *c
  * head_dim; it may be the same buffer) and is read for 16 or 64 query rows
  * of any sequences at a time, not once a sequence; prefix_len 0 (prefix and prefix_shape NULL) is plain
  * batched attention.  A query that sees no row yields zeros.  Softmax
- * statistics and sums are f32; for QBK_F32 queries and weights are split in
- * two halves so that the products keep f32's precision.  The result does
- * not depend on what other calls run.  workspace of at least
+ * statistics, scores and sums are f32 (the largest channel of a query times
+ * the largest of a key is to stay below 2^128; past it a score is not a
+ * number); for QBK_F32 queries and weights are split in two halves so that
+ * the products keep f32's precision.  The result does not depend on what
+ * other calls run.  workspace of at least
  * qbk_attention_kv_workspace_size bytes, 16-byte aligned; calls that share
  * one must not overlap. */
 size_t qbk_attention_kv_workspace_size(const qbk_kv_shape *shape, size_t n_heads, size_t n, size_t seq_q,

@@ -194,11 +194,12 @@ struct __attribute__((packed, aligned(sizeof(T)))) Kva4 {
 
 // Queries row0 .. row0 + n_rows - 1 (at most 16 NT) of kv head hk into LDS as
 // the B operands of K q^T, [tile][step][lane][16 bytes], for f32 queries the
-// low halves behind them; cqs[r]: the factor that scores of row r still need.
+// low halves behind them; qps[r]: the power of two that scores of row r still
+// need, NaN for a row that holds a NaN or an infinity.
 // 16 DC lanes a row, four channels a lane, every row's load before the first
 // is used (32 requests behind 8192 rows, by a row at a time 41 us, so 29).
 template <int DC, int NT, typename T>
-__device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float *cqs, uint32_t row0, uint32_t n_rows,
+__device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float *qps, uint32_t row0, uint32_t n_rows,
                                             uint32_t hk) {
     constexpr int STEPS = 2 * DC, LANES = 16 * DC, AT_ONCE = KVA_WAVES * 64 / LANES, N = 16 * NT / AT_ONCE;
     const int tid = threadIdx.x, hd = (int)a.own.hd, c = 4 * (tid % LANES), r0 = tid / LANES;
@@ -233,8 +234,8 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
         // the largest channel to [8, 16): both halves of every channel within fp16
         const bool whole = top[k] < 0x7f800000u;
         uint32_t ex = top[k] >> 23;
-        ex = ex < 8 ? 8 : ex;  // rows below 2^-119 stay below 8: the factor below is a normal number down to here
-        const float f = __uint_as_float((257 - ex) << 23);  // NaN rows: the scores become NaN by cqs
+        ex = ex < 4 ? 4 : ex;  // rows below 2^-123 stay below 8: the power of two is a normal number down to here
+        const float f = __uint_as_float((257 - ex) << 23);  // NaN rows: the scores become NaN by qps
         kva_h2_t hi[2], lo[2];
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
@@ -250,11 +251,11 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
         if constexpr (sizeof(T) == 4)
             *(uint2 *)(qs + NT * STEPS * 1024 + at) =
                 uint2{__builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1])};
-        top[k] = whole ? __float_as_uint(a.scale * __uint_as_float((ex - 3) << 23)) : 0x7fc00000u;
+        top[k] = whole ? (ex - 3) << 23 : 0x7fc00000u;
     }
     if (c == 0)
 #pragma unroll
-        for (int k = 0; k < N; k++) cqs[r0 + k * AT_ONCE] = __uint_as_float(top[k]);
+        for (int k = 0; k < N; k++) qps[r0 + k * AT_ONCE] = __uint_as_float(top[k]);
 }
 
 // The largest value scale vm of a tile against vref, a power of two at or above
@@ -270,6 +271,15 @@ __device__ __forceinline__ void kva_value_scales(float vm, float &vref, float &v
         for (int ct = 0; ct < CT; ct++) o[ct] *= f;
         vref = to;
     }
+}
+
+// Sums of code products as q k: times the key's scale and the row's power of
+// two, those two first.  Codes reach 448 and a scaled query 16, so a sum by its
+// key's scale alone would pass f32 for keys from some 2^117 on; the two
+// together pass it where |q| |k| does.
+__device__ __forceinline__ void kva_scores(kva_f4_t (&s)[4], const kva_f4_t (&ks)[4], float qp) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[i] *= ks[i] * qp;
 }
 
 // Scores t and value scales vs of a lane's 16 keys (16 i + j past key) that its
@@ -288,14 +298,14 @@ __device__ __forceinline__ void kva_mask(kva_f4_t (&t)[4], kva_f4_t (&vs)[4], ui
 // The row's reference moves when a score passes it eightfold, its sum and
 // outputs with it.
 template <int CT>
-__device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float cq, float &ref, float &sum,
+__device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float scale, float &ref, float &sum,
                                               kva_f4_t (&o)[CT]) {
     float m[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) m[i] = fmaxf(fmaxf(t[i][0], t[i][1]), fmaxf(t[i][2], t[i][3]));
     const float tm = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    if (__ballot(tm * cq > ref + 3.0f)) {
-        const float to = fmaxf(ref, ceilf(kva_max4(tm) * cq));
+    if (__ballot(tm * scale > ref + 3.0f)) {
+        const float to = fmaxf(ref, ceilf(kva_max4(tm) * scale));
         const float f = kva_rescale(ref, to);
         sum *= f;
 #pragma unroll
@@ -304,10 +314,10 @@ __device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float cq, 
     }
 }
 
-// Scores to weights: p = exp2(t cq - ref) into sum, p times the value scales
+// Scores to weights: p = exp2(t scale - ref) into sum, p times the value scales
 // as operands ph (and pl, what the first half leaves).
 template <bool HI>
-__device__ __forceinline__ void kva_weights(const kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float cq, float ref,
+__device__ __forceinline__ void kva_weights(const kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float scale, float ref,
                                             float &sum, kva_h8_t (&ph)[2], kva_h8_t (&pl)[2]) {
     const float base = ref == -INFINITY ? 0.0f : ref;  // a row that has seen nothing: every p is 0
     float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -318,7 +328,7 @@ __device__ __forceinline__ void kva_weights(const kva_f4_t (&t)[4], const kva_f4
             kva_f2_t w;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j + e], cq, -base));
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j + e], scale, -base));
                 l[i] += p;
                 w[e] = p * vs[i][j + e];
             }
@@ -339,10 +349,10 @@ __device__ __forceinline__ void kva_weights(const kva_f4_t (&t)[4], const kva_f4
 template <int DC>
 struct KvaState {
     kva_f4_t o[4 * DC];
-    float ref, sum, cq, vref, vinv;
+    float ref, sum, qp, vref, vinv;
     uint32_t lim;
-    __device__ __forceinline__ KvaState(float cq, uint32_t lim)
-        : ref(-INFINITY), sum(0.0f), cq(cq), vref(0.0f), vinv(0.0f), lim(lim) {
+    __device__ __forceinline__ KvaState(float qp, uint32_t lim)
+        : ref(-INFINITY), sum(0.0f), qp(qp), vref(0.0f), vinv(0.0f), lim(lim) {
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++) o[ct] = kva_f4_t{0, 0, 0, 0};
     }
@@ -385,7 +395,7 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: loops and addresses by it are too
     const int hd = (int)a.own.hd, nc = hd / 16;
     char *qs = smem;
-    float *cqs = (float *)(smem + L::BODY), *refs = cqs + 16, *sums = refs + KVA_WAVES * 16;
+    float *qps = (float *)(smem + L::BODY), *refs = qps + 16, *sums = refs + KVA_WAVES * 16;
 
     // A tile's codes and scales travel while the one before is worked on: keys
     // and their scales are asked for again as soon as the scores are formed,
@@ -418,9 +428,9 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
         load_k(first);
         load_v(first);
     }
-    kva_queries<DC, 1, T>(a, qs, cqs, row0, n_rows, hk);
+    kva_queries<DC, 1, T>(a, qs, qps, row0, n_rows, hk);
     __syncthreads();
-    KvaState<DC> st(cqs[col], limit((uint32_t)col < n_rows ? col : n_rows - 1));
+    KvaState<DC> st(qps[col], limit((uint32_t)col < n_rows ? col : n_rows - 1));
     const uint32_t least = kva_scalar(limit(0));  // keys below it are seen by every row
 
     for (uint32_t tt = first; tt < tile1; tt += KVA_WAVES) {
@@ -452,9 +462,8 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
                 for (int i = 0; i < 4; i++) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], ql, s[i], 0, 0, 0);
             }
         }
-        // scores in units of 1 / cq; the key registers are free again
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[i] *= ks[i];
+        // the key registers are free again
+        kva_scores(s, ks, st.qp);
         if (more) load_k(tt + KVA_WAVES);
         float vm = 0.0f;
 #pragma unroll
@@ -464,8 +473,8 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
         for (int i = 0; i < 4; i++) vs[i] *= st.vinv;
         kva_h8_t ph[2], pl[2];
         if (masked) kva_mask(s, vs, key0 + 4 * g, st.lim);
-        kva_reference(s, st.cq, st.ref, st.sum, st.o);
-        kva_weights<HI>(s, vs, st.cq, st.ref, st.sum, ph, pl);
+        kva_reference(s, a.scale, st.ref, st.sum, st.o);
+        kva_weights<HI>(s, vs, a.scale, st.ref, st.sum, ph, pl);
         // fp8 rows that were never written may hold NaN codes
         kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
         if (FMT == QBK_KV_FP8 && masked) keep = kva_keep(key0, written, g);
@@ -566,7 +575,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: loops and addresses by it are too
     const int hd = (int)a.own.hd, nc = hd / 16;
-    float *cqs = (float *)(smem + L::BODY);
+    float *qps = (float *)(smem + L::BODY);
 
     // This wave's part of a tile: the keys of block `wave` and every fourth
     // channel tile of the values.
@@ -609,7 +618,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
     };
     if (tile0 < tile1) load(tile0, 0);
     if (BUFS > 1 && tile0 + 1 < tile1) load(tile0 + 1, BUFS - 1);
-    kva_queries<DC, KVA_WAVES, T>(a, smem, cqs, row0, n_rows, hk);
+    kva_queries<DC, KVA_WAVES, T>(a, smem, qps, row0, n_rows, hk);
     __syncthreads();
     kva_h8_t qh[STEPS], ql[STEPS];
 #pragma unroll
@@ -620,7 +629,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
     }
     const uint32_t my0 = wave * 16, r = my0 + col;  // this wave's first row, this lane's
     const bool rows = my0 < n_rows;
-    KvaState<DC> st(cqs[r], limit(r < n_rows ? r : n_rows - 1));
+    KvaState<DC> st(qps[r], limit(r < n_rows ? r : n_rows - 1));
     const uint32_t least = kva_scalar(limit(rows ? my0 : 0)), end = my0 + 16 < n_rows ? my0 + 16 : n_rows;
     const uint32_t most = rows ? kva_scalar(limit(end - 1)) : 0;  // no row of the wave sees keys from here on
     __syncthreads();  // the queries are read
@@ -646,14 +655,12 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
             }
         kva_value_scales(vm, st.vref, st.vinv, st.o);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            vs[i] *= st.vinv;
-            s[i] *= ks[i];
-        }
+        for (int i = 0; i < 4; i++) vs[i] *= st.vinv;
+        kva_scores(s, ks, st.qp);
         if (key0 + 64 > least) kva_mask(s, vs, key0 + 4 * g, st.lim);
-        kva_reference(s, st.cq, st.ref, st.sum, st.o);
+        kva_reference(s, a.scale, st.ref, st.sum, st.o);
         kva_h8_t ph[2], pl[2];
-        kva_weights<HI>(s, vs, st.cq, st.ref, st.sum, ph, pl);
+        kva_weights<HI>(s, vs, a.scale, st.ref, st.sum, ph, pl);
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++)
 #pragma unroll

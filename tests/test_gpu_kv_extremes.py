@@ -87,3 +87,18 @@ def test_queries_near_the_bottom_of_the_range(ctx, fmt, dtype, shape):
     q = (1e-36 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
     want, tol = reference(q, p, own, rows)
     att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_keys_near_the_top_of_the_range(ctx, fmt, dtype, shape):
+    """Keys of 1e37 against queries of 1e-36: the scores are ordinary numbers, and so is the answer."""
+    n, heads, kv, d, sq, rows, plen = shape
+
+    def poke(k, v):
+        k *= 1e37
+    cache, own, shared, p = both(ctx, fmt, shape, poke)
+    q = (1e-36 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
+    want, tol = reference(q, p, own, rows)
+    att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol)
