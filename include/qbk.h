@@ -501,8 +501,10 @@ int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *c
  * 0 .. lens[i] - seq_q + t.  The prefix is rows 0 .. prefix_len - 1 of
  * sequence prefix_seq of `prefix` (a cache of the same format, kv heads and
  * head_dim; it may be the same buffer) and is read for 16 or 64 query rows
- * of any sequences at a time, not once a sequence; prefix_len 0 (prefix and prefix_shape NULL) is plain
- * batched attention.  A query that sees no row yields zeros.  Softmax
+ * of any sequences at a time, not once a sequence; prefix_len 0 (prefix and
+ * prefix_shape NULL) is plain batched attention.  A query that sees no row
+ * yields zeros, whatever it holds; one that sees rows and holds a NaN or an
+ * infinity, or sees a row that stands for NaN, yields NaN.  Softmax
  * statistics, scores and sums are f32 (the largest channel of a query times
  * the largest of a key is to stay below 2^128; past it a score is not a
  * number); for QBK_F32 queries and weights are split in two halves so that

@@ -102,3 +102,17 @@ def test_keys_near_the_top_of_the_range(ctx, fmt, dtype, shape):
     q = (1e-36 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
     want, tol = reference(q, p, own, rows)
     att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,d,sq,rows", [(4, 2, 64, 3, 1), (128, 128, 128, 130, 64), (64, 64, 256, 70, 1)])
+def test_a_nan_query_that_sees_nothing_is_zeros(ctx, dtype, heads, kv, d, sq, rows):
+    """Query t sees own rows 0 .. rows - sq + t: the first ones none, whatever they hold."""
+    cache = att.make(ctx, "int8", 1, rows, kv, d)
+    own = att.fill(cache, 20, [rows])
+    q = normal(21, (1, sq, heads, d)).to(getattr(torch, dtype))
+    q[0, 0, 1, 3], q[0, 1, 0, 0] = float("nan"), float("inf")
+    got = att.attend(cache, q, words([rows]), dtype)
+    assert bool((got[0, :sq - rows] == 0).all())
+    want, tol = reference(q.nan_to_num(0.0, 0.0, 0.0), att.empty_prefix(kv, d), own, [rows])
+    att.check(got, want, tol)
