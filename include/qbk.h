@@ -507,9 +507,12 @@ int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *c
  * infinity, or sees a row that stands for NaN, yields NaN.  Softmax
  * statistics, scores and sums are f32 (the largest channel of a query times
  * the largest of a key is to stay below 2^128; past it a score is not a
- * number); for QBK_F32 queries and weights are split in two halves so that
- * the products keep f32's precision.  The result does not depend on what
- * other calls run.  workspace of at least
+ * number).  The products take queries, and weights times their values'
+ * scales, as fp16 numbers relative to the row's largest: two halves, 22 bits,
+ * for QBK_F32, one, 11 bits, for QBK_BF16, whose outputs hold 8; a weight
+ * times scale keeps them down to 2^-26 of the largest that the query sees,
+ * and is off by 2^-36 of that at most below.  Rows that a query does not see
+ * have no part in its result, and other calls neither.  workspace of at least
  * qbk_attention_kv_workspace_size bytes, 16-byte aligned; calls that share
  * one must not overlap. */
 size_t qbk_attention_kv_workspace_size(const qbk_kv_shape *shape, size_t n_heads, size_t n, size_t seq_q,

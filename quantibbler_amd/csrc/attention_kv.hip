@@ -18,8 +18,9 @@
 //
 // Roundings: q is scaled by a power of two and held as fp16 (bf16 queries:
 // exact but for channels 2^-28 of the row's largest) or as two fp16 halves
-// (f32 queries: 22 bits); p times scale likewise, 2^12 above the reference so
-// that a weight keeps its bits down to 2^-26 of the largest.  Sums are f32.
+// (f32 queries: 22 bits); p times scale likewise, 2^12 above a reference of its
+// own, the row's largest of them, so that a weight keeps its bits down to 2^-26
+// of that.  Sums are f32.
 #include <math.h>
 
 #include <atomic>
@@ -258,21 +259,6 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
         for (int k = 0; k < N; k++) qps[r0 + k * AT_ONCE] = __uint_as_float(top[k]);
 }
 
-// The largest value scale vm of a tile against vref, a power of two at or above
-// every one so far: the outputs follow when it moves, vinv = 2^12 / vref.
-template <int CT>
-__device__ __forceinline__ void kva_value_scales(float vm, float &vref, float &vinv, kva_f4_t (&o)[CT]) {
-    if (vm > vref) {  // the same in every lane
-        const uint32_t e = (__float_as_uint(vm) >> 23) + 1;  // scales are 2^-107 .. 2^122
-        const float to = __uint_as_float(e << 23);
-        vinv = __uint_as_float((266 - e) << 23);
-        const float f = vref * __uint_as_float((254 - e) << 23);
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) o[ct] *= f;
-        vref = to;
-    }
-}
-
 // Sums of code products as q k: times the key's scale and the row's power of
 // two, those two first.  Codes reach 448 and a scaled query 16, so a sum by its
 // key's scale alone would pass f32 for keys from some 2^117 on; the two
@@ -295,64 +281,99 @@ __device__ __forceinline__ void kva_mask(kva_f4_t (&t)[4], kva_f4_t (&vs)[4], ui
         }
 }
 
-// The row's reference moves when a score passes it eightfold, its sum and
-// outputs with it.
-template <int CT>
-__device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float scale, float &ref, float &sum,
-                                              kva_f4_t (&o)[CT]) {
+// The largest of a lane's 16.
+__device__ __forceinline__ float kva_most(const kva_f4_t (&t)[4]) {
     float m[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) m[i] = fmaxf(fmaxf(t[i][0], t[i][1]), fmaxf(t[i][2], t[i][3]));
-    const float tm = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+// The row's reference moves when a score passes it eightfold, its sum with it;
+// what the outputs stand for stays, so wref moves the other way.
+__device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float scale, float &ref, float &sum,
+                                              float &wref) {
+    const float tm = kva_most(t);
     if (__ballot(tm * scale > ref + 3.0f)) {
         const float to = fmaxf(ref, ceilf(kva_max4(tm) * scale));
         const float f = kva_rescale(ref, to);
         sum *= f;
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) o[ct] *= f;
+        wref *= f;
         ref = to;
     }
 }
 
-// Scores to weights: p = exp2(t scale - ref) into sum, p times the value scales
-// as operands ph (and pl, what the first half leaves).
-template <bool HI>
-__device__ __forceinline__ void kva_weights(const kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float scale, float ref,
-                                            float &sum, kva_h8_t (&ph)[2], kva_h8_t (&pl)[2]) {
+// Scores to weights: p = exp2(t scale - ref) into sum, t becomes p times the
+// value's scale.
+__device__ __forceinline__ void kva_weights(kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float scale, float ref,
+                                            float &sum) {
     const float base = ref == -INFINITY ? 0.0f : ref;  // a row that has seen nothing: every p is 0
     float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            kva_f2_t w;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j + e], scale, -base));
-                l[i] += p;
-                w[e] = p * vs[i][j + e];
-            }
-            const kva_h2_t h = __builtin_convertvector(w, kva_h2_t);
-            ph[i >> 1][4 * (i & 1) + j] = h[0];
-            ph[i >> 1][4 * (i & 1) + j + 1] = h[1];
-            if constexpr (HI) {
-                const kva_h2_t r = __builtin_convertvector(w - __builtin_convertvector(h, kva_f2_t), kva_h2_t);
-                pl[i >> 1][4 * (i & 1) + j] = r[0];
-                pl[i >> 1][4 * (i & 1) + j + 1] = r[1];
-            }
+        for (int j = 0; j < 4; j++) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j], scale, -base));
+            l[i] += p;
+            t[i][j] = p * vs[i][j];
         }
     sum += (l[0] + l[1]) + (l[2] + l[3]);
 }
 
+// Weights w = p times value scale against wref, a power of two above every one
+// that the row has seen (or an eighth of it): the outputs follow when it moves.
+// It is the row's own and of rows that it sees alone, and p is in it, so that
+// neither a value that the mask hides nor a large one of little weight costs
+// the others their bits.  A row's likeliest key has p of 1/2 and more and a
+// scale of 2^-109 and more, so wref is 2^-113 and more as soon as a weight is
+// not 0, and at most 2^126.
+template <int CT>
+__device__ __forceinline__ void kva_weight_reference(const kva_f4_t (&w)[4], float &wref, kva_f4_t (&o)[CT]) {
+    const float wm = kva_most(w);
+    if (__ballot(wm > 8.0f * wref)) {
+        const float most = kva_max4(wm);
+        if (most > 8.0f * wref) {
+            uint32_t e = (__float_as_uint(most) >> 23) + 1;
+            e = e < 12 ? 12 : e > 253 ? 253 : e;  // what a row that is no number has seen
+            const float f = wref * __uint_as_float((254 - e) << 23);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) o[ct] *= f;
+            wref = __uint_as_float(e << 23);
+        }
+    }
+}
+
+// Weights in units of 2^-12 wref as operands ph (and pl, what the first half
+// leaves).
+template <bool HI>
+__device__ __forceinline__ void kva_operands(const kva_f4_t (&w)[4], float wref, kva_h8_t (&ph)[2],
+                                             kva_h8_t (&pl)[2]) {
+    const float inv = __uint_as_float((266u << 23) - __float_as_uint(wref));  // 2^12 / wref; of 0 a number, weights are 0
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            const kva_f2_t x = {w[i][j] * inv, w[i][j + 1] * inv};
+            const kva_h2_t h = __builtin_convertvector(x, kva_h2_t);
+            ph[i >> 1][4 * (i & 1) + j] = h[0];
+            ph[i >> 1][4 * (i & 1) + j + 1] = h[1];
+            if constexpr (HI) {
+                const kva_h2_t r = __builtin_convertvector(x - __builtin_convertvector(h, kva_f2_t), kva_h2_t);
+                pl[i >> 1][4 * (i & 1) + j] = r[0];
+                pl[i >> 1][4 * (i & 1) + j + 1] = r[1];
+            }
+        }
+}
+
 // A wave's running state for its 16 rows: reference, sum of weights and
-// weighted values (O^T, channel 16 ct + 4 g + j of row col) over vref's 2^12.
+// weighted values (O^T, channel 16 ct + 4 g + j of row col) over wref's 2^12.
 template <int DC>
 struct KvaState {
     kva_f4_t o[4 * DC];
-    float ref, sum, qp, vref, vinv;
+    float ref, sum, qp, wref;
     uint32_t lim;
     __device__ __forceinline__ KvaState(float qp, uint32_t lim)
-        : ref(-INFINITY), sum(0.0f), qp(qp), vref(0.0f), vinv(0.0f), lim(lim) {
+        : ref(-INFINITY), sum(0.0f), qp(qp), wref(0.0f), lim(lim) {
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++) o[ct] = kva_f4_t{0, 0, 0, 0};
     }
@@ -465,16 +486,12 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
         // the key registers are free again
         kva_scores(s, ks, st.qp);
         if (more) load_k(tt + KVA_WAVES);
-        float vm = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) vm = fmaxf(fmaxf(fmaxf(vm, vs[i][0]), fmaxf(vs[i][1], vs[i][2])), vs[i][3]);
-        if (__ballot(vm > st.vref)) kva_value_scales(kva_scalar(kva_max4(vm)), st.vref, st.vinv, st.o);
-#pragma unroll
-        for (int i = 0; i < 4; i++) vs[i] *= st.vinv;
-        kva_h8_t ph[2], pl[2];
         if (masked) kva_mask(s, vs, key0 + 4 * g, st.lim);
-        kva_reference(s, a.scale, st.ref, st.sum, st.o);
-        kva_weights<HI>(s, vs, a.scale, st.ref, st.sum, ph, pl);
+        kva_reference(s, a.scale, st.ref, st.sum, st.wref);
+        kva_weights(s, vs, a.scale, st.ref, st.sum);
+        kva_weight_reference(s, st.wref, st.o);
+        kva_h8_t ph[2], pl[2];
+        kva_operands<HI>(s, st.wref, ph, pl);
         // fp8 rows that were never written may hold NaN codes
         kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
         if (FMT == QBK_KV_FP8 && masked) keep = kva_keep(key0, written, g);
@@ -513,7 +530,7 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     constexpr int OC = L::OC, LD = OC + 4;
     float *ob = (float *)smem;  // [wave][16 rows][LD]
     const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0;
-    const float f = kva_rescale(st.ref, largest(col)) * st.vref * 0x1p-12f;
+    const float f = kva_rescale(st.ref, largest(col)) * st.wref * 0x1p-12f;
 #pragma unroll
     for (int c0 = 0; c0 < 64 * DC; c0 += OC) {
         if (c0 >= hd) continue;
@@ -554,7 +571,7 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
 // behind 16384, 32/8 heads of 128: 244 MB in 54.4 us, 4.5 TB/s.
 template <int DC>
 struct KvaStage {
-    static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 528, BUFS = DC < 4 ? 2 : 1;
+    static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 512, BUFS = DC < 4 ? 2 : 1;
 };
 template <int DC, bool HI>
 struct KvaWideLds {
@@ -611,9 +628,6 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
         if (wave < 2) {
             const float x = tail && key0 + lane >= written ? 0.0f : sc[at];
             *(float *)(buf + 2 * KEYS + wave * 256 + lane * 4) = x;
-            // the largest value scale, NaN aside: no scale is negative
-            const uint32_t most = kva_row_max<64>(x == x ? __float_as_uint(x) : 0u);
-            if (tid == 64) *(uint32_t *)(buf + 2 * KEYS + 512) = most;
         }
     };
     if (tile0 < tile1) load(tile0, 0);
@@ -638,7 +652,6 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
         const uint32_t key0 = tt * 64;
         if (key0 >= most) return;
         kva_f4_t ks[4], vs[4], s[4];
-        const float vm = kva_scalar(*(const float *)(buf + 2 * KEYS + 512));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             ks[i] = *(const kva_f4_t *)(buf + 2 * KEYS + (16 * i + 4 * g) * 4);
@@ -653,14 +666,13 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
                 s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[x], s[i], 0, 0, 0);
                 if constexpr (HI) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[x], s[i], 0, 0, 0);
             }
-        kva_value_scales(vm, st.vref, st.vinv, st.o);
-#pragma unroll
-        for (int i = 0; i < 4; i++) vs[i] *= st.vinv;
         kva_scores(s, ks, st.qp);
         if (key0 + 64 > least) kva_mask(s, vs, key0 + 4 * g, st.lim);
-        kva_reference(s, a.scale, st.ref, st.sum, st.o);
+        kva_reference(s, a.scale, st.ref, st.sum, st.wref);
+        kva_weights(s, vs, a.scale, st.ref, st.sum);
+        kva_weight_reference(s, st.wref, st.o);
         kva_h8_t ph[2], pl[2];
-        kva_weights<HI>(s, vs, a.scale, st.ref, st.sum, ph, pl);
+        kva_operands<HI>(s, st.wref, ph, pl);
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++)
 #pragma unroll
@@ -682,7 +694,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
             if (tt + BUFS < tile1) load(tt + BUFS, p);
             work(tt, buf);
         }
-    const float l = kva_sum4(st.sum), f = st.vref * 0x1p-12f;
+    const float l = kva_sum4(st.sum), f = st.wref * 0x1p-12f;
     if (r >= n_rows) return;
     if (last) {
         T *dst = kva_out_row<T>(a, row0 + r, hk) + 4 * g;

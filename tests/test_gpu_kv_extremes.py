@@ -116,3 +116,56 @@ def test_a_nan_query_that_sees_nothing_is_zeros(ctx, dtype, heads, kv, d, sq, ro
     assert bool((got[0, :sq - rows] == 0).all())
     want, tol = reference(q.nan_to_num(0.0, 0.0, 0.0), att.empty_prefix(kv, d), own, [rows])
     att.check(got, want, tol)
+
+
+@pytest.mark.parametrize("power", [20, 45, 100])
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[4] > 1])
+def test_a_value_that_only_the_last_query_sees(ctx, fmt, dtype, shape, power):
+    """The last query's own row is 2^power times the others: the queries before it answer as if it were not there."""
+    n, heads, kv, d, sq, rows, plen = shape
+
+    def poke(k, v):
+        if v.shape[0] == sum(rows):
+            v[np.cumsum(rows) - 1] *= 2.0 ** power
+    cache, own, shared, p = both(ctx, fmt, shape, poke)
+    q = normal(n + d, (n, sq, heads, d)).to(getattr(torch, dtype))
+    got = att.attend(cache, q, words(rows), dtype, shared, plen)
+    want, tol = reference(q, p, own, rows)
+    att.check(got, want, tol)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("where", [0, 7, -1])
+def test_a_large_value_of_next_to_no_weight(ctx, fmt, dtype, shape, where):
+    """A row of 1e15 whose weight is some e^-60 of the others': seen by every query, and still nothing to it."""
+    n, heads, kv, d, sq, rows, plen = shape
+
+    def poke(k, v):
+        k *= 0.3
+        at = where if plen or where >= 0 else 3
+        if v.shape[0] != sum(rows) or not plen:
+            k[at], v[at] = -60.0 * d ** -0.5, v[at] * 1e15
+    cache, own, shared, p = both(ctx, fmt, shape, poke)
+    q = (1.0 + 0.1 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
+    want, tol = reference(q, p, own, rows)
+    att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHAPES[:6])
+def test_contributions_that_change_places(ctx, dtype, shape):
+    """Scores that rise by 30 every 16 rows, twice in 48, while the values fall by 2^45 each time or rise by as much."""
+    n, heads, kv, d, sq, rows, plen = shape
+    for fall in (-45.0, 45.0):
+        def poke(k, v):
+            tile = (torch.arange(k.shape[0], device="cuda") // 16 % 3).float()[:, None, None]
+            k.mul_(0.1).add_(tile * 30.0 * d ** -0.5)
+            v.mul_(torch.exp2(tile * fall))
+        cache, own, shared, p = both(ctx, "int8", shape, poke)
+        q = (1.0 + 0.1 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
+        want, tol = reference(q, p, own, rows)
+        att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol, f"{fall}")
