@@ -295,7 +295,8 @@ __device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float scal
                                               float &wref) {
     const float tm = kva_most(t);
     if (__ballot(tm * scale > ref + 3.0f)) {
-        const float to = fmaxf(ref, ceilf(kva_max4(tm) * scale));
+        const float most = kva_max4(tm) * scale;
+        const float to = most > ref + 3.0f ? ceilf(most) : ref;  // other rows' scores move no more than theirs
         const float f = kva_rescale(ref, to);
         sum *= f;
         wref *= f;

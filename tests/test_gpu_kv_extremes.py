@@ -169,3 +169,20 @@ def test_contributions_that_change_places(ctx, dtype, shape):
         q = (1.0 + 0.1 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
         want, tol = reference(q, p, own, rows)
         att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol, f"{fall}")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[4] > 1])
+def test_what_a_query_does_not_see_has_no_part(ctx, dtype, shape):
+    """The last query's own row, changed: the queries before it stay as they were, bit for bit."""
+    n, heads, kv, d, sq, rows, plen = shape
+    q = normal(n + d, (n, sq, heads, d)).to(getattr(torch, dtype))
+    got = []
+    for factor in (1.0, 40.0):
+        def poke(k, v):
+            if v.shape[0] == sum(rows):
+                k[np.cumsum(rows) - 1] *= factor
+                v[np.cumsum(rows) - 1] *= factor ** 8
+        cache, own, shared, p = both(ctx, "int8", shape, poke)
+        got.append(att.attend(cache, q, words(rows), dtype, shared, plen))
+    assert torch.equal(got[0][:, :-1], got[1][:, :-1]) and not torch.equal(got[0][:, -1], got[1][:, -1])
