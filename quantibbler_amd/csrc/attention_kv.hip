@@ -7,7 +7,7 @@
 // sequence's own rows are seen by its sq G rows alone.  Both kinds are items of
 // one launch:
 //   item = (kv head, 16 or 64 rows, run of 64-row key tiles)
-// and leave a partial result (sum of weights, weighted values, reference) per
+// and leave a partial result (sum of weights, mean of values, reference) per
 // row; a second launch joins them.  A key tile and 16 rows, a wave:
 //   S^T = K q^T      v_mfma_f32_16x16x32_f16, codes widened to fp16 (exact)
 //   p = exp2(s - M)  online, per query column; M is a whole number, so moving
@@ -62,7 +62,7 @@ struct KvAttArgs {
     const void *q;
     void *out;
     const uint32_t *lens;
-    float *po;    // [split][hk][rho][hd] weighted values
+    float *po;    // [split][hk][rho][hd] weighted means of the values
     float2 *ml;   // [split][hk][rho] reference, sum of weights
     uint32_t first_seq, prefix_seq, prefix_len, max_len;
     uint32_t plus;                   // 1: lens are positions, the rows before the one just written
@@ -392,6 +392,12 @@ __device__ __forceinline__ kva_u4_t kva_keep(uint32_t key0, uint32_t written, in
     return keep;
 }
 
+// What outputs times wref are a mean of values by (a last place of f32 off):
+// sums of values may pass f32 where their mean does not, so none is formed.
+__device__ __forceinline__ float kva_per(float sum) {
+    return sum == 0.0f ? 0.0f : 0x1p-12f * __builtin_amdgcn_rcpf(sum);
+}
+
 // Where row rho's output goes.
 template <typename T>
 __device__ __forceinline__ T *kva_out_row(const KvAttArgs &a, uint32_t rho, uint32_t hk) {
@@ -516,29 +522,22 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
         sums[wave * 16 + col] = l;
     }
     __syncthreads();
-    auto largest = [&](int r) {
-        float m = refs[r];
+    float2 row = {refs[col], 0.0f};  // row col's reference and sum of weights
 #pragma unroll
-        for (int w = 1; w < KVA_WAVES; w++) m = fmaxf(m, refs[w * 16 + r]);
-        return m;
-    };
-    auto total = [&](int r, float m) {
-        float l = 0.0f;
+    for (int w = 1; w < KVA_WAVES; w++) row.x = fmaxf(row.x, refs[w * 16 + col]);
 #pragma unroll
-        for (int w = 0; w < KVA_WAVES; w++) l += sums[w * 16 + r] * kva_rescale(refs[w * 16 + r], m);
-        return l;
-    };
+    for (int w = 0; w < KVA_WAVES; w++) row.y += sums[w * 16 + col] * kva_rescale(refs[w * 16 + col], row.x);
     constexpr int OC = L::OC, LD = OC + 4;
     float *ob = (float *)smem;  // [wave][16 rows][LD]
     const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0;
-    const float f = kva_rescale(st.ref, largest(col)) * st.wref * 0x1p-12f;
+    const float per = kva_per(row.y), f = kva_rescale(st.ref, row.x) * st.wref;
 #pragma unroll
     for (int c0 = 0; c0 < 64 * DC; c0 += OC) {
         if (c0 >= hd) continue;
         if (c0) __syncthreads();  // what the region held has been read
 #pragma unroll
         for (int k = 0; k < OC / 16; k++)
-            *(kva_f4_t *)(ob + (wave * 16 + col) * LD + 16 * k + 4 * g) = st.o[c0 / 16 + k] * f;
+            *(kva_f4_t *)(ob + (wave * 16 + col) * LD + 16 * k + 4 * g) = st.o[c0 / 16 + k] * per * f;
         __syncthreads();
         for (int x = tid; x < 16 * OC; x += 64 * KVA_WAVES) {
             const int r = x / OC, c = x % OC;
@@ -546,18 +545,11 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < KVA_WAVES; w++) v += ob[(w * 16 + r) * LD + c];
-            if (last) {
-                const float l = total(r, largest(r));
-                kva_out_row<T>(a, row0 + r, hk)[c0 + c] = kva_out<T>(l == 0.0f ? 0.0f : v / l);
-            } else {
-                a.po[(part + r) * hd + c0 + c] = v;
-            }
+            if (last) kva_out_row<T>(a, row0 + r, hk)[c0 + c] = kva_out<T>(v);
+            else a.po[(part + r) * hd + c0 + c] = v;
         }
     }
-    if (!last && tid < (int)n_rows) {
-        const float m = largest(tid);
-        a.ml[part + tid] = float2{m, total(tid, m)};
-    }
+    if (!last && tid < (int)n_rows) a.ml[part + tid] = row;
 }
 
 // The body of many rows: four waves of 16 rows, every wave every key tile.  A
@@ -695,7 +687,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
             if (tt + BUFS < tile1) load(tt + BUFS, p);
             work(tt, buf);
         }
-    const float l = kva_sum4(st.sum), f = st.wref * 0x1p-12f;
+    const float l = kva_sum4(st.sum), per = kva_per(l);
     if (r >= n_rows) return;
     if (last) {
         T *dst = kva_out_row<T>(a, row0 + r, hk) + 4 * g;
@@ -703,13 +695,13 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
         for (int ct = 0; ct < 4 * DC; ct++)
             if (ct < nc)
 #pragma unroll
-                for (int j = 0; j < 4; j++) dst[16 * ct + j] = kva_out<T>(l == 0.0f ? 0.0f : st.o[ct][j] * f / l);
+                for (int j = 0; j < 4; j++) dst[16 * ct + j] = kva_out<T>(st.o[ct][j] * per * st.wref);
     } else {
         const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0 + r;
         float *dst = a.po + part * hd + 4 * g;
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++)
-            if (ct < nc) *(kva_f4_t *)(dst + 16 * ct) = st.o[ct] * f;
+            if (ct < nc) *(kva_f4_t *)(dst + 16 * ct) = st.o[ct] * per * st.wref;
         if (g == 0) a.ml[part] = float2{st.ref, l};
     }
 }
@@ -790,7 +782,7 @@ __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
     const uint32_t c = 4 * (lane % LANES), sub = lane / LANES;
     const float *src = a.po + ((size_t)hk * a.rows + rho) * hd + (c < hd ? c : 0);
     const size_t apart = (size_t)Hk * a.rows * hd;
-    float M = -INFINITY, f = 0.0f, lf = 0.0f;
+    float share = 0.0f;  // of the row's weights, this lane's split's
     kva_f4_t v = {0, 0, 0, 0};
 #pragma unroll
     for (int b = 0; b < N; b += BATCH) {
@@ -802,18 +794,19 @@ __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
             if ((b + k) * STEP < (int)splits) x[k] = *(const kva_f4_t *)(src + (s < splits ? s : splits - 1) * apart);
         }
         if (b == 0) {
-            M = m;
+            float M = m;
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-            f = lane < splits ? kva_rescale(m, M) : 0.0f;
-            lf = lane < splits ? l * f : 0.0f;
+            const float own = lane < splits ? l * kva_rescale(m, M) : 0.0f;
+            float sum = own;
 #pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) lf += __shfl_xor(lf, o, 64);
+            for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            share = sum == 0.0f ? 0.0f : own / sum;
         }
 #pragma unroll
         for (int k = 0; k < BATCH; k++) {
             const uint32_t s = (b + k) * STEP + sub;
-            const float fs = __shfl(f, (int)(s < 64 ? s : 63), 64);
+            const float fs = __shfl(share, (int)(s < 64 ? s : 63), 64);
             if (s < splits) v += x[k] * fs;
         }
     }
@@ -824,7 +817,7 @@ __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
     if (lane >= LANES || c >= hd) return;
     T *dst = kva_out_row<T>(a, rho, hk) + c;
 #pragma unroll
-    for (int e = 0; e < 4; e++) dst[e] = kva_out<T>(lf == 0.0f ? 0.0f : v[e] / lf);
+    for (int e = 0; e < 4; e++) dst[e] = kva_out<T>(v[e]);
 }
 
 // How a call is cut: row tiles (16 or 64 rows) and splits of the prefix and of

@@ -186,3 +186,18 @@ def test_what_a_query_does_not_see_has_no_part(ctx, dtype, shape):
         cache, own, shared, p = both(ctx, "int8", shape, poke)
         got.append(att.attend(cache, q, words(rows), dtype, shared, plen))
     assert torch.equal(got[0][:, :-1], got[1][:, :-1]) and not torch.equal(got[0][:, -1], got[1][:, -1])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_values_near_the_top_of_the_range(ctx, fmt, dtype, shape):
+    """Values of some 1e38, all of one sign, with weights all alike: their mean is a number, if their sum is not."""
+    n, heads, kv, d, sq, rows, plen = shape
+
+    def poke(k, v):
+        v.uniform_(0.7e38, 1.3e38)
+    cache, own, shared, p = both(ctx, fmt, shape, poke)
+    q = (0.05 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
+    want, tol = reference(q, p, own, rows)
+    att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol)
