@@ -919,9 +919,8 @@ static int kva_check(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq,
         (n && (unsigned __int128)n * sq * (n_heads / s->n_kv_heads) > 0x7FFFFFFFull))
         return fail(QBK_ERR_VALIDATION, "kv attention: too many query rows for one launch");
     const KvaPlan p = n ? kva_plan(s, n_heads, n, sq, max_len, prefix_len) : KvaPlan{};
-    // a launch is below 2^32 threads; the join, launched unless one split is all there is, takes four rows a workgroup
-    const bool join = p.sp + p.ss != 1;
-    if (p.items > 0xFFFFFF || (unsigned __int128)n * sq * n_heads > (join ? 4 * 0xFFFFFFull : 0x7FFFFFFFull))
+    // a launch is below 2^32 threads; the join takes four rows a workgroup
+    if (p.items > 0xFFFFFF || (unsigned __int128)n * sq * n_heads > (p.bytes ? 4 * 0xFFFFFFull : 0x7FFFFFFFull))
         return fail(QBK_ERR_VALIDATION, "kv attention: too many query rows for one launch");
     return QBK_OK;
 }
