@@ -219,6 +219,19 @@ def _bf16_values(a) -> np.ndarray:
     return (r << 16).view(np.float32)
 
 
+def _memory_of(stream):
+    """torch's allocations within come from the pool of ``stream`` (as the
+    device calls take it): no other stream's work is still using them, and
+    once freed they go to work that this stream runs later."""
+    import torch
+
+    if not stream:
+        stream = torch.cuda.default_stream()
+    elif not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream if isinstance(stream, int) else stream.cuda_stream)
+    return torch.cuda.stream(stream)
+
+
 class DeviceModel:
     """The transformer trunk on the device at bf16 serving (Engine::forward,
     engine/mod.rs:802-806, and forward_prefill's per-token loop, :811-822):
@@ -275,7 +288,15 @@ class DeviceModel:
             b.reset()
         self.pos = 0
         self.positions = [0] * self.n_seqs
+        self._wait_shared()
         self._shared = None
+
+    def _wait_shared(self):
+        """Steps behind a shared prefix, on whatever stream, are through with its memory."""
+        import torch
+
+        if self._shared is not None:
+            torch.cuda.synchronize()
 
     def prefill(self, tokens, stream=None, seq: int = 0):
         """forward_prefill (engine/mod.rs:811-822) of a new sequence (held as
@@ -304,10 +325,11 @@ class DeviceModel:
         md = self.md
         ids = [int(t) for t in tokens]
         n = len(ids)
-        h = torch.empty((n, md.d_model), dtype=torch.float32, device="cuda")
-        embed(self.ctx, self.embedding, md.vocab_size, md.d_model, ids, h, stream)
         need = max(b.prefill_workspace_size(n) for b in self.blocks)
-        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        with _memory_of(stream):
+            h = torch.empty((n, md.d_model), dtype=torch.float32, device="cuda")
+            ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        embed(self.ctx, self.embedding, md.vocab_size, md.d_model, ids, h, stream)
         for b in self.blocks:
             b.prefill_seq_dev(int(seq), h, n, ws, need, stream)
         self.positions[int(seq)] = n
@@ -371,10 +393,11 @@ class DeviceModel:
             raise ValueError(f"a batch of {n} sequences on a model holding {self.n_seqs}")
         if n not in self._batch:
             wn = max(b.decode_batch_workspace_size(n) for b in self.blocks)
-            self._batch[n] = (torch.empty((n, md.d_model), dtype=torch.float32, device="cuda"),
-                              torch.empty((n, md.d_model), dtype=torch.float32, device="cuda"),
-                              torch.empty((n, md.vocab_size), dtype=torch.float32, device="cuda"),
-                              torch.empty(wn, dtype=torch.uint8, device="cuda"), wn)
+            with _memory_of(stream):
+                self._batch[n] = (torch.empty((n, md.d_model), dtype=torch.float32, device="cuda"),
+                                  torch.empty((n, md.d_model), dtype=torch.float32, device="cuda"),
+                                  torch.empty((n, md.vocab_size), dtype=torch.float32, device="cuda"),
+                                  torch.empty(wn, dtype=torch.uint8, device="cuda"), wn)
         h, hn, logits, ws, wn = self._batch[n]
         if dev_ids:
             embed_dev(self.ctx, self.embedding, md.vocab_size, md.d_model, tokens, n, h, stream)
@@ -412,6 +435,7 @@ class DeviceModel:
             return KvCache.size(fmt, seqs, rows, md.n_kv_heads, md.head_dim)
 
         size(1, n), size(int(n_seqs), int(capacity))  # refusals come before sequence 0 is replaced
+        self._wait_shared()
         logits = self.prefill(tokens, stream)
 
         def cache(seqs, rows):
@@ -419,21 +443,21 @@ class DeviceModel:
             return KvCache(self.ctx, fmt, seqs, rows, md.n_kv_heads, md.head_dim,
                            torch.empty(need, dtype=torch.uint8, device="cuda"))
 
-        pos = torch.zeros(int(n_seqs), dtype=torch.int32, device="cuda")
-        torch.cuda.current_stream().synchronize()  # the positions are there, whatever stream reads them
-        prefixes, caches = [], []
-        for b in self.blocks:
-            k, v = b.cache_ptrs()
-            prefixes.append(cache(1, n))
-            prefixes[-1].write_dev(k, v, "float32", pos, n, row_stride=kd, stream=stream)
-            caches.append(cache(int(n_seqs), int(capacity)))
-        need = max(b.decode_kv_workspace_size(c, int(n_seqs), prefix_len=n) for b, c in zip(self.blocks, caches))
-        d = md.d_model
-        self._shared = {"n": int(n_seqs), "prefix": prefixes, "len": n, "own": caches, "pos": pos, "steps": 0,
-                        "h": torch.empty((int(n_seqs), d), dtype=torch.float32, device="cuda"),
-                        "hn": torch.empty((int(n_seqs), d), dtype=torch.float32, device="cuda"),
-                        "logits": torch.empty((int(n_seqs), md.vocab_size), dtype=torch.float32, device="cuda"),
-                        "ws": torch.empty(need, dtype=torch.uint8, device="cuda"), "need": need}
+        d, seqs = md.d_model, int(n_seqs)
+        with _memory_of(stream):
+            pos = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+            prefixes, caches = [], []
+            for b in self.blocks:
+                k, v = b.cache_ptrs()
+                prefixes.append(cache(1, n))
+                prefixes[-1].write_dev(k, v, "float32", pos, n, row_stride=kd, stream=stream)
+                caches.append(cache(seqs, int(capacity)))
+            need = max(b.decode_kv_workspace_size(c, seqs, prefix_len=n) for b, c in zip(self.blocks, caches))
+            self._shared = {"n": seqs, "prefix": prefixes, "len": n, "own": caches, "pos": pos, "steps": 0,
+                            "h": torch.empty((seqs, d), dtype=torch.float32, device="cuda"),
+                            "hn": torch.empty((seqs, d), dtype=torch.float32, device="cuda"),
+                            "logits": torch.empty((seqs, md.vocab_size), dtype=torch.float32, device="cuda"),
+                            "ws": torch.empty(need, dtype=torch.uint8, device="cuda"), "need": need}
         return logits
 
     def step_shared(self, tokens, stream=None):
