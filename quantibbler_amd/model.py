@@ -30,6 +30,8 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
+from ._lib import KernelError
+
 
 class ModelError(ValueError):
     """A model directory that cannot be read (the reference's load error)."""
@@ -354,6 +356,8 @@ class DeviceModel:
         ids = [int(t) for t in tokens]
         if len(ids) < 2:
             raise ValueError(f"a score needs at least two tokens, got {len(ids)}")
+        if not 0 <= k <= min(64, md.vocab_size):  # as logprobs_dev, before the sequence is replaced
+            raise KernelError(f"logprobs top_k must be at most 64 and the vocabulary of {md.vocab_size}, got {k}")
         h, n, ws = self._prefill_rows(ids, stream, seq)
         targets = torch.tensor(ids[1:], dtype=torch.int32, device="cuda")
         torch.cuda.current_stream().synchronize()  # the targets are there, whatever stream reads them
