@@ -56,6 +56,63 @@ def _stream(s):
     raise TypeError(f"cannot take a stream handle of {type(s)!r}")
 
 
+_SERVING_DTYPES = {"float32": _lib.QBK_F32, "bfloat16": _lib.QBK_BF16}
+_TORCH_DTYPES = {}
+
+
+def _device_values(x, dtype: str, n: int, ctx, what: str, strided: bool = False):
+    """The address of ``x``: None, a raw device address the caller vouches
+    for, or a contiguous tensor of ``dtype`` on the context's device with at
+    least n values -- strided: any, with n values of its memory from its
+    first one on."""
+    if x is None or isinstance(x, int):
+        return x
+    try:
+        if dtype not in _TORCH_DTYPES:
+            import torch
+
+            _TORCH_DTYPES[dtype] = getattr(torch, dtype)
+        if x.dtype is _TORCH_DTYPES[dtype] and x.get_device() == ctx.device_index and (
+                x.is_contiguous() and x.numel() >= n or
+                strided and x.untyped_storage().nbytes() // x.element_size() - x.storage_offset() >= n):
+            return x.data_ptr()
+        got = f"{x.dtype} of {tuple(x.shape)}{'' if x.is_contiguous() else ', not contiguous,'} on {x.device}"
+    except AttributeError:
+        got = repr(type(x))
+    raise _lib.KernelError(f"{what} must be a{' contiguous' * (not strided)} {dtype} tensor on device {ctx.device_index} "
+                           f"with room for {n} values; got {got}")
+
+
+def _device_bytes(x, n: int, ctx, what: str):
+    """The address of ``x``: None, a raw device address, or a contiguous
+    tensor of any type on the context's device of at least n bytes."""
+    if x is None or isinstance(x, int):
+        return x
+    try:
+        if x.get_device() == ctx.device_index and x.is_contiguous() and x.numel() * x.element_size() >= n:
+            return x.data_ptr()
+        got = f"{x.numel() * x.element_size()} bytes on {x.device}"
+    except AttributeError:
+        got = repr(type(x))
+    raise _lib.KernelError(f"{what} must be a contiguous tensor on device {ctx.device_index} of at least {n} bytes; got "
+                           f"{got}")
+
+
+def _device_words(x, n: int, ctx, what: str):
+    """The address of ``x``: None, a raw device address the caller vouches
+    for, or a contiguous 32-bit integer tensor on the context's device of at
+    least n entries."""
+    if x is None or isinstance(x, int):
+        return x
+    if not hasattr(x, "is_cuda"):
+        raise _lib.KernelError(f"{what} must be a device tensor or a device address")
+    if not x.is_cuda or x.element_size() != 4 or x.is_floating_point() or not x.is_contiguous() or x.numel() < n \
+            or x.get_device() != ctx.device_index:
+        raise _lib.KernelError(f"{what} must be a contiguous 32-bit device tensor of at least {n} entries; got "
+                               f"{x.dtype} of {x.numel()} on {x.device}")
+    return x.data_ptr()
+
+
 def gpu_available() -> bool:
     """gpu.rs:187-189."""
     return bool(_lib.load().qbk_gpu_available())
@@ -285,10 +342,21 @@ def logprobs_dev(ctx: GpuContext, logits, rows: int, vocab: int, targets, logpro
     and the ``top_k`` likeliest tokens, ids and log probabilities in order,
     into ``top_ids`` / ``top_logprobs`` [rows][top_k] (equal logits: the lower
     id first).  ``targets`` with ``logprobs``, and ``entropy``, may be None."""
-    check(_lib.load().qbk_logprobs_dev(ctx.handle, _ptr(logits), _DTYPES[dtype][0], int(rows), int(vocab),
-                                       int(vocab if row_stride is None else row_stride), _ptr(targets),
-                                       _ptr(logprobs), _ptr(entropy), int(top_k), _ptr(top_ids), _ptr(top_logprobs),
-                                       _ptr(workspace), int(workspace_size), _stream(stream)))
+    code = _SERVING_DTYPES.get(dtype)
+    if code is None:
+        raise _lib.KernelError(f"logprobs takes 'float32' or 'bfloat16' logits, got {dtype!r}")
+    rows, vocab, k, stride = int(rows), int(vocab), int(top_k), int(vocab if row_stride is None else row_stride)
+    if min(rows, vocab, k, stride) < 0:
+        raise _lib.KernelError("logprobs sizes must not be negative")
+    x = _device_values(logits, dtype, (rows - 1) * stride + vocab if rows else 0, ctx, "logprobs: logits",
+                       row_stride is not None)
+    check(_lib.load().qbk_logprobs_dev(
+        ctx.handle, x, code, rows, vocab, stride, _device_words(targets, rows, ctx, "targets"),
+        _device_values(logprobs, "float32", rows, ctx, "logprobs: logprobs"),
+        _device_values(entropy, "float32", rows, ctx, "logprobs: entropy"), k,
+        _device_words(top_ids, rows * k, ctx, "top_ids"),
+        _device_values(top_logprobs, "float32", rows * k, ctx, "logprobs: top_logprobs"),
+        _device_bytes(workspace, workspace_size, ctx, "logprobs: workspace"), int(workspace_size), _stream(stream)))
 
 
 class KvCache:
@@ -326,15 +394,15 @@ class KvCache:
         return need
 
     def _rows(self, fn, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start, row_stride, stream):
-        code = _KV_DTYPES.get(dtype)
+        code = _SERVING_DTYPES.get(dtype)
         if code is None:
             raise _lib.KernelError(f"kv cache rows must be 'float32' or 'bfloat16', got {dtype!r}")
         n = self.n_seqs - first_seq if n_seqs is None else n_seqs
         stride = self.n_kv_heads * self.head_dim if row_stride is None else row_stride
         if n_rows < 0 or first_seq < 0 or n < 0 or stride < 0:
             raise _lib.KernelError("kv cache rows, sequences and strides must not be negative")
-        at = _device_words(pos, n, "positions")
-        starts = None if row_start is None else _device_words(row_start, n + 1, "row starts")
+        at = _device_words(pos, n, self.ctx, "positions")
+        starts = None if row_start is None else _device_words(row_start, n + 1, self.ctx, "row starts")
         check(fn(self.ctx.handle, self._shape_ref, self._base, _ptr(k), _ptr(v), code, stride, n_rows, starts, at,
                  first_seq, n, _stream(stream)))
 
@@ -374,7 +442,7 @@ class KvCache:
         among them), at most ``max_len`` (the capacity if None).  Every query
         also sees rows 0 .. prefix_len - 1 of ``prefix``'s sequence
         ``prefix_seq``, read for 16 or 64 query rows of the batch at a time."""
-        code = _KV_DTYPES.get(dtype)
+        code = _SERVING_DTYPES.get(dtype)
         if code is None:
             raise _lib.KernelError(f"kv attention takes 'float32' or 'bfloat16' queries, got {dtype!r}")
         n = self.n_seqs - first_seq if n_seqs is None else n_seqs
@@ -383,27 +451,11 @@ class KvCache:
             raise _lib.KernelError("kv attention sizes must not be negative")
         if prefix_len and prefix is None:
             raise _lib.KernelError("a prefix_len needs the cache that holds the prefix")
-        words = _device_words(lens, n, "lengths")
+        words = _device_words(lens, n, self.ctx, "lengths")
         shared, base = (prefix._shape_ref, prefix._base) if prefix_len else (None, None)
         check(_lib.load().qbk_attention_kv_dev(
             self.ctx.handle, self._shape_ref, self._base, first_seq, n, words, most, shared, base, prefix_seq,
             prefix_len, n_heads, seq_q, _ptr(q), code, _ptr(out), _ptr(workspace), workspace_size, _stream(stream)))
-
-
-_KV_DTYPES = {"float32": _lib.QBK_F32, "bfloat16": _lib.QBK_BF16}
-
-
-def _device_words(x, n: int, what: str) -> int:
-    """The address of ``x``, a contiguous 32-bit integer device tensor of at
-    least n entries, or a raw device address the caller vouches for."""
-    if isinstance(x, int):
-        return x
-    if not hasattr(x, "is_cuda"):
-        raise _lib.KernelError(f"{what} must be a device tensor or a device address")
-    if not x.is_cuda or x.element_size() != 4 or x.is_floating_point() or not x.is_contiguous() or x.numel() < n:
-        raise _lib.KernelError(f"{what} must be a contiguous 32-bit device tensor of at least {n} entries; got "
-                               f"{x.dtype} of {x.numel()} on {x.device}")
-    return x.data_ptr()
 
 
 class SageDecodeState:
@@ -581,7 +633,7 @@ class DecoderBlock:
             raise _lib.KernelError("kv decode sizes must not be negative")
         if prefix_len and prefix is None:
             raise _lib.KernelError("a prefix_len needs the cache that holds the prefix")
-        words = _device_words(pos, n, "positions")
+        words = _device_words(pos, n, self.ctx, "positions")
         shared, base = (prefix._shape_ref, prefix._base) if prefix_len else (None, None)
         check(_lib.load().qbk_block_decode_kv_dev(
             self.ctx.handle, self._h, _ptr(h), words, n, cache._shape_ref, cache._base, first_seq, most, shared, base,
