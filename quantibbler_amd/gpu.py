@@ -51,66 +51,74 @@ def _stream(s):
         return None
     if isinstance(s, int):
         return s
-    if hasattr(s, "cuda_stream"):
+    try:
         return s.cuda_stream
-    raise TypeError(f"cannot take a stream handle of {type(s)!r}")
+    except AttributeError:
+        raise TypeError(f"cannot take a stream handle of {type(s)!r}") from None
 
 
 _SERVING_DTYPES = {"float32": _lib.QBK_F32, "bfloat16": _lib.QBK_BF16}
-_TORCH_DTYPES = {}
+_TORCH_DTYPES = {}  # by name, once a tensor has been seen
 
+
+def _torch_dtypes():
+    import torch
+
+    _TORCH_DTYPES.update(float32=torch.float32, bfloat16=torch.bfloat16, words=(torch.int32, torch.uint32))
+    return _TORCH_DTYPES
+
+
+def _refuse(x, what: str, wanted: str):
+    got = repr(type(x))
+    if hasattr(x, "is_contiguous"):
+        got = f"{x.dtype} of {tuple(x.shape)}{'' if x.is_contiguous() else ', not contiguous,'} on {x.device}"
+    raise _lib.KernelError(f"{what} must be {wanted}; got {got}")
+
+
+# A tensor's address, once it is what a call takes it for.  None and raw device
+# addresses, which the caller vouches for, pass as they are.
 
 def _device_values(x, dtype: str, n: int, ctx, what: str, strided: bool = False):
-    """The address of ``x``: None, a raw device address the caller vouches
-    for, or a contiguous tensor of ``dtype`` on the context's device with at
+    """Of a contiguous tensor of ``dtype`` on the context's device with at
     least n values -- strided: any, with n values of its memory from its
     first one on."""
     if x is None or isinstance(x, int):
         return x
     try:
-        if dtype not in _TORCH_DTYPES:
-            import torch
-
-            _TORCH_DTYPES[dtype] = getattr(torch, dtype)
-        if x.dtype is _TORCH_DTYPES[dtype] and x.get_device() == ctx.device_index and (
+        if x.dtype is (_TORCH_DTYPES or _torch_dtypes())[dtype] and x.get_device() == ctx.device_index and (
                 x.is_contiguous() and x.numel() >= n or
                 strided and x.untyped_storage().nbytes() // x.element_size() - x.storage_offset() >= n):
             return x.data_ptr()
-        got = f"{x.dtype} of {tuple(x.shape)}{'' if x.is_contiguous() else ', not contiguous,'} on {x.device}"
     except AttributeError:
-        got = repr(type(x))
-    raise _lib.KernelError(f"{what} must be a{' contiguous' * (not strided)} {dtype} tensor on device {ctx.device_index} "
-                           f"with room for {n} values; got {got}")
+        pass
+    _refuse(x, what, f"a{' contiguous' * (not strided)} {dtype} tensor on the context's device with room for {n} values")
 
 
 def _device_bytes(x, n: int, ctx, what: str):
-    """The address of ``x``: None, a raw device address, or a contiguous
-    tensor of any type on the context's device of at least n bytes."""
+    """Of a contiguous tensor of any type on the context's device of at
+    least n bytes."""
     if x is None or isinstance(x, int):
         return x
     try:
-        if x.get_device() == ctx.device_index and x.is_contiguous() and x.numel() * x.element_size() >= n:
+        if x.element_size() * x.numel() >= n and x.get_device() == ctx.device_index and x.is_contiguous():
             return x.data_ptr()
-        got = f"{x.numel() * x.element_size()} bytes on {x.device}"
     except AttributeError:
-        got = repr(type(x))
-    raise _lib.KernelError(f"{what} must be a contiguous tensor on device {ctx.device_index} of at least {n} bytes; got "
-                           f"{got}")
+        pass
+    _refuse(x, what, f"a contiguous tensor on the context's device of at least {n} bytes")
 
 
 def _device_words(x, n: int, ctx, what: str):
-    """The address of ``x``: None, a raw device address the caller vouches
-    for, or a contiguous 32-bit integer tensor on the context's device of at
+    """Of a contiguous 32-bit integer tensor on the context's device of at
     least n entries."""
     if x is None or isinstance(x, int):
         return x
-    if not hasattr(x, "is_cuda"):
-        raise _lib.KernelError(f"{what} must be a device tensor or a device address")
-    if not x.is_cuda or x.element_size() != 4 or x.is_floating_point() or not x.is_contiguous() or x.numel() < n \
-            or x.get_device() != ctx.device_index:
-        raise _lib.KernelError(f"{what} must be a contiguous 32-bit device tensor of at least {n} entries; got "
-                               f"{x.dtype} of {x.numel()} on {x.device}")
-    return x.data_ptr()
+    try:
+        if x.numel() >= n and x.dtype in (_TORCH_DTYPES or _torch_dtypes())["words"] and x.is_contiguous() \
+                and x.get_device() == ctx.device_index:
+            return x.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(x, what, f"a contiguous 32-bit device tensor of at least {n} entries")
 
 
 def gpu_available() -> bool:
@@ -346,7 +354,7 @@ def logprobs_dev(ctx: GpuContext, logits, rows: int, vocab: int, targets, logpro
     if code is None:
         raise _lib.KernelError(f"logprobs takes 'float32' or 'bfloat16' logits, got {dtype!r}")
     rows, vocab, k, stride = int(rows), int(vocab), int(top_k), int(vocab if row_stride is None else row_stride)
-    if min(rows, vocab, k, stride) < 0:
+    if rows < 0 or vocab < 0 or k < 0 or stride < 0:
         raise _lib.KernelError("logprobs sizes must not be negative")
     x = _device_values(logits, dtype, (rows - 1) * stride + vocab if rows else 0, ctx, "logprobs: logits",
                        row_stride is not None)
@@ -378,7 +386,8 @@ class KvCache:
         self.n_seqs, self.capacity = int(n_seqs), int(capacity)
         self.n_kv_heads, self.head_dim = int(n_kv_heads), int(head_dim)
         self._shape = KvShape(self.FORMATS[fmt], self.n_seqs, self.capacity, self.n_kv_heads, self.head_dim)
-        self._shape_ref, self._base = C.byref(self._shape), _ptr(buffer)
+        self._shape_ref = C.byref(self._shape)
+        self._base = _device_bytes(buffer, need, ctx, "kv cache buffer")
 
     @classmethod
     def size(cls, fmt: str, n_seqs: int, capacity: int, n_kv_heads: int, head_dim: int) -> int:
@@ -393,6 +402,12 @@ class KvCache:
             raise _lib.KernelError(_lib.load().qbk_last_error().decode())
         return need
 
+    def _as_prefix_of(self, cache: "KvCache"):
+        if self.ctx.device_index != cache.ctx.device_index:
+            raise _lib.KernelError(f"the prefix's cache is on device {self.ctx.device_index}, the sequences' on "
+                                   f"{cache.ctx.device_index}")
+        return self._shape_ref, self._base
+
     def _rows(self, fn, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start, row_stride, stream):
         code = _SERVING_DTYPES.get(dtype)
         if code is None:
@@ -401,9 +416,12 @@ class KvCache:
         stride = self.n_kv_heads * self.head_dim if row_stride is None else row_stride
         if n_rows < 0 or first_seq < 0 or n < 0 or stride < 0:
             raise _lib.KernelError("kv cache rows, sequences and strides must not be negative")
+        room = (n_rows - 1) * stride + self.n_kv_heads * self.head_dim if n_rows else 0
+        keys = _device_values(k, dtype, room, self.ctx, "kv cache: keys", row_stride is not None)
+        values = _device_values(v, dtype, room, self.ctx, "kv cache: values", row_stride is not None)
         at = _device_words(pos, n, self.ctx, "positions")
         starts = None if row_start is None else _device_words(row_start, n + 1, self.ctx, "row starts")
-        check(fn(self.ctx.handle, self._shape_ref, self._base, _ptr(k), _ptr(v), code, stride, n_rows, starts, at,
+        check(fn(self.ctx.handle, self._shape_ref, self._base, keys, values, code, stride, n_rows, starts, at,
                  first_seq, n, _stream(stream)))
 
     def write_dev(self, k, v, dtype: str, pos, n_rows: int, first_seq: int = 0, n_seqs: int | None = None,
@@ -447,15 +465,19 @@ class KvCache:
             raise _lib.KernelError(f"kv attention takes 'float32' or 'bfloat16' queries, got {dtype!r}")
         n = self.n_seqs - first_seq if n_seqs is None else n_seqs
         most = self.capacity if max_len is None else max_len
-        if min(n, most, first_seq, n_heads, seq_q, prefix_seq, prefix_len) < 0:
+        if n < 0 or most < 0 or first_seq < 0 or n_heads < 0 or seq_q < 0 or prefix_seq < 0 or prefix_len < 0:
             raise _lib.KernelError("kv attention sizes must not be negative")
         if prefix_len and prefix is None:
             raise _lib.KernelError("a prefix_len needs the cache that holds the prefix")
         words = _device_words(lens, n, self.ctx, "lengths")
-        shared, base = (prefix._shape_ref, prefix._base) if prefix_len else (None, None)
+        room = n * seq_q * n_heads * self.head_dim
+        queries = _device_values(q, dtype, room, self.ctx, "kv attention: queries")
+        to = _device_values(out, dtype, room, self.ctx, "kv attention: out")
+        ws = _device_bytes(workspace, workspace_size, self.ctx, "kv attention: workspace")
+        shared, base = prefix._as_prefix_of(self) if prefix_len else (None, None)
         check(_lib.load().qbk_attention_kv_dev(
             self.ctx.handle, self._shape_ref, self._base, first_seq, n, words, most, shared, base, prefix_seq,
-            prefix_len, n_heads, seq_q, _ptr(q), code, _ptr(out), _ptr(workspace), workspace_size, _stream(stream)))
+            prefix_len, n_heads, seq_q, queries, code, to, ws, workspace_size, _stream(stream)))
 
 
 class SageDecodeState:
@@ -633,11 +655,15 @@ class DecoderBlock:
             raise _lib.KernelError("kv decode sizes must not be negative")
         if prefix_len and prefix is None:
             raise _lib.KernelError("a prefix_len needs the cache that holds the prefix")
+        if cache.ctx.device_index != self.ctx.device_index:
+            raise _lib.KernelError(f"the kv cache is on device {cache.ctx.device_index}, the block on "
+                                   f"{self.ctx.device_index}")
         words = _device_words(pos, n, self.ctx, "positions")
-        shared, base = (prefix._shape_ref, prefix._base) if prefix_len else (None, None)
+        ws = _device_bytes(workspace, workspace_size, self.ctx, "kv decode: workspace")
+        shared, base = prefix._as_prefix_of(cache) if prefix_len else (None, None)
         check(_lib.load().qbk_block_decode_kv_dev(
             self.ctx.handle, self._h, _ptr(h), words, n, cache._shape_ref, cache._base, first_seq, most, shared, base,
-            prefix_seq, prefix_len, _ptr(workspace), int(workspace_size), _stream(stream)))
+            prefix_seq, prefix_len, ws, int(workspace_size), _stream(stream)))
 
     def set_positions(self, positions):
         """The host record after device-position steps: sequence i holds
@@ -664,7 +690,7 @@ class DecoderBlock:
     def _check_rows(self, h, n: int, what: str):
         if hasattr(h, "is_cuda"):
             if not h.is_cuda or str(h.dtype) != "torch.float32" or not h.is_contiguous() \
-                    or h.numel() != self.d_model * n:
+                    or h.numel() != self.d_model * n or h.get_device() != self.ctx.device_index:
                 raise _lib.KernelError(
                     f"{what} must be a contiguous float32 device tensor of {n} x {self.d_model} "
                     f"values; got {h.dtype} of {h.numel()} on {h.device}")
