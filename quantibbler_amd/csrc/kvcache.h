@@ -13,8 +13,8 @@
 // K q^T (lane l: row l % 16, channels of chunk l / 16), values as the A rows
 // of V^T p^T (lane l: channel l % 16, the sixteen rows whose scores the lane's
 // group l / 16 holds after K q^T).  Nothing is transposed or exchanged between
-// lanes when the cache is read; the writer pays with four byte-wide stores a
-// value dword.
+// lanes when the cache is read; the writer pays, row by row with four byte-wide
+// stores a value dword, by 64-row tiles with a turn of 4 x 4 bytes in LDS.
 // An int8 code c is held as the byte c + 128: 0x6400 | byte is the fp16 number
 // 1024 + byte, from which one packed subtraction of 1152 leaves c.
 #pragma once
