@@ -197,12 +197,12 @@ struct __attribute__((packed, aligned(sizeof(T)))) Kva4 {
 
 // Queries row0 .. row0 + n_rows - 1 (at most 16 NT) of kv head hk into LDS as
 // the B operands of K q^T, [tile][step][lane][16 bytes], for f32 queries the
-// low halves behind them; qps[r]: the power of two that scores of row r still
-// need, NaN for a row that holds a NaN or an infinity.
+// low halves behind them; qfs[r]: the factor that scores of row r still need,
+// NaN for a row that holds a NaN or an infinity.
 // 16 DC lanes a row, four channels a lane, every row's load before the first
 // is used (32 requests behind 8192 rows, by a row at a time 41 us, so 29).
 template <int DC, int NT, typename T>
-__device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float *qps, uint32_t row0, uint32_t n_rows,
+__device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float *qfs, uint32_t row0, uint32_t n_rows,
                                             uint32_t hk) {
     constexpr int STEPS = 2 * DC, LANES = 16 * DC, AT_ONCE = KVA_WAVES * 64 / LANES, N = 16 * NT / AT_ONCE;
     const int tid = threadIdx.x, hd = (int)a.own.hd, c = 4 * (tid % LANES), r0 = tid / LANES;
@@ -237,8 +237,8 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
         // the largest channel to [8, 16): both halves of every channel within fp16
         const bool whole = top[k] < 0x7f800000u;
         uint32_t ex = top[k] >> 23;
-        ex = ex < 4 ? 4 : ex;  // rows below 2^-123 stay below 8: the power of two is a normal number down to here
-        const float f = __uint_as_float((257 - ex) << 23);  // NaN rows: the scores become NaN by qps
+        ex = ex < 8 ? 8 : ex;  // rows below 2^-119 stay below 8: the factor is a normal number down to here
+        const float f = __uint_as_float((257 - ex) << 23);  // NaN rows: the scores become NaN by qfs
         kva_h2_t hi[2], lo[2];
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
@@ -254,20 +254,22 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
         if constexpr (sizeof(T) == 4)
             *(uint2 *)(qs + NT * STEPS * 1024 + at) =
                 uint2{__builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1])};
-        top[k] = whole ? (ex - 3) << 23 : 0x7fc00000u;
+        top[k] = whole ? __float_as_uint(a.scale * __uint_as_float((ex - 3) << 23)) : 0x7fc00000u;
     }
     if (c == 0)
 #pragma unroll
-        for (int k = 0; k < N; k++) qps[r0 + k * AT_ONCE] = __uint_as_float(top[k]);
+        for (int k = 0; k < N; k++) qfs[r0 + k * AT_ONCE] = __uint_as_float(top[k]);
 }
 
-// Sums of code products as q k: times the key's scale and the row's power of
-// two, those two first.  Codes reach 448 and a scaled query 16, so a sum by its
-// key's scale alone would pass f32 for keys from some 2^117 on; the two
-// together pass it where |q| |k| does.
-__device__ __forceinline__ void kva_scores(kva_f4_t (&s)[4], const kva_f4_t (&ks)[4], float qp) {
+// Sums of code products to scores in base 2: times the key's scale and the
+// row's factor, those two first.  Codes reach 448 and a scaled query 16, so a
+// sum by its key's scale alone would pass f32 for keys from some 2^117 on; the
+// two together pass it where |q| |k| does.  From here on a score is this
+// rounded number: a reference taken from it is as large as the largest, while
+// of a fused product's remainders past 2^31 some are above 2^128 by themselves.
+__device__ __forceinline__ void kva_scores(kva_f4_t (&s)[4], const kva_f4_t (&ks)[4], float qf) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) s[i] *= ks[i] * qp;
+    for (int i = 0; i < 4; i++) s[i] *= ks[i] * qf;
 }
 
 // Scores t and value scales vs of a lane's 16 keys (16 i + j past key) that its
@@ -293,11 +295,10 @@ __device__ __forceinline__ float kva_most(const kva_f4_t (&t)[4]) {
 
 // The row's reference moves when a score passes it eightfold, its sum with it;
 // what the outputs stand for stays, so wref moves the other way.
-__device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float scale, float &ref, float &sum,
-                                              float &wref) {
+__device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float &ref, float &sum, float &wref) {
     const float tm = kva_most(t);
-    if (__ballot(tm * scale > ref + 3.0f)) {
-        const float most = kva_max4(tm) * scale;
+    if (__ballot(tm > ref + 3.0f)) {
+        const float most = kva_max4(tm);
         const float to = most > ref + 3.0f ? ceilf(most) : ref;  // other rows' scores move no more than theirs
         const float f = kva_rescale(ref, to);
         sum *= f;
@@ -306,17 +307,16 @@ __device__ __forceinline__ void kva_reference(const kva_f4_t (&t)[4], float scal
     }
 }
 
-// Scores to weights: p = exp2(t scale - ref) into sum, t becomes p times the
-// value's scale.
-__device__ __forceinline__ void kva_weights(kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float scale, float ref,
-                                            float &sum) {
+// Scores to weights: p = exp2(t - ref) into sum, t becomes p times the value's
+// scale.
+__device__ __forceinline__ void kva_weights(kva_f4_t (&t)[4], const kva_f4_t (&vs)[4], float ref, float &sum) {
     const float base = ref == -INFINITY ? 0.0f : ref;  // a row that has seen nothing: every p is 0
     float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t[i][j], scale, -base));
+            const float p = __builtin_amdgcn_exp2f(t[i][j] - base);
             l[i] += p;
             t[i][j] = p * vs[i][j];
         }
@@ -373,10 +373,10 @@ __device__ __forceinline__ void kva_operands(const kva_f4_t (&w)[4], float wref,
 template <int DC>
 struct KvaState {
     kva_f4_t o[4 * DC];
-    float ref, sum, qp, wref;
+    float ref, sum, qf, wref;
     uint32_t lim;
-    __device__ __forceinline__ KvaState(float qp, uint32_t lim)
-        : ref(-INFINITY), sum(0.0f), qp(qp), wref(0.0f), lim(lim) {
+    __device__ __forceinline__ KvaState(float qf, uint32_t lim)
+        : ref(-INFINITY), sum(0.0f), qf(qf), wref(0.0f), lim(lim) {
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++) o[ct] = kva_f4_t{0, 0, 0, 0};
     }
@@ -425,7 +425,7 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: loops and addresses by it are too
     const int hd = (int)a.own.hd, nc = hd / 16;
     char *qs = smem;
-    float *qps = (float *)(smem + L::BODY), *refs = qps + 16, *sums = refs + KVA_WAVES * 16;
+    float *qfs = (float *)(smem + L::BODY), *refs = qfs + 16, *sums = refs + KVA_WAVES * 16;
 
     // A tile's codes and scales travel while the one before is worked on: keys
     // and their scales are asked for again as soon as the scores are formed,
@@ -458,9 +458,9 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
         load_k(first);
         load_v(first);
     }
-    kva_queries<DC, 1, T>(a, qs, qps, row0, n_rows, hk);
+    kva_queries<DC, 1, T>(a, qs, qfs, row0, n_rows, hk);
     __syncthreads();
-    KvaState<DC> st(qps[col], limit((uint32_t)col < n_rows ? col : n_rows - 1));
+    KvaState<DC> st(qfs[col], limit((uint32_t)col < n_rows ? col : n_rows - 1));
     const uint32_t least = kva_scalar(limit(0));  // keys below it are seen by every row
 
     for (uint32_t tt = first; tt < tile1; tt += KVA_WAVES) {
@@ -493,11 +493,11 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
             }
         }
         // the key registers are free again
-        kva_scores(s, ks, st.qp);
+        kva_scores(s, ks, st.qf);
         if (more) load_k(tt + KVA_WAVES);
         if (masked) kva_mask(s, vs, key0 + 4 * g, st.lim);
-        kva_reference(s, a.scale, st.ref, st.sum, st.wref);
-        kva_weights(s, vs, a.scale, st.ref, st.sum);
+        kva_reference(s, st.ref, st.sum, st.wref);
+        kva_weights(s, vs, st.ref, st.sum);
         kva_weight_reference(s, st.wref, st.o);
         kva_h8_t ph[2], pl[2];
         kva_operands<HI>(s, st.wref, ph, pl);
@@ -587,7 +587,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: loops and addresses by it are too
     const int hd = (int)a.own.hd, nc = hd / 16;
-    float *qps = (float *)(smem + L::BODY);
+    float *qfs = (float *)(smem + L::BODY);
 
     // This wave's part of a tile: the keys of block `wave` and every fourth
     // channel tile of the values.
@@ -627,7 +627,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
     };
     if (tile0 < tile1) load(tile0, 0);
     if (BUFS > 1 && tile0 + 1 < tile1) load(tile0 + 1, BUFS - 1);
-    kva_queries<DC, KVA_WAVES, T>(a, smem, qps, row0, n_rows, hk);
+    kva_queries<DC, KVA_WAVES, T>(a, smem, qfs, row0, n_rows, hk);
     __syncthreads();
     kva_h8_t qh[STEPS], ql[STEPS];
 #pragma unroll
@@ -638,7 +638,7 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
     }
     const uint32_t my0 = wave * 16, r = my0 + col;  // this wave's first row, this lane's
     const bool rows = my0 < n_rows;
-    KvaState<DC> st(qps[r], limit(r < n_rows ? r : n_rows - 1));
+    KvaState<DC> st(qfs[r], limit(r < n_rows ? r : n_rows - 1));
     const uint32_t least = kva_scalar(limit(rows ? my0 : 0)), end = my0 + 16 < n_rows ? my0 + 16 : n_rows;
     const uint32_t most = rows ? kva_scalar(limit(end - 1)) : 0;  // no row of the wave sees keys from here on
     __syncthreads();  // the queries are read
@@ -661,10 +661,10 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
                 s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[x], s[i], 0, 0, 0);
                 if constexpr (HI) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[x], s[i], 0, 0, 0);
             }
-        kva_scores(s, ks, st.qp);
+        kva_scores(s, ks, st.qf);
         if (key0 + 64 > least) kva_mask(s, vs, key0 + 4 * g, st.lim);
-        kva_reference(s, a.scale, st.ref, st.sum, st.wref);
-        kva_weights(s, vs, a.scale, st.ref, st.sum);
+        kva_reference(s, st.ref, st.sum, st.wref);
+        kva_weights(s, vs, st.ref, st.sum);
         kva_weight_reference(s, st.wref, st.o);
         kva_h8_t ph[2], pl[2];
         kva_operands<HI>(s, st.wref, ph, pl);

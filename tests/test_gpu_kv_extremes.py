@@ -201,3 +201,40 @@ def test_values_near_the_top_of_the_range(ctx, fmt, dtype, shape):
     q = (0.05 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
     want, tol = reference(q, p, own, rows)
     att.check(att.attend(cache, q, words(rows), dtype, shared, plen), want, tol)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("size", [3e4, 1e7, 1e14])
+def test_scores_past_the_exponents_range(ctx, fmt, dtype, shape, size):
+    """Scores of 1e9, 1e14 and 1e28: the likeliest key has all the weight, and its value is the answer (where float64
+    tells it from the next by more than the scores' own roundings)."""
+    n, heads, kv, d, sq, rows, plen = shape
+
+    def poke(k, v):
+        k *= size
+    cache, own, shared, p = both(ctx, fmt, shape, poke)
+    q = (size * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
+    got = att.attend(cache, q, words(rows), dtype, shared, plen).double()
+    assert bool(got.isfinite().all())
+    told = 0
+    for b in range(n):
+        k, v = (torch.cat([x, y[:rows[b]]]) for x, y in zip(p, own[b]))
+        index = torch.arange(len(k), device="cuda")[None]
+        seen = index < plen + rows[b] - sq + 1 + torch.arange(sq, device="cuda")[:, None]
+        for h in range(heads):
+            kk, vv, qq = k[:, h // (heads // kv)], v[:, h // (heads // kv)], q[b, :, h].double()
+            s = torch.where(seen, qq @ kk.t().contiguous(), torch.full_like(seen, -torch.inf, dtype=torch.float64))
+            two, at = s.topk(2, -1)
+            # a score is off by (d + 8) eps and, f32, 2^-23 of its terms; fp16's smallest step against the largest channel
+            off = (((d + 8) * EPS + 2.0 ** -23) * (qq.abs() @ kk.abs().t().contiguous()).amax(-1) +
+                   2.0 ** -28 * qq.abs().amax(-1) * kk.abs().sum(-1).max())
+            clear = two[:, 0] - two[:, 1] > 2 * off + 60.0 * d ** 0.5
+            told += int(clear.sum())
+            want = vv[at[:, 0]]
+            # the weight is 1 and rides with the value's scale: rounded as a weight is (fp16's half step 2^-11, in two
+            # halves 2^-22), the exact product with the code by some f32 roundings on the way, and as an output
+            step = 2.0 ** -8 + 2.0 ** -11 if dtype == "bfloat16" else EPS + 2.0 ** -22
+            assert bool(((got[b, :, h] - want).abs() <= (step + 70 * EPS) * want.abs())[clear].all()), f"row {b} head {h}"
+    assert told > n * sq * heads // 2
