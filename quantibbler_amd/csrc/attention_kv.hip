@@ -411,7 +411,7 @@ __device__ __forceinline__ T *kva_out_row(const KvAttArgs &a, uint32_t rho, uint
 // Up to 16 rows, row0 .. row0 + n_rows - 1 of kv head hk, over key tiles tile0
 // .. tile1 - 1 of the slab k, v, ks, vs: a wave every fourth tile, in registers
 // alone (few rows are bound by the cache's bytes; 32 sequences of up to 2085
-// rows, 32/8 heads of 128: 107 MB in 23.2 us, 4.6 TB/s).  Row r of the body sees
+// rows, 32/8 heads of 128: 107 MB in 23.0 us, 4.7 TB/s).  Row r of the body sees
 // keys below limit(r), none of them at or past `written`.
 template <int FMT, int DC, typename T, class Limit>
 __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows, uint32_t hk,
@@ -563,7 +563,7 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
 // at unlike places (one alone issues a vector operation every four cycles, two
 // of one workgroup stand at its barriers together); 32 rows a wave would halve
 // the widening but do not fit 256 registers.  64 requests of up to 2048 rows
-// behind 16384, 32/8 heads of 128: 244 MB in 54.7 us, 4.5 TB/s.
+// behind 16384, 32/8 heads of 128: 244 MB in 54 to 55 us, 4.5 TB/s.
 template <int DC>
 struct KvaStage {
     static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 512, BUFS = DC < 4 ? 2 : 1;
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
 // A wave a row and kv head: the partial results of its splits on their largest
 // reference.  Four channels a lane and, up to 128 channels, two or four splits
 // at a time; everything is asked for before anything is used, so that the
-// partial rows and their references take one latency (1024 rows: 4.0 us).
+// partial rows and their references take one latency (1024 rows: 4.3 us).
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
     constexpr int STEP = 64 / LANES, N = (2 * KVA_MAX_SPLITS + STEP - 1) / STEP, BATCH = N < 16 ? N : 16;

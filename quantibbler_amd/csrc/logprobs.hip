@@ -17,7 +17,7 @@
 // which all differ: only k threads hold keys above the k-th largest of theirs.
 //
 // Many rows are bound by memory: 2048 x 128256 f32, 1.05 GB in 179 us, 5.9 TB/s.
-// One row of 128256 is bound by two dependent launches, 9.3 to 10.3 and 5.8 us,
+// One row of 128256 is bound by two dependent launches, 9.3 to 10.1 and 5.8 us,
 // the first of sixteen workgroups: a chunk is 8192 logits whatever the call.
 #include <math.h>
 
