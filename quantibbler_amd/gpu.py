@@ -314,8 +314,9 @@ def embed(ctx: GpuContext, table, vocab: int, d_model: int, tokens, out, stream=
 
 def embed_dev(ctx: GpuContext, table, vocab: int, d_model: int, tokens, n: int, out, stream=None):
     """Device token ids (int32); an out-of-range id yields a NaN row."""
-    check(_lib.load().qbk_embed_dev(ctx.handle, _ptr(table), int(vocab), int(d_model), _ptr(tokens), int(n),
-                                    _ptr(out), _stream(stream)))
+    ids = _device_words(tokens, int(n), ctx, "token ids")
+    check(_lib.load().qbk_embed_dev(ctx.handle, _ptr(table), int(vocab), int(d_model), ids, int(n), _ptr(out),
+                                    _stream(stream)))
 
 
 def rms_norm_dev(ctx: GpuContext, x, rows: int, d: int, w, eps: float, out, stream=None, serving: str = "bf16"):

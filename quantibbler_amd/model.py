@@ -467,7 +467,9 @@ class DeviceModel:
     def step_shared(self, tokens, stream=None):
         """The next position of every request of share_prefix(): ``tokens`` as
         step_batch's, one a request.  Returns the logits [n][vocab] (a device
-        tensor, overwritten by the next call)."""
+        tensor, overwritten by the next call).  A captured step serves this
+        shared prefix alone and counts once towards the requests' capacity,
+        however often it is replayed; replays past it write no rows."""
         from .gpu import advance_positions_dev, embed, embed_dev, rms_norm_dev
 
         md, s = self.md, self._shared

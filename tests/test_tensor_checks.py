@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from quantibbler_amd import DecoderBlock, KernelError, KvCache
-from quantibbler_amd.gpu import logprobs_dev, logprobs_workspace_size
+from quantibbler_amd.gpu import embed_dev, logprobs_dev, logprobs_workspace_size
 
 
 class OnDevice:
@@ -183,3 +183,15 @@ def test_a_blocks_step_takes_what_it_says():
     refused("prefix's cache is on device 1, the sequences' on 0", step, prefix=make(other, 1), prefix_len=3)
     refused("positions must be", step, pos=dev(SEQS, dtype=torch.int32, index=1))
     refused("batched decode input must be", step, h=dev(SEQS, 256, index=1))
+
+
+def test_token_ids_are_32_bits():
+    """What argmax of torch gives is 64 bits, and was read as pairs of ids."""
+    def ids(tokens):
+        embed_dev(CTX, 4096, VOCAB, 64, tokens, ROWS, 4096)
+
+    refused("null qbk_ctx", ids, tokens=dev(ROWS, dtype=torch.int32))
+    refused("null qbk_ctx", ids, tokens=4096)
+    for bad in (dev(ROWS, dtype=torch.int64), dev(ROWS - 1, dtype=torch.int32), dev(ROWS),
+                torch.zeros(ROWS, dtype=torch.int32), dev(ROWS, dtype=torch.int32, index=1)):
+        refused("^token ids must be", ids, tokens=bad)
