@@ -446,7 +446,7 @@ int qbk_sage_blk_quantize_dev(qbk_ctx *ctx, const qbk_attn_shape *shape, const u
                               int8_t *khat, float *kscale, float *kmean, uint16_t *vh,
                               void *stream);
 
-/* ---- 8-bit KV cache and the attention that reads it ------------------------ */
+/* ---- KV cache in 8 or 4 bits and the attention that reads it ---------------- */
 
 /* No counterpart in the reference (its KvCache is f32, engine/mod.rs:
  * 1189-1269): n_seqs sequences of up to `capacity` rows, each row's key and
@@ -456,13 +456,21 @@ int qbk_sage_blk_quantize_dev(qbk_ctx *ctx, const qbk_attn_shape *shape, const u
  *   scale = A (1 / L),  code = nearest(x (L (1 / A))) (f32 steps; ties to
  * even; int8: to an integer, fp8: to an OCP e4m3 value), and the row stands
  * for code * scale.
+ * The 4-bit format (fp4) holds e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4 and 6) and,
+ * for every 32 channels, the last ones where head_dim leaves fewer, an e4m3
+ * multiplier m of them: with a the largest |x| of those channels
+ *   m = nearest(a (448 (1 / A))),  code = nearest((x (2688 (1 / A))) (1 / m)),
+ *   scale = A (1 / 2688),  value = (code * m) * scale
+ * in f32 steps, ties to even, codes past 6 held at 6; m = 0 (channels of zeros,
+ * or next to nothing beside A) stands for zeros.  A row of 128 channels is 72
+ * bytes, of the 8-bit formats 132.
  * A head's row that holds a NaN or an infinity reads back as NaN throughout.
  * head_dim is a multiple of 16 up to 256.  The cache is one device buffer of
  * qbk_kv_cache_size bytes, 16-byte aligned, that the caller owns; its inner
  * layout is the attention kernel's, rows enter and leave it through
  * qbk_kv_cache_write_dev / _read_dev.  A new buffer needs no clearing: rows
  * never written are never looked at while lengths say so. */
-enum { QBK_KV_INT8 = 0, QBK_KV_FP8 = 1 };
+enum { QBK_KV_INT8 = 0, QBK_KV_FP8 = 1, QBK_KV_FP4 = 4 };
 typedef struct {
     int format;
     size_t n_seqs, capacity, n_kv_heads, head_dim;
@@ -484,7 +492,7 @@ size_t qbk_kv_cache_size(const qbk_kv_shape *shape);
 int qbk_kv_cache_write_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, void *cache, const void *k, const void *v,
                            int dtype, size_t row_stride, size_t n_rows, const uint32_t *row_start,
                            const uint32_t *pos, size_t first_seq, size_t n, void *stream);
-/* The same rows back as values (code * scale in f32, rounded once for
+/* The same rows back as values (as above, in f32, rounded once for
  * QBK_BF16); a row whose position is at or past the capacity, or that no
  * sequence claims, is NaN. */
 int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, void *k, void *v, int dtype,

@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(HERE, "libqbk.so")
 
 QBK_OK, QBK_ERR_VALIDATION, QBK_ERR_DEVICE, QBK_ERR_INIT = 0, 1, 2, 3
 QBK_F64, QBK_F32, QBK_BF16 = 0, 1, 2
-QBK_KV_INT8, QBK_KV_FP8 = 0, 1
+QBK_KV_INT8, QBK_KV_FP8, QBK_KV_FP4 = 0, 1, 4
 
 
 class KernelError(ValueError):
@@ -36,7 +36,7 @@ class AttnShape(C.Structure):
 
 
 class KvShape(C.Structure):
-    """qbk_kv_shape: an 8-bit KV cache's format and sizes."""
+    """qbk_kv_shape: an 8-bit or 4-bit KV cache's format and sizes."""
     _fields_ = [("format", C.c_int)] + [(n, C.c_size_t) for n in ("n_seqs", "capacity", "n_kv_heads", "head_dim")]
 
 

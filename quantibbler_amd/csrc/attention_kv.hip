@@ -1,5 +1,5 @@
-// attention_kv.hip -- attention of a batch over the 8-bit KV cache, behind a
-// prefix that every sequence shares.
+// attention_kv.hip -- attention of a batch over the 8-bit or 4-bit KV cache,
+// behind a prefix that every sequence shares.
 //
 // Rows: query row rho = (b sq + t) G + hg of kv head hk is sequence b's query
 // t, head hk G + hg.  Every row sees the prefix, so the prefix's items take
@@ -9,7 +9,7 @@
 //   item = (kv head, 16 or 64 rows, run of 64-row key tiles)
 // and leave a partial result (sum of weights, mean of values, reference) per
 // row; a second launch joins them.  A key tile and 16 rows, a wave:
-//   S^T = K q^T      v_mfma_f32_16x16x32_f16, codes widened to fp16 (exact)
+//   S^T = K q^T      v_mfma_f32_16x16x32_f16, codes (fp4: times their multipliers) widened to fp16 (exact)
 //   p = exp2(s - M)  online, per query column; M is a whole number, so moving
 //                    to another M and joining partials scale by powers of two
 //   O^T += V^T p^T   p times the value row's scale, in fp16
@@ -37,6 +37,7 @@ typedef _Float16 kva_h8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 kva_h2_t __attribute__((ext_vector_type(2)));
 typedef float kva_f2_t __attribute__((ext_vector_type(2)));
 typedef float kva_f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t kva_u2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t kva_u4_t __attribute__((ext_vector_type(4)));
 
 #define KVA_WAVES 4
@@ -104,6 +105,40 @@ __device__ __forceinline__ kva_h8_t kva_wide(uint32_t lo, uint32_t hi) {
         p[3] = __builtin_bit_cast(kva_h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true));
     }
     return kva_h8_t{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
+}
+
+// The same of the 4-bit format: eight codes in one dword.
+__device__ __forceinline__ void kva_wide4(uint32_t w, kva_h2_t (&p)[4]) {
+    p[0] = __builtin_bit_cast(kva_h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0));
+    p[1] = __builtin_bit_cast(kva_h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1));
+    p[2] = __builtin_bit_cast(kva_h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2));
+    p[3] = __builtin_bit_cast(kva_h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3));
+}
+__device__ __forceinline__ kva_h8_t kva_h8(const kva_h2_t (&p)[4]) {
+    return kva_h8_t{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
+}
+// Two multipliers of a dword's four.
+template <int HALF>
+__device__ __forceinline__ kva_h2_t kva_mul4(uint32_t w) {
+    return __builtin_bit_cast(kva_h2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HALF));
+}
+// A key's eight channels of one group times the group's multiplier; a value's
+// eight rows (row pairs of dwords m0 and m1) times theirs.
+__device__ __forceinline__ kva_h8_t kva_key4(uint32_t w, _Float16 mul) {
+    kva_h2_t p[4];
+    kva_wide4(w, p);
+#pragma unroll
+    for (int e = 0; e < 4; e++) p[e] *= kva_h2_t{mul, mul};
+    return kva_h8(p);
+}
+__device__ __forceinline__ kva_h8_t kva_val4(uint32_t w, uint32_t m0, uint32_t m1) {
+    kva_h2_t p[4];
+    kva_wide4(w, p);
+    p[0] *= kva_mul4<0>(m0);
+    p[1] *= kva_mul4<1>(m0);
+    p[2] *= kva_mul4<0>(m1);
+    p[3] *= kva_mul4<1>(m1);
+    return kva_h8(p);
 }
 
 // The largest of a value over the four lanes of a query column (l ^ 16, l ^ 32).
@@ -262,7 +297,7 @@ __device__ __forceinline__ void kva_queries(const KvAttArgs &a, char *qs, float 
 }
 
 // Sums of code products to scores in base 2: times the key's scale and the
-// row's factor, those two first.  Codes reach 448 and a scaled query 16, so a
+// row's factor, those two first.  Codes reach 448 (fp4: 2688) and a scaled query 16, so a
 // sum by its key's scale alone would pass f32 for keys from some 2^117 on; the
 // two together pass it where |q| |k| does.  From here on a score is this
 // rounded number: a reference taken from it is as large as the largest, while
@@ -328,7 +363,7 @@ __device__ __forceinline__ void kva_weights(kva_f4_t (&t)[4], const kva_f4_t (&v
 // It is the row's own and of rows that it sees alone, and p is in it, so that
 // neither a value that the mask hides nor a large one of little weight costs
 // the others their bits.  A row's likeliest key has p of 1/2 and more and a
-// scale of 2^-109 and more, so wref is 2^-113 and more as soon as a weight is
+// scale of 2^-112 and more, so wref is 2^-114 and more as soon as a weight is
 // not 0, and at most 2^126.
 template <int CT>
 __device__ __forceinline__ void kva_weight_reference(const kva_f4_t (&w)[4], float &wref, kva_f4_t (&o)[CT]) {
@@ -408,6 +443,99 @@ __device__ __forceinline__ T *kva_out_row(const KvAttArgs &a, uint32_t rho, uint
     return (T *)a.out + ((size_t)query * a.H + (size_t)hk * a.G + head) * a.own.hd;
 }
 
+// A slab's codes, multipliers (fp4) and scales.
+struct KvaSlab {
+    const uint8_t *k, *v, *km, *vm;
+    const float *ks, *vs;
+    uint32_t ng;
+    template <int FMT>
+    static __device__ __forceinline__ KvaSlab of(const KvView &c, size_t slab) {
+        KvaSlab s;
+        s.ng = c.groups();
+        if constexpr (FMT == QBK_KV_FP4) {
+            s.k = c.k + slab * (c.hd / 2);
+            s.v = c.v + slab * (16 * s.ng);
+            s.km = c.km + slab * s.ng;
+            s.vm = c.vm + slab * s.ng;
+        } else {
+            s.k = c.k + slab * c.hd;
+            s.v = c.v + slab * c.hd;
+            s.km = s.vm = nullptr;
+        }
+        s.ks = c.ks + slab;
+        s.vs = c.vs + slab;
+        return s;
+    }
+};
+
+// A key tile's codes on their way to a wave, and its operands.
+template <int FMT, int DC>
+struct KvaTile {
+    kva_u4_t kc[DC][4], vc[4 * DC];
+    __device__ __forceinline__ void load_k(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+        const int nc = hd / 16;
+        const uint8_t *kt = c.k + (size_t)tt * 64 * hd + col * 16;
+#pragma unroll
+        for (int x = 0; x < DC; x++) {
+            const int chunk = 4 * x + g < nc ? 4 * x + g : nc - 1;  // past the last chunk q is zero
+#pragma unroll
+            for (int i = 0; i < 4; i++) kc[x][i] = *(const kva_u4_t *)(kt + (i * nc + chunk) * 256);
+        }
+    }
+    __device__ __forceinline__ void load_v(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+        const int nc = hd / 16;
+        const uint8_t *vt = c.v + (size_t)tt * 64 * hd + col * 64 + g * 16;
+#pragma unroll
+        for (int ct = 0; ct < 4 * DC; ct++)
+            vc[ct] = *(const kva_u4_t *)(vt + (ct < nc ? ct : nc - 1) * 1024);  // past the last tile: not stored
+    }
+    __device__ __forceinline__ kva_h8_t key(int x, int i) const {
+        return kva_wide<FMT>(kc[x / 2][i][2 * (x & 1)], kc[x / 2][i][2 * (x & 1) + 1]);
+    }
+    // keep: rows that were written; fp8 rows that were not may hold NaN codes
+    __device__ __forceinline__ kva_h8_t val(int ct, int u, const kva_u4_t &keep) const {
+        const kva_u4_t w = FMT == QBK_KV_FP8 ? vc[ct] & keep : vc[ct];
+        return kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
+    }
+};
+template <int DC>
+struct KvaTile<QBK_KV_FP4, DC> {
+    kva_u4_t kc[DC][2], vc[2 * DC], vm[2 * DC];
+    uint32_t km[DC];
+    __device__ __forceinline__ void load_k(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+        const int nc = hd / 16, ng = (int)c.ng;
+        const uint8_t *kt = c.k + (size_t)tt * 32 * hd + col * 16;
+        const uint8_t *mt = c.km + (size_t)tt * 64 * ng + col * 4;
+#pragma unroll
+        for (int x = 0; x < DC; x++) {
+            const int chunk = 4 * x + g < nc ? 4 * x + g : nc - 1;  // past the last chunk q is zero
+            km[x] = *(const uint32_t *)(mt + (chunk >> 1) * 64);
+#pragma unroll
+            for (int p = 0; p < 2; p++) kc[x][p] = *(const kva_u4_t *)(kt + (p * nc + chunk) * 256);
+        }
+    }
+    __device__ __forceinline__ void load_v(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+        const int ng = (int)c.ng;
+        const uint8_t *vt = c.v + (size_t)tt * 1024 * ng + col * 64 + g * 16;
+        const uint8_t *mt = c.vm + (size_t)tt * 64 * ng + g * 16;
+#pragma unroll
+        for (int m = 0; m < 2 * DC; m++) {
+            const int at = m < ng ? m : ng - 1;  // past the last tile: not stored
+            vm[m] = *(const kva_u4_t *)(mt + at * 64);
+            vc[m] = *(const kva_u4_t *)(vt + at * 1024);
+        }
+    }
+    __device__ __forceinline__ kva_h8_t key(int x, int i) const {
+        const kva_h2_t m = i < 2 ? kva_mul4<0>(km[x / 2]) : kva_mul4<1>(km[x / 2]);
+        return kva_key4(kc[x / 2][i >> 1][2 * (i & 1) + (x & 1)], m[i & 1]);
+    }
+    // keep: rows that were written; those that were not may hold NaN multipliers
+    __device__ __forceinline__ kva_h8_t val(int ct, int u, const kva_u4_t &keep) const {
+        const kva_u4_t m = vm[ct >> 1] & keep;
+        return kva_val4(vc[ct >> 1][2 * (ct & 1) + u], m[2 * u], m[2 * u + 1]);
+    }
+};
+
 // Up to 16 rows, row0 .. row0 + n_rows - 1 of kv head hk, over key tiles tile0
 // .. tile1 - 1 of the slab k, v, ks, vs: a wave every fourth tile, in registers
 // alone (few rows are bound by the cache's bytes; 32 sequences of up to 2085
@@ -415,8 +543,7 @@ __device__ __forceinline__ T *kva_out_row(const KvAttArgs &a, uint32_t rho, uint
 // keys below limit(r), none of them at or past `written`.
 template <int FMT, int DC, typename T, class Limit>
 __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows, uint32_t hk,
-                                         const uint8_t *kcode, const uint8_t *vcode, const float *ksc,
-                                         const float *vsc, uint32_t tile0, uint32_t tile1, uint32_t written,
+                                         const KvaSlab &slab, uint32_t tile0, uint32_t tile1, uint32_t written,
                                          Limit limit, uint32_t split, bool last) {
     constexpr bool HI = sizeof(T) == 4;
     using L = KvaLds<DC, HI>;
@@ -430,28 +557,19 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     // A tile's codes and scales travel while the one before is worked on: keys
     // and their scales are asked for again as soon as the scores are formed,
     // values once they are added, the first of both before the queries are read.
-    kva_u4_t kc[DC][4], vc[4 * DC];
+    KvaTile<FMT, DC> tile;
     kva_f4_t ks[4], vs[4];
     auto load_k = [&](uint32_t tt) {
-        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + col * 16;
-        const float *st = ksc + (size_t)tt * 64 + 4 * g;
+        const float *st = slab.ks + (size_t)tt * 64 + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; i++) ks[i] = *(const kva_f4_t *)(st + 16 * i);
-#pragma unroll
-        for (int c = 0; c < DC; c++) {
-            const int chunk = 4 * c + g < nc ? 4 * c + g : nc - 1;  // past the last chunk q is zero
-#pragma unroll
-            for (int i = 0; i < 4; i++) kc[c][i] = *(const kva_u4_t *)(kt + (i * nc + chunk) * 256);
-        }
+        tile.load_k(slab, tt, hd, col, g);
     };
     auto load_v = [&](uint32_t tt) {
-        const uint8_t *vt = vcode + (size_t)tt * 64 * hd + col * 64 + g * 16;
-        const float *st = vsc + (size_t)tt * 64 + 4 * g;
+        const float *st = slab.vs + (size_t)tt * 64 + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; i++) vs[i] = *(const kva_f4_t *)(st + 16 * i);
-#pragma unroll
-        for (int ct = 0; ct < 4 * DC; ct++)
-            vc[ct] = *(const kva_u4_t *)(vt + (ct < nc ? ct : nc - 1) * 1024);  // past the last tile: not stored
+        tile.load_v(slab, tt, hd, col, g);
     };
     const uint32_t first = tile0 + wave;
     if (first < tile1) {
@@ -483,7 +601,7 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
             kva_h8_t kf[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                kf[i] = kva_wide<FMT>(kc[x / 2][i][2 * (x & 1)], kc[x / 2][i][2 * (x & 1) + 1]);
+                kf[i] = tile.key(x, i);
                 s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qf, s[i], 0, 0, 0);
             }
             if constexpr (HI) {
@@ -501,15 +619,13 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
         kva_weight_reference(s, st.wref, st.o);
         kva_h8_t ph[2], pl[2];
         kva_operands<HI>(s, st.wref, ph, pl);
-        // fp8 rows that were never written may hold NaN codes
         kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
-        if (FMT == QBK_KV_FP8 && masked) keep = kva_keep(key0, written, g);
+        if (FMT != QBK_KV_INT8 && masked) keep = kva_keep(key0, written, g);
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++) {
-            const kva_u4_t w = FMT == QBK_KV_FP8 ? vc[ct] & keep : vc[ct];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const kva_h8_t vf = kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
+                const kva_h8_t vf = tile.val(ct, u, keep);
                 st.o[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[u], st.o[ct], 0, 0, 0);
                 if constexpr (HI) st.o[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[u], st.o[ct], 0, 0, 0);
             }
@@ -576,10 +692,58 @@ struct KvaWideLds {
     static constexpr int BYTES = BODY + 16 * KVA_WAVES * 4;
 };
 
+// A wave's quarter of a tile on its way: the keys of block `wave` and every
+// fourth channel tile of the values.
+template <int FMT, int DC>
+struct KvaPart {
+    kva_u4_t kc[DC], vc[DC];
+    __device__ __forceinline__ void load(const KvaSlab &c, uint32_t tt, int hd, int col, int g, int wave) {
+        const int nc = hd / 16;
+        const uint8_t *kt = c.k + (size_t)tt * 64 * hd + (wave * nc) * 256 + col * 16;
+        const uint8_t *vt = c.v + (size_t)tt * 64 * hd + col * 64 + g * 16;
+#pragma unroll
+        for (int x = 0; x < DC; x++) {
+            const int chunk = 4 * x + g, ct = 4 * x + wave;
+            kc[x] = *(const kva_u4_t *)(kt + (chunk < nc ? chunk : nc - 1) * 256);  // past the last chunk q is zero
+            vc[x] = *(const kva_u4_t *)(vt + (ct < nc ? ct : nc - 1) * 1024);       // past the last tile: not stored
+        }
+    }
+    __device__ __forceinline__ kva_h8_t key(int x, int u) const { return kva_wide<FMT>(kc[x][2 * u], kc[x][2 * u + 1]); }
+    __device__ __forceinline__ kva_h8_t val(int x, int u, const kva_u4_t &keep) const {
+        const kva_u4_t w = FMT == QBK_KV_FP8 ? vc[x] & keep : vc[x];
+        return kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
+    }
+};
+template <int DC>
+struct KvaPart<QBK_KV_FP4, DC> {
+    kva_u2_t kc[DC], vc[DC];
+    kva_u4_t vm[DC];
+    uint32_t km[DC];
+    __device__ __forceinline__ void load(const KvaSlab &c, uint32_t tt, int hd, int col, int g, int wave) {
+        const int nc = hd / 16, ng = (int)c.ng;
+        const uint8_t *kt = c.k + (size_t)tt * 32 * hd + ((wave >> 1) * nc) * 256 + col * 16 + (wave & 1) * 8;
+        const uint8_t *vt = c.v + (size_t)tt * 1024 * ng + col * 64 + g * 16 + (wave & 1) * 8;
+        const uint8_t *kmt = c.km + (size_t)tt * 64 * ng + col * 4 + wave, *vmt = c.vm + (size_t)tt * 64 * ng + g * 16;
+#pragma unroll
+        for (int x = 0; x < DC; x++) {
+            const int chunk = 4 * x + g < nc ? 4 * x + g : nc - 1;  // past the last chunk q is zero
+            const int m = 2 * x + (wave >> 1) < ng ? 2 * x + (wave >> 1) : ng - 1;  // past the last tile: not stored
+            kc[x] = *(const kva_u2_t *)(kt + chunk * 256);
+            km[x] = kmt[(chunk >> 1) * 64];
+            vc[x] = *(const kva_u2_t *)(vt + m * 1024);
+            vm[x] = *(const kva_u4_t *)(vmt + m * 64);
+        }
+    }
+    __device__ __forceinline__ kva_h8_t key(int x, int u) const { return kva_key4(kc[x][u], kva_mul4<0>(km[x])[0]); }
+    __device__ __forceinline__ kva_h8_t val(int x, int u, const kva_u4_t &keep) const {
+        const kva_u4_t m = vm[x] & keep;
+        return kva_val4(vc[x][u], m[2 * u], m[2 * u + 1]);
+    }
+};
+
 template <int FMT, int DC, typename T, class Limit>
 __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows,
-                                              uint32_t hk, const uint8_t *kcode, const uint8_t *vcode,
-                                              const float *ksc, const float *vsc, uint32_t tile0, uint32_t tile1,
+                                              uint32_t hk, const KvaSlab &slab, uint32_t tile0, uint32_t tile1,
                                               uint32_t written, Limit limit, uint32_t split, bool last) {
     constexpr bool HI = sizeof(T) == 4;
     constexpr int STEPS = 2 * DC, KEYS = KvaStage<DC>::KEYS, BUFS = KvaStage<DC>::BUFS;
@@ -591,33 +755,23 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
 
     // This wave's part of a tile: the keys of block `wave` and every fourth
     // channel tile of the values.
-    kva_u4_t kc[BUFS][DC], vc[BUFS][DC];
+    KvaPart<FMT, DC> part[BUFS];
     float sc[BUFS];  // waves 0 and 1: a key's and a value's scale a lane
     auto load = [&](uint32_t tt, int at) {
-        const uint8_t *kt = kcode + (size_t)tt * 64 * hd + (wave * nc) * 256 + col * 16;
-        const uint8_t *vt = vcode + (size_t)tt * 64 * hd + col * 64 + g * 16;
-#pragma unroll
-        for (int c = 0; c < DC; c++) {
-            const int chunk = 4 * c + g, ct = 4 * c + wave;
-            kc[at][c] = *(const kva_u4_t *)(kt + (chunk < nc ? chunk : nc - 1) * 256);  // past the last chunk q is zero
-            vc[at][c] = *(const kva_u4_t *)(vt + (ct < nc ? ct : nc - 1) * 1024);       // past the last tile: not stored
-        }
-        if (wave < 2) sc[at] = (wave ? vsc : ksc)[(size_t)tt * 64 + lane];
+        part[at].load(slab, tt, hd, col, g, wave);
+        if (wave < 2) sc[at] = (wave ? slab.vs : slab.ks)[(size_t)tt * 64 + lane];
     };
     auto stage = [&](uint32_t tt, int at, char *buf) {
         const uint32_t key0 = tt * 64;
         const bool tail = key0 + 64 > written;  // rows that were never written take no part, whatever they hold
         kva_u4_t keep = {~0u, ~0u, ~0u, ~0u};
-        if (FMT == QBK_KV_FP8 && tail) keep = kva_keep(key0, written, g);  // NaN codes
+        if (FMT != QBK_KV_INT8 && tail) keep = kva_keep(key0, written, g);  // NaN codes or multipliers
 #pragma unroll
         for (int c = 0; c < DC; c++) {
-            const kva_u4_t w = FMT == QBK_KV_FP8 ? vc[at][c] & keep : vc[at][c];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                *(kva_h8_t *)(buf + ((wave * STEPS + 2 * c + u) * 64 + lane) * 16) =
-                    kva_wide<FMT>(kc[at][c][2 * u], kc[at][c][2 * u + 1]);
-                *(kva_h8_t *)(buf + KEYS + ((2 * (4 * c + wave) + u) * 64 + lane) * 16) =
-                    kva_wide<FMT>(w[2 * u], w[2 * u + 1]);
+                *(kva_h8_t *)(buf + ((wave * STEPS + 2 * c + u) * 64 + lane) * 16) = part[at].key(c, u);
+                *(kva_h8_t *)(buf + KEYS + ((2 * (4 * c + wave) + u) * 64 + lane) * 16) = part[at].val(c, u, keep);
             }
         }
         if (wave < 2) {
@@ -699,12 +853,12 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
 #pragma unroll
                 for (int j = 0; j < 4; j++) dst[16 * ct + j] = kva_out<T>(st.o[ct][j] * per * st.wref);
     } else {
-        const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0 + r;
-        float *dst = a.po + part * hd + 4 * g;
+        const size_t at = ((size_t)split * a.own.Hk + hk) * a.rows + row0 + r;
+        float *dst = a.po + at * hd + 4 * g;
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++)
             if (ct < nc) *(kva_f4_t *)(dst + 16 * ct) = st.o[ct] * per * st.wref;
-        if (g == 0) a.ml[part] = float2{st.ref, l};
+        if (g == 0) a.ml[at] = float2{st.ref, l};
     }
 }
 
@@ -727,10 +881,9 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
         const uint32_t row0 = rt * R, n_rows = a.rows - row0 < R ? a.rows - row0 : R;
         const uint32_t tiles = (a.prefix_len + 63) / 64, run = a.by_sp.split(tiles + a.sp - 1, rest);
         const uint32_t t0 = split * run < tiles ? split * run : tiles, t1 = t0 + run < tiles ? t0 + run : tiles;
-        const size_t slab = a.pre.slab(a.prefix_seq, hk);
+        const KvaSlab slab = KvaSlab::of<FMT>(a.pre, a.pre.slab(a.prefix_seq, hk));
         const uint32_t len = a.prefix_len;
-        kva_any<FMT, DC, WIDEP, T>(a, smem, row0, n_rows, hk, a.pre.k + slab * a.pre.hd, a.pre.v + slab * a.pre.hd,
-                                  a.pre.ks + slab, a.pre.vs + slab, t0, t1, len, [&](uint32_t) { return len; }, split,
+        kva_any<FMT, DC, WIDEP, T>(a, smem, row0, n_rows, hk, slab, t0, t1, len, [&](uint32_t) { return len; }, split,
                                   last);
         return;
     }
@@ -752,9 +905,8 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
     const uint32_t most = (kva_scalar(limit(n_rows - 1)) + 63) / 64;
     uint32_t t1 = split * run + run;
     t1 = t1 < most ? t1 : most;
-    const size_t slab = a.own.slab(a.first_seq + b, hk);
-    kva_any<FMT, DC, WIDES, T>(a, smem, b * per + r0, n_rows, hk, a.own.k + slab * a.own.hd, a.own.v + slab * a.own.hd,
-                              a.own.ks + slab, a.own.vs + slab, split * run, t1, len, limit, a.sp + split, last);
+    const KvaSlab slab = KvaSlab::of<FMT>(a.own, a.own.slab(a.first_seq + b, hk));
+    kva_any<FMT, DC, WIDES, T>(a, smem, b * per + r0, n_rows, hk, slab, split * run, t1, len, limit, a.sp + split, last);
 }
 
 // A wave a row and kv head: the partial results of its splits on their largest
@@ -1003,9 +1155,12 @@ int attention_kv_run(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache,
         if (shape->format == QBK_KV_INT8)
             rc = dtype == QBK_F32 ? kva_dispatch<QBK_KV_INT8, float>(a, p, ctx->device, st)
                                   : kva_dispatch<QBK_KV_INT8, uint16_t>(a, p, ctx->device, st);
-        else
+        else if (shape->format == QBK_KV_FP8)
             rc = dtype == QBK_F32 ? kva_dispatch<QBK_KV_FP8, float>(a, p, ctx->device, st)
                                   : kva_dispatch<QBK_KV_FP8, uint16_t>(a, p, ctx->device, st);
+        else
+            rc = dtype == QBK_F32 ? kva_dispatch<QBK_KV_FP4, float>(a, p, ctx->device, st)
+                                  : kva_dispatch<QBK_KV_FP4, uint16_t>(a, p, ctx->device, st);
         if (rc) return rc;
     }
     if (p.sp + p.ss == 1) return QBK_OK;  // the items wrote the output

@@ -11,7 +11,7 @@
 // a few rows are bound by the launch, 3 us).
 #include <math.h>
 
-#include "kvcache.h"
+#include "kvcache_rows.h"
 
 #pragma clang fp contract(off)
 
@@ -19,8 +19,8 @@ namespace qbk {
 
 int kv_check_shape(const qbk_kv_shape *s, size_t *bytes) {
     if (!s) return fail(QBK_ERR_VALIDATION, "null shape");
-    if (s->format != QBK_KV_INT8 && s->format != QBK_KV_FP8)
-        return fail(QBK_ERR_VALIDATION, fmt("kv cache format must be int8 (0) or fp8 (1), got %d", s->format));
+    if (s->format != QBK_KV_INT8 && s->format != QBK_KV_FP8 && s->format != QBK_KV_FP4)
+        return fail(QBK_ERR_VALIDATION, fmt("kv cache format must be int8 (0), fp8 (1) or fp4 (4), got %d", s->format));
     if (s->n_seqs == 0 || s->capacity == 0 || s->n_kv_heads == 0)
         return fail(QBK_ERR_VALIDATION, "kv cache requires non-empty sequences, capacity and heads");
     if (s->head_dim == 0 || s->head_dim % 16 != 0 || s->head_dim > 256)
@@ -31,7 +31,9 @@ int kv_check_shape(const qbk_kv_shape *s, size_t *bytes) {
         return fail(QBK_ERR_VALIDATION, "kv cache sizes must be below 2^31");
     // 64-bit throughout: at most 2^31 * 2^31 slabs before the check below
     const unsigned __int128 rows = (unsigned __int128)s->n_seqs * s->n_kv_heads * round_up(s->capacity, 64);
-    const unsigned __int128 total = rows * (2 * (s->head_dim + 4));
+    const size_t groups = div_ceil(s->head_dim, 32);
+    const size_t per = s->format == QBK_KV_FP4 ? s->head_dim / 2 + 16 * groups + 2 * groups + 8 : 2 * (s->head_dim + 4);
+    const unsigned __int128 total = rows * per;
     if (total > ((unsigned __int128)1 << 48)) return fail(QBK_ERR_VALIDATION, "kv cache of more than 2^48 bytes");
     *bytes = (size_t)total;
     return QBK_OK;
@@ -46,53 +48,18 @@ KvView kv_view(const qbk_kv_shape *s, const void *cache) {
     v.hd = (uint32_t)s->head_dim;
     const size_t rows = s->n_seqs * s->n_kv_heads * v.cap64;
     v.k = (uint8_t *)const_cast<void *>(cache);
-    v.v = v.k + rows * v.hd;
-    v.ks = (float *)(v.v + rows * v.hd);
+    if (s->format == QBK_KV_FP4) {
+        v.v = v.k + rows * (v.hd / 2);
+        v.km = v.v + rows * (16 * v.groups());
+        v.vm = v.km + rows * v.groups();
+        v.ks = (float *)(v.vm + rows * v.groups());
+    } else {
+        v.v = v.k + rows * v.hd;
+        v.km = v.vm = nullptr;
+        v.ks = (float *)(v.v + rows * v.hd);
+    }
     v.vs = v.ks + rows;
     return v;
-}
-
-struct KvRows {
-    KvView c;
-    const uint32_t *row_start, *pos;  // row_start null: `per` rows a sequence
-    size_t stride;                    // values from one row to the next
-    uint32_t n_rows, n, per, first;
-    bool tiles;  // by 64-row tiles
-};
-
-// The sequence (0 .. n - 1) and position of row r; false for a row that no
-// sequence claims or that lies past the capacity.  Whatever row_start holds,
-// a row that passes addresses the cache in bounds.
-__device__ __forceinline__ bool kv_place(const KvRows &a, uint32_t r, uint32_t &seq, size_t &at) {
-    uint32_t s, start;
-    if (a.row_start) {
-        uint32_t lo = 0, hi = a.n;  // the last s with row_start[s] <= r
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (a.row_start[mid] <= r) lo = mid;
-            else hi = mid;
-        }
-        s = lo;
-        start = a.row_start[s];
-        if (r < start || r >= a.row_start[s + 1]) return false;
-    } else {
-        s = r / a.per;
-        start = s * a.per;
-    }
-    seq = a.first + s;
-    at = (size_t)a.pos[s] + (r - start);
-    return at < a.c.cap;
-}
-
-template <typename T>
-__device__ __forceinline__ float kv_in(T x) {
-    if constexpr (sizeof(T) == 4) return x;
-    else return bf16_to_f32(x);
-}
-template <typename T>
-__device__ __forceinline__ T kv_out(float x) {
-    if constexpr (sizeof(T) == 4) return x;
-    else return f32_to_bf16(x);
 }
 
 // A wave a row and kv head: lanes 0-31 its key, 32-63 its value, four
@@ -192,77 +159,7 @@ __global__ void __launch_bounds__(256) kv_read(KvRows a, T *k, T *v) {
     }
 }
 
-// Four values at any alignment (one access on this machine).
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Kv4 {
-    T v[4];
-};
-
 // ---- many rows a sequence: a workgroup a 64-row tile of one kv head ----------
-
-// The workgroup's tile: input rows row .. row + hi - lo - 1 stand at rows lo ..
-// hi - 1 of the tile that begins at position first of sequence seq; seq -1:
-// rows that no sequence claims (lo 0).
-struct KvTile {
-    int32_t seq;
-    uint32_t row, lo, hi;
-    uint64_t first;
-};
-// Segments of the rows: 0 those before the first sequence's, 1 .. n the
-// sequences', n + 1 those behind the last one's.  Segment i's tiles are numbered
-// from (its first row) / 64 + 2 i on, which leaves room for the two that its
-// rows touch past those they fill, so that a tile finds its segment among 64 in
-// one load and one ballot, without the other segments' counts (a running sum
-// over them took 6.6 ms for 16384 sequences of four rows).
-__device__ __forceinline__ bool kv_tile(const KvRows &a, uint32_t tile, KvTile *t) {
-    const uint32_t lane = threadIdx.x & 63;
-    auto bound = [&](uint32_t i) -> uint32_t {  // first row of segment i, 0 .. n + 2
-        if (i == 0) return 0;
-        if (i == a.n + 2) return a.n_rows;
-        const uint32_t r = a.row_start ? a.row_start[i - 1] : (i - 1) * a.per;
-        return r < a.n_rows ? r : a.n_rows;
-    };
-    uint32_t seg = 0, len = a.n + 2;  // seg .. seg + len - 1 hold it; the first of them begins at or before tile
-    while (len > 1) {
-        const uint32_t step = (len + 63) / 64, off = lane * step;
-        bool below = false;
-        if (off < len) below = bound(seg + off) / 64 + 2 * (seg + off) <= tile;
-        const uint64_t above = ~__ballot(below);
-        const uint32_t at = (above ? (uint32_t)__builtin_ctzll(above) : 64u) - 1;
-        const uint32_t skip = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at * step));
-        seg += skip;
-        len = len - skip < step ? len - skip : step;
-    }
-    const bool claimed = seg >= 1 && seg <= a.n;
-    const uint32_t from = bound(seg), to = bound(seg + 1), k = tile - (from / 64 + 2 * seg);
-    const uint32_t at = claimed ? a.pos[seg - 1] : 0, skip = at & 63;
-    if (to <= from || k >= (skip + (uint64_t)(to - from) + 63) / 64) return false;
-    t->seq = claimed ? (int32_t)(seg - 1) : -1;
-    t->lo = k == 0 ? skip : 0;
-    t->row = from + (k == 0 ? 0 : 64 * k - skip);
-    t->hi = to - t->row < 64 - t->lo ? t->lo + (to - t->row) : 64;
-    t->first = (uint64_t)(at - skip) + 64ull * k;
-    return true;
-}
-
-// 4 x 4 bytes: out[i] = bytes i of in[0 .. 3].
-__device__ __forceinline__ void kv_transpose4(const uint32_t (&in)[4], uint32_t (&out)[4]) {
-    const uint32_t a = __builtin_amdgcn_perm(in[1], in[0], 0x05010400u), b = __builtin_amdgcn_perm(in[3], in[2], 0x05010400u);
-    const uint32_t c = __builtin_amdgcn_perm(in[1], in[0], 0x07030602u), d = __builtin_amdgcn_perm(in[3], in[2], 0x07030602u);
-    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
-    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
-}
-
-// Largest over 16 lanes.
-__device__ __forceinline__ uint32_t kv_max16(uint32_t v) {
-    auto up = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));  // row_ror 8, 4, 2, 1
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
-    v = up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
-    return up(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
-}
 
 template <int FMT>
 __device__ __forceinline__ uint32_t kv_codes(const float (&x)[4], float inv) {
@@ -484,9 +381,6 @@ static bool kv_by_tiles(size_t n_rows, size_t n, const qbk_kv_shape *s) {
     return (unsigned __int128)n_rows * s->n_kv_heads > 4096 && n_rows * s->head_dim / 512 >= n;
 }
 
-// Tile numbers of a call (kv_tile): at most two a segment past the tiles that the rows fill.
-static size_t kv_tiles(size_t n_rows, size_t n) { return n_rows / 64 + 2 * (n + 2); }
-
 // Checks shared by the write and the read; *a filled for a launch, n_rows 0
 // where there is nothing to do.
 static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void *k, const void *v, int dtype,
@@ -509,7 +403,7 @@ static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void
     if (n_rows != 0 && !row_start && n_rows % n != 0)
         return fail(QBK_ERR_VALIDATION, fmt("%zu rows do not split evenly over %zu sequences", n_rows, n));
     // a launch is below 2^32 threads
-    a->tiles = kv_by_tiles(n_rows, n, shape);
+    a->tiles = shape->format != QBK_KV_FP4 && kv_by_tiles(n_rows, n, shape);
     const size_t groups = a->tiles ? kv_tiles(n_rows, n) * shape->n_kv_heads
                                    : div_ceil(n_rows * shape->n_kv_heads, 4);
     if (groups > 0xFFFFFF) return fail(QBK_ERR_VALIDATION, "kv cache: too many rows for one call");
@@ -571,7 +465,8 @@ int qbk_kv_cache_write_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, void *cache,
     if (a.n_rows == 0) return QBK_OK;
     if ((rc = bind(ctx))) return rc;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == QBK_F32)
+    if (shape->format == QBK_KV_FP4) kv4_write_go(a, k, v, dtype, s);
+    else if (dtype == QBK_F32)
         shape->format == QBK_KV_INT8 ? kv_write_go<QBK_KV_INT8>(a, (const float *)k, (const float *)v, s)
                                      : kv_write_go<QBK_KV_FP8>(a, (const float *)k, (const float *)v, s);
     else
@@ -591,7 +486,8 @@ int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *c
     if (a.n_rows == 0) return QBK_OK;
     if ((rc = bind(ctx))) return rc;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == QBK_F32)
+    if (shape->format == QBK_KV_FP4) kv4_read_go(a, k, v, dtype, s);
+    else if (dtype == QBK_F32)
         shape->format == QBK_KV_INT8 ? kv_read_go<QBK_KV_INT8>(a, (float *)k, (float *)v, s)
                                      : kv_read_go<QBK_KV_FP8>(a, (float *)k, (float *)v, s);
     else

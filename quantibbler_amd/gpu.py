@@ -369,14 +369,15 @@ def logprobs_dev(ctx: GpuContext, logits, rows: int, vocab: int, targets, logpro
 
 
 class KvCache:
-    """A KV cache in 8 bits for ``n_seqs`` sequences of up to ``capacity``
-    rows: per row and kv head, head_dim codes ("int8" or "fp8", OCP e4m3) and
-    one f32 scale, quantised as rows are written.  ``buffer`` is the caller's
+    """A KV cache in 8 or 4 bits for ``n_seqs`` sequences of up to ``capacity``
+    rows: per row and kv head, head_dim codes ("int8", "fp8", OCP e4m3, or
+    "fp4", OCP e2m1 with an e4m3 multiplier for every 32 channels) and one f32
+    scale, quantised as rows are written.  ``buffer`` is the caller's
     device memory of ``size(...)`` bytes.  Positions, lengths and row starts
     are device uint32 (or int32) read when a call runs, so a captured graph of
     a step serves every later position."""
 
-    FORMATS = {"int8": _lib.QBK_KV_INT8, "fp8": _lib.QBK_KV_FP8}
+    FORMATS = {"int8": _lib.QBK_KV_INT8, "fp8": _lib.QBK_KV_FP8, "fp4": _lib.QBK_KV_FP4}
 
     def __init__(self, ctx: GpuContext, fmt: str, n_seqs: int, capacity: int, n_kv_heads: int, head_dim: int, buffer):
         need = self.size(fmt, n_seqs, capacity, n_kv_heads, head_dim)

@@ -66,7 +66,7 @@ pub struct AttentionShape {
     pub val_dim: usize,
 }
 
-/// qbk_kv_shape: an 8-bit KV cache's format and sizes.
+/// qbk_kv_shape: an 8-bit or 4-bit KV cache's format and sizes.
 #[repr(C)]
 #[derive(Clone, Copy, Debug, PartialEq, Eq)]
 pub struct KvShape {
