@@ -573,6 +573,85 @@ int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *block, float *h, const uint
                             const qbk_kv_shape *prefix_shape, const void *prefix, size_t prefix_seq,
                             size_t prefix_len, void *workspace, size_t workspace_size, void *stream);
 
+/* ---- rotary positions -------------------------------------------------------- */
+
+/* How the pairs of a head turn with the position (the reference has one way,
+ * rope_rotate, engine/mod.rs:1169-1187: half layout, the whole head, unscaled,
+ * which a block applies by itself).  A plain value that the caller keeps and
+ * passes; qbk_rope_init fills it.  Pair i of rotary_dim / 2 turns by the
+ * position times f_i, f_i = theta^(-2 i / rotary_dim) unless scaled, and is
+ * channels i and i + rotary_dim / 2, or, interleaved, 2 i and 2 i + 1; channels
+ * from rotary_dim on stay.  turns: f_i / 2 pi in units of 2^-64, so that a
+ * position times it is the angle's fraction of a turn, at any position. */
+typedef struct {
+    uint32_t head_dim, rotary_dim, interleaved, reserved;
+    double size; /* what cos and sin are multiplied by */
+    uint64_t turns[128];
+} qbk_rope;
+/* A context stretched by `factor`:
+ *   LINEAR  f_i / factor
+ *   BASE    theta becomes theta factor^(rotary_dim / (rotary_dim - 2))
+ *   RAMP    with t = original_len f_i / 2 pi, the turns of the pair in the
+ *           original context: f_i from t = high on, f_i / factor up to t = low,
+ *           between them k f_i + (1 - k) f_i / factor, k = (t - low) / (high - low)
+ *   YARN    the same by the pair's number, k = 1 up to floor of the number that
+ *           makes `high` turns, 0 from ceil of that which makes `low` on, and
+ *           size = 0.1 ln(factor) + 1 (Peng et al., 2023) */
+enum { QBK_ROPE_PLAIN = 0, QBK_ROPE_LINEAR = 1, QBK_ROPE_BASE = 2, QBK_ROPE_RAMP = 3, QBK_ROPE_YARN = 4 };
+typedef struct {
+    int kind;
+    double factor, original_len, low, high;
+} qbk_rope_scaling;
+/* head_dim even up to 256, rotary_dim even up to head_dim; scaling NULL: none. */
+int qbk_rope_init(qbk_rope *rope, size_t head_dim, size_t rotary_dim, int interleaved, double theta,
+                  const qbk_rope_scaling *scaling);
+/* Queries and keys of n_rows rows, each head RMS-normed (x / sqrt(mean x^2 +
+ * eps) * w over head_dim; q_norm and k_norm f32 [head_dim], either may be NULL:
+ * not normed) and turned to its row's position, in one pass: f32 throughout,
+ * rounded once on the way out (unlike the block's own norm, which rounds its
+ * operand and result to bf16 as the reference's does).  q: rows of n_heads
+ * heads, k: rows of n_kv_heads heads (dtype QBK_F32 or QBK_BF16, row strides in
+ * values: a fused projection's rows are taken in place); k with n_kv_heads 0, or
+ * q with n_heads 0, may be NULL.  Rows belong to n sequences as those of
+ * qbk_kv_cache_write_dev do (row_start NULL: evenly), row row_start[i] + t at
+ * position before + pos[i] + t; rows that no sequence claims are left out.
+ * q_out and k_out may be q and k (with the same strides). */
+int qbk_rotate_heads_dev(qbk_ctx *ctx, const qbk_rope *rope, const void *q, const void *k, int dtype, size_t n_rows,
+                         size_t n_heads, size_t n_kv_heads, size_t q_stride, size_t k_stride, const uint32_t *row_start,
+                         const uint32_t *pos, size_t n, size_t before, const float *q_norm, const float *k_norm,
+                         double eps, void *q_out, void *k_out, size_t q_out_stride, size_t k_out_stride, void *stream);
+
+/* ---- drafted tokens ------------------------------------------------------------ */
+
+/* Verification of drafted tokens against the target's probabilities (no
+ * counterpart in the reference, whose sampler is greedy).  Request i has m =
+ * n_drafts[i] drafts (device uint32, at most k; NULL: k) ids[i][0 .. m - 1]
+ * (device int32), the target's logits in rows i (k + 1) .. i (k + 1) + m of
+ * `logits` and, where the drafts were drawn from a model, that model's in rows
+ * i k .. i k + m - 1 of draft_logits (both QBK_F32 or both QBK_BF16, row strides
+ * in values); draft_logits NULL: drafts that were looked up.  With p_j and q_j
+ * the softmax of row j's logits over temperature[i] (device f32; NULL: 1; not
+ * above 0: all on the likeliest id, the lowest of equals, as qbk_argmax_dev has
+ * it) and q_j = 1 at the draft where there are no draft logits, draft j is kept
+ * while uniforms[i][j] q_j(d) < p_j(d); at the first that is not, or at j = m,
+ * one token is drawn with uniforms[i][m] from max(p_j - q_j, 0), at j = m from
+ * p_m: the first id whose running sum is above the number times the sum (numbers
+ * are in [0, 1); weights all 0: from p_j).  A mask is a logit of -inf.  tokens
+ * [n][k + 1] gets the drafts that were kept, the drawn one and -1 behind; counts
+ * [n] how many that are; pos (may be NULL, device uint32) is advanced by it.  So
+ * what is emitted is distributed as tokens drawn from p one by one; k = 0 draws
+ * one token a request.  A draft outside the vocabulary is not kept; a target row
+ * with a NaN or +inf or nothing above -inf ends its request without a drawn token
+ * (-1, not counted), such a row of draft logits keeps no draft and draws from p.
+ * Exponentials and sums are 64-bit.  workspace of at least
+ * qbk_verify_drafts_workspace_size bytes (draft_logits: whether there are any),
+ * 16-byte aligned. */
+size_t qbk_verify_drafts_workspace_size(size_t n, size_t k, size_t vocab, int draft_logits);
+int qbk_verify_drafts_dev(qbk_ctx *ctx, const void *logits, const void *draft_logits, int dtype, size_t n, size_t k,
+                          size_t vocab, size_t row_stride, size_t draft_row_stride, const int32_t *ids,
+                          const uint32_t *n_drafts, const float *uniforms, const float *temperature, int32_t *tokens,
+                          int32_t *counts, uint32_t *pos, void *workspace, size_t workspace_size, void *stream);
+
 /* ---- log probabilities ------------------------------------------------------ */
 
 /* What the API's logprobs report and a perplexity sums (no counterpart in the

@@ -40,6 +40,17 @@ class KvShape(C.Structure):
     _fields_ = [("format", C.c_int)] + [(n, C.c_size_t) for n in ("n_seqs", "capacity", "n_kv_heads", "head_dim")]
 
 
+class RopeC(C.Structure):
+    """qbk_rope: how the pairs of a head turn with the position."""
+    _fields_ = [(n, C.c_uint32) for n in ("head_dim", "rotary_dim", "interleaved", "reserved")] + \
+        [("size", C.c_double), ("turns", C.c_uint64 * 128)]
+
+
+class RopeScaling(C.Structure):
+    """qbk_rope_scaling."""
+    _fields_ = [("kind", C.c_int)] + [(n, C.c_double) for n in ("factor", "original_len", "low", "high")]
+
+
 _P, _Z, _I = C.c_void_p, C.c_size_t, C.c_int
 _SIGS = {
     "qbk_backend_version": (C.c_char_p, []),
@@ -124,6 +135,11 @@ _SIGS = {
     "qbk_block_decode_kv_workspace_size": (_Z, [_P, C.POINTER(KvShape), _Z, _Z, _Z]),
     "qbk_block_decode_kv_dev": (_I, [_P, _P, _P, _P, _Z, C.POINTER(KvShape), _P, _Z, _Z, C.POINTER(KvShape), _P, _Z,
                                      _Z, _P, _Z, _P]),
+    "qbk_rope_init": (_I, [C.POINTER(RopeC), _Z, _Z, _I, C.c_double, C.POINTER(RopeScaling)]),
+    "qbk_rotate_heads_dev": (_I, [_P, C.POINTER(RopeC), _P, _P, _I, _Z, _Z, _Z, _Z, _Z, _P, _P, _Z, _Z, _P, _P,
+                                  C.c_double, _P, _P, _Z, _Z, _P]),
+    "qbk_verify_drafts_workspace_size": (_Z, [_Z, _Z, _Z, _I]),
+    "qbk_verify_drafts_dev": (_I, [_P, _P, _P, _I, _Z, _Z, _Z, _Z, _Z, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "qbk_logprobs_workspace_size": (_Z, [_Z, _Z, _Z]),
     "qbk_logprobs_dev": (_I, [_P, _P, _I, _Z, _Z, _Z, _P, _P, _P, _Z, _P, _P, _P, _Z, _P]),
     "qbk_sage_blk_workspace_size": (_Z, [C.POINTER(AttnShape)]),

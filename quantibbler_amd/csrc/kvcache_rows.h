@@ -14,29 +14,35 @@ struct KvRows {
     bool tiles;  // by 64-row tiles
 };
 
-// The sequence (0 .. n - 1) and position of row r; false for a row that no
-// sequence claims or that lies past the capacity.  Whatever row_start holds,
-// a row that passes addresses the cache in bounds.  start .. end - 1: the call's
-// rows of that sequence.
-__device__ __forceinline__ bool kv_place(const KvRows &a, uint32_t r, uint32_t &seq, size_t &at, uint32_t &start,
-                                         uint32_t &end) {
-    uint32_t s;
-    if (a.row_start) {
-        uint32_t lo = 0, hi = a.n;  // the last s with row_start[s] <= r
+// The sequence s (0 .. n - 1) that claims row r, and the call's rows start ..
+// end - 1 of it; row_start null: `per` rows a sequence.
+__device__ __forceinline__ bool kv_claim(const uint32_t *row_start, uint32_t n, uint32_t per, uint32_t r, uint32_t &s,
+                                         uint32_t &start, uint32_t &end) {
+    if (row_start) {
+        uint32_t lo = 0, hi = n;  // the last s with row_start[s] <= r
         while (hi - lo > 1) {
             const uint32_t mid = lo + (hi - lo) / 2;
-            if (a.row_start[mid] <= r) lo = mid;
+            if (row_start[mid] <= r) lo = mid;
             else hi = mid;
         }
         s = lo;
-        start = a.row_start[s];
-        end = a.row_start[s + 1];
-        if (r < start || r >= end) return false;
-    } else {
-        s = r / a.per;
-        start = s * a.per;
-        end = start + a.per;
+        start = row_start[s];
+        end = row_start[s + 1];
+        return r >= start && r < end;
     }
+    s = r / per;
+    start = s * per;
+    end = start + per;
+    return true;
+}
+
+// The sequence (0 .. n - 1) and position of row r; false for a row that no
+// sequence claims or that lies past the capacity.  Whatever row_start holds,
+// a row that passes addresses the cache in bounds.
+__device__ __forceinline__ bool kv_place(const KvRows &a, uint32_t r, uint32_t &seq, size_t &at, uint32_t &start,
+                                         uint32_t &end) {
+    uint32_t s;
+    if (!kv_claim(a.row_start, a.n, a.per, r, s, start, end)) return false;
     seq = a.first + s;
     at = (size_t)a.pos[s] + (r - start);
     return at < a.c.cap;

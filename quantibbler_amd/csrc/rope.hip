@@ -1,0 +1,236 @@
+// rope.hip -- heads normed and turned to their positions in one pass.
+//
+// Pair i of a row at position t: angle 2 pi frac(t turns_i), turns_i = f_i / 2 pi
+// in units of 2^-64: an integer product modulo 2^64 is the fraction of a turn
+// itself, to 2^-32 of a turn at position 2^32, where a float product has none of
+// it left from 2^24 turns on.  Cos and sin of what is left of the nearest quarter
+// turn are series in 64 bits (once a row, for all its heads; a f64 FMA takes what
+// a f32 one does), rounded once to f32.
+#include <math.h>
+
+#include "kvcache_rows.h"
+
+#pragma clang fp contract(off)
+
+namespace qbk {
+
+struct RotArgs {
+    const void *q, *k;
+    void *qo, *ko;
+    const float *wq, *wk;
+    const uint32_t *row_start, *pos;
+    size_t qs, ks, qos, kos;  // values from one row to the next
+    uint64_t before;
+    uint32_t n_rows, n, per, H, Hk;
+    float eps;
+    qbk_rope rope;
+};
+
+// cos and sin of 2 pi turns / 2^64.  |x| <= pi / 4: the series' next terms are
+// below 2^-60.
+__device__ __forceinline__ float2 rot_turn(uint64_t turns, double size) {
+    const uint64_t quarter = (turns + (1ull << 61)) >> 62;
+    const double x = (double)(int64_t)(turns - (quarter << 62)) * (6.283185307179586477 * 0x1p-64), z = x * x;
+    double c = -1.0 / 87178291200.0, s = 1.0 / 6227020800.0;
+    c = __builtin_fma(c, z, 1.0 / 479001600.0);
+    s = __builtin_fma(s, z, -1.0 / 39916800.0);
+    c = __builtin_fma(c, z, -1.0 / 3628800.0);
+    s = __builtin_fma(s, z, 1.0 / 362880.0);
+    c = __builtin_fma(c, z, 1.0 / 40320.0);
+    s = __builtin_fma(s, z, -1.0 / 5040.0);
+    c = __builtin_fma(c, z, -1.0 / 720.0);
+    s = __builtin_fma(s, z, 1.0 / 120.0);
+    c = __builtin_fma(c, z, 1.0 / 24.0);
+    s = __builtin_fma(s, z, -1.0 / 6.0);
+    c = __builtin_fma(c, z, -0.5);
+    c = __builtin_fma(c, z, 1.0);
+    s = __builtin_fma(s * z, x, x);
+    if (quarter & 1) {
+        const double t = c;
+        c = -s;
+        s = t;
+    }
+    const double by = quarter & 2 ? -size : size;
+    return float2{(float)(c * by), (float)(s * by)};
+}
+
+template <typename T>
+__device__ __forceinline__ float rot_in(T x) {
+    if constexpr (sizeof(T) == 4) return x;
+    else return bf16_to_f32(x);
+}
+template <typename T>
+__device__ __forceinline__ T rot_out(float x) {
+    if constexpr (sizeof(T) == 4) return x;
+    else return f32_to_bf16(x);
+}
+
+// The row's position; false where no sequence claims it.
+__device__ __forceinline__ bool rot_place(const RotArgs &a, uint32_t r, uint64_t &at) {
+    uint32_t s, start, end;
+    if (!kv_claim(a.row_start, a.n, a.per, r, s, start, end)) return false;
+    at = a.before + a.pos[s] + (r - start);
+    return true;
+}
+
+// A wave a row and head, a pair or a channel a lane at a time: any layout.
+template <typename T>
+__global__ void __launch_bounds__(256) rot_any(RotArgs a) {
+    const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t all = a.H + a.Hk, r = (uint32_t)(item / all), head = (uint32_t)(item % all), lane = threadIdx.x & 63;
+    uint64_t at;
+    if (r >= a.n_rows || !rot_place(a, r, at)) return;
+    const uint32_t hd = a.rope.head_dim, half = a.rope.rotary_dim / 2;
+    const bool is_q = head < a.H;
+    const uint32_t h = is_q ? head : head - a.H;
+    const T *src = is_q ? (const T *)a.q + r * a.qs + (size_t)h * hd : (const T *)a.k + r * a.ks + (size_t)h * hd;
+    T *dst = is_q ? (T *)a.qo + r * a.qos + (size_t)h * hd : (T *)a.ko + r * a.kos + (size_t)h * hd;
+    const float *w = is_q ? a.wq : a.wk;
+    float inv = 1.0f;
+    if (w) {
+        float ss = 0.0f;
+        for (uint32_t c = lane; c < hd; c += 64) {
+            const float x = rot_in<T>(src[c]);
+            ss += x * x;
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        inv = 1.0f / sqrtf(ss / (float)hd + a.eps);
+    }
+    auto value = [&](uint32_t c) {
+        const float x = rot_in<T>(src[c]);
+        return w ? x * inv * w[c] : x;
+    };
+    for (uint32_t i = lane; i < half; i += 64) {
+        const uint32_t c0 = a.rope.interleaved ? 2 * i : i, c1 = a.rope.interleaved ? 2 * i + 1 : i + half;
+        const float2 t = rot_turn(a.rope.turns[i] * at, a.rope.size);
+        const float x = value(c0), y = value(c1);
+        dst[c0] = rot_out<T>(x * t.x - y * t.y);
+        dst[c1] = rot_out<T>(y * t.x + x * t.y);
+    }
+    for (uint32_t c = 2 * half + lane; c < hd; c += 64) dst[c] = rot_out<T>(value(c));
+}
+
+static int rot_check(const qbk_rope *r) {
+    if (!r) return fail(QBK_ERR_VALIDATION, "null argument");
+    if (r->head_dim == 0 || r->head_dim % 2 || r->head_dim > 256 || r->rotary_dim % 2 || r->rotary_dim > r->head_dim)
+        return fail(QBK_ERR_VALIDATION, fmt("rope needs an even head_dim up to 256 and an even rotary_dim up to it, got %u "
+                                            "and %u", r->head_dim, r->rotary_dim));
+    return QBK_OK;
+}
+
+}  // namespace qbk
+
+using namespace qbk;
+
+extern "C" {
+
+int qbk_rope_init(qbk_rope *rope, size_t head_dim, size_t rotary_dim, int interleaved, double theta,
+                  const qbk_rope_scaling *scaling) {
+    if (!rope) return fail(QBK_ERR_VALIDATION, "null argument");
+    if (head_dim == 0 || head_dim % 2 || head_dim > 256 || rotary_dim == 0 || rotary_dim % 2 || rotary_dim > head_dim)
+        return fail(QBK_ERR_VALIDATION, fmt("rope needs an even head_dim up to 256 and an even rotary_dim up to it, got %zu "
+                                            "and %zu", head_dim, rotary_dim));
+    if (!(theta > 0.0) || !isfinite(theta)) return fail(QBK_ERR_VALIDATION, fmt("rope theta must be positive, got %g", theta));
+    const int kind = scaling ? scaling->kind : QBK_ROPE_PLAIN;
+    if (kind < QBK_ROPE_PLAIN || kind > QBK_ROPE_YARN) return fail(QBK_ERR_VALIDATION, fmt("unknown rope scaling %d", kind));
+    const double factor = kind ? scaling->factor : 1.0;
+    if (!(factor > 0.0) || !isfinite(factor))
+        return fail(QBK_ERR_VALIDATION, fmt("rope scaling factor must be positive, got %g", factor));
+    const bool parts = kind == QBK_ROPE_RAMP || kind == QBK_ROPE_YARN;
+    if (parts && (!(scaling->original_len > 0.0) || !(scaling->low > 0.0) || !(scaling->high > scaling->low) ||
+                  !isfinite(scaling->original_len) || !isfinite(scaling->high)))
+        return fail(QBK_ERR_VALIDATION, fmt("rope scaling by parts needs original_len > 0 and 0 < low < high, got %g, %g and %g",
+                                            scaling->original_len, scaling->low, scaling->high));
+    if (kind == QBK_ROPE_YARN && !(theta > 1.0))
+        return fail(QBK_ERR_VALIDATION, fmt("rope scaling by the pair's number needs theta above 1, got %g", theta));
+    const long double tau = 6.28318530717958647692528676655900577L;
+    long double base = theta;
+    if (kind == QBK_ROPE_BASE && rotary_dim > 2)
+        base *= powl((long double)factor, (long double)rotary_dim / (long double)(rotary_dim - 2));
+    double first = 0.0, last = 0.0;
+    if (kind == QBK_ROPE_YARN) {
+        auto pair = [&](double turns) {
+            return (double)rotary_dim * log(scaling->original_len / (turns * (double)tau)) / (2.0 * log(theta));
+        };
+        first = fmax(floor(pair(scaling->high)), 0.0);
+        last = fmin(ceil(pair(scaling->low)), (double)rotary_dim - 1.0);
+    }
+    qbk_rope r{};
+    r.head_dim = (uint32_t)head_dim;
+    r.rotary_dim = (uint32_t)rotary_dim;
+    r.interleaved = interleaved != 0;
+    r.size = kind == QBK_ROPE_YARN ? 0.1 * log(factor) + 1.0 : 1.0;
+    for (size_t i = 0; i < rotary_dim / 2; i++) {
+        long double f = powl(base, -2.0L * (long double)i / (long double)rotary_dim), keep = 1.0L;
+        if (kind == QBK_ROPE_LINEAR) keep = 0.0L;
+        if (kind == QBK_ROPE_RAMP)
+            keep = (scaling->original_len * f / tau - scaling->low) / ((long double)scaling->high - scaling->low);
+        if (kind == QBK_ROPE_YARN) keep = 1.0 - ((double)i - first) / fmax(last - first, 0.001);
+        keep = keep < 0.0L ? 0.0L : keep > 1.0L ? 1.0L : keep;
+        f = f * keep + f / factor * (1.0L - keep);
+        if (!isfinite((double)f)) return fail(QBK_ERR_VALIDATION, fmt("rope frequencies of theta %g pass the range", theta));
+        const long double part = f / tau;
+        r.turns[i] = (uint64_t)((part - floorl(part)) * 0x1p64L);
+    }
+    *rope = r;
+    return QBK_OK;
+}
+
+int qbk_rotate_heads_dev(qbk_ctx *ctx, const qbk_rope *rope, const void *q, const void *k, int dtype, size_t n_rows,
+                         size_t n_heads, size_t n_kv_heads, size_t q_stride, size_t k_stride, const uint32_t *row_start,
+                         const uint32_t *pos, size_t n, size_t before, const float *q_norm, const float *k_norm,
+                         double eps, void *q_out, void *k_out, size_t q_out_stride, size_t k_out_stride, void *stream) {
+    int rc;
+    if ((rc = rot_check(rope))) return rc;
+    if (dtype != QBK_F32 && dtype != QBK_BF16)
+        return fail(QBK_ERR_VALIDATION, fmt("rotate_heads takes float32 or bfloat16 rows (dtype %d)", dtype));
+    if (n_heads > 65536 || n_kv_heads > 65536) return fail(QBK_ERR_VALIDATION, "rotate_heads takes up to 65536 heads");
+    const size_t hd = rope->head_dim, most = (size_t)1 << 40;
+    const size_t strides[4] = {q_stride, q_out_stride, k_stride, k_out_stride};
+    for (int i = 0; i < 4; i++) {
+        const size_t width = (i < 2 ? n_heads : n_kv_heads) * hd;
+        if (n_rows > 1 && width && (strides[i] < width || strides[i] > most))
+            return fail(QBK_ERR_VALIDATION, fmt("a row stride of %zu does not fit a row of %zu values", strides[i], width));
+    }
+    if (n_rows > 0x7FFFFFFFull || before > 0xFFFFFFFFull || n > 0x7FFFFFFFull)
+        return fail(QBK_ERR_VALIDATION, "rotate_heads: too many rows for one call");
+    if (n_rows != 0 && n == 0) return fail(QBK_ERR_VALIDATION, "rotate_heads: rows of no sequence");
+    if (n_rows != 0 && !row_start && n_rows % n != 0)
+        return fail(QBK_ERR_VALIDATION, fmt("%zu rows do not split evenly over %zu sequences", n_rows, n));
+    if (!(eps >= 0.0) && (q_norm || k_norm)) return fail(QBK_ERR_VALIDATION, fmt("rotate_heads: eps must not be negative, got %g", eps));
+    const size_t groups = div_ceil(n_rows * (n_heads + n_kv_heads), 4);
+    if (groups > 0xFFFFFF) return fail(QBK_ERR_VALIDATION, "rotate_heads: too many rows for one call");
+    if (groups == 0) return QBK_OK;
+    if (!pos || (n_heads && (!q || !q_out)) || (n_kv_heads && (!k || !k_out)))
+        return fail(QBK_ERR_VALIDATION, "null argument");
+    if ((rc = bind(ctx))) return rc;
+    RotArgs a{};
+    a.q = q;
+    a.k = k;
+    a.qo = q_out;
+    a.ko = k_out;
+    a.wq = q_norm;
+    a.wk = k_norm;
+    a.row_start = row_start;
+    a.pos = pos;
+    a.qs = q_stride;
+    a.ks = k_stride;
+    a.qos = q_out_stride;
+    a.kos = k_out_stride;
+    a.before = before;
+    a.n_rows = (uint32_t)n_rows;
+    a.n = (uint32_t)n;
+    a.per = (uint32_t)(n_rows / n ? n_rows / n : 1);
+    a.H = (uint32_t)n_heads;
+    a.Hk = (uint32_t)n_kv_heads;
+    a.eps = (float)eps;
+    a.rope = *rope;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == QBK_F32) hipLaunchKernelGGL(rot_any<float>, dim3((unsigned)groups), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(rot_any<uint16_t>, dim3((unsigned)groups), dim3(256), 0, s, a);
+    QBK_HIP(hipGetLastError());
+    return QBK_OK;
+}
+
+}  // extern "C"

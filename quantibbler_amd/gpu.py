@@ -18,7 +18,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import AttnShape, KvShape, check
+from ._lib import AttnShape, KvShape, RopeC, RopeScaling, check
 
 _DTYPES = {"float64": (_lib.QBK_F64, np.float64), "float32": (_lib.QBK_F32, np.float32),
            "bfloat16": (_lib.QBK_BF16, np.uint16)}
@@ -366,6 +366,132 @@ def logprobs_dev(ctx: GpuContext, logits, rows: int, vocab: int, targets, logpro
         _device_words(top_ids, rows * k, ctx, "top_ids"),
         _device_values(top_logprobs, "float32", rows * k, ctx, "logprobs: top_logprobs"),
         _device_bytes(workspace, workspace_size, ctx, "logprobs: workspace"), int(workspace_size), _stream(stream)))
+
+
+def verify_drafts_workspace_size(n: int, drafts: int, vocab: int, draft_logits: bool = False) -> int:
+    """Bytes of workspace ``verify_drafts_dev`` needs."""
+    if min(int(n), int(drafts), int(vocab)) < 0:
+        raise _lib.KernelError("verify_drafts sizes must not be negative")
+    return int(_lib.load().qbk_verify_drafts_workspace_size(int(n), int(drafts), int(vocab), int(bool(draft_logits))))
+
+
+def verify_drafts_dev(ctx: GpuContext, logits, n: int, drafts: int, vocab: int, ids, uniforms, tokens, counts,
+                      workspace, workspace_size: int, draft_logits=None, n_drafts=None, temperature=None, pos=None,
+                      dtype: str = "float32", row_stride: int | None = None, draft_row_stride: int | None = None,
+                      stream=None):
+    """Drafted tokens against the target's probabilities, for n requests of up
+    to ``drafts`` (64) each: keeps a request's drafts ``ids`` [n][drafts] (device
+    int32) while uniforms[i][j] q_j(draft) < p_j(draft) and draws one more token,
+    so that what is emitted is distributed as the target's own tokens.
+
+    ``logits`` [n][drafts + 1][vocab]: the target's at each draft and behind the
+    last; ``draft_logits`` [n][drafts][vocab]: those the drafts were drawn from
+    (None: drafts that were looked up, q_j = 1), both ``dtype`` ("float32" or
+    "bfloat16"), rows ``row_stride`` / ``draft_row_stride`` values apart;
+    ``uniforms`` [n][drafts + 1] f32 in [0, 1), of which a request's number
+    n_drafts[i] draws; ``n_drafts`` device words (None: all have ``drafts``);
+    ``temperature`` device f32 a request (None: 1; 0: the likeliest id).
+    ``tokens`` [n][drafts + 1] int32 gets the kept drafts, the drawn token and -1
+    behind, ``counts`` [n] how many there are, and ``pos``, where given, is
+    advanced by as many.  drafts = 0 draws a token a request."""
+    code = _SERVING_DTYPES.get(dtype)
+    if code is None:
+        raise _lib.KernelError(f"verify_drafts takes 'float32' or 'bfloat16' logits, got {dtype!r}")
+    n, k, vocab = int(n), int(drafts), int(vocab)
+    stride = vocab if row_stride is None else int(row_stride)
+    dstride = vocab if draft_row_stride is None else int(draft_row_stride)
+    if min(n, k, vocab, stride, dstride) < 0:
+        raise _lib.KernelError("verify_drafts sizes must not be negative")
+    rows, drows = n * (k + 1), n * k
+    x = _device_values(logits, dtype, (rows - 1) * stride + vocab if rows else 0, ctx, "verify_drafts: logits",
+                       row_stride is not None)
+    y = _device_values(draft_logits, dtype, (drows - 1) * dstride + vocab if drows else 0, ctx,
+                       "verify_drafts: draft_logits", draft_row_stride is not None)
+    check(_lib.load().qbk_verify_drafts_dev(
+        ctx.handle, x, y, code, n, k, vocab, stride, dstride, _device_words(ids, drows, ctx, "ids"),
+        _device_words(n_drafts, n, ctx, "n_drafts"), _device_values(uniforms, "float32", rows, ctx,
+                                                                    "verify_drafts: uniforms"),
+        _device_values(temperature, "float32", n, ctx, "verify_drafts: temperature"),
+        _device_words(tokens, rows, ctx, "tokens"), _device_words(counts, n, ctx, "counts"),
+        _device_words(pos, n, ctx, "positions"),
+        _device_bytes(workspace, workspace_size, ctx, "verify_drafts: workspace"), int(workspace_size),
+        _stream(stream)))
+
+
+class Rope:
+    """How the pairs of a head turn with the position (rotate_heads_dev): pair
+    i of ``rotary_dim`` / 2 (None: the whole head) by theta^(-2 i / rotary_dim) a
+    position, channels i and i + rotary_dim / 2 or, ``interleaved``, 2 i and
+    2 i + 1.  ``scaling`` stretches the context: None, or a dict with "kind" and
+    "factor": "linear" (slower throughout), "base" (a larger theta), "ramp" or
+    "yarn" (slower where a pair makes few turns in "original_len" positions:
+    "low" (1) and fewer by the factor, "high" (4; yarn 32) and more not at all;
+    yarn counts by the pair's number and scales cos and sin)."""
+
+    KINDS = {"linear": 1, "base": 2, "ramp": 3, "yarn": 4}
+
+    def __init__(self, head_dim: int, theta: float, rotary_dim: int | None = None, interleaved: bool = False,
+                 scaling: dict | None = None):
+        s = None
+        if scaling is not None:
+            given = dict(scaling)
+            kind = given.pop("kind", None)
+            if kind not in self.KINDS:
+                raise _lib.KernelError(f"rope scaling kind must be one of {sorted(self.KINDS)}, got {kind!r}")
+            values = {"factor": given.pop("factor", None)}
+            if kind in ("ramp", "yarn"):
+                values.update(original_len=given.pop("original_len", None), low=given.pop("low", 1.0),
+                              high=given.pop("high", 4.0 if kind == "ramp" else 32.0))
+            missing = sorted(k for k, v in values.items() if v is None)
+            if missing or given:
+                raise _lib.KernelError(f"rope scaling {kind!r}: missing {missing}, unknown {sorted(given)}")
+            s = C.byref(RopeScaling(self.KINDS[kind], **{k: float(v) for k, v in values.items()}))
+        hd, rd = int(head_dim), int(head_dim if rotary_dim is None else rotary_dim)
+        if hd < 0 or rd < 0:
+            raise _lib.KernelError("rope sizes must not be negative")
+        self._rope = RopeC()
+        check(_lib.load().qbk_rope_init(C.byref(self._rope), hd, rd, int(bool(interleaved)), float(theta), s))
+        self._ref = C.byref(self._rope)
+        self.head_dim, self.rotary_dim, self.interleaved = hd, rd, bool(interleaved)
+
+
+def rotate_heads_dev(ctx: GpuContext, rope: Rope, q, k, dtype: str, n_rows: int, n_heads: int, n_kv_heads: int, pos,
+                     q_out, k_out, n_seqs: int = 1, row_start=None, before: int = 0, q_norm=None, k_norm=None,
+                     eps: float = 1e-6, q_stride: int | None = None, k_stride: int | None = None,
+                     q_out_stride: int | None = None, k_out_stride: int | None = None, stream=None):
+    """Queries [n_rows][n_heads][head_dim] and keys [n_rows][n_kv_heads][head_dim]
+    ("float32" or "bfloat16", rows ``*_stride`` values apart, so a fused
+    projection's are taken in place), each head RMS-normed where it has a weight
+    (``q_norm``, ``k_norm``: device f32 [head_dim]) and turned to its row's
+    position, into q_out and k_out, which may be q and k: rows row_start[i] ..
+    row_start[i + 1] - 1 are sequence i's at before + pos[i], before + pos[i] + 1,
+    ... (as KvCache.write_dev's; ``row_start`` None splits the rows evenly over
+    ``n_seqs``); rows no sequence claims are left out.  n_heads or n_kv_heads may
+    be 0, with None for the tensors."""
+    code = _SERVING_DTYPES.get(dtype)
+    if code is None:
+        raise _lib.KernelError(f"rotate_heads takes 'float32' or 'bfloat16' rows, got {dtype!r}")
+    hd = rope.head_dim
+    if min(n_rows, n_heads, n_kv_heads, n_seqs, before) < 0:
+        raise _lib.KernelError("rotate_heads sizes must not be negative")
+
+    def rows(x, heads, stride, what):
+        s = heads * hd if stride is None else stride
+        if s < 0:
+            raise _lib.KernelError("rotate_heads strides must not be negative")
+        room = (n_rows - 1) * s + heads * hd if n_rows and heads else 0
+        return _device_values(x, dtype, room, ctx, f"rotate_heads: {what}", stride is not None), s
+
+    qi, qs = rows(q, n_heads, q_stride, "q")
+    ki, ks = rows(k, n_kv_heads, k_stride, "k")
+    qo, qos = rows(q_out, n_heads, q_out_stride, "q_out")
+    ko, kos = rows(k_out, n_kv_heads, k_out_stride, "k_out")
+    check(_lib.load().qbk_rotate_heads_dev(
+        ctx.handle, rope._ref, qi, ki, code, n_rows, n_heads, n_kv_heads, qs, ks,
+        _device_words(row_start, n_seqs + 1, ctx, "row starts"), _device_words(pos, n_seqs, ctx, "positions"), n_seqs,
+        before, _device_values(q_norm, "float32", hd, ctx, "rotate_heads: q_norm"),
+        _device_values(k_norm, "float32", hd, ctx, "rotate_heads: k_norm"), float(eps), qo, ko, qos, kos,
+        _stream(stream)))
 
 
 class KvCache:

@@ -77,6 +77,29 @@ pub struct KvShape {
     pub head_dim: usize,
 }
 
+/// qbk_rope: how the pairs of a head turn with the position (qbk_rope_init).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Rope {
+    pub head_dim: u32,
+    pub rotary_dim: u32,
+    pub interleaved: u32,
+    pub reserved: u32,
+    pub size: f64,
+    pub turns: [u64; 128],
+}
+
+/// qbk_rope_scaling: a context stretched by `factor` (kind: 1 linear, 2 base, 3 ramp, 4 yarn).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct RopeScaling {
+    pub kind: c_int,
+    pub factor: f64,
+    pub original_len: f64,
+    pub low: f64,
+    pub high: f64,
+}
+
 extern "C" {
     pub fn qbk_backend_version() -> *const c_char;
     pub fn qbk_last_error() -> *const c_char;
@@ -243,6 +266,19 @@ extern "C" {
                                    prefix_shape: *const KvShape, prefix: *const c_void, prefix_seq: usize,
                                    prefix_len: usize, workspace: *mut c_void, workspace_size: usize,
                                    stream: *mut c_void) -> c_int;
+    pub fn qbk_rope_init(rope: *mut Rope, head_dim: usize, rotary_dim: usize, interleaved: c_int, theta: f64,
+                         scaling: *const RopeScaling) -> c_int;
+    pub fn qbk_rotate_heads_dev(ctx: *mut QbkCtx, rope: *const Rope, q: *const c_void, k: *const c_void, dtype: c_int,
+                                n_rows: usize, n_heads: usize, n_kv_heads: usize, q_stride: usize, k_stride: usize,
+                                row_start: *const u32, pos: *const u32, n: usize, before: usize, q_norm: *const f32,
+                                k_norm: *const f32, eps: f64, q_out: *mut c_void, k_out: *mut c_void,
+                                q_out_stride: usize, k_out_stride: usize, stream: *mut c_void) -> c_int;
+    pub fn qbk_verify_drafts_workspace_size(n: usize, k: usize, vocab: usize, draft_logits: c_int) -> usize;
+    pub fn qbk_verify_drafts_dev(ctx: *mut QbkCtx, logits: *const c_void, draft_logits: *const c_void, dtype: c_int,
+                                 n: usize, k: usize, vocab: usize, row_stride: usize, draft_row_stride: usize,
+                                 ids: *const i32, n_drafts: *const u32, uniforms: *const f32,
+                                 temperature: *const f32, tokens: *mut i32, counts: *mut i32, pos: *mut u32,
+                                 workspace: *mut c_void, workspace_size: usize, stream: *mut c_void) -> c_int;
     pub fn qbk_logprobs_workspace_size(rows: usize, vocab: usize, top_k: usize) -> usize;
     pub fn qbk_logprobs_dev(ctx: *mut QbkCtx, logits: *const c_void, dtype: c_int, rows: usize, vocab: usize,
                             row_stride: usize, targets: *const i32, logprobs: *mut f32, entropy: *mut f32,
