@@ -14,6 +14,8 @@
 
 namespace qbk {
 
+#define ROT_WAVES 8192
+
 struct RotArgs {
     const void *q, *k;
     void *qo, *ko;
@@ -23,6 +25,7 @@ struct RotArgs {
     uint64_t before;
     uint32_t n_rows, n, per, H, Hk;
     float eps;
+    uint32_t waves;  // a row's
     qbk_rope rope;
 };
 
@@ -73,6 +76,115 @@ __device__ __forceinline__ bool rot_place(const RotArgs &a, uint32_t r, uint64_t
     return true;
 }
 
+// The sum over aligned runs of LANES lanes.
+template <int LANES>
+__device__ __forceinline__ float rot_sum(float v) {
+    auto add = [](float x, int moved) { return x + __uint_as_float((uint32_t)moved); };
+    if constexpr (LANES >= 2) v = add(v, __builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0xB1, 0xf, 0xf, true));   // lane ^ 1
+    if constexpr (LANES >= 4) v = add(v, __builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x4E, 0xf, 0xf, true));   // lane ^ 2
+    if constexpr (LANES >= 8) v = add(v, __builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x141, 0xf, 0xf, true));  // 7 - lane
+    if constexpr (LANES >= 16) v = add(v, __builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x140, 0xf, 0xf, true)); // 15 - lane
+    if constexpr (LANES >= 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    return v;
+}
+
+// Four values at any alignment, one access.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Rot4 {
+    T v[4];
+};
+
+// LANES lanes a head, two runs of four channels a lane: in the half layout
+// channels 4 l .. and rotary / 2 + 4 l .., the two halves of four pairs,
+// interleaved and past rotary_dim 8 l .. 8 l + 7.  A wave takes 64 / LANES heads
+// of a row at a time and turns all of them by the four angles it has formed
+// once.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) rot_quads(RotArgs a) {
+    constexpr uint32_t HEADS = 64 / LANES;
+    const uint64_t item = (uint64_t)blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t r = (uint32_t)(item / a.waves), wave = (uint32_t)(item % a.waves);
+    uint64_t at;
+    if (r >= a.n_rows || !rot_place(a, r, at)) return;
+    const uint32_t lane = threadIdx.x & 63, l = lane % LANES, hd = a.rope.head_dim, half = a.rope.rotary_dim / 2;
+    const bool in = 8 * l < hd, turned = 8 * l < 2 * half, inter = a.rope.interleaved;
+    const uint32_t c0 = turned && !inter ? 4 * l : 8 * l, c1 = turned && !inter ? half + 4 * l : 8 * l + 4;
+    float2 t[4];
+    if (turned)
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] = rot_turn(a.rope.turns[4 * l + i] * at, a.rope.size);
+    const uint32_t all = a.H + a.Hk;
+    for (uint32_t first = wave * HEADS; first < all; first += a.waves * HEADS) {
+        const uint32_t head = first + lane / LANES;
+        const bool is_q = head < a.H, live = in && head < all;
+        const uint32_t h = is_q ? head : head - a.H;
+        const T *src = is_q ? (const T *)a.q + r * a.qs + (size_t)h * hd : (const T *)a.k + r * a.ks + (size_t)h * hd;
+        T *dst = is_q ? (T *)a.qo + r * a.qos + (size_t)h * hd : (T *)a.ko + r * a.kos + (size_t)h * hd;
+        const float *w = is_q ? a.wq : a.wk;
+        float x[8];
+        if (live) {
+            const Rot4<T> lo = *(const Rot4<T> *)(src + c0), hi = *(const Rot4<T> *)(src + c1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[e] = rot_in<T>(lo.v[e]);
+                x[4 + e] = rot_in<T>(hi.v[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = 0.0f;
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss += x[e] * x[e];
+        ss = rot_sum<LANES>(ss);
+        if (!live) continue;
+        if (w) {
+            const float inv = __builtin_amdgcn_rsqf(ss / (float)hd + a.eps);
+            const Rot4<float> lo = *(const Rot4<float> *)(w + c0), hi = *(const Rot4<float> *)(w + c1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[e] = x[e] * inv * lo.v[e];
+                x[4 + e] = x[4 + e] * inv * hi.v[e];
+            }
+        }
+        if (turned) {
+            if (inter) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float p = x[2 * i], q = x[2 * i + 1];
+                    x[2 * i] = p * t[i].x - q * t[i].y;
+                    x[2 * i + 1] = q * t[i].x + p * t[i].y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float p = x[i], q = x[4 + i];
+                    x[i] = p * t[i].x - q * t[i].y;
+                    x[4 + i] = q * t[i].x + p * t[i].y;
+                }
+            }
+        }
+        Rot4<T> lo, hi;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                lo.v[e] = x[e];
+                hi.v[e] = x[4 + e];
+            }
+        } else {
+            const uint2 u = {f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3])};
+            const uint2 v = {f32x2_to_bf16x2(x[4], x[5]), f32x2_to_bf16x2(x[6], x[7])};
+            lo = __builtin_bit_cast(Rot4<T>, u);
+            hi = __builtin_bit_cast(Rot4<T>, v);
+        }
+        *(Rot4<T> *)(dst + c0) = lo;
+        *(Rot4<T> *)(dst + c1) = hi;
+    }
+}
+
 // A wave a row and head, a pair or a channel a lane at a time: any layout.
 template <typename T>
 __global__ void __launch_bounds__(256) rot_any(RotArgs a) {
@@ -109,6 +221,28 @@ __global__ void __launch_bounds__(256) rot_any(RotArgs a) {
         dst[c1] = rot_out<T>(y * t.x + x * t.y);
     }
     for (uint32_t c = 2 * half + lane; c < hd; c += 64) dst[c] = rot_out<T>(value(c));
+}
+
+// Whether a head falls into runs of four pairs and eight channels.
+static bool rot_by_quads(const qbk_rope &r) { return r.head_dim % 8 == 0 && r.rotary_dim % 8 == 0; }
+
+template <typename T>
+static void rot_go(RotArgs a, hipStream_t s) {
+    const size_t all = a.H + a.Hk;
+    if (!rot_by_quads(a.rope)) {
+        hipLaunchKernelGGL(rot_any<T>, dim3((unsigned)div_ceil(a.n_rows * all, 4)), dim3(256), 0, s, a);
+        return;
+    }
+    const uint32_t hd = a.rope.head_dim;
+    const int lanes = hd <= 16 ? 2 : hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
+    const size_t passes = div_ceil(all, (size_t)(64 / lanes)), want = div_ceil(ROT_WAVES, (size_t)a.n_rows);
+    a.waves = (uint32_t)(want < 1 ? 1 : want < passes ? want : passes);
+    void (*k)(RotArgs) = lanes == 2   ? rot_quads<T, 2>
+                         : lanes == 4 ? rot_quads<T, 4>
+                         : lanes == 8 ? rot_quads<T, 8>
+                         : lanes == 16 ? rot_quads<T, 16>
+                                       : rot_quads<T, 32>;
+    hipLaunchKernelGGL(k, dim3((unsigned)div_ceil((size_t)a.n_rows * a.waves, 4)), dim3(256), 0, s, a);
 }
 
 static int rot_check(const qbk_rope *r) {
@@ -227,8 +361,8 @@ int qbk_rotate_heads_dev(qbk_ctx *ctx, const qbk_rope *rope, const void *q, cons
     a.eps = (float)eps;
     a.rope = *rope;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == QBK_F32) hipLaunchKernelGGL(rot_any<float>, dim3((unsigned)groups), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(rot_any<uint16_t>, dim3((unsigned)groups), dim3(256), 0, s, a);
+    if (dtype == QBK_F32) rot_go<float>(a, s);
+    else rot_go<uint16_t>(a, s);
     QBK_HIP(hipGetLastError());
     return QBK_OK;
 }
