@@ -403,7 +403,7 @@ static int kv_rows_args(const qbk_kv_shape *shape, const void *cache, const void
     if (n_rows != 0 && !row_start && n_rows % n != 0)
         return fail(QBK_ERR_VALIDATION, fmt("%zu rows do not split evenly over %zu sequences", n_rows, n));
     // a launch is below 2^32 threads
-    a->tiles = shape->format != QBK_KV_FP4 && kv_by_tiles(n_rows, n, shape);
+    a->tiles = kv_by_tiles(n_rows, n, shape);
     const size_t groups = a->tiles ? kv_tiles(n_rows, n) * shape->n_kv_heads
                                    : div_ceil(n_rows * shape->n_kv_heads, 4);
     if (groups > 0xFFFFFF) return fail(QBK_ERR_VALIDATION, "kv cache: too many rows for one call");

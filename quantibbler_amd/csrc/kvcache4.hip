@@ -165,16 +165,282 @@ __global__ void __launch_bounds__(256) kv4_read(KvRows a, T *k, T *v) {
     }
 }
 
-void kv4_write_go(const KvRows &a, const void *k, const void *v, int dtype, hipStream_t s) {
-    const dim3 grid((unsigned)div_ceil((size_t)a.n_rows * a.c.Hk, 4));
-    if (dtype == QBK_F32) hipLaunchKernelGGL(kv4_write<float>, grid, dim3(256), 0, s, a, (const float *)k, (const float *)v);
-    else hipLaunchKernelGGL(kv4_write<uint16_t>, grid, dim3(256), 0, s, a, (const uint16_t *)k, (const uint16_t *)v);
+// ---- many rows a sequence: a workgroup a 64-row tile of one kv head ----------
+
+// Four codes of 16 bits as four bytes, and back.
+__device__ __forceinline__ uint32_t kv4_bytes(uint32_t w) {
+    w = (w | w << 8) & 0x00ff00ffu;
+    return (w | w << 4) & 0x0f0f0f0fu;
+}
+__device__ __forceinline__ uint32_t kv4_nibbles(uint32_t b) {
+    b |= b >> 4;
+    return __builtin_amdgcn_perm(0u, b, 0x0c0c0200u);
+}
+// 4 x 4 codes: out[i] = codes i of in[0 .. 3].
+__device__ __forceinline__ void kv4_turn(const uint32_t (&in)[4], uint32_t (&out)[4]) {
+    uint32_t b[4], t[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = kv4_bytes(in[i]);
+    kv_transpose4(b, t);
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = kv4_nibbles(t[i]);
+}
+// The largest over aligned runs of eight lanes.
+__device__ __forceinline__ uint32_t kv4_max8(uint32_t v) {
+    v = kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));   // lane ^ 1
+    v = kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));   // lane ^ 2
+    return kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));  // 7 - lane
+}
+// Bits of the codes of rows 4 k .. 4 k + 3 that lie in lo .. hi - 1.
+__device__ __forceinline__ uint32_t kv4_rows_in(uint32_t row, uint32_t lo, uint32_t hi) {
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) m |= row + j >= lo && row + j < hi ? 15u << (4 * j) : 0u;
+    return m;
 }
 
+// Sixteen lanes a row, four channels a lane and P times 64 channels, sixteen
+// rows at a time and every row's loads before the first is used.  Codes go
+// through LDS, 16 bits for four channels of a row, and leave 16 bytes at a time:
+// keys as two rows' sixteen channels, values, turned by 4 x 4, as two channels'
+// sixteen rows; multipliers through LDS in the cache's order.
+template <int P, typename T>
+__global__ void __launch_bounds__(256) kv4_write_tiles(KvRows a, const T *k, const T *v) {
+    constexpr int PAD = 16 * P + 4;  // of an LDS row, in four channels: keys are read eight bytes at a time
+    __shared__ __attribute__((aligned(16))) uint16_t codes[64 * PAD];
+    __shared__ __attribute__((aligned(16))) uint8_t mul[2 * P * 64];
+    const uint32_t h = blockIdx.x % a.c.Hk, tid = threadIdx.x, hd = a.c.hd, ng = a.c.groups(), nc = hd / 16;
+    KvTile t;
+    if (!kv_tile(a, blockIdx.x / a.c.Hk, &t) || t.seq < 0 || t.first >= a.c.cap) return;
+    const size_t slab = a.c.slab(a.first + t.seq, h);
+    uint32_t hi = t.hi;
+    if (t.first + hi > a.c.cap) hi = (uint32_t)(a.c.cap - t.first);
+    const bool full = t.lo == 0 && hi == 64;
+    const uint32_t c0 = 4 * (tid & 15);
+    const T *srcs[2] = {k, v};
+    Kv4<T> raw[4][P];
+    auto load = [&](int val) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t r = 16 * q + (tid >> 4);
+            const bool in = r >= t.lo && r < hi;
+            const T *src = srcs[val] + (size_t)(t.row + (in ? r - t.lo : 0)) * a.stride + (size_t)h * hd;
+#pragma unroll
+            for (int p = 0; p < P; p++) raw[q][p] = *(const Kv4<T> *)(src + (c0 + 64 * p < hd ? c0 + 64 * p : 0));
+        }
+    };
+    load(0);
+#pragma unroll
+    for (int val = 0; val < 2; val++) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t r = 16 * q + (tid >> 4);
+            float x[P][4];
+            uint32_t group[P], top = 0;
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                group[p] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[p][e] = c0 + 64 * p < hd ? kv_in<T>(raw[q][p].v[e]) : 0.0f;
+                    group[p] = kv4_most(group[p], __float_as_uint(x[p][e]) & 0x7fffffffu);
+                }
+                group[p] = kv4_max8(group[p]);
+                top = kv4_most(top, group[p]);
+            }
+            top = kv4_most(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x128, 0xf, 0xf, true));  // row_ror 8
+            const Kv4Row row(top);
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                const uint32_t c = c0 + 64 * p;
+                if (c >= hd) continue;
+                float by;
+                const uint32_t m = kv4_mul(row, group[p], by);
+                codes[r * PAD + c / 4] = (uint16_t)kv4_codes(row, x[p], by);
+                if ((tid & 7) == 0)
+                    mul[c / 32 * 64 + (val ? (r >> 2 & 3) * 16 + (r >> 4) * 4 + (r & 3) : (r & 15) * 4 + (r >> 4))] = (uint8_t)m;
+            }
+            if (r >= t.lo && r < hi && (tid & 15) == 0) (val ? a.c.vs : a.c.ks)[slab + t.first + r] = row.scale;
+        }
+        if (val == 0) load(1);  // on their way while the keys leave
+        __syncthreads();
+        uint8_t *md = (val ? a.c.vm : a.c.km) + slab * ng + t.first * ng;
+        for (uint32_t x = tid; x < 16 * ng; x += 256) {  // four rows of a group: key 16 i + x % 16, value 16 i + 4 g + j
+            const uint32_t w = *(const uint32_t *)(mul + 4 * x);
+            if (full) {
+                *(uint32_t *)(md + 4 * x) = w;
+                continue;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t r = val ? (x & 3) * 16 + (x >> 2 & 3) * 4 + i : 16 * i + (x & 15);
+                if (r >= t.lo && r < hi) md[4 * x + i] = (uint8_t)(w >> (8 * i));
+            }
+        }
+        if (val == 0) {
+            uint8_t *dst = a.c.k + slab * (hd / 2) + t.first * (hd / 2);
+            for (uint32_t x = tid; x < 32 * nc; x += 256) {  // rows r and r + 16, one run of 16 channels
+                const uint32_t pair = x / (16 * nc), y = x - pair * 16 * nc, chunk = y >> 4, r = 32 * pair + (y & 15);
+                const uint2 one = *(const uint2 *)(codes + r * PAD + 4 * chunk);
+                const uint2 two = *(const uint2 *)(codes + (r + 16) * PAD + 4 * chunk);
+                const bool in1 = r >= t.lo && r < hi, in2 = r + 16 >= t.lo && r + 16 < hi;
+                uint8_t *d = dst + (size_t)x * 16;
+                if (in1 && in2) *(uint4 *)d = uint4{one.x, one.y, two.x, two.y};
+                else if (in1) *(uint2 *)d = one;
+                else if (in2) *(uint2 *)(d + 8) = two;
+            }
+        } else {
+            uint8_t *dst = a.c.v + slab * (16 * ng) + t.first * (16 * ng);
+            for (uint32_t x = tid; x < 16 * ng; x += 256) {  // channels 4 q .. of both halves of a group, rows of one g
+                const uint32_t g = x & 3, q = x >> 2 & 3, m = x >> 4;
+                uint32_t out[2][4][4];  // [half][i][channel]
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t in[4];
+                        const uint32_t c4 = 8 * m + 4 * half + q;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) in[j] = 4 * c4 < hd ? codes[(16 * i + 4 * g + j) * PAD + c4] : 0u;
+                        kv4_turn(in, out[half][i]);
+                    }
+                uint32_t keep[2] = {0u, 0u};  // codes that stay as they were
+                if (!full) {
+                    keep[0] = ~(kv4_rows_in(4 * g, t.lo, hi) | kv4_rows_in(16 + 4 * g, t.lo, hi) << 16);
+                    keep[1] = ~(kv4_rows_in(32 + 4 * g, t.lo, hi) | kv4_rows_in(48 + 4 * g, t.lo, hi) << 16);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint4 *d = (uint4 *)(dst + m * 1024 + (4 * q + e) * 64 + g * 16);
+                    uint4 w;
+                    w.x = out[0][0][e] | out[0][1][e] << 16;
+                    w.y = out[0][2][e] | out[0][3][e] << 16;
+                    w.z = out[1][0][e] | out[1][1][e] << 16;
+                    w.w = out[1][2][e] | out[1][3][e] << 16;
+                    if (!full) {
+                        const uint4 o = *d;
+                        w.x = (w.x & ~keep[0]) | (o.x & keep[0]);
+                        w.y = (w.y & ~keep[1]) | (o.y & keep[1]);
+                        w.z = (w.z & ~keep[0]) | (o.z & keep[0]);
+                        w.w = (w.w & ~keep[1]) | (o.w & keep[1]);
+                    }
+                    *d = w;
+                }
+            }
+        }
+        if (val == 0) __syncthreads();
+    }
+}
+
+// The other way: codes into LDS, 16 bits for four channels of a row, values
+// turned by 4 x 4, and out as rows: four channels a lane (f32) or eight.
+template <typename T>
+__global__ void __launch_bounds__(256) kv4_read_tiles(KvRows a, T *k, T *v) {
+    constexpr uint32_t PAD = 68, PER = sizeof(T) == 4 ? 4 : 8;  // channels a lane
+    __shared__ __attribute__((aligned(16))) uint16_t codes[2][64 * PAD];
+    __shared__ __attribute__((aligned(16))) uint8_t mul[2][8 * 64];
+    __shared__ float scale[2][64];
+    const uint32_t h = blockIdx.x % a.c.Hk, tid = threadIdx.x, hd = a.c.hd, ng = a.c.groups(), nc = hd / 16;
+    KvTile t;
+    if (!kv_tile(a, blockIdx.x / a.c.Hk, &t)) return;
+    const bool held = t.seq >= 0 && t.first < a.c.cap;
+    const size_t slab = a.c.slab(a.first + (held ? t.seq : 0), h);
+    const uint64_t first = held ? t.first : 0;
+    if (held) {
+        const uint8_t *ks = a.c.k + slab * (hd / 2) + first * (hd / 2);
+        for (uint32_t x = tid; x < 32 * nc; x += 256) {
+            const uint32_t pair = x / (16 * nc), y = x - pair * 16 * nc, chunk = y >> 4, r = 32 * pair + (y & 15);
+            const uint4 w = *(const uint4 *)(ks + (size_t)x * 16);
+            *(uint2 *)(codes[0] + r * PAD + 4 * chunk) = uint2{w.x, w.y};
+            *(uint2 *)(codes[0] + (r + 16) * PAD + 4 * chunk) = uint2{w.z, w.w};
+        }
+        const uint8_t *vs = a.c.v + slab * (16 * ng) + first * (16 * ng);
+        for (uint32_t x = tid; x < 32 * ng; x += 256) {  // channels 4 q .. of one half of a group, rows of one g
+            const uint32_t g = x & 3, q = x >> 2 & 3, half = x >> 4 & 1, m = x >> 5, c4 = 8 * m + 4 * half + q;
+            if (4 * c4 >= hd) continue;
+            uint2 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = *(const uint2 *)(vs + m * 1024 + (4 * q + e) * 64 + g * 16 + half * 8);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t in[4], out[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) in[e] = (i < 2 ? w[e].x : w[e].y) >> (16 * (i & 1)) & 0xffffu;
+                kv4_turn(in, out);
+#pragma unroll
+                for (int j = 0; j < 4; j++) codes[1][(16 * i + 4 * g + j) * PAD + c4] = (uint16_t)out[j];
+            }
+        }
+        for (uint32_t x = tid; x < 32 * ng; x += 256) {  // keys' multipliers, then values'
+            const uint32_t val = x >= 16 * ng, y = x - val * 16 * ng;
+            *(uint32_t *)(mul[val] + 4 * y) = *(const uint32_t *)((val ? a.c.vm : a.c.km) + slab * ng + first * ng + 4 * y);
+        }
+    }
+    if (tid < 128) {
+        const uint32_t r = tid & 63;
+        const bool in = held && r >= t.lo && first + r < a.c.cap;
+        scale[tid >> 6][r] = in ? (tid < 64 ? a.c.ks : a.c.vs)[slab + first + r] : __builtin_nanf("");
+    }
+    __syncthreads();
+    // x / words by a multiplication: x < 2^12, words <= 2^6, so that x times the factor's excess is below 2^20
+    const uint32_t words = hd / PER, by = ((1u << 20) + words - 1) / words, all = (t.hi - t.lo) * words;
+    for (uint32_t x = tid; x < all; x += 256) {
+        const uint32_t row = x * by >> 20, w = x - row * words, r = t.lo + row, c = w * PER;
+        const size_t to = (size_t)(t.row + row) * a.stride + (size_t)h * hd + c;
+#pragma unroll
+        for (int val = 0; val < 2; val++) {
+            const uint32_t m = held ? mul[val][c / 32 * 64 + (val ? (r >> 2 & 3) * 16 + (r >> 4) * 4 + (r & 3)
+                                                                  : (r & 15) * 4 + (r >> 4))] : 0u;
+            const float s = scale[val][r];
+            float y[PER];
+#pragma unroll
+            for (uint32_t e = 0; e < PER; e += 4) {
+                float z[4];
+                kv4_values(held ? codes[val][r * PAD + (c + e) / 4] : 0u, m, s, z);
+#pragma unroll
+                for (int f = 0; f < 4; f++) y[e + f] = z[f];
+            }
+            T *d = (val ? v : k) + to;
+            if constexpr (sizeof(T) == 4) {
+                *(Kv4<float> *)d = Kv4<float>{{y[0], y[1], y[2], y[3]}};
+            } else {
+                struct __attribute__((packed, aligned(2))) Out {
+                    uint32_t v[4];
+                } o;
+#pragma unroll
+                for (int e = 0; e < 4; e++) o.v[e] = f32x2_to_bf16x2(y[2 * e], y[2 * e + 1]);
+                *(Out *)d = o;
+            }
+        }
+    }
+}
+
+template <typename T>
+static void kv4_write_any(const KvRows &a, const T *k, const T *v, hipStream_t s) {
+    if (a.tiles) {
+        void (*kern)(KvRows, const T *, const T *) = a.c.hd <= 64    ? kv4_write_tiles<1, T>
+                                                     : a.c.hd <= 128 ? kv4_write_tiles<2, T>
+                                                                     : kv4_write_tiles<4, T>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk)), dim3(256), 0, s, a, k, v);
+    } else {
+        hipLaunchKernelGGL(kv4_write<T>, dim3((unsigned)div_ceil((size_t)a.n_rows * a.c.Hk, 4)), dim3(256), 0, s, a, k, v);
+    }
+}
+void kv4_write_go(const KvRows &a, const void *k, const void *v, int dtype, hipStream_t s) {
+    if (dtype == QBK_F32) kv4_write_any(a, (const float *)k, (const float *)v, s);
+    else kv4_write_any(a, (const uint16_t *)k, (const uint16_t *)v, s);
+}
+
+template <typename T>
+static void kv4_read_any(const KvRows &a, T *k, T *v, hipStream_t s) {
+    if (a.tiles)
+        hipLaunchKernelGGL(kv4_read_tiles<T>, dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk)), dim3(256), 0, s, a, k, v);
+    else
+        hipLaunchKernelGGL(kv4_read<T>, dim3((unsigned)div_ceil((size_t)a.n_rows * a.c.Hk, 4)), dim3(256), 0, s, a, k, v);
+}
 void kv4_read_go(const KvRows &a, void *k, void *v, int dtype, hipStream_t s) {
-    const dim3 grid((unsigned)div_ceil((size_t)a.n_rows * a.c.Hk, 4));
-    if (dtype == QBK_F32) hipLaunchKernelGGL(kv4_read<float>, grid, dim3(256), 0, s, a, (float *)k, (float *)v);
-    else hipLaunchKernelGGL(kv4_read<uint16_t>, grid, dim3(256), 0, s, a, (uint16_t *)k, (uint16_t *)v);
+    if (dtype == QBK_F32) kv4_read_any(a, (float *)k, (float *)v, s);
+    else kv4_read_any(a, (uint16_t *)k, (uint16_t *)v, s);
 }
 
 }  // namespace qbk

@@ -472,26 +472,25 @@ def rotate_heads_dev(ctx: GpuContext, rope: Rope, q, k, dtype: str, n_rows: int,
     if code is None:
         raise _lib.KernelError(f"rotate_heads takes 'float32' or 'bfloat16' rows, got {dtype!r}")
     hd = rope.head_dim
-    if min(n_rows, n_heads, n_kv_heads, n_seqs, before) < 0:
+    if n_rows < 0 or n_heads < 0 or n_kv_heads < 0 or n_seqs < 0 or before < 0:
         raise _lib.KernelError("rotate_heads sizes must not be negative")
-
-    def rows(x, heads, stride, what):
-        s = heads * hd if stride is None else stride
-        if s < 0:
-            raise _lib.KernelError("rotate_heads strides must not be negative")
-        room = (n_rows - 1) * s + heads * hd if n_rows and heads else 0
-        return _device_values(x, dtype, room, ctx, f"rotate_heads: {what}", stride is not None), s
-
-    qi, qs = rows(q, n_heads, q_stride, "q")
-    ki, ks = rows(k, n_kv_heads, k_stride, "k")
-    qo, qos = rows(q_out, n_heads, q_out_stride, "q_out")
-    ko, kos = rows(k_out, n_kv_heads, k_out_stride, "k_out")
+    qw, kw, last = n_heads * hd, n_kv_heads * hd, n_rows - 1
+    qs, ks = qw if q_stride is None else q_stride, kw if k_stride is None else k_stride
+    qos, kos = qw if q_out_stride is None else q_out_stride, kw if k_out_stride is None else k_out_stride
+    if qs < 0 or ks < 0 or qos < 0 or kos < 0:
+        raise _lib.KernelError("rotate_heads strides must not be negative")
+    qn, kn = n_rows and qw, n_rows and kw  # values of a row, if there are any
     check(_lib.load().qbk_rotate_heads_dev(
-        ctx.handle, rope._ref, qi, ki, code, n_rows, n_heads, n_kv_heads, qs, ks,
-        _device_words(row_start, n_seqs + 1, ctx, "row starts"), _device_words(pos, n_seqs, ctx, "positions"), n_seqs,
-        before, _device_values(q_norm, "float32", hd, ctx, "rotate_heads: q_norm"),
-        _device_values(k_norm, "float32", hd, ctx, "rotate_heads: k_norm"), float(eps), qo, ko, qos, kos,
-        _stream(stream)))
+        ctx.handle, rope._ref,
+        _device_values(q, dtype, qn and last * qs + qw, ctx, "rotate_heads: q", q_stride is not None),
+        _device_values(k, dtype, kn and last * ks + kw, ctx, "rotate_heads: k", k_stride is not None),
+        code, n_rows, n_heads, n_kv_heads, qs, ks, _device_words(row_start, n_seqs + 1, ctx, "row starts"),
+        _device_words(pos, n_seqs, ctx, "positions"), n_seqs, before,
+        _device_values(q_norm, "float32", hd, ctx, "rotate_heads: q_norm"),
+        _device_values(k_norm, "float32", hd, ctx, "rotate_heads: k_norm"), eps,
+        _device_values(q_out, dtype, qn and last * qos + qw, ctx, "rotate_heads: q_out", q_out_stride is not None),
+        _device_values(k_out, dtype, kn and last * kos + kw, ctx, "rotate_heads: k_out", k_out_stride is not None),
+        qos, kos, _stream(stream)))
 
 
 class KvCache:
