@@ -670,6 +670,219 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     if (!last && tid < (int)n_rows) a.ml[part + tid] = row;
 }
 
+// The 4-bit cache's body of up to four rows (a step's, of four query heads a kv
+// head): a wave as kva_body's, but the 16 columns of the products are the rows
+// four times over, and columns 4 t .. 4 t + 3 take the keys of block t alone,
+// 16 t .. 16 t + 15 of a tile.  So a lane weighs four keys, not sixteen of which
+// three quarters are of columns that nobody asks for, and since it does, values
+// stay codes and their multipliers go to the weights: some 340 vector operations
+// a tile, in kva_body 560.  The columns of a row are joined as the waves are.
+// 32 sequences of up to 2085 rows, 32/8 heads of 128: 59 MB in 18.0 us, by
+// kva_body 20.9, by eight waves a workgroup 17.8 (64 sequences of 600 18.2, by
+// four 11.6); 128 of up to 4000 446 MB in 85.5, 5.2 TB/s.
+template <int DC>
+struct KvaFew {
+    kva_u4_t kc[DC][2], vc[2 * DC];
+    uint32_t km[DC], vm[2 * DC];
+    kva_f4_t ks, vs;
+    __device__ __forceinline__ void load_k(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+        const int nc = hd / 16, ng = (int)c.ng;
+        const uint8_t *kt = c.k + (size_t)tt * 32 * hd + col * 16;
+        const uint8_t *mt = c.km + (size_t)tt * 64 * ng + col * 4;
+        ks = *(const kva_f4_t *)(c.ks + (size_t)tt * 64 + 16 * (col >> 2) + 4 * g);
+#pragma unroll
+        for (int x = 0; x < DC; x++) {
+            const int chunk = 4 * x + g < nc ? 4 * x + g : nc - 1;  // past the last chunk q is zero
+            km[x] = *(const uint32_t *)(mt + (chunk >> 1) * 64);
+#pragma unroll
+            for (int p = 0; p < 2; p++) kc[x][p] = *(const kva_u4_t *)(kt + (p * nc + chunk) * 256);
+        }
+    }
+    __device__ __forceinline__ void load_v(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+        const int ng = (int)c.ng;
+        const uint8_t *vt = c.v + (size_t)tt * 1024 * ng + col * 64 + g * 16;
+        const uint8_t *mt = c.vm + (size_t)tt * 64 * ng + g * 16 + (col >> 2) * 4;
+        vs = *(const kva_f4_t *)(c.vs + (size_t)tt * 64 + 16 * (col >> 2) + 4 * g);
+#pragma unroll
+        for (int m = 0; m < 2 * DC; m++) {
+            const int at = m < ng ? m : ng - 1;  // past the last tile: not stored
+            vm[m] = *(const uint32_t *)(mt + at * 64);
+            vc[m] = *(const kva_u4_t *)(vt + at * 1024);
+        }
+    }
+};
+
+template <int DC, typename T, class Limit>
+__device__ __forceinline__ void kva_few(const KvAttArgs &a, char *smem, uint32_t row0, uint32_t n_rows, uint32_t hk,
+                                        const KvaSlab &slab, uint32_t tile0, uint32_t tile1, uint32_t written,
+                                        Limit limit, uint32_t split, bool last) {
+    constexpr bool HI = sizeof(T) == 4;
+    using L = KvaLds<DC, HI>;
+    constexpr int STEPS = 2 * DC;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int row = col & 3, block = col >> 2;  // of this lane's column
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hd = (int)a.own.hd, nc = hd / 16;
+    char *qs = smem;
+    float *qfs = (float *)(smem + L::BODY), *refs = qfs + 16, *sums = refs + KVA_WAVES * 16;
+    KvaFew<DC> tile;
+    const uint32_t first = tile0 + wave;
+    if (first < tile1) {
+        tile.load_k(slab, first, hd, col, g);
+        tile.load_v(slab, first, hd, col, g);
+    }
+    kva_queries<DC, 1, T>(a, qs, qfs, row0, n_rows, hk);
+    __syncthreads();
+    KvaState<DC> st(qfs[row], limit((uint32_t)row < n_rows ? row : n_rows - 1));
+    const uint32_t least = kva_scalar(limit(0));  // keys below it are seen by every row
+    const int qlane = (g * 16 + row) * 16;
+    const uint32_t mine[4] = {block == 0 ? ~0u : 0u, block == 1 ? ~0u : 0u, block == 2 ? ~0u : 0u, block == 3 ? ~0u : 0u};
+
+    for (uint32_t tt = first; tt < tile1; tt += KVA_WAVES) {
+        const uint32_t key0 = tt * 64, key = key0 + 16 * block + 4 * g;
+        const bool masked = key0 + 64 > least, more = tt + KVA_WAVES < tile1;
+        kva_f4_t s[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = kva_f4_t{0, 0, 0, 0};
+        asm volatile("" ::: "memory");  // the queries are read from LDS again, not kept in registers that spill
+#pragma unroll
+        for (int x = 0; x < STEPS; x++) {
+            const kva_h8_t qf = *(const kva_h8_t *)(qs + x * 1024 + qlane);
+            kva_h8_t kf[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const kva_h2_t m = i < 2 ? kva_mul4<0>(tile.km[x / 2]) : kva_mul4<1>(tile.km[x / 2]);
+                kf[i] = kva_key4(tile.kc[x / 2][i >> 1][2 * (i & 1) + (x & 1)], m[i & 1]);
+                s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qf, s[i], 0, 0, 0);
+            }
+            if constexpr (HI) {
+                const kva_h8_t ql = *(const kva_h8_t *)(qs + (STEPS + x) * 1024 + qlane);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], ql, s[i], 0, 0, 0);
+            }
+        }
+        kva_f4_t t = s[0], vs = tile.vs;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {  // this column's block
+            const float lo = block & 1 ? s[1][j] : s[0][j], hi = block & 1 ? s[3][j] : s[2][j];
+            t[j] = block & 2 ? hi : lo;
+        }
+        t *= tile.ks * st.qf;
+        if (more) tile.load_k(slab, tt + KVA_WAVES, hd, col, g);
+        uint32_t keep = ~0u;
+        if (masked) {  // what was never written, or lies past the row's keys, takes no part, whatever it holds
+            const uint32_t left = written > key ? written - key : 0;
+            keep = left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool out = key + j >= st.lim;
+                t[j] = out ? -INFINITY : t[j];
+                vs[j] = out || key + j >= written ? 0.0f : vs[j];
+            }
+        }
+        const float tm = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        if (__ballot(tm > st.ref + 3.0f)) {  // as kva_reference
+            const float most = kva_max4(tm);
+            const float to = most > st.ref + 3.0f ? ceilf(most) : st.ref;
+            const float f = kva_rescale(st.ref, to);
+            st.sum *= f;
+            st.wref *= f;
+            st.ref = to;
+        }
+        const float base = st.ref == -INFINITY ? 0.0f : st.ref;
+        float l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float p = __builtin_amdgcn_exp2f(t[j] - base);
+            l += p;
+            t[j] = p * vs[j];
+        }
+        st.sum += l;
+        const float wm = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        if (__ballot(wm > 8.0f * st.wref)) {  // as kva_weight_reference
+            const float most = kva_max4(wm);
+            if (most > 8.0f * st.wref) {
+                uint32_t e = (__float_as_uint(most) >> 23) + 1;
+                e = e < 12 ? 12 : e > 253 ? 253 : e;
+                const float f = st.wref * __uint_as_float((254 - e) << 23);
+#pragma unroll
+                for (int ct = 0; ct < 4 * DC; ct++) st.o[ct] *= f;
+                st.wref = __uint_as_float(e << 23);
+            }
+        }
+        // weights in units of 2^-12 wref, times their group's multiplier over 2^9 (at most 7 / 8, so within fp16 still)
+        t *= __uint_as_float((266u << 23) - __float_as_uint(st.wref));
+#pragma unroll
+        for (int m = 0; m < 2 * DC; m++) {
+            const uint32_t mw = tile.vm[m] & keep;
+            const kva_f2_t m0 = __builtin_bit_cast(kva_f2_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(mw, 0x1p-9f, false));
+            const kva_f2_t m1 = __builtin_bit_cast(kva_f2_t, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(mw, 0x1p-9f, true));
+            const kva_f2_t x0 = {t[0] * m0[0], t[1] * m0[1]}, x1 = {t[2] * m1[0], t[3] * m1[1]};
+            const kva_h2_t h0 = __builtin_convertvector(x0, kva_h2_t), h1 = __builtin_convertvector(x1, kva_h2_t);
+            const uint32_t w0 = __builtin_bit_cast(uint32_t, h0), w1 = __builtin_bit_cast(uint32_t, h1);
+            uint32_t r0 = 0, r1 = 0;
+            if constexpr (HI) {
+                const kva_h2_t e0 = __builtin_convertvector(x0 - __builtin_convertvector(h0, kva_f2_t), kva_h2_t);
+                const kva_h2_t e1 = __builtin_convertvector(x1 - __builtin_convertvector(h1, kva_f2_t), kva_h2_t);
+                r0 = __builtin_bit_cast(uint32_t, e0);
+                r1 = __builtin_bit_cast(uint32_t, e1);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const kva_h8_t ph = __builtin_bit_cast(kva_h8_t, kva_u4_t{w0 & mine[2 * u], w1 & mine[2 * u], w0 & mine[2 * u + 1], w1 & mine[2 * u + 1]});
+                kva_h8_t pl;
+                if constexpr (HI)
+                    pl = __builtin_bit_cast(kva_h8_t, kva_u4_t{r0 & mine[2 * u], r1 & mine[2 * u], r0 & mine[2 * u + 1], r1 & mine[2 * u + 1]});
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    kva_h2_t v[4];
+                    kva_wide4(tile.vc[m][2 * h + u], v);
+                    const kva_h8_t vf = kva_h8(v);
+                    st.o[2 * m + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, st.o[2 * m + h], 0, 0, 0);
+                    if constexpr (HI) st.o[2 * m + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, st.o[2 * m + h], 0, 0, 0);
+                }
+            }
+        }
+        if (more) tile.load_v(slab, tt + KVA_WAVES, hd, col, g);
+    }
+
+    // join the waves' and the blocks' columns on each row's largest reference
+    const float l = kva_sum4(st.sum);
+    if (g == 0) {
+        refs[wave * 16 + col] = st.ref;
+        sums[wave * 16 + col] = l;
+    }
+    __syncthreads();
+    float2 all = {refs[row], 0.0f};  // row's reference and sum of weights
+#pragma unroll
+    for (int w = 1; w < 4 * KVA_WAVES; w++) all.x = fmaxf(all.x, refs[w * 4 + row]);
+#pragma unroll
+    for (int w = 0; w < 4 * KVA_WAVES; w++) all.y += sums[w * 4 + row] * kva_rescale(refs[w * 4 + row], all.x);
+    constexpr int OC = L::OC, LD = OC + 4;
+    float *ob = (float *)smem;  // [wave][16 columns][LD]
+    const size_t part = ((size_t)split * a.own.Hk + hk) * a.rows + row0;
+    const float per = 512.0f * kva_per(all.y), f = kva_rescale(st.ref, all.x) * st.wref;
+#pragma unroll
+    for (int c0 = 0; c0 < 64 * DC; c0 += OC) {
+        if (c0 >= hd) continue;
+        if (c0) __syncthreads();  // what the region held has been read
+#pragma unroll
+        for (int k = 0; k < OC / 16; k++)
+            *(kva_f4_t *)(ob + (wave * 16 + col) * LD + 16 * k + 4 * g) = st.o[c0 / 16 + k] * per * f;
+        __syncthreads();
+        for (int x = tid; x < 4 * OC; x += 64 * KVA_WAVES) {
+            const int r = x / OC, c = x % OC;
+            if (r >= (int)n_rows || c0 + c >= hd) continue;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4 * KVA_WAVES; w++) v += ob[(w * 4 + r) * LD + c];
+            if (last) kva_out_row<T>(a, row0 + r, hk)[c0 + c] = kva_out<T>(v);
+            else a.po[(part + r) * hd + c0 + c] = v;
+        }
+    }
+    if (!last && tid < (int)n_rows) a.ml[part + tid] = all;
+}
+
 // The body of many rows: four waves of 16 rows, every wave every key tile.  A
 // tile is widened once for the four of them, a quarter by each, into LDS in
 // operand order (each 16-byte access of a wave is 1 KiB in a row) while the
@@ -862,13 +1075,16 @@ __device__ __forceinline__ void kva_wide_body(const KvAttArgs &a, char *smem, ui
     }
 }
 
-template <int FMT, int DC, bool WIDE, typename T, class... ARGS>
+enum { KVA_ROWS16 = 0, KVA_ROWS64 = 1, KVA_ROWS4 = 2 };  // a body's rows
+
+template <int FMT, int DC, int ROWS, typename T, class... ARGS>
 __device__ __forceinline__ void kva_any(ARGS &&...args) {
-    if constexpr (WIDE) kva_wide_body<FMT, DC, T>(args...);
+    if constexpr (ROWS == KVA_ROWS64) kva_wide_body<FMT, DC, T>(args...);
+    else if constexpr (ROWS == KVA_ROWS4) kva_few<DC, T>(args...);
     else kva_body<FMT, DC, T>(args...);
 }
 
-template <int FMT, int DC, bool WIDEP, bool WIDES, typename T>
+template <int FMT, int DC, bool WIDEP, int OWN, typename T>
 __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAttArgs a) {
     extern __shared__ char smem[];
     const uint32_t Hk = a.own.Hk;
@@ -883,7 +1099,7 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
         const uint32_t t0 = split * run < tiles ? split * run : tiles, t1 = t0 + run < tiles ? t0 + run : tiles;
         const KvaSlab slab = KvaSlab::of<FMT>(a.pre, a.pre.slab(a.prefix_seq, hk));
         const uint32_t len = a.prefix_len;
-        kva_any<FMT, DC, WIDEP, T>(a, smem, row0, n_rows, hk, slab, t0, t1, len, [&](uint32_t) { return len; }, split,
+        kva_any<FMT, DC, WIDEP ? KVA_ROWS64 : KVA_ROWS16, T>(a, smem, row0, n_rows, hk, slab, t0, t1, len, [&](uint32_t) { return len; }, split,
                                   last);
         return;
     }
@@ -892,7 +1108,7 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
     const uint32_t split = a.by_n.split(a.by_rts.split(a.by_hk.split(item, hk), rt), b);
     const uint32_t len = kva_len(a, b), tiles = (len + 63) / 64, run = kva_run(a, len);
     if (split * run >= tiles && split > 0) return;  // split 0 is there for a sequence with no rows
-    constexpr uint32_t R = WIDES ? 64 : 16;
+    constexpr uint32_t R = OWN == KVA_ROWS64 ? 64 : 16;
     const uint32_t per = a.sq * a.G, r0 = rt * R, n_rows = per - r0 < R ? per - r0 : R;
     const uint32_t sq = a.sq;
     const KvaRow rows(a, r0);
@@ -906,7 +1122,7 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
     uint32_t t1 = split * run + run;
     t1 = t1 < most ? t1 : most;
     const KvaSlab slab = KvaSlab::of<FMT>(a.own, a.own.slab(a.first_seq + b, hk));
-    kva_any<FMT, DC, WIDES, T>(a, smem, b * per + r0, n_rows, hk, slab, split * run, t1, len, limit, a.sp + split, last);
+    kva_any<FMT, DC, OWN, T>(a, smem, b * per + r0, n_rows, hk, slab, split * run, t1, len, limit, a.sp + split, last);
 }
 
 // A wave a row and kv head: the partial results of its splits on their largest
@@ -978,6 +1194,7 @@ __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
 // the sequences' own rows.
 struct KvaPlan {
     bool widep, wides;  // bodies of 64 rows
+    bool few;           // own rows by the body of four
     uint32_t rtp, rts, sp, ss;
     uint64_t items;
     size_t bytes;
@@ -998,22 +1215,29 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
     // 31.4, 49.2 / 53.9; heads of 64 behind 500 and 2048: 128 tiles 12.1 / 10.3, 14.2 / 12.6, 512 24.3 / 24.8, 29.6 /
     // 32.4; heads of 256: 32 tiles 19.8 / 14.2, 21.6 / 23.2, 64 tiles 20.8 / 21.0, 24.0 / 26.8).
     p.widep = p.wides || (prefix_len && (uint64_t)Hk * div_ceil(rows, 16) >= (dc == 1 ? 512 : 256 / dc));
+    p.few = s->format == QBK_KV_FP4 && per <= 4;
     p.rtp = (uint32_t)div_ceil(rows, p.widep ? 64 : 16);
     p.rts = (uint32_t)div_ceil(per, p.wides ? 64 : 16);
-    const uint64_t op = (uint64_t)Hk * p.rtp, os = (uint64_t)n * Hk * p.rts;
+    const uint64_t op = prefix_len ? (uint64_t)Hk * p.rtp : 0, os = (uint64_t)n * Hk * p.rts;
     // Splits: a workgroup a CU for the prefix, of four key tiles at least, and two for own rows where the sequences
     // alone leave CUs idle; past that a run of at most 64 tiles, so that no workgroup outlasts the rest on one long
     // sequence.  More of them write and join more partial rows (us for 128, 256 and 512 workgroups of the prefix: 32
     // requests behind 8192 30.0, 21.9, 22.8, 64 behind 16384 86.8, 54.6, 70.9; own rows of 32 sequences up to 2085: one
     // split 23.5, two 25.1, of 8 sequences for 128, 256, 512 workgroups 15.8, 13.1, 13.2; 32 sequences up to 16384,
     // runs of 16, 64 and 512 tiles: 159.8, 154.1, 161.9).
+    const size_t tp = div_ceil(prefix_len, 64), ts = div_ceil(max_len, 64);
     auto splits = [](uint64_t want, size_t tiles) -> uint32_t {
         const uint64_t most = div_ceil(tiles, KVA_WAVES);
         want = want < most ? want : most;
         return (uint32_t)(want < 1 ? 1 : want > KVA_MAX_SPLITS ? KVA_MAX_SPLITS : want);
     };
-    const size_t tp = div_ceil(prefix_len, 64), ts = div_ceil(max_len, 64);
     if (prefix_len) p.sp = splits(div_ceil(256, op), tp);
+    // fp4, whose tiles take a wave as long for half the bytes: whole rounds of the waves (80 rows behind 4001, f32, 8
+    // heads of 80, runs of nine tiles and of eight: 17.2 and 15.9 us)
+    if (prefix_len && s->format == QBK_KV_FP4 && !p.widep) {
+        const size_t run = div_ceil(tp, p.sp), whole = run / KVA_WAVES * KVA_WAVES;
+        if (whole) p.sp = splits(div_ceil(tp, whole), tp);
+    }
     if (max_len) p.ss = splits(os >= 256 ? div_ceil(ts, 64) : div_ceil(512, os), ts);
     // a second launch takes longer than one more tile a wave (one sequence of 512 rows in one launch 7.9 us, split 9.2;
     // of 768 9.6 and 9.4, of 1024 11.1 and 9.4)
@@ -1023,13 +1247,13 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
     return p;
 }
 
-template <int FMT, int DC, bool WIDEP, bool WIDES, typename T>
+template <int FMT, int DC, bool WIDEP, int OWN, typename T>
 static int kva_launch(const KvAttArgs &a, uint64_t items, int device, hipStream_t st) {
     constexpr bool HI = sizeof(T) == 4;
-    constexpr int N = KvaLds<DC, HI>::BYTES, W = KvaWideLds<DC, HI>::BYTES;
-    constexpr int lds = !WIDEP ? N : WIDES || W > N ? W : N;
-    static_assert(!WIDES || WIDEP, "own rows are no more than the prefix's");
-    void (*k)(KvAttArgs) = kva_items<FMT, DC, WIDEP, WIDES, T>;
+    constexpr int N = KvaLds<DC, HI>::BYTES, WIDE = KvaWideLds<DC, HI>::BYTES;
+    constexpr int lds = !WIDEP ? N : OWN == KVA_ROWS64 || WIDE > N ? WIDE : N;
+    static_assert(OWN != KVA_ROWS64 || WIDEP, "own rows are no more than the prefix's");
+    void (*k)(KvAttArgs) = kva_items<FMT, DC, WIDEP, OWN, T>;
     if (lds > 64 * 1024) {  // once a device
         static std::atomic<uint64_t> asked{0};
         const uint64_t bit = device < 64 ? 1ull << device : 0;
@@ -1045,9 +1269,15 @@ static int kva_launch(const KvAttArgs &a, uint64_t items, int device, hipStream_
 
 template <int FMT, int DC, typename T>
 static int kva_dispatch_dc(const KvAttArgs &a, const KvaPlan &p, int device, hipStream_t st) {
-    if (p.wides) return kva_launch<FMT, DC, true, true, T>(a, p.items, device, st);
-    if (p.widep) return kva_launch<FMT, DC, true, false, T>(a, p.items, device, st);
-    return kva_launch<FMT, DC, false, false, T>(a, p.items, device, st);
+    if (p.wides) return kva_launch<FMT, DC, true, KVA_ROWS64, T>(a, p.items, device, st);
+    if constexpr (FMT == QBK_KV_FP4) {
+        if (p.few) {
+            if (p.widep) return kva_launch<FMT, DC, true, KVA_ROWS4, T>(a, p.items, device, st);
+            return kva_launch<FMT, DC, false, KVA_ROWS4, T>(a, p.items, device, st);
+        }
+    }
+    if (p.widep) return kva_launch<FMT, DC, true, KVA_ROWS16, T>(a, p.items, device, st);
+    return kva_launch<FMT, DC, false, KVA_ROWS16, T>(a, p.items, device, st);
 }
 
 template <int FMT, typename T>
