@@ -553,7 +553,7 @@ int qbk_head_logits_dev(qbk_ctx *ctx, const qbk_head *head, const float *hidden,
                         void *stream);
 
 /* One decode position of n sequences (1 .. 64) through a block whose rows
- * stand in an 8-bit cache in place of the block's own f32 cache (which, with
+ * stand in an 8-bit or 4-bit cache in place of the block's own f32 cache (which, with
  * its attention state, is left as it is): the batched step of
  * qbk_block_decode_batch_dev with its attention over `cache` behind the
  * shared prefix.  h f32 [n][d_model], replaced by the block's outputs; pos:
@@ -572,6 +572,20 @@ int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *block, float *h, const uint
                             const qbk_kv_shape *shape, void *cache, size_t first_seq, size_t max_len,
                             const qbk_kv_shape *prefix_shape, const void *prefix, size_t prefix_seq,
                             size_t prefix_len, void *workspace, size_t workspace_size, void *stream);
+/* The same of `tokens` positions a sequence at once, n * tokens up to 64: a
+ * request's last token and its drafts, whose logits qbk_verify_drafts_dev takes.
+ * h f32 [n][tokens][d_model]; token t of sequence first_seq + i stands at own
+ * position pos[i] + t and sees the rows up to its own.  max_len: a host bound on
+ * pos[i] + tokens, at most the cache's capacity; tokens at positions past it have
+ * no meaning, and those before them in the same step neither.  Advancing pos by
+ * fewer than `tokens` takes the rest back: later rows are written over theirs. */
+size_t qbk_block_decode_kv_tokens_workspace_size(const qbk_block *block, const qbk_kv_shape *shape, size_t n,
+                                                 size_t tokens, size_t max_len, size_t prefix_len);
+int qbk_block_decode_kv_tokens_dev(qbk_ctx *ctx, qbk_block *block, float *h, const uint32_t *pos, size_t n,
+                                   size_t tokens, const qbk_kv_shape *shape, void *cache, size_t first_seq,
+                                   size_t max_len, const qbk_kv_shape *prefix_shape, const void *prefix,
+                                   size_t prefix_seq, size_t prefix_len, void *workspace, size_t workspace_size,
+                                   void *stream);
 
 /* ---- rotary positions -------------------------------------------------------- */
 

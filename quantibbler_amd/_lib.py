@@ -135,6 +135,9 @@ _SIGS = {
     "qbk_block_decode_kv_workspace_size": (_Z, [_P, C.POINTER(KvShape), _Z, _Z, _Z]),
     "qbk_block_decode_kv_dev": (_I, [_P, _P, _P, _P, _Z, C.POINTER(KvShape), _P, _Z, _Z, C.POINTER(KvShape), _P, _Z,
                                      _Z, _P, _Z, _P]),
+    "qbk_block_decode_kv_tokens_workspace_size": (_Z, [_P, C.POINTER(KvShape), _Z, _Z, _Z, _Z]),
+    "qbk_block_decode_kv_tokens_dev": (_I, [_P, _P, _P, _P, _Z, _Z, C.POINTER(KvShape), _P, _Z, _Z, C.POINTER(KvShape),
+                                            _P, _Z, _Z, _P, _Z, _P]),
     "qbk_rope_init": (_I, [C.POINTER(RopeC), _Z, _Z, _I, C.c_double, C.POINTER(RopeScaling)]),
     "qbk_rotate_heads_dev": (_I, [_P, C.POINTER(RopeC), _P, _P, _I, _Z, _Z, _Z, _Z, _Z, _P, _P, _Z, _Z, _P, _P,
                                   C.c_double, _P, _P, _Z, _Z, _P]),

@@ -68,7 +68,7 @@ struct KvAttArgs {
     float *po;    // [split][hk][rho][hd] weighted means of the values
     float2 *ml;   // [split][hk][rho] reference, sum of weights
     uint32_t first_seq, prefix_seq, prefix_len, max_len;
-    uint32_t plus;                   // 1: lens are positions, the rows before the one just written
+    uint32_t plus;                   // lens are positions, so many rows behind them just written
     uint32_t n, sq, H, G, rows;      // rows = n sq G
     uint32_t sp, ss, rtp, rts;       // splits and row tiles of prefix and own items
     uint32_t n_pre;                  // prefix items
@@ -80,7 +80,7 @@ struct KvAttArgs {
 // at least one a wave, so that short sequences use few splits.
 __device__ __forceinline__ uint32_t kva_len(const KvAttArgs &a, uint32_t b) {
     const uint32_t l = a.lens[b];
-    return l < a.max_len ? l + a.plus : a.max_len;
+    return l < a.max_len && a.plus < a.max_len - l ? l + a.plus : a.max_len;
 }
 __device__ __forceinline__ uint32_t kva_run(const KvAttArgs &a, uint32_t len) {
     uint32_t rest;
@@ -1309,8 +1309,7 @@ static int kva_check(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq,
     return QBK_OK;
 }
 
-// qbk_attention_kv_dev; plus 1: lens[i] counts the rows before the queries'
-// last one.
+// qbk_attention_kv_dev; plus seq_q: lens[i] counts the rows before the queries'.
 int attention_kv_run(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, size_t first_seq, size_t n,
                      const uint32_t *lens, uint32_t plus, size_t max_len, const qbk_kv_shape *prefix_shape,
                      const void *prefix, size_t prefix_seq, size_t prefix_len, size_t n_heads, size_t seq_q,

@@ -758,15 +758,15 @@ __global__ void __launch_bounds__(64) blkb_qk_rope(const float *q, const float *
     }
 }
 
-// The same for a step over an 8-bit cache: row t at position before + pos[t],
-// q to qr [n][H hd], k to kr [n][Hk hd] (the cache takes k from there and v
+// The same for a step over an 8-bit or 4-bit cache of `per` tokens a sequence:
+// row t at position before + pos[t / per] + t % per, q to qr [n][H hd], k to kr [n][Hk hd] (the cache takes k from there and v
 // from the projection); zeros past the block's positions.
 __global__ void __launch_bounds__(64) blkb_qk_rope_rows(const float *q, const float *k, const float2 *rope,
-                                                        const uint32_t *pos, uint32_t before, size_t cap,
+                                                        const uint32_t *pos, uint32_t before, uint32_t per, size_t cap,
                                                         const float *wq, const float *wk, float eps, float *qr,
                                                         float *kr, int H, int Hk, int hd) {
     const int head = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
-    const size_t p = (size_t)pos[t] + before;
+    const size_t p = (size_t)pos[t / per] + t % per + before;
     const bool is_q = head < H;
     const size_t at = is_q ? ((size_t)t * H + head) * hd : ((size_t)t * Hk + head - H) * hd;
     float *dst = (is_q ? qr : kr) + at;
@@ -1348,27 +1348,28 @@ size_t qbk_block_decode_batch_workspace_size(const qbk_block *B, size_t n) {
 // attention stepping every sequence's kept state.
 }  // extern "C"
 
-// A batched step over an 8-bit cache in place of the block's own (qbk.h,
-// qbk_block_decode_kv_dev).
+// A batched step over an 8-bit or 4-bit cache in place of the block's own
+// (qbk.h, qbk_block_decode_kv_tokens_dev).
 struct BlkKv {
     const qbk_kv_shape *shape, *prefix_shape;
     void *cache;
     const void *prefix;
-    size_t first_seq, max_len, prefix_seq, prefix_len;
+    size_t first_seq, max_len, prefix_seq, prefix_len, tokens;
 };
-// Its workspace: the batched step's, the rotated keys, the attention's.
-static size_t blkkv_workspace(const qbk_block *B, const qbk_kv_shape *shape, size_t n, size_t max_len,
+// Its workspace, for n rows in all: the batched step's, the rotated keys, the
+// attention's.
+static size_t blkkv_workspace(const qbk_block *B, const qbk_kv_shape *shape, size_t n, size_t tokens, size_t max_len,
                               size_t prefix_len, size_t *o_kr, size_t *o_att, size_t *att) {
     *o_kr = blkb_plan(B, n).bytes;
     *o_att = *o_kr + round_up(n * B->Hk * B->hd * 4, 256);
-    *att = qbk_attention_kv_workspace_size(shape, B->H, n, 1, max_len, prefix_len);
+    *att = qbk_attention_kv_workspace_size(shape, B->H, n / tokens, tokens, max_len, prefix_len);
     return *o_att + *att;
 }
 
 // With pos_dev (device, n entries) in place of pos: each sequence at the
 // position its word holds when the step runs; the host record of cached
-// positions is then left to the caller.  With kv (pos_dev given): rows and
-// attention on that cache.
+// positions is then left to the caller.  With kv (pos_dev given, an entry a
+// sequence): n rows, kv->tokens a sequence, rows and attention on that cache.
 static int block_decode_batch(qbk_ctx *ctx, qbk_block *B, float *h, const size_t *pos, const uint32_t *pos_dev,
                               size_t n, void *workspace, size_t workspace_size, void *stream,
                               const BlkKv *kv = nullptr) {
@@ -1377,7 +1378,10 @@ static int block_decode_batch(qbk_ctx *ctx, qbk_block *B, float *h, const size_t
     if (B->face == QBK_ATTN_EXACT && !kv) return fail(QBK_ERR_VALIDATION, kExactFaceOnly);
     if (B->serving == QBK_F32) return fail(QBK_ERR_VALIDATION, kF32Only);
     if (n == 0 || n > (kv ? BLKB_MAXSEQ : B->nseq))
-        return fail(QBK_ERR_VALIDATION, kv ? fmt("a step over a kv cache takes 1 .. %d sequences, got %zu", BLKB_MAXSEQ, n)
+        return fail(QBK_ERR_VALIDATION, kv ? kv->tokens == 1
+                                                 ? fmt("a step over a kv cache takes 1 .. %d sequences, got %zu", BLKB_MAXSEQ, n)
+                                                 : fmt("a step over a kv cache takes 1 .. %d rows, got %zu of %zu tokens a "
+                                                       "sequence", BLKB_MAXSEQ, n, kv->tokens)
                                            : fmt("batch of %zu sequences on a block holding %zu", n, B->nseq));
     for (size_t i = 0; !pos_dev && i < n; i++) {
         if (pos[i] >= B->cap)
@@ -1389,7 +1393,8 @@ static int block_decode_batch(qbk_ctx *ctx, qbk_block *B, float *h, const size_t
     }
     const BlkbPlan P = blkb_plan(B, n);
     size_t o_kr = 0, o_att = 0, att = 0;
-    const size_t need = kv ? blkkv_workspace(B, kv->shape, n, kv->max_len, kv->prefix_len, &o_kr, &o_att, &att) : P.bytes;
+    const size_t need = kv ? blkkv_workspace(B, kv->shape, n, kv->tokens, kv->max_len, kv->prefix_len, &o_kr, &o_att, &att)
+                           : P.bytes;
     if (!workspace || workspace_size < need)
         return fail(QBK_ERR_VALIDATION,
                     fmt("workspace of %zu bytes is smaller than the %zu this step needs", workspace_size, need));
@@ -1435,13 +1440,14 @@ static int block_decode_batch(qbk_ctx *ctx, qbk_block *B, float *h, const size_t
     if (kv) {
         float *kr = (float *)(w + o_kr);
         hipLaunchKernelGGL(blkb_qk_rope_rows, dim3(H + Hk, (unsigned)n), dim3(64), 0, s, q, k, B->rope, pos_dev,
-                           (uint32_t)kv->prefix_len, B->cap, B->w_q, B->w_k, B->eps, qr, kr, H, Hk, hd);
+                           (uint32_t)kv->prefix_len, (uint32_t)kv->tokens, B->cap, B->w_q, B->w_k, B->eps, qr, kr, H, Hk, hd);
         QBK_HIP(hipGetLastError());
+        const size_t seqs = n / kv->tokens;
         if ((rc = qbk_kv_cache_write_dev(ctx, kv->shape, kv->cache, kr, v, QBK_F32, kd, n, nullptr, pos_dev,
-                                         kv->first_seq, n, stream)) ||
-            (rc = attention_kv_run(ctx, kv->shape, kv->cache, kv->first_seq, n, pos_dev, 1, kv->max_len,
-                                   kv->prefix_shape, kv->prefix, kv->prefix_seq, kv->prefix_len, B->H, 1, qr, QBK_F32,
-                                   at, w + o_att, att, stream)))
+                                         kv->first_seq, seqs, stream)) ||
+            (rc = attention_kv_run(ctx, kv->shape, kv->cache, kv->first_seq, seqs, pos_dev, (uint32_t)kv->tokens,
+                                   kv->max_len, kv->prefix_shape, kv->prefix, kv->prefix_seq, kv->prefix_len, B->H,
+                                   kv->tokens, qr, QBK_F32, at, w + o_att, att, stream)))
             return rc;
     } else {
         hipLaunchKernelGGL(blkb_qk_rope, dim3(H + Hk, (unsigned)n), dim3(64), 0, s, q, k, v, B->rope, bp, pos_dev,
@@ -1534,17 +1540,35 @@ int qbk_block_decode_batch_pos_dev(qbk_ctx *ctx, qbk_block *B, float *h, const u
     return block_decode_batch(ctx, B, h, nullptr, pos, n, workspace, workspace_size, stream);
 }
 
+size_t qbk_block_decode_kv_tokens_workspace_size(const qbk_block *B, const qbk_kv_shape *shape, size_t n, size_t tokens,
+                                                 size_t max_len, size_t prefix_len) {
+    if (!B || n == 0 || tokens == 0 || n > BLKB_MAXSEQ || tokens > BLKB_MAXSEQ / n || !shape ||
+        qbk_kv_cache_size(shape) == 0)
+        return 0;
+    size_t o_kr, o_att, att;
+    return blkkv_workspace(B, shape, n * tokens, tokens, max_len, prefix_len, &o_kr, &o_att, &att);
+}
+
 size_t qbk_block_decode_kv_workspace_size(const qbk_block *B, const qbk_kv_shape *shape, size_t n, size_t max_len,
                                           size_t prefix_len) {
-    if (!B || n == 0 || n > BLKB_MAXSEQ || !shape || qbk_kv_cache_size(shape) == 0) return 0;
-    size_t o_kr, o_att, att;
-    return blkkv_workspace(B, shape, n, max_len, prefix_len, &o_kr, &o_att, &att);
+    return qbk_block_decode_kv_tokens_workspace_size(B, shape, n, 1, max_len, prefix_len);
 }
 
 int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *B, float *h, const uint32_t *pos, size_t n,
                             const qbk_kv_shape *shape, void *cache, size_t first_seq, size_t max_len,
                             const qbk_kv_shape *prefix_shape, const void *prefix, size_t prefix_seq, size_t prefix_len,
                             void *workspace, size_t workspace_size, void *stream) {
+    return qbk_block_decode_kv_tokens_dev(ctx, B, h, pos, n, 1, shape, cache, first_seq, max_len, prefix_shape, prefix,
+                                          prefix_seq, prefix_len, workspace, workspace_size, stream);
+}
+
+int qbk_block_decode_kv_tokens_dev(qbk_ctx *ctx, qbk_block *B, float *h, const uint32_t *pos, size_t n, size_t tokens,
+                                   const qbk_kv_shape *shape, void *cache, size_t first_seq, size_t max_len,
+                                   const qbk_kv_shape *prefix_shape, const void *prefix, size_t prefix_seq,
+                                   size_t prefix_len, void *workspace, size_t workspace_size, void *stream) {
+    if (tokens == 0 || tokens > BLKB_MAXSEQ)
+        return fail(QBK_ERR_VALIDATION, fmt("a step over a kv cache takes 1 .. %d tokens a sequence, got %zu", BLKB_MAXSEQ,
+                                            tokens));
     if (!B || !h || !pos || !shape || !cache || (prefix_len && (!prefix_shape || !prefix)))
         return fail(QBK_ERR_VALIDATION, "null argument");
     if (qbk_kv_cache_size(shape) == 0) return QBK_ERR_VALIDATION;
@@ -1570,8 +1594,10 @@ int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *B, float *h, const uint32_t
     if (((uintptr_t)cache | (uintptr_t)(prefix_len ? prefix : nullptr) | (uintptr_t)workspace) & 15)
         return fail(QBK_ERR_VALIDATION, "kv cache buffers and the workspace must be 16-byte aligned");
     if (B->H > 8192) return fail(QBK_ERR_VALIDATION, "kv attention takes up to 8192 heads");
-    const BlkKv kv{shape, prefix_shape, cache, prefix, first_seq, max_len, prefix_seq, prefix_len};
-    return block_decode_batch(ctx, B, h, nullptr, pos, n, workspace, workspace_size, stream, &kv);
+    const BlkKv kv{shape, prefix_shape, cache, prefix, first_seq, max_len, prefix_seq, prefix_len, tokens};
+    // no sequences, and more than there are rows for, are refused there as a step of one token's are
+    return block_decode_batch(ctx, B, h, nullptr, pos, n > BLKB_MAXSEQ ? n : n * tokens, workspace, workspace_size, stream,
+                              &kv);
 }
 
 }  // extern "C"

@@ -145,8 +145,8 @@ struct DecRope {
     int H;
 };
 
-// qbk_attention_kv_dev (attention_kv.hip); plus 1: lens[i] counts the rows
-// before the queries' last one, as a step's positions do.
+// qbk_attention_kv_dev (attention_kv.hip); plus seq_q: lens[i] counts the rows
+// before the queries', as a step's positions do.
 int attention_kv_run(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, size_t first_seq, size_t n,
                      const uint32_t *lens, uint32_t plus, size_t max_len, const qbk_kv_shape *prefix_shape,
                      const void *prefix, size_t prefix_seq, size_t prefix_len, size_t n_heads, size_t seq_q,

@@ -458,6 +458,7 @@ class DeviceModel:
                 caches.append(cache(seqs, int(capacity)))
             need = max(b.decode_kv_workspace_size(c, seqs, prefix_len=n) for b, c in zip(self.blocks, caches))
             self._shared = {"n": seqs, "prefix": prefixes, "len": n, "own": caches, "pos": pos, "steps": 0,
+                            "bound": False, "drafts": {},  # steps: rows a request holds, or a bound; drafts: by tokens
                             "h": torch.empty((seqs, d), dtype=torch.float32, device="cuda"),
                             "hn": torch.empty((seqs, d), dtype=torch.float32, device="cuda"),
                             "logits": torch.empty((seqs, md.vocab_size), dtype=torch.float32, device="cuda"),
@@ -479,8 +480,7 @@ class DeviceModel:
         n = int(tokens.numel()) if dev_ids else len(tokens)
         if n != s["n"]:
             raise ValueError(f"{n} tokens for {s['n']} requests")
-        if s["steps"] >= s["own"][0].capacity:
-            raise ValueError(f"the requests hold their {s['steps']} rows already")
+        self._room(1, stream)
         if dev_ids:
             embed_dev(self.ctx, self.embedding, md.vocab_size, md.d_model, tokens, n, s["h"], stream)
         else:
@@ -493,6 +493,80 @@ class DeviceModel:
         self.head.logits_dev(s["hn"], n, s["logits"], stream)
         s["steps"] += 1
         return s["logits"]
+
+    def _room(self, rows: int, stream):
+        """Refuses a step of so many rows a request that its cache has no room
+        for.  What requests hold is known here as a bound, since the device
+        counts the drafts that it keeps; the count is fetched where the bound
+        does not do."""
+        import torch
+
+        s = self._shared
+        capacity = s["own"][0].capacity
+        if s["steps"] + rows > capacity and s["bound"]:
+            with _memory_of(stream):
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.synchronize()
+                    s["steps"], s["bound"] = int(s["pos"].max()), False
+        if s["steps"] + rows > capacity:
+            raise ValueError(f"the requests hold their {s['steps']} rows already" if rows == 1 else
+                             f"no room for {rows} rows behind {s['steps']} of a capacity of {capacity}")
+
+    def verify_shared(self, tokens, uniforms, draft_logits=None, n_drafts=None, temperature=None, stream=None):
+        """Drafted tokens of every request of share_prefix() in one step:
+        ``tokens`` [n][k + 1] (device int32, or host ids) holds a request's last
+        token, which no step has taken yet, and k drafts behind it, n (k + 1) up
+        to 64.  The model's logits behind each of them verify the drafts as
+        verify_drafts_dev does, with ``uniforms`` [n][k + 1] f32 in [0, 1) and, if
+        any, ``draft_logits`` [n][k][vocab] f32, ``n_drafts`` and ``temperature``
+        [n] (device tensors).  Returns device int32 tensors, overwritten by the
+        next call of the same k: the emitted tokens [n][k + 1], -1 behind the
+        last, and how many there are, by which the requests' positions advance;
+        a request's next step begins with its last emitted token.  k = 0 draws a
+        token a request.  As a captured step_shared, a captured call counts once
+        towards the capacity."""
+        import torch
+
+        from .gpu import embed_dev, rms_norm_dev, verify_drafts_dev, verify_drafts_workspace_size
+
+        md, s = self.md, self._shared
+        if s is None:
+            raise ValueError("verify_shared needs share_prefix first")
+        with _memory_of(stream):
+            if not hasattr(tokens, "is_cuda"):
+                tokens = torch.tensor([[int(t) for t in row] for row in tokens], dtype=torch.int32, device="cuda")
+            if tokens.dim() != 2 or tokens.shape[0] != s["n"] or tokens.shape[1] == 0:
+                raise ValueError(f"tokens of {tuple(tokens.shape)} for {s['n']} requests")
+            n, per = (int(v) for v in tokens.shape)
+            if n * per > 64:
+                raise ValueError(f"{n} requests of {per} tokens are more than the 64 rows of a step")
+            k, rows, d = per - 1, n * per, md.d_model
+            self._room(per, stream)
+            if per not in s["drafts"]:
+                need = max(b.decode_kv_workspace_size(c, n, prefix_len=s["len"], n_tokens=per)
+                           for b, c in zip(self.blocks, s["own"]))
+                vneed = max(verify_drafts_workspace_size(n, k, md.vocab_size, given) for given in (False, k > 0))
+                s["drafts"][per] = {"h": torch.empty((rows, d), dtype=torch.float32, device="cuda"),
+                                    "hn": torch.empty((rows, d), dtype=torch.float32, device="cuda"),
+                                    "logits": torch.empty((rows, md.vocab_size), dtype=torch.float32, device="cuda"),
+                                    "tokens": torch.empty((n, per), dtype=torch.int32, device="cuda"),
+                                    "counts": torch.empty(n, dtype=torch.int32, device="cuda"),
+                                    "ws": torch.empty(need, dtype=torch.uint8, device="cuda"), "need": need,
+                                    "vws": torch.empty(vneed, dtype=torch.uint8, device="cuda"), "vneed": vneed}
+            b = s["drafts"][per]
+            ids = tokens[:, 1:].contiguous()
+            embed_dev(self.ctx, self.embedding, md.vocab_size, d, tokens, rows, b["h"], stream)
+            for block, own, prefix in zip(self.blocks, s["own"], s["prefix"]):
+                block.decode_kv_dev(b["h"], s["pos"], n, own, b["ws"], b["need"], prefix=prefix, prefix_len=s["len"],
+                                    stream=stream, n_tokens=per)
+            rms_norm_dev(self.ctx, b["h"], rows, d, self.final_norm, md.rms_norm_eps, b["hn"], stream)
+            self.head.logits_dev(b["hn"], rows, b["logits"], stream)
+            verify_drafts_dev(self.ctx, b["logits"], n, k, md.vocab_size, ids, uniforms, b["tokens"], b["counts"],
+                              b["vws"], b["vneed"], draft_logits=draft_logits, n_drafts=n_drafts,
+                              temperature=temperature, pos=s["pos"], stream=stream)
+        s["steps"] += per
+        s["bound"] = True
+        return b["tokens"], b["counts"]
 
     def step(self, token: int, stream=None):
         """The next position's logits (a device tensor, overwritten by the

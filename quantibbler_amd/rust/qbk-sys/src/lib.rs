@@ -266,6 +266,13 @@ extern "C" {
                                    prefix_shape: *const KvShape, prefix: *const c_void, prefix_seq: usize,
                                    prefix_len: usize, workspace: *mut c_void, workspace_size: usize,
                                    stream: *mut c_void) -> c_int;
+    pub fn qbk_block_decode_kv_tokens_workspace_size(block: *const QbkBlock, shape: *const KvShape, n: usize,
+                                                     tokens: usize, max_len: usize, prefix_len: usize) -> usize;
+    pub fn qbk_block_decode_kv_tokens_dev(ctx: *mut QbkCtx, block: *mut QbkBlock, h: *mut f32, pos: *const u32, n: usize,
+                                          tokens: usize, shape: *const KvShape, cache: *mut c_void, first_seq: usize,
+                                          max_len: usize, prefix_shape: *const KvShape, prefix: *const c_void,
+                                          prefix_seq: usize, prefix_len: usize, workspace: *mut c_void,
+                                          workspace_size: usize, stream: *mut c_void) -> c_int;
     pub fn qbk_rope_init(rope: *mut Rope, head_dim: usize, rotary_dim: usize, interleaved: c_int, theta: f64,
                          scaling: *const RopeScaling) -> c_int;
     pub fn qbk_rotate_heads_dev(ctx: *mut QbkCtx, rope: *const Rope, q: *const c_void, k: *const c_void, dtype: c_int,
