@@ -1200,6 +1200,30 @@ struct KvaPlan {
     size_t bytes;
 };
 
+// fp4: splits of a prefix of tp tiles for op row tiles, `own` tiles of own rows beside it.  A workgroup takes its run of
+// tiles (the body of 16 rows: four at a time) and as long as C more; two on a CU take 1.45 (16 rows: 1.65) times one's
+// time, of heads past 128 twice, since one fills it.  Own rows are read by the second workgroup of a CU while the first
+// computes, so that the prefix stays within one a CU where they are as many tiles (16 rows: a third; us for 256 / 512
+// workgroups, 32/8 heads of 128, 64 rows: 128 row tiles of 16 behind 16384 55.0 / 48.2, with 1000 own rows each 55.9 /
+// 53.2, with 2000 57.3 / 63.7; 512 tiles behind 4096 58.5 / 51.7, behind 16384 185 / 133; 16 rows: 64 tiles behind 16384
+// 34.8 / 31.0, with 2000 own rows 35.8 / 40.3; 40 of heads of 80 behind 4001, 240 and 280 to 320 14.5 / 17.2, 16.0).
+static uint32_t kva_prefix_splits(uint64_t op, size_t tp, bool wide, size_t dc, uint64_t own) {
+    const uint64_t round = wide ? 1 : KVA_WAVES, fixed = wide ? 200 : 50, both = dc == 4 ? 40 : wide ? 29 : 33;  // by 20
+    const uint64_t most = div_ceil(tp, KVA_WAVES) < KVA_MAX_SPLITS ? div_ceil(tp, KVA_WAVES) : KVA_MAX_SPLITS;
+    uint64_t best = 1, least = ~0ull;
+    for (uint64_t sp = 1; sp <= most; sp++) {
+        const uint64_t groups = op * sp;
+        if (sp > 1 && groups > (own * (wide ? 1 : 3) > op * tp ? 256 : 512)) break;
+        const uint64_t rest = groups % 512, slots = groups / 512 * both + (rest > 256 ? both : rest ? 20 : 0);
+        const uint64_t cost = (20 * div_ceil(div_ceil(tp, sp), round) + fixed) * slots;
+        if (cost < least) {
+            least = cost;
+            best = sp;
+        }
+    }
+    return (uint32_t)div_ceil(tp, div_ceil(tp, best));  // none without a tile
+}
+
 static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t sq, size_t max_len, size_t prefix_len) {
     KvaPlan p{};
     const size_t Hk = s->n_kv_heads, G = n_heads / Hk, rows = n * sq * G, per = sq * G;
@@ -1210,12 +1234,21 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
     // 19.4, 2048 21 / 35; up to 1500: 27.8 / 21.1, 36.2 / 36.4, 45 / 66; heads of 64, 1024 items 9.5 / 11.7 and 24.8 /
     // 21.8; heads of 256, 256 items 24.5 / 17.6 and 41.5 / 31.3, 512 24.9 / 29.3 and 53.8 / 51.9).
     p.wides = per > 16 && max_len && (uint64_t)n * Hk * div_ceil(per, 16) > 1024 / dc;
+    // fp4, whose tiles take longer to widen, past 512 keys only from more items on and where most of the 64 rows are
+    // there (32/8 heads of 128, 1024 items up to 300 15.9 / 17.7, up to 700 24.8 / 23.8, up to 1500 41.9 / 34.8, with 32
+    // rows a sequence 43.2 / 35.7; 2048 up to 1500 48.8 / 62.9; heads of 64, 1024 28.9 / 23.6, 2048 33.3 / 38.5; of 256,
+    // 512 items up to 300 28.9 / 23.5, 1024 31 / 45 and 89 / 86).
+    const bool fp4 = s->format == QBK_KV_FP4;
+    if (fp4 && (max_len > 512 || dc == 4))
+        p.wides = p.wides && per > 32 && (uint64_t)n * Hk * div_ceil(per, 16) > (dc == 4 ? 1023 : 1024);
     // The prefix, split over the card by either, from the row tiles on whose reading of the same codes shows (8 kv heads
     // of 128 behind 500, 8192 and 16384: 64 tiles 13.9 / 11.5, 23.7 / 20.7, 31.2 / 32.5; 128 tiles 14.9 / 15.8, 32.4 /
     // 31.4, 49.2 / 53.9; heads of 64 behind 500 and 2048: 128 tiles 12.1 / 10.3, 14.2 / 12.6, 512 24.3 / 24.8, 29.6 /
     // 32.4; heads of 256: 32 tiles 19.8 / 14.2, 21.6 / 23.2, 64 tiles 20.8 / 21.0, 24.0 / 26.8).
-    p.widep = p.wides || (prefix_len && (uint64_t)Hk * div_ceil(rows, 16) >= (dc == 1 ? 512 : 256 / dc));
-    p.few = s->format == QBK_KV_FP4 && per <= 4;
+    // fp4 keeps to the first for heads of 256 (behind 16384: 128 tiles 122 / 101, 256 tiles 223 / 180, 512 422 / 351).
+    p.widep = p.wides || (prefix_len && !(fp4 && dc == 4) &&
+                          (uint64_t)Hk * div_ceil(rows, 16) >= (dc == 1 ? 512 : 256 / dc));
+    p.few = fp4 && per <= 4;
     p.rtp = (uint32_t)div_ceil(rows, p.widep ? 64 : 16);
     p.rts = (uint32_t)div_ceil(per, p.wides ? 64 : 16);
     const uint64_t op = prefix_len ? (uint64_t)Hk * p.rtp : 0, os = (uint64_t)n * Hk * p.rts;
@@ -1231,13 +1264,7 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
         want = want < most ? want : most;
         return (uint32_t)(want < 1 ? 1 : want > KVA_MAX_SPLITS ? KVA_MAX_SPLITS : want);
     };
-    if (prefix_len) p.sp = splits(div_ceil(256, op), tp);
-    // fp4, whose tiles take a wave as long for half the bytes: whole rounds of the waves (80 rows behind 4001, f32, 8
-    // heads of 80, runs of nine tiles and of eight: 17.2 and 15.9 us)
-    if (prefix_len && s->format == QBK_KV_FP4 && !p.widep) {
-        const size_t run = div_ceil(tp, p.sp), whole = run / KVA_WAVES * KVA_WAVES;
-        if (whole) p.sp = splits(div_ceil(tp, whole), tp);
-    }
+    if (prefix_len) p.sp = fp4 ? kva_prefix_splits(op, tp, p.widep, dc, os * ts) : splits(div_ceil(256, op), tp);
     if (max_len) p.ss = splits(os >= 256 ? div_ceil(ts, 64) : div_ceil(512, os), ts);
     // a second launch takes longer than one more tile a wave (one sequence of 512 rows in one launch 7.9 us, split 9.2;
     // of 768 9.6 and 9.4, of 1024 11.1 and 9.4)
@@ -1270,13 +1297,14 @@ static int kva_launch(const KvAttArgs &a, uint64_t items, int device, hipStream_
 template <int FMT, int DC, typename T>
 static int kva_dispatch_dc(const KvAttArgs &a, const KvaPlan &p, int device, hipStream_t st) {
     if (p.wides) return kva_launch<FMT, DC, true, KVA_ROWS64, T>(a, p.items, device, st);
-    if constexpr (FMT == QBK_KV_FP4) {
-        if (p.few) {
-            if (p.widep) return kva_launch<FMT, DC, true, KVA_ROWS4, T>(a, p.items, device, st);
-            return kva_launch<FMT, DC, false, KVA_ROWS4, T>(a, p.items, device, st);
-        }
+    constexpr bool FP4 = FMT == QBK_KV_FP4;
+    if constexpr (FP4) {
+        if constexpr (DC < 4)
+            if (p.few && p.widep) return kva_launch<FMT, DC, true, KVA_ROWS4, T>(a, p.items, device, st);
+        if (p.few) return kva_launch<FMT, DC, false, KVA_ROWS4, T>(a, p.items, device, st);
     }
-    if (p.widep) return kva_launch<FMT, DC, true, KVA_ROWS16, T>(a, p.items, device, st);
+    if constexpr (!FP4 || DC < 4)
+        if (p.widep) return kva_launch<FMT, DC, true, KVA_ROWS16, T>(a, p.items, device, st);
     return kva_launch<FMT, DC, false, KVA_ROWS16, T>(a, p.items, device, st);
 }
 
