@@ -377,8 +377,14 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
 //   the same read: 512 rows 4.3 / 5.1, 1024 6.2 / 5.6, 2048 9.9 / 6.8
 //   1024 sequences, written: two rows each 31 / 47, four 57 / 49, sixteen 135 / 57; read 26 / 34, 49 / 35, 71 / 42
 //   4096 sequences, 2 heads of 64, written: four rows 20.5 / 37, eight 37.5 / 38, sixteen 69 / 39
+// fp4 has more to do a tile, and its rows go in twos: from eight rows a sequence
+// on
+//   one sequence, written: 512 rows 6.1 / 8.3, 1024 8.7 / 8.3, 2048 15.3 / 9.7; read 3.9 / 5.4, 5.4 / 5.9, 7.9 / 6.9
+//   1024 sequences, written: four rows each 55 / 72, eight 76 / 72, sixteen 123 / 73; read 30 / 28, 36 / 29, 48 / 32
+//   the same, 2 heads of 64: eight rows 13.8 / 19.8, sixteen 22.7 / 19.6; heads of 256: two 67 / 138, eight 207 / 136
 static bool kv_by_tiles(size_t n_rows, size_t n, const qbk_kv_shape *s) {
-    return (unsigned __int128)n_rows * s->n_kv_heads > 4096 && n_rows * s->head_dim / 512 >= n;
+    return (unsigned __int128)n_rows * s->n_kv_heads > 4096 &&
+           (s->format == QBK_KV_FP4 ? n_rows / 8 : n_rows * s->head_dim / 512) >= n;
 }
 
 // Checks shared by the write and the read; *a filled for a launch, n_rows 0

@@ -162,6 +162,32 @@ def test_rows_written_a_few_at_a_time(ctx, kv):
         kvc.check(vo, want, f"value {i}")
 
 
+@pytest.mark.parametrize("d", [48, 128])
+def test_rows_written_by_parts_of_tiles(ctx, d):
+    """Eight rows a sequence and more, as tiles go, from any row of a tile to any: what earlier calls wrote stays, in the
+    other half of a byte too."""
+    rng = np.random.default_rng(9)
+    n, kv, cap = 3, 180, 210
+    cache = kvc.make(ctx, "fp4", n, cap, kv, d)
+    x = torch.from_numpy(kvc.rows_of(rng, n * cap, kv, d)).cuda().view(n, cap, kv, d)
+    at = [0, 3, 62]
+    first = list(at)
+    while max(at) + 33 < cap:
+        step = [0, 0, 0]
+        while sum(step) < 24:
+            step = [int(v) for v in rng.integers(0, 34, n)]
+        rows = torch.cat([x[i, at[i]:at[i] + step[i]] for i in range(n)])
+        cache.write_dev(rows, rows, "float32", words(at), len(rows), row_start=words(np.concatenate([[0], np.cumsum(step)])))
+        at = [a + s for a, s in zip(at, step)]
+    for i in range(n):
+        m = at[i] - first[i]
+        ko, vo = torch.empty((m, kv, d), device="cuda"), torch.empty((m, kv, d), device="cuda")
+        cache.read_dev(ko, vo, "float32", words([first[i]]), m, first_seq=i, n_seqs=1)
+        want = stored(x[i, first[i]:at[i]].cpu().numpy())
+        kvc.check(ko, want, f"key {i}")
+        kvc.check(vo, want, f"value {i}")
+
+
 @pytest.mark.parametrize("kv", [1, 400])
 def test_row_starts_that_say_nothing_sensible(ctx, kv):
     d, cap = 16, 40
