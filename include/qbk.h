@@ -488,7 +488,8 @@ size_t qbk_kv_cache_size(const qbk_kv_shape *shape);
  * arrays are read when the call runs, so a captured graph serves every later
  * position.  A row whose position is at or past the capacity, or that no
  * sequence claims, is left out; cache rows no position names keep what they
- * held. */
+ * held. In the 4-bit format neighbouring rows share bytes: calls that write rows of
+ * one sequence must not run at the same time. */
 int qbk_kv_cache_write_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, void *cache, const void *k, const void *v,
                            int dtype, size_t row_stride, size_t n_rows, const uint32_t *row_start,
                            const uint32_t *pos, size_t first_seq, size_t n, void *stream);

@@ -14,8 +14,6 @@
 
 namespace qbk {
 
-#define ROT_WAVES 8192
-
 struct RotArgs {
     const void *q, *k;
     void *qo, *ko;
@@ -223,7 +221,9 @@ __global__ void __launch_bounds__(256) rot_any(RotArgs a) {
     for (uint32_t c = 2 * half + lane; c < hd; c += 64) dst[c] = rot_out<T>(value(c));
 }
 
-// Whether a head falls into runs of four pairs and eight channels.
+// Whether a head falls into runs of four pairs and eight channels.  Pair by pair
+// otherwise (us by runs / by pairs, 8192 rows of 32 and 8 heads of 128, bf16: 29 /
+// 142, 32 rows 3.3 / 3.6).
 static bool rot_by_quads(const qbk_rope &r) { return r.head_dim % 8 == 0 && r.rotary_dim % 8 == 0; }
 
 template <typename T>
@@ -235,8 +235,14 @@ static void rot_go(RotArgs a, hipStream_t s) {
     }
     const uint32_t hd = a.rope.head_dim;
     const int lanes = hd <= 16 ? 2 : hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
-    const size_t passes = div_ceil(all, (size_t)(64 / lanes)), want = div_ceil(ROT_WAVES, (size_t)a.n_rows);
-    a.waves = (uint32_t)(want < 1 ? 1 : want < passes ? want : passes);
+    // Waves a row: two a SIMD, up to eight while each has five passes over heads to form its angles for (us for one wave a
+    // row, two a SIMD, eight; 32 and 8 heads of 128, bf16: 1 row 7.1 / 3.5 / 3.2, 1024 rows 8.9 / 7.1 / 8.5, 4096 18.8 /
+    // 18.6 / 17.0; 16 and 4 heads of 64: 32 rows 4.2 / 3.2 / 3.2, 4096 7.6 / 7.6 / 8.9; all passes apart, 8192 rows of
+    // heads of 128 29 -> 48).
+    const size_t passes = div_ceil(all, (size_t)(64 / lanes)), two = div_ceil((size_t)2048, (size_t)a.n_rows);
+    const size_t eight = div_ceil((size_t)8192, (size_t)a.n_rows), five = div_ceil(passes, (size_t)5);
+    const size_t want = eight < five ? eight : five > two ? five : two;
+    a.waves = (uint32_t)(want < passes ? want : passes);
     void (*k)(RotArgs) = lanes == 2   ? rot_quads<T, 2>
                          : lanes == 4 ? rot_quads<T, 4>
                          : lanes == 8 ? rot_quads<T, 8>
@@ -339,6 +345,9 @@ int qbk_rotate_heads_dev(qbk_ctx *ctx, const qbk_rope *rope, const void *q, cons
     if (!pos || (n_heads && (!q || !q_out)) || (n_kv_heads && (!k || !k_out)))
         return fail(QBK_ERR_VALIDATION, "null argument");
     if ((rc = bind(ctx))) return rc;
+    if (n_rows > 1 && ((n_heads && q == q_out && q_stride != q_out_stride) ||
+                       (n_kv_heads && k == k_out && k_stride != k_out_stride)))
+        return fail(QBK_ERR_VALIDATION, "rotate_heads in place needs one stride for rows in and out");
     RotArgs a{};
     a.q = q;
     a.k = k;

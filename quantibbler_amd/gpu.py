@@ -558,7 +558,9 @@ class KvCache:
         in place) into sequences first_seq .. first_seq + n_seqs - 1: rows
         row_start[i] .. row_start[i + 1] - 1 go to sequence first_seq + i at
         positions pos[i], pos[i] + 1, ...; ``row_start`` None splits the rows
-        evenly.  Rows past the capacity are left out."""
+        evenly.  Rows past the capacity are left out.  In "fp4" neighbouring
+        rows share bytes: two calls that write rows of one sequence must not
+        run at the same time."""
         self._rows(_lib.load().qbk_kv_cache_write_dev, k, v, dtype, pos, n_rows, first_seq, n_seqs, row_start,
                    row_stride, stream)
 

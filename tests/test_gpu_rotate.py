@@ -254,3 +254,21 @@ def test_rows_that_fill_the_card(ctx):
     for x, x64 in zip(out, (q64, k64)):
         want, tol = reference(x64[pick], w.cpu().numpy(), 17 + pick, 500000.0, d, False, SCALINGS[3])
         check(x[torch.from_numpy(pick).cuda()], want, tol)
+
+
+def test_in_place_takes_one_stride(ctx):
+    from quantibbler_amd import KernelError
+
+    d, heads, kv, n = 64, 4, 2, 3
+    wide = torch.randn((n, 500), device="cuda")
+    kept = wide.clone()
+    q, k = wide[:, :heads * d], wide[:, heads * d:(heads + kv) * d]
+    out = torch.empty((n, 500), device="cuda")
+    for strides in (dict(k_out_stride=500), dict(q_out_stride=500)):
+        with pytest.raises(KernelError, match="in place needs one stride"):
+            rotate_heads_dev(ctx, Rope(d, 10000.0), q, k, "float32", n, heads, kv, words([1]), q, k, q_stride=500,
+                             k_stride=500, **strides)
+    rotate_heads_dev(ctx, Rope(d, 10000.0), q, None, "float32", n, heads, 0, words([1]), out, None, q_stride=500,
+                     q_out_stride=500)
+    torch.cuda.synchronize()
+    assert torch.equal(wide, kept)
