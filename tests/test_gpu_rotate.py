@@ -266,8 +266,8 @@ def test_in_place_takes_one_stride(ctx):
     out = torch.empty((n, 500), device="cuda")
     for strides in (dict(k_out_stride=500), dict(q_out_stride=500)):
         with pytest.raises(KernelError, match="in place needs one stride"):
-            rotate_heads_dev(ctx, Rope(d, 10000.0), q, k, "float32", n, heads, kv, words([1]), q, k, q_stride=500,
-                             k_stride=500, **strides)
+            rotate_heads_dev(ctx, Rope(d, 10000.0), q.data_ptr(), k.data_ptr(), "float32", n, heads, kv, words([1]),
+                             q.data_ptr(), k.data_ptr(), q_stride=500, k_stride=500, **strides)
     rotate_heads_dev(ctx, Rope(d, 10000.0), q, None, "float32", n, heads, 0, words([1]), out, None, q_stride=500,
                      q_out_stride=500)
     torch.cuda.synchronize()
