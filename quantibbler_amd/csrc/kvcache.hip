@@ -1,5 +1,6 @@
 // kvcache.hip -- the 8-bit KV cache's rows in and out: quantised as they are
-// written, one f32 scale a row and kv head, and read back as values.
+// written, one f32 scale a row and kv head, and read back as values; and the
+// entries of the 4-bit one (kvcache4.hip).
 //
 //   A = max(max |x|, 2^-100), L = 127 (int8) or 448 (e4m3)
 //   scale = A (1 / L),  code = nearest(x (L (1 / A))),  value = code * scale
@@ -379,9 +380,9 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
 //   4096 sequences, 2 heads of 64, written: four rows 20.5 / 37, eight 37.5 / 38, sixteen 69 / 39
 // fp4 has more to do a tile, and its rows go in twos: from eight rows a sequence
 // on
-//   one sequence, written: 512 rows 6.1 / 8.3, 1024 8.7 / 8.3, 2048 15.3 / 9.7; read 3.9 / 5.4, 5.4 / 5.9, 7.9 / 6.9
-//   1024 sequences, written: four rows each 55 / 72, eight 76 / 72, sixteen 123 / 73; read 30 / 28, 36 / 29, 48 / 32
-//   the same, 2 heads of 64: eight rows 13.8 / 19.8, sixteen 22.7 / 19.6; heads of 256: two 67 / 138, eight 207 / 136
+//   one sequence, written: 1024 rows 8.7 / 6.4, 2048 15.3 / 7.8; read 5.4 / 5.9, 7.9 / 6.9
+//   1024 sequences, written: four rows each 55 / 78, eight 76 / 79, sixteen 123 / 81; read 30 / 28, 36 / 29, 48 / 32
+//   the same, 2 heads of 64: eight rows 13.8 / 20, sixteen 22.7 / 20; heads of 256: two 67 / 138, eight 207 / 134
 static bool kv_by_tiles(size_t n_rows, size_t n, const qbk_kv_shape *s) {
     return (unsigned __int128)n_rows * s->n_kv_heads > 4096 &&
            (s->format == QBK_KV_FP4 ? n_rows / 8 : n_rows * s->head_dim / 512) >= n;

@@ -8,6 +8,12 @@
 // each step rounded once to f32 (to nearest, even at a tie), codes past 6 held
 // at 6 (2688 = 6 448).  The multiplier of the group that holds A is 448, the
 // others' follow their own largest within 2^-4.
+//
+// One pass over rows and codes, bound by memory where there are many (98816 f32
+// rows of 8 heads of 128 written 199 us, 4.6 TB/s; 10391 written 31, read back
+// 18.4, 3.1 and 5.3 TB/s; 50000 of one sequence read as bf16 33 us), by the launch
+// and one row's chain of reductions where there are few (32 rows written 5.3,
+// read 3.9).
 #include <math.h>
 
 #include "kvcache_rows.h"
@@ -200,10 +206,11 @@ __device__ __forceinline__ uint32_t kv4_rows_in(uint32_t row, uint32_t lo, uint3
 }
 
 // Sixteen lanes a row, four channels a lane and P times 64 channels, sixteen
-// rows at a time and every row's loads before the first is used.  Codes go
-// through LDS, 16 bits for four channels of a row, and leave 16 bytes at a time:
-// keys as two rows' sixteen channels, values, turned by 4 x 4, as two channels'
-// sixteen rows; multipliers through LDS in the cache's order.
+// rows at a time and every row's loads before the first is used; keys and values
+// by workgroups of their own.  Codes go through LDS, 16 bits for four channels of
+// a row: keys leave as two rows' sixteen channels, 16 bytes, values, turned by
+// 4 x 4, as a channel's sixteen rows, 8 bytes; multipliers through LDS in the
+// cache's order.
 template <int P, typename T>
 __global__ void __launch_bounds__(256) kv4_write_tiles(KvRows a, const T *k, const T *v) {
     constexpr int PAD = 16 * P + 4;  // of an LDS row, in four channels: keys are read eight bytes at a time
@@ -217,118 +224,101 @@ __global__ void __launch_bounds__(256) kv4_write_tiles(KvRows a, const T *k, con
     if (t.first + hi > a.c.cap) hi = (uint32_t)(a.c.cap - t.first);
     const bool full = t.lo == 0 && hi == 64;
     const uint32_t c0 = 4 * (tid & 15);
-    const T *srcs[2] = {k, v};
+    const bool val = blockIdx.y;
     Kv4<T> raw[4][P];
-    auto load = [&](int val) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t r = 16 * q + (tid >> 4);
-            const bool in = r >= t.lo && r < hi;
-            const T *src = srcs[val] + (size_t)(t.row + (in ? r - t.lo : 0)) * a.stride + (size_t)h * hd;
+    for (int q = 0; q < 4; q++) {
+        const uint32_t r = 16 * q + (tid >> 4);
+        const bool in = r >= t.lo && r < hi;
+        const T *src = (val ? v : k) + (size_t)(t.row + (in ? r - t.lo : 0)) * a.stride + (size_t)h * hd;
 #pragma unroll
-            for (int p = 0; p < P; p++) raw[q][p] = *(const Kv4<T> *)(src + (c0 + 64 * p < hd ? c0 + 64 * p : 0));
+        for (int p = 0; p < P; p++) raw[q][p] = *(const Kv4<T> *)(src + (c0 + 64 * p < hd ? c0 + 64 * p : 0));
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const uint32_t r = 16 * q + (tid >> 4);
+        float x[P][4];
+        uint32_t group[P], top = 0;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            group[p] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[p][e] = c0 + 64 * p < hd ? kv_in<T>(raw[q][p].v[e]) : 0.0f;
+                group[p] = kv4_most(group[p], __float_as_uint(x[p][e]) & 0x7fffffffu);
+            }
+            group[p] = kv4_max8(group[p]);
+            top = kv4_most(top, group[p]);
         }
-    };
-    load(0);
+        top = kv4_most(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x128, 0xf, 0xf, true));  // row_ror 8
+        const Kv4Row row(top);
 #pragma unroll
-    for (int val = 0; val < 2; val++) {
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t r = 16 * q + (tid >> 4);
-            float x[P][4];
-            uint32_t group[P], top = 0;
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                group[p] = 0;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[p][e] = c0 + 64 * p < hd ? kv_in<T>(raw[q][p].v[e]) : 0.0f;
-                    group[p] = kv4_most(group[p], __float_as_uint(x[p][e]) & 0x7fffffffu);
-                }
-                group[p] = kv4_max8(group[p]);
-                top = kv4_most(top, group[p]);
-            }
-            top = kv4_most(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x128, 0xf, 0xf, true));  // row_ror 8
-            const Kv4Row row(top);
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                const uint32_t c = c0 + 64 * p;
-                if (c >= hd) continue;
-                float by;
-                const uint32_t m = kv4_mul(row, group[p], by);
-                codes[r * PAD + c / 4] = (uint16_t)kv4_codes(row, x[p], by);
-                if ((tid & 7) == 0)
-                    mul[c / 32 * 64 + (val ? (r >> 2 & 3) * 16 + (r >> 4) * 4 + (r & 3) : (r & 15) * 4 + (r >> 4))] = (uint8_t)m;
-            }
-            if (r >= t.lo && r < hi && (tid & 15) == 0) (val ? a.c.vs : a.c.ks)[slab + t.first + r] = row.scale;
+        for (int p = 0; p < P; p++) {
+            const uint32_t c = c0 + 64 * p;
+            if (c >= hd) continue;
+            float by;
+            const uint32_t m = kv4_mul(row, group[p], by);
+            codes[r * PAD + c / 4] = (uint16_t)kv4_codes(row, x[p], by);
+            if ((tid & 7) == 0)
+                mul[c / 32 * 64 + (val ? (r >> 2 & 3) * 16 + (r >> 4) * 4 + (r & 3) : (r & 15) * 4 + (r >> 4))] = (uint8_t)m;
         }
-        if (val == 0) load(1);  // on their way while the keys leave
-        __syncthreads();
-        uint8_t *md = (val ? a.c.vm : a.c.km) + slab * ng + t.first * ng;
-        for (uint32_t x = tid; x < 16 * ng; x += 256) {  // four rows of a group: key 16 i + x % 16, value 16 i + 4 g + j
-            const uint32_t w = *(const uint32_t *)(mul + 4 * x);
-            if (full) {
-                *(uint32_t *)(md + 4 * x) = w;
-                continue;
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                const uint32_t r = val ? (x & 3) * 16 + (x >> 2 & 3) * 4 + i : 16 * i + (x & 15);
-                if (r >= t.lo && r < hi) md[4 * x + i] = (uint8_t)(w >> (8 * i));
-            }
+        if (r >= t.lo && r < hi && (tid & 15) == 0) (val ? a.c.vs : a.c.ks)[slab + t.first + r] = row.scale;
+    }
+    __syncthreads();
+    uint8_t *md = (val ? a.c.vm : a.c.km) + slab * ng + t.first * ng;
+    for (uint32_t x = tid; x < 16 * ng; x += 256) {  // four rows of a group: key 16 i + x % 16, value 16 i + 4 g + j
+        const uint32_t w = *(const uint32_t *)(mul + 4 * x);
+        if (full) {
+            *(uint32_t *)(md + 4 * x) = w;
+            continue;
         }
-        if (val == 0) {
-            uint8_t *dst = a.c.k + slab * (hd / 2) + t.first * (hd / 2);
-            for (uint32_t x = tid; x < 32 * nc; x += 256) {  // rows r and r + 16, one run of 16 channels
-                const uint32_t pair = x / (16 * nc), y = x - pair * 16 * nc, chunk = y >> 4, r = 32 * pair + (y & 15);
-                const uint2 one = *(const uint2 *)(codes + r * PAD + 4 * chunk);
-                const uint2 two = *(const uint2 *)(codes + (r + 16) * PAD + 4 * chunk);
-                const bool in1 = r >= t.lo && r < hi, in2 = r + 16 >= t.lo && r + 16 < hi;
-                uint8_t *d = dst + (size_t)x * 16;
-                if (in1 && in2) *(uint4 *)d = uint4{one.x, one.y, two.x, two.y};
-                else if (in1) *(uint2 *)d = one;
-                else if (in2) *(uint2 *)(d + 8) = two;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t r = val ? (x & 3) * 16 + (x >> 2 & 3) * 4 + i : 16 * i + (x & 15);
+            if (r >= t.lo && r < hi) md[4 * x + i] = (uint8_t)(w >> (8 * i));
+        }
+    }
+    if (!val) {
+        uint8_t *dst = a.c.k + slab * (hd / 2) + t.first * (hd / 2);
+        for (uint32_t x = tid; x < 32 * nc; x += 256) {  // rows r and r + 16, one run of 16 channels
+            const uint32_t pair = x / (16 * nc), y = x - pair * 16 * nc, chunk = y >> 4, r = 32 * pair + (y & 15);
+            const uint2 one = *(const uint2 *)(codes + r * PAD + 4 * chunk);
+            const uint2 two = *(const uint2 *)(codes + (r + 16) * PAD + 4 * chunk);
+            const bool in1 = r >= t.lo && r < hi, in2 = r + 16 >= t.lo && r + 16 < hi;
+            uint8_t *d = dst + (size_t)x * 16;
+            if (in1 && in2) *(uint4 *)d = uint4{one.x, one.y, two.x, two.y};
+            else if (in1) *(uint2 *)d = one;
+            else if (in2) *(uint2 *)(d + 8) = two;
+        }
+    } else {
+        uint8_t *dst = a.c.v + slab * (16 * ng) + t.first * (16 * ng);
+        for (uint32_t x = tid; x < 32 * ng; x += 256) {  // channels 4 q .. of one half of a group, rows of one g
+            const uint32_t half = x & 1, g = x >> 1 & 3, q = x >> 3 & 3, m = x >> 5, c4 = 8 * m + 4 * half + q;
+            uint32_t out[4][4];  // [i][channel]
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t in[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) in[j] = 4 * c4 < hd ? codes[(16 * i + 4 * g + j) * PAD + c4] : 0u;
+                kv4_turn(in, out[i]);
             }
-        } else {
-            uint8_t *dst = a.c.v + slab * (16 * ng) + t.first * (16 * ng);
-            for (uint32_t x = tid; x < 16 * ng; x += 256) {  // channels 4 q .. of both halves of a group, rows of one g
-                const uint32_t g = x & 3, q = x >> 2 & 3, m = x >> 4;
-                uint32_t out[2][4][4];  // [half][i][channel]
+            uint32_t keep[2] = {0u, 0u};  // codes that stay as they were
+            if (!full) {
+                keep[0] = ~(kv4_rows_in(4 * g, t.lo, hi) | kv4_rows_in(16 + 4 * g, t.lo, hi) << 16);
+                keep[1] = ~(kv4_rows_in(32 + 4 * g, t.lo, hi) | kv4_rows_in(48 + 4 * g, t.lo, hi) << 16);
+            }
 #pragma unroll
-                for (int half = 0; half < 2; half++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t in[4];
-                        const uint32_t c4 = 8 * m + 4 * half + q;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) in[j] = 4 * c4 < hd ? codes[(16 * i + 4 * g + j) * PAD + c4] : 0u;
-                        kv4_turn(in, out[half][i]);
-                    }
-                uint32_t keep[2] = {0u, 0u};  // codes that stay as they were
+            for (int e = 0; e < 4; e++) {
+                uint2 *d = (uint2 *)(dst + m * 1024 + (4 * q + e) * 64 + g * 16 + half * 8);
+                uint2 w{out[0][e] | out[1][e] << 16, out[2][e] | out[3][e] << 16};
                 if (!full) {
-                    keep[0] = ~(kv4_rows_in(4 * g, t.lo, hi) | kv4_rows_in(16 + 4 * g, t.lo, hi) << 16);
-                    keep[1] = ~(kv4_rows_in(32 + 4 * g, t.lo, hi) | kv4_rows_in(48 + 4 * g, t.lo, hi) << 16);
+                    const uint2 o = *d;
+                    w.x = (w.x & ~keep[0]) | (o.x & keep[0]);
+                    w.y = (w.y & ~keep[1]) | (o.y & keep[1]);
                 }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint4 *d = (uint4 *)(dst + m * 1024 + (4 * q + e) * 64 + g * 16);
-                    uint4 w;
-                    w.x = out[0][0][e] | out[0][1][e] << 16;
-                    w.y = out[0][2][e] | out[0][3][e] << 16;
-                    w.z = out[1][0][e] | out[1][1][e] << 16;
-                    w.w = out[1][2][e] | out[1][3][e] << 16;
-                    if (!full) {
-                        const uint4 o = *d;
-                        w.x = (w.x & ~keep[0]) | (o.x & keep[0]);
-                        w.y = (w.y & ~keep[1]) | (o.y & keep[1]);
-                        w.z = (w.z & ~keep[0]) | (o.z & keep[0]);
-                        w.w = (w.w & ~keep[1]) | (o.w & keep[1]);
-                    }
-                    *d = w;
-                }
+                *d = w;
             }
         }
-        if (val == 0) __syncthreads();
     }
 }
 
@@ -417,11 +407,11 @@ __global__ void __launch_bounds__(256) kv4_read_tiles(KvRows a, T *k, T *v) {
 
 template <typename T>
 static void kv4_write_any(const KvRows &a, const T *k, const T *v, hipStream_t s) {
-    if (a.tiles) {
+    if (a.tiles) {  // keys, then values
         void (*kern)(KvRows, const T *, const T *) = a.c.hd <= 64    ? kv4_write_tiles<1, T>
                                                      : a.c.hd <= 128 ? kv4_write_tiles<2, T>
                                                                      : kv4_write_tiles<4, T>;
-        hipLaunchKernelGGL(kern, dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk)), dim3(256), 0, s, a, k, v);
+        hipLaunchKernelGGL(kern, dim3((unsigned)(kv_tiles(a.n_rows, a.n) * a.c.Hk), 2), dim3(256), 0, s, a, k, v);
     } else {
         hipLaunchKernelGGL(kv4_write<T>, dim3((unsigned)div_ceil((size_t)a.n_rows * a.c.Hk, 4)), dim3(256), 0, s, a, k, v);
     }
