@@ -8,15 +8,16 @@ two hot paths behind the reference's own API surface:
   scheme) and ``GpuContext.attention_sage_blk_dev`` (block-scaled INT8 Q/K,
   fp16 P.V).
 
-Beside them, for serving: an 8-bit KV cache and batched attention over it
-behind a shared prefix (``KvCache``) and log probabilities
-(``gpu.logprobs_dev``).
+Beside them, for serving: a KV cache in 8 or 4 bits and batched attention
+over it behind a shared prefix (``KvCache``), heads normed and rotated
+(``Rope``, ``gpu.rotate_heads_dev``), verification of drafted tokens
+(``gpu.verify_drafts_dev``) and log probabilities (``gpu.logprobs_dev``).
 
 All compute runs in libqbk.so (hand-written HIP, C ABI in include/qbk.h).
 """
 from ._lib import DeviceError, InitError, KernelError, load as _load_lib  # noqa: F401
 from .gpu import (AttentionShape, DecoderBlock, FactorLayer, FactorSet, GpuContext,  # noqa: F401
-                  KvCache, LmHead, SageDecodeState, gpu_available)
+                  KvCache, LmHead, Rope, SageDecodeState, gpu_available)
 
 _load_lib()
 

@@ -892,7 +892,8 @@ __device__ __forceinline__ void kva_few(const KvAttArgs &a, char *smem, uint32_t
 // at unlike places (one alone issues a vector operation every four cycles, two
 // of one workgroup stand at its barriers together); 32 rows a wave would halve
 // the widening but do not fit 256 registers.  64 requests of up to 2048 rows
-// behind 16384, 32/8 heads of 128: 244 MB in 54 to 55 us, 4.5 TB/s.
+// behind 16384, 32/8 heads of 128: 244 MB in 54 to 55 us, 4.5 TB/s; fp4, bound by
+// the widening, 134 MB in 58.
 template <int DC>
 struct KvaStage {
     static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 512, BUFS = DC < 4 ? 2 : 1;

@@ -419,10 +419,11 @@ class DeviceModel:
 
     def share_prefix(self, tokens, n_seqs: int, capacity: int, fmt: str = "int8", stream=None):
         """Serves ``n_seqs`` (up to 64) requests behind one prompt: the tokens
-        are prefilled once (as sequence 0), their cache rows quantised into an
-        8-bit cache per block, and every request gets room for ``capacity``
-        rows of its own there; step_shared() then steps them together, each
-        block reading the prompt's rows for many of them at a time.  bf16 serving;
+        are prefilled once (as sequence 0), their cache rows quantised into a
+        cache of ``fmt`` ("int8", "fp8", or "fp4" in 4 bits) per block, and
+        every request gets room for ``capacity`` rows of its own there;
+        step_shared() then steps them together, verify_shared() with drafts,
+        each block reading the prompt's rows for many of them at a time.  bf16 serving;
         prompt and capacity together within the model's capacity.  Returns the
         prompt's last logits, as prefill."""
         import torch
