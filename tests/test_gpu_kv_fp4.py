@@ -237,6 +237,31 @@ def test_attention_that_fills_the_card(ctx, dtype, n, heads, kv, d, sq, rows, pl
     many.test_attention_against_float64(ctx, "fp4", dtype, n, heads, kv, d, sq, rows, plen)
 
 
+# bodies of 64 rows as this format takes them, and splits of a prefix by what they cost
+WIDE = [(4, 64, 64, 256, 64, [64, 65, 130, 90], 64), (6, 64, 64, 240, 33, [33, 34, 200, 3, 0, 65], 0),
+        (1, 256, 256, 256, 70, [90], 30), (2, 128, 128, 128, 80, [80, 900], 0), (1, 256, 256, 64, 70, [600], 100),
+        (2, 96, 96, 112, 100, [513, 700], 65)]
+LONG = [(16, 8, 8, 80, 5, [5 + 3 * i for i in range(16)], 4001), (33, 35, 5, 80, 2, [2 + i % 7 for i in range(33)], 8200),
+        (20, 32, 8, 128, 4, [4 + 40 * i for i in range(20)], 5001), (2, 8, 2, 256, 9, [9, 300], 9000)]
+
+
+@BOTH
+@pytest.mark.parametrize("n,heads,kv,d,sq,rows,plen", WIDE + LONG)
+def test_attention_by_64_rows_and_by_long_prefixes(ctx, dtype, n, heads, kv, d, sq, rows, plen):
+    many.test_attention_against_float64(ctx, "fp4", dtype, n, heads, kv, d, sq, rows, plen)
+
+
+@BOTH
+def test_the_ends_of_the_range_by_64_rows_of_256_channels(ctx, dtype):
+    shape = (1, 256, 256, 256, 70, [90], 30)
+    ext.test_queries_near_the_bottom_of_the_range(ctx, "fp4", dtype, shape)
+    ext.test_keys_near_the_top_of_the_range(ctx, "fp4", dtype, shape)
+    ext.test_values_near_the_top_of_the_range(ctx, "fp4", dtype, shape)
+    ext.test_a_large_value_of_next_to_no_weight(ctx, "fp4", dtype, shape, -1)
+    ext.test_a_value_that_only_the_last_query_sees(ctx, "fp4", dtype, shape, 45)
+    ext.test_scores_past_the_exponents_range(ctx, "fp4", dtype, shape, 1e7)
+
+
 @BOTH
 def test_values_out_of_the_ordinary(ctx, dtype):
     att.test_values_out_of_the_ordinary(ctx, "fp4", dtype)
