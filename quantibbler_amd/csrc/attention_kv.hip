@@ -1269,7 +1269,10 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
     if (max_len) p.ss = splits(os >= 256 ? div_ceil(ts, 64) : div_ceil(512, os), ts);
     // a second launch takes longer than one more tile a wave (one sequence of 512 rows in one launch 7.9 us, split 9.2;
     // of 768 9.6 and 9.4, of 1024 11.1 and 9.4)
-    if (!prefix_len && ts <= 2 * KVA_WAVES) p.ss = 1;
+    // (the body of four rows, heads of 64: 1024 rows 8.0 and 6.9, 1500 8.2 and 8.3; of 128: 768 9.2 and 8.4, 1024 9.2 and
+    // 9.5; of 256: 512 10.5, 600 11.4 and 12.5)
+    const size_t tiles = !p.few || dc == 4 ? 2 : dc == 2 ? 3 : 4;  // a wave's
+    if (!prefix_len && ts <= tiles * KVA_WAVES) p.ss = 1;
     p.items = op * p.sp + os * p.ss;
     p.bytes = p.sp + p.ss > 1 ? round_up((size_t)(p.sp + p.ss) * Hk * rows * (s->head_dim * 4 + 8), 256) : 0;
     return p;
