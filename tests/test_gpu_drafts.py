@@ -360,3 +360,58 @@ def test_a_program_of_its_own(ctx, dtype):
         check(f"replay {rep}")
     del graph
     head.close()
+
+
+def test_two_captured_calls_that_share_a_workspace(ctx):
+    """Verification and attention of two sizes captured apart on one workspace, replayed in turn and in any order: the
+    eager calls' results; the same calls on two streams at once, each with a workspace of its own, too."""
+    vocab, kv, heads, d = 5003, 2, 8, 128
+    cache, held = att.make(ctx, "fp4", 6, 700, kv, d), [700, 64, 5, 333, 650, 5]
+    att.fill(cache, 150, held)
+    jobs = []
+    for n, k in ((6, 3), (2, 1)):
+        per = k + 1
+        x, y = torch.randn((n * per, vocab), device="cuda") * 3, torch.randn((n * k, vocab), device="cuda") * 3
+        ids = torch.randint(0, vocab, (n, k), dtype=torch.int32, device="cuda")
+        u = torch.rand((n, per), device="cuda")
+        tok, cnt = torch.empty((n, per), dtype=torch.int32, device="cuda"), torch.empty(n, dtype=torch.int32, device="cuda")
+        q = torch.randn((n, per, heads, d), device="cuda")
+        lens, out = words(held[:n]), torch.empty_like(q)
+        need = max(verify_drafts_workspace_size(n, k, vocab), cache.attention_workspace_size(heads, n, seq_q=per))
+
+        def run(ws, s, n=n, k=k, per=per, x=x, y=y, ids=ids, u=u, tok=tok, cnt=cnt, q=q, lens=lens, out=out, need=need):
+            verify_drafts_dev(ctx, x, n, k, vocab, ids, u, tok, cnt, ws, need, draft_logits=y, stream=s)
+            cache.attention_dev(q, "float32", heads, lens, out, ws, need, n_seqs=n, seq_q=per, stream=s)
+        jobs.append((run, need, (tok, cnt, out), (x, u, q)))
+    shared = torch.full((max(j[1] for j in jobs),), 0xFF, dtype=torch.uint8, device="cuda")
+    apart = [torch.full((j[1],), 0xFF, dtype=torch.uint8, device="cuda") for j in jobs]
+    streams, graphs = [torch.cuda.Stream() for _ in jobs], []
+    for run, _, _, _ in jobs:
+        run(shared, torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            run(shared, torch.cuda.current_stream())
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1, 0)):
+        for _, _, _, inputs in jobs:
+            inputs[0].normal_(), inputs[1].uniform_(0.0, 0.999), inputs[2].normal_()
+        torch.cuda.synchronize()
+        want = []
+        for (run, _, outs, _), ws in zip(jobs, apart):
+            run(ws, torch.cuda.current_stream())
+            torch.cuda.synchronize()
+            want.append([t.clone() for t in outs])
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for (_, _, outs, _), w in zip(jobs, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs, w))
+            for t in outs:
+                t.zero_()
+        torch.cuda.synchronize()
+        for (run, _, _, _), ws, st in zip(jobs, apart, streams):
+            run(ws, st)
+        torch.cuda.synchronize()
+        for (_, _, outs, _), w in zip(jobs, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs, w))
+    del graphs
