@@ -12,8 +12,8 @@
 // One pass over rows and codes, bound by memory where there are many (98816 f32
 // rows of 8 heads of 128 written 199 us, 4.6 TB/s; 10391 written 31, read back
 // 18.4, 3.1 and 5.3 TB/s; 50000 of one sequence read as bf16 33 us), by the launch
-// and one row's chain of reductions where there are few (32 rows written 5.3,
-// read 3.9).
+// and one row's chain of reductions where there are few (32 rows of 8 heads of 128,
+// from a graph, written 4.0, read 3.0).
 #include <math.h>
 
 #include "kvcache_rows.h"
@@ -26,6 +26,19 @@ namespace qbk {
 #define KV4_TOP 2688.0f
 
 __device__ __forceinline__ uint32_t kv4_most(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// The largest over aligned runs of eight lanes.
+__device__ __forceinline__ uint32_t kv4_max8(uint32_t v) {
+    v = kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));   // lane ^ 1
+    v = kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));   // lane ^ 2
+    return kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));  // 7 - lane
+}
+// Of that, over aligned runs of 32.
+__device__ __forceinline__ uint32_t kv4_max32(uint32_t v) {
+    v = kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));  // row_ror 8
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return kv4_most(a[0], a[1]);
+}
 
 // What a row's values are multiplied by: per = 1 / A, 0 for a row that holds a
 // NaN or an infinity (then nothing is kept but the scale, NaN).
@@ -88,13 +101,9 @@ __global__ void __launch_bounds__(256) kv4_write(KvRows a, const T *k, const T *
                 x[p][e] = c < hd ? kv_in<T>(src[c]) : 0.0f;
                 group[p] = kv4_most(group[p], __float_as_uint(x[p][e]) & 0x7fffffffu);
             }
-#pragma unroll
-            for (int o = 1; o <= 4; o <<= 1) group[p] = kv4_most(group[p], (uint32_t)__shfl_xor((int)group[p], o, 64));
+            group[p] = kv4_max8(group[p]);
         }
-        uint32_t top = kv4_most(group[0], group[1]);
-#pragma unroll
-        for (int o = 8; o <= 16; o <<= 1) top = kv4_most(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        const Kv4Row row(top);
+        const Kv4Row row(kv4_max32(kv4_most(group[0], group[1])));
 #pragma unroll
         for (int p = 0; p < 2; p++) {
             const uint32_t c = c0 + 128 * p;
@@ -190,12 +199,6 @@ __device__ __forceinline__ void kv4_turn(const uint32_t (&in)[4], uint32_t (&out
     kv_transpose4(b, t);
 #pragma unroll
     for (int i = 0; i < 4; i++) out[i] = kv4_nibbles(t[i]);
-}
-// The largest over aligned runs of eight lanes.
-__device__ __forceinline__ uint32_t kv4_max8(uint32_t v) {
-    v = kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));   // lane ^ 1
-    v = kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));   // lane ^ 2
-    return kv4_most(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));  // 7 - lane
 }
 // Bits of the codes of rows 4 k .. 4 k + 3 that lie in lo .. hi - 1.
 __device__ __forceinline__ uint32_t kv4_rows_in(uint32_t row, uint32_t lo, uint32_t hi) {
