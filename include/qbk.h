@@ -577,9 +577,10 @@ int qbk_block_decode_kv_dev(qbk_ctx *ctx, qbk_block *block, float *h, const uint
  * request's last token and its drafts, whose logits qbk_verify_drafts_dev takes.
  * h f32 [n][tokens][d_model]; token t of sequence first_seq + i stands at own
  * position pos[i] + t and sees the rows up to its own.  max_len: a host bound on
- * pos[i] + tokens, at most the cache's capacity; tokens at positions past it have
- * no meaning, and those before them in the same step neither.  Advancing pos by
- * fewer than `tokens` takes the rest back: later rows are written over theirs. */
+ * the rows, at most the cache's capacity; what tokens at positions from it on
+ * yield has no meaning, those before them in the same step are as any.  Advancing
+ * pos by fewer than `tokens` takes the rest back: later rows are written over
+ * theirs. */
 size_t qbk_block_decode_kv_tokens_workspace_size(const qbk_block *block, const qbk_kv_shape *shape, size_t n,
                                                  size_t tokens, size_t max_len, size_t prefix_len);
 int qbk_block_decode_kv_tokens_dev(qbk_ctx *ctx, qbk_block *block, float *h, const uint32_t *pos, size_t n,

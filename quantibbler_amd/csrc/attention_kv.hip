@@ -1111,13 +1111,15 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
     if (split * run >= tiles && split > 0) return;  // split 0 is there for a sequence with no rows
     constexpr uint32_t R = OWN == KVA_ROWS64 ? 64 : 16;
     const uint32_t per = a.sq * a.G, r0 = rt * R, n_rows = per - r0 < R ? per - r0 : R;
-    const uint32_t sq = a.sq;
+    const uint32_t sq = a.sq, l = a.lens[b], end = (l < a.max_len ? l : a.max_len) + a.plus;
     const KvaRow rows(a, r0);
-    auto limit = [&](uint32_t r) {  // own rows seen by row r of the body: len - sq + t + 1, none where that is negative
+    // own rows seen by row r of the body: end - sq + t + 1, none where that is negative; end is past len where a step's
+    // last tokens have no room, which does not move the others
+    auto limit = [&](uint32_t r) {
         uint32_t t, head;
         rows.at(r, t, head);
-        const uint32_t up = len + t + 1;
-        return up > sq ? up - sq : 0;
+        const uint32_t up = end + t + 1, seen = up > sq ? up - sq : 0;
+        return seen < len ? seen : len;
     };
     const uint32_t most = (kva_scalar(limit(n_rows - 1)) + 63) / 64;
     uint32_t t1 = split * run + run;
