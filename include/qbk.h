@@ -667,6 +667,17 @@ int qbk_verify_drafts_dev(qbk_ctx *ctx, const void *logits, const void *draft_lo
                           size_t vocab, size_t row_stride, size_t draft_row_stride, const int32_t *ids,
                           const uint32_t *n_drafts, const float *uniforms, const float *temperature, int32_t *tokens,
                           int32_t *counts, uint32_t *pos, void *workspace, size_t workspace_size, void *stream);
+/* The same where a request's rows end: pos[i] is that of its first token's row,
+ * and rows from pos_limit on (at most 2^32 - 1; past that none ends) are not
+ * there.  At most pos_limit - pos[i] - 1 of its drafts are looked at, as if
+ * n_drafts[i] were that, and a request whose pos[i] is at or past pos_limit emits
+ * nothing: tokens of -1, a count of 0.  So a captured step that is replayed never
+ * passes its cache's capacity. */
+int qbk_verify_drafts_within_dev(qbk_ctx *ctx, const void *logits, const void *draft_logits, int dtype, size_t n,
+                                 size_t k, size_t vocab, size_t row_stride, size_t draft_row_stride, const int32_t *ids,
+                                 const uint32_t *n_drafts, const float *uniforms, const float *temperature,
+                                 int32_t *tokens, int32_t *counts, uint32_t *pos, size_t pos_limit, void *workspace,
+                                 size_t workspace_size, void *stream);
 
 /* ---- log probabilities ------------------------------------------------------ */
 

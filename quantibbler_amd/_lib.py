@@ -143,6 +143,8 @@ _SIGS = {
                                   C.c_double, _P, _P, _Z, _Z, _P]),
     "qbk_verify_drafts_workspace_size": (_Z, [_Z, _Z, _Z, _I]),
     "qbk_verify_drafts_dev": (_I, [_P, _P, _P, _I, _Z, _Z, _Z, _Z, _Z, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "qbk_verify_drafts_within_dev": (_I, [_P, _P, _P, _I, _Z, _Z, _Z, _Z, _Z, _P, _P, _P, _P, _P, _P, _P, _Z, _P, _Z,
+                                          _P]),
     "qbk_logprobs_workspace_size": (_Z, [_Z, _Z, _Z]),
     "qbk_logprobs_dev": (_I, [_P, _P, _I, _Z, _Z, _Z, _P, _P, _P, _Z, _P, _P, _P, _Z, _P]),
     "qbk_sage_blk_workspace_size": (_Z, [C.POINTER(AttnShape)]),

@@ -9,7 +9,9 @@
 // at the first j that is not, or at j = n, one more token is drawn,
 //   with weights w = max(p_j - q_j, 0)  (all 0: p_j), at j = n w = p_n:
 //   the first v of w(v) > 0 with w(0) + .. + w(v) > u_n (w(0) + .. + w(last)).
-// What is emitted is then distributed as the target's own tokens are.
+// What is emitted is then distributed as the target's own tokens are.  Where a
+// request's rows end, it has no more drafts than rows behind its first token, and
+// without a row for that it emits nothing.
 //
 // Which v that is hangs on sums of a vocabulary's weights: off by 1e-7 of the
 // whole, as f32 leaves them, one draw in a hundred over 128256 ids of like
@@ -59,14 +61,23 @@ struct VfArgs {
     const uint32_t *n_drafts;
     int32_t *tokens, *counts;
     uint32_t *pos;
+    uint64_t limit;  // of the positions; 2^32: none
     VfPart *part;  // [request][row][unit], a request's rows: target's 0 .. k, drafts' 0 .. k - 1
     double *rest;  // [request][unit]
     VfEnd *end;    // [request]
     uint32_t n, k, rows, vocab, units;
 };
 
+// Rows that request i has left, and the drafts that are looked at.
+__device__ __forceinline__ uint64_t vf_room(const VfArgs &a, uint32_t i) {
+    if (a.limit >> 32) return a.limit;
+    const uint32_t at = a.pos[i];
+    return a.limit > at ? a.limit - at : 0;
+}
 __device__ __forceinline__ uint32_t vf_drafts(const VfArgs &a, uint32_t i) {
-    return a.n_drafts ? (a.n_drafts[i] < a.k ? a.n_drafts[i] : a.k) : a.k;
+    const uint32_t m = a.n_drafts ? (a.n_drafts[i] < a.k ? a.n_drafts[i] : a.k) : a.k;
+    const uint64_t room = vf_room(a, i);
+    return m < room ? m : room ? (uint32_t)room - 1 : 0;
 }
 // log2(e) / T, 0 for T = 0 (or less, or no number): the likeliest token.  A T
 // past 2^110 counts as that: what is -inf stays masked.
@@ -491,6 +502,10 @@ __global__ void __launch_bounds__(VF_THREADS) vf_choose(VfArgs a) {
         }
         token = (int32_t)(one != ~0u ? one : end - 1);
     }
+    if (!(a.limit >> 32)) {
+        if (vf_room(a, i) == 0) token = -1;  // e.row is 0
+        __syncthreads();                     // every wave has read the position
+    }
     const uint32_t got = e.row + (token >= 0 ? 1u : 0u);
     for (uint32_t j = tid; j <= a.k; j += VF_THREADS)
         a.tokens[(size_t)i * (a.k + 1) + j] = j < e.row ? a.ids[(size_t)i * a.k + j] : j == e.row ? token : -1;
@@ -556,6 +571,16 @@ int qbk_verify_drafts_dev(qbk_ctx *ctx, const void *logits, const void *draft_lo
                           size_t vocab, size_t row_stride, size_t draft_row_stride, const int32_t *ids,
                           const uint32_t *n_drafts, const float *uniforms, const float *temperature, int32_t *tokens,
                           int32_t *counts, uint32_t *pos, void *workspace, size_t workspace_size, void *stream) {
+    return qbk_verify_drafts_within_dev(ctx, logits, draft_logits, dtype, n, k, vocab, row_stride, draft_row_stride, ids,
+                                        n_drafts, uniforms, temperature, tokens, counts, pos, SIZE_MAX, workspace,
+                                        workspace_size, stream);
+}
+
+int qbk_verify_drafts_within_dev(qbk_ctx *ctx, const void *logits, const void *draft_logits, int dtype, size_t n,
+                                 size_t k, size_t vocab, size_t row_stride, size_t draft_row_stride, const int32_t *ids,
+                                 const uint32_t *n_drafts, const float *uniforms, const float *temperature,
+                                 int32_t *tokens, int32_t *counts, uint32_t *pos, size_t pos_limit, void *workspace,
+                                 size_t workspace_size, void *stream) {
     int rc;
     const bool given = draft_logits != nullptr;
     if ((rc = vf_check(n, k, vocab, given))) return rc;
@@ -568,6 +593,7 @@ int qbk_verify_drafts_dev(qbk_ctx *ctx, const void *logits, const void *draft_lo
                                             draft_row_stride, vocab));
     if (n == 0) return QBK_OK;
     if (!logits || !uniforms || !tokens || !counts || (k && !ids)) return fail(QBK_ERR_VALIDATION, "null argument");
+    if (pos_limit >> 32 == 0 && !pos) return fail(QBK_ERR_VALIDATION, "verify_drafts: a limit of positions without positions");
     const VfPlan p = vf_plan(n, k, vocab, given);
     if (!workspace || workspace_size < p.bytes)
         return fail(QBK_ERR_VALIDATION, fmt("verify_drafts workspace of %zu bytes is smaller than the %zu needed",
@@ -586,6 +612,7 @@ int qbk_verify_drafts_dev(qbk_ctx *ctx, const void *logits, const void *draft_lo
     a.tokens = tokens;
     a.counts = counts;
     a.pos = pos;
+    a.limit = pos_limit >> 32 ? 1ull << 32 : pos_limit;
     a.part = (VfPart *)workspace;
     a.rest = (double *)((char *)workspace + p.o_rest);
     a.end = (VfEnd *)((char *)workspace + p.o_end);

@@ -368,6 +368,9 @@ def logprobs_dev(ctx: GpuContext, logits, rows: int, vocab: int, targets, logpro
         _device_bytes(workspace, workspace_size, ctx, "logprobs: workspace"), int(workspace_size), _stream(stream)))
 
 
+_NO_LIMIT = 1 << 32
+
+
 def verify_drafts_workspace_size(n: int, drafts: int, vocab: int, draft_logits: bool = False) -> int:
     """Bytes of workspace ``verify_drafts_dev`` needs."""
     if min(int(n), int(drafts), int(vocab)) < 0:
@@ -378,7 +381,7 @@ def verify_drafts_workspace_size(n: int, drafts: int, vocab: int, draft_logits: 
 def verify_drafts_dev(ctx: GpuContext, logits, n: int, drafts: int, vocab: int, ids, uniforms, tokens, counts,
                       workspace, workspace_size: int, draft_logits=None, n_drafts=None, temperature=None, pos=None,
                       dtype: str = "float32", row_stride: int | None = None, draft_row_stride: int | None = None,
-                      stream=None):
+                      stream=None, pos_limit: int | None = None):
     """Drafted tokens against the target's probabilities, for n requests of up
     to ``drafts`` (64) each: keeps a request's drafts ``ids`` [n][drafts] (device
     int32) while uniforms[i][j] q_j(draft) < p_j(draft) and draws one more token,
@@ -393,27 +396,30 @@ def verify_drafts_dev(ctx: GpuContext, logits, n: int, drafts: int, vocab: int, 
     ``temperature`` device f32 a request (None: 1; 0: the likeliest id).
     ``tokens`` [n][drafts + 1] int32 gets the kept drafts, the drawn token and -1
     behind, ``counts`` [n] how many there are, and ``pos``, where given, is
-    advanced by as many.  drafts = 0 draws a token a request."""
+    advanced by as many.  drafts = 0 draws a token a request.  With ``pos_limit``
+    (a cache's capacity) a request at pos[i] has at most pos_limit - pos[i] - 1
+    drafts, and one at the limit emits nothing (a count of 0)."""
     code = _SERVING_DTYPES.get(dtype)
     if code is None:
         raise _lib.KernelError(f"verify_drafts takes 'float32' or 'bfloat16' logits, got {dtype!r}")
     n, k, vocab = int(n), int(drafts), int(vocab)
     stride = vocab if row_stride is None else int(row_stride)
     dstride = vocab if draft_row_stride is None else int(draft_row_stride)
-    if min(n, k, vocab, stride, dstride) < 0:
+    limit = _NO_LIMIT if pos_limit is None else int(pos_limit)
+    if min(n, k, vocab, stride, dstride, limit) < 0:
         raise _lib.KernelError("verify_drafts sizes must not be negative")
     rows, drows = n * (k + 1), n * k
     x = _device_values(logits, dtype, (rows - 1) * stride + vocab if rows else 0, ctx, "verify_drafts: logits",
                        row_stride is not None)
     y = _device_values(draft_logits, dtype, (drows - 1) * dstride + vocab if drows else 0, ctx,
                        "verify_drafts: draft_logits", draft_row_stride is not None)
-    check(_lib.load().qbk_verify_drafts_dev(
+    check(_lib.load().qbk_verify_drafts_within_dev(
         ctx.handle, x, y, code, n, k, vocab, stride, dstride, _device_words(ids, drows, ctx, "ids"),
         _device_words(n_drafts, n, ctx, "n_drafts"), _device_values(uniforms, "float32", rows, ctx,
                                                                     "verify_drafts: uniforms"),
         _device_values(temperature, "float32", n, ctx, "verify_drafts: temperature"),
         _device_words(tokens, rows, ctx, "tokens"), _device_words(counts, n, ctx, "counts"),
-        _device_words(pos, n, ctx, "positions"),
+        _device_words(pos, n, ctx, "positions"), limit,
         _device_bytes(workspace, workspace_size, ctx, "verify_drafts: workspace"), int(workspace_size),
         _stream(stream)))
 

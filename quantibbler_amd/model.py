@@ -459,7 +459,8 @@ class DeviceModel:
                 caches.append(cache(seqs, int(capacity)))
             need = max(b.decode_kv_workspace_size(c, seqs, prefix_len=n) for b, c in zip(self.blocks, caches))
             self._shared = {"n": seqs, "prefix": prefixes, "len": n, "own": caches, "pos": pos, "steps": 0,
-                            "bound": False, "drafts": {},  # steps: rows a request holds, or a bound; drafts: by tokens
+                            # steps: rows a request holds, or a bound; replayed: or not even that; drafts: by tokens
+                            "bound": False, "replayed": False, "drafts": {},
                             "h": torch.empty((seqs, d), dtype=torch.float32, device="cuda"),
                             "hn": torch.empty((seqs, d), dtype=torch.float32, device="cuda"),
                             "logits": torch.empty((seqs, md.vocab_size), dtype=torch.float32, device="cuda"),
@@ -470,8 +471,9 @@ class DeviceModel:
         """The next position of every request of share_prefix(): ``tokens`` as
         step_batch's, one a request.  Returns the logits [n][vocab] (a device
         tensor, overwritten by the next call).  A captured step serves this
-        shared prefix alone and counts once towards the requests' capacity,
-        however often it is replayed; replays past it write no rows."""
+        shared prefix alone; replays past the requests' capacity write no rows,
+        and the calls that are made behind a capture look up what requests hold
+        (a synchronization each)."""
         from .gpu import advance_positions_dev, embed, embed_dev, rms_norm_dev
 
         md, s = self.md, self._shared
@@ -481,7 +483,7 @@ class DeviceModel:
         n = int(tokens.numel()) if dev_ids else len(tokens)
         if n != s["n"]:
             raise ValueError(f"{n} tokens for {s['n']} requests")
-        self._room(1, stream)
+        captured = self._room(1, stream)
         if dev_ids:
             embed_dev(self.ctx, self.embedding, md.vocab_size, md.d_model, tokens, n, s["h"], stream)
         else:
@@ -493,25 +495,29 @@ class DeviceModel:
         rms_norm_dev(self.ctx, s["h"], n, md.d_model, self.final_norm, md.rms_norm_eps, s["hn"], stream)
         self.head.logits_dev(s["hn"], n, s["logits"], stream)
         s["steps"] += 1
+        s["replayed"] |= captured
         return s["logits"]
 
     def _room(self, rows: int, stream):
         """Refuses a step of so many rows a request that its cache has no room
-        for.  What requests hold is known here as a bound, since the device
-        counts the drafts that it keeps; the count is fetched where the bound
-        does not do."""
+        for; returns whether the step is being captured.  What requests hold is
+        known here as a bound, since the device counts the drafts that it keeps
+        and replays are not seen: the count is fetched where the bound does not
+        do."""
         import torch
 
         s = self._shared
         capacity = s["own"][0].capacity
-        if s["steps"] + rows > capacity and s["bound"]:
-            with _memory_of(stream):
-                if not torch.cuda.is_current_stream_capturing():
+        with _memory_of(stream):
+            capturing = torch.cuda.is_current_stream_capturing()
+            if s["replayed"] or (s["bound"] and s["steps"] + rows > capacity):
+                if not capturing:
                     torch.cuda.synchronize()
                     s["steps"], s["bound"] = int(s["pos"].max()), False
         if s["steps"] + rows > capacity:
             raise ValueError(f"the requests hold their {s['steps']} rows already" if rows == 1 else
                              f"no room for {rows} rows behind {s['steps']} of a capacity of {capacity}")
+        return capturing
 
     def verify_shared(self, tokens, uniforms, draft_logits=None, n_drafts=None, temperature=None, stream=None):
         """Drafted tokens of every request of share_prefix() in one step:
@@ -524,8 +530,10 @@ class DeviceModel:
         next call of the same k: the emitted tokens [n][k + 1], -1 behind the
         last, and how many there are, by which the requests' positions advance;
         a request's next step begins with its last emitted token.  k = 0 draws a
-        token a request.  As a captured step_shared, a captured call counts once
-        towards the capacity."""
+        token a request.  A captured call's replays keep to the capacity: a request
+        takes as many drafts as it has rows for, and emits nothing (a count of 0)
+        where it has none; the calls that are made behind a capture look up what
+        requests hold (a synchronization each)."""
         import torch
 
         from .gpu import embed_dev, rms_norm_dev, verify_drafts_dev, verify_drafts_workspace_size
@@ -542,7 +550,7 @@ class DeviceModel:
             if n * per > 64:
                 raise ValueError(f"{n} requests of {per} tokens are more than the 64 rows of a step")
             k, rows, d = per - 1, n * per, md.d_model
-            self._room(per, stream)
+            captured = self._room(per, stream)
             if per not in s["drafts"]:
                 need = max(b.decode_kv_workspace_size(c, n, prefix_len=s["len"], n_tokens=per)
                            for b, c in zip(self.blocks, s["own"]))
@@ -564,9 +572,11 @@ class DeviceModel:
             self.head.logits_dev(b["hn"], rows, b["logits"], stream)
             verify_drafts_dev(self.ctx, b["logits"], n, k, md.vocab_size, ids, uniforms, b["tokens"], b["counts"],
                               b["vws"], b["vneed"], draft_logits=draft_logits, n_drafts=n_drafts,
-                              temperature=temperature, pos=s["pos"], stream=stream)
+                              temperature=temperature, pos=s["pos"], stream=stream,
+                              pos_limit=s["own"][0].capacity)
         s["steps"] += per
         s["bound"] = True
+        s["replayed"] |= captured
         return b["tokens"], b["counts"]
 
     def step(self, token: int, stream=None):

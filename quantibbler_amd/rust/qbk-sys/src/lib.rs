@@ -286,6 +286,12 @@ extern "C" {
                                  ids: *const i32, n_drafts: *const u32, uniforms: *const f32,
                                  temperature: *const f32, tokens: *mut i32, counts: *mut i32, pos: *mut u32,
                                  workspace: *mut c_void, workspace_size: usize, stream: *mut c_void) -> c_int;
+    pub fn qbk_verify_drafts_within_dev(ctx: *mut QbkCtx, logits: *const c_void, draft_logits: *const c_void,
+                                        dtype: c_int, n: usize, k: usize, vocab: usize, row_stride: usize,
+                                        draft_row_stride: usize, ids: *const i32, n_drafts: *const u32,
+                                        uniforms: *const f32, temperature: *const f32, tokens: *mut i32,
+                                        counts: *mut i32, pos: *mut u32, pos_limit: usize, workspace: *mut c_void,
+                                        workspace_size: usize, stream: *mut c_void) -> c_int;
     pub fn qbk_logprobs_workspace_size(rows: usize, vocab: usize, top_k: usize) -> usize;
     pub fn qbk_logprobs_dev(ctx: *mut QbkCtx, logits: *const c_void, dtype: c_int, rows: usize, vocab: usize,
                             row_stride: usize, targets: *const i32, logprobs: *mut f32, entropy: *mut f32,

@@ -1,4 +1,5 @@
-"""GPU: drafted tokens where a request's rows end."""
+"""GPU: drafted tokens where a request's rows end: a step that passes the capacity,
+verification within a limit, replays that reach it."""
 import numpy as np
 import pytest
 
@@ -7,6 +8,7 @@ torch = pytest.importorskip("torch")
 
 import test_gpu_attention_kv as att
 import test_gpu_block_kv as bkv
+import test_gpu_verify as ver
 from quantibbler_amd import DecoderBlock, GpuContext
 
 words, EPS = att.words, 2.0 ** -24
@@ -51,3 +53,81 @@ def test_tokens_that_fit_before_those_that_do_not(ctx, orc, fmt, per, plen, lens
             off = np.abs(got[i, t] - want) - bound - 2 * EPS * np.abs(want)
             assert (off <= 0).all(), f"sequence {i}, token {t}: past its bound by {off.max()}"
     block.close()
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("n_drafts", [False, True])
+def test_verification_within_a_limit(ctx, given, n_drafts):
+    """A request's drafts end where its rows do, whichever end comes first; without a row it emits nothing and stays."""
+    n, k, vocab, limit = 12, 6, 5003, 100
+    at = [0, 93, 94, 95, 97, 98, 99, 100, 101, 2 ** 31 - 1, -1, 50]  # -1: 2^32 - 1
+    have = [6, 5, 6, 9, 1, 6, 0, 6, 2, 6, 6, 3] if n_drafts else [k] * n
+    x, y, ids, u = ver.make(3, n, k, vocab, "float32", given)
+    u[::2] *= 0.05
+    heat = np.where(np.arange(n) % 3 == 1, 0.0, 0.8).astype(np.float32)
+    pos = words(at)
+    tokens, counts = ver.verify(ctx, x, y, ids, u, words(have) if n_drafts else None, ver.tensor(heat), pos=pos,
+                                pos_limit=limit)
+    live = [i for i in range(n) if 0 <= at[i] < limit]
+    some = [min(have[i], limit - 1 - at[i]) for i in live]
+    ver.check(tokens[live], counts[live], x[live], None if y is None else y[live], ids[live], u[live], some, heat[live])
+    for i in set(range(n)) - set(live):
+        assert tokens[i].tolist() == [-1] * (k + 1) and int(counts[i]) == 0
+    assert pos.tolist() == [a + c for a, c in zip(at, counts.tolist())]
+    # from 2^32 on, no limit
+    pos = words(at)
+    free = ver.verify(ctx, x, y, ids, u, words(have) if n_drafts else None, ver.tensor(heat), pos=pos, pos_limit=1 << 32)
+    ver.check(*free, x, y, ids, u, have, heat)
+
+
+def model(ctx, orc, capacity):
+    from test_gpu_trunk import synthetic_model
+
+    from quantibbler_amd.model import DeviceModel
+
+    return DeviceModel(ctx, synthetic_model(orc, 808), capacity=capacity)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp4"])
+def test_replays_up_to_the_capacity(ctx, orc, fmt):
+    """A captured verification replayed until its requests are full: drafts are taken as far as there is room, the drawn
+    token follows the last row, and a request without room emits nothing and stays where it is; an eager call is then
+    refused with the rows that are held."""
+    m = model(ctx, orc, 60)
+    vocab, n, k, cap = m.md.vocab_size, 4, 3, 17
+    rng = np.random.default_rng(3)
+    m.share_prefix(rng.integers(0, vocab, 33).tolist(), n, cap, fmt=fmt)
+    tokens, u = torch.zeros((n, k + 1), dtype=torch.int32, device="cuda"), torch.zeros((n, k + 1), device="cuda")
+    heat = torch.tensor([0.8, 0.0, 1.5, 1.0], device="cuda")
+    counts_in = words([k, 1, 2, k])
+    m.verify_shared(tokens, u, n_drafts=counts_in, temperature=heat)
+    torch.cuda.synchronize()
+    m._shared["pos"].copy_(words([0, 3, 1, 2]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, counts = m.verify_shared(tokens, u, n_drafts=counts_in, temperature=heat, stream=torch.cuda.current_stream())
+    logits = m._shared["drafts"][k + 1]["logits"].view(n, k + 1, vocab)
+    full = 0
+    for rep in range(24):
+        before = m._shared["pos"].tolist()
+        tokens.copy_(words(rng.integers(0, vocab, n * (k + 1))).view(n, k + 1))
+        u.copy_(torch.from_numpy((0.02 * rng.random((n, k + 1))).astype(np.float32)))
+        graph.replay()
+        torch.cuda.synchronize()
+        room = [cap - b for b in before]
+        most = [max(0, min(c, r - 1)) for c, r in zip([k, 1, 2, k], room)]
+        live = [i for i in range(n) if room[i] > 0]
+        ver.check(out[live], counts[live], logits[live], None, tokens[live, 1:], u[live], [most[i] for i in live],
+                  heat[live], f"replay {rep}")
+        for i in range(n):
+            if room[i] <= 0:
+                full += 1
+                assert out[i].tolist() == [-1] * (k + 1) and int(counts[i]) == 0
+        after = m._shared["pos"].tolist()
+        assert after == [b + c for b, c in zip(before, counts.tolist())] and max(after) <= cap
+    assert full and max(after) == cap
+    for call in (lambda: m.verify_shared(tokens, u), lambda: m.step_shared([1] * n)):
+        with pytest.raises(ValueError, match="no room for 4 rows behind 17 of|hold their 17 rows already"):
+            call()
+    del graph
+    m.close()
