@@ -503,7 +503,8 @@ class DeviceModel:
         for; returns whether the step is being captured.  What requests hold is
         known here as a bound, since the device counts the drafts that it keeps
         and replays are not seen: the count is fetched where the bound does not
-        do."""
+        do.  A capture fetches nothing; what its replays have no room for is the
+        device's to leave out."""
         import torch
 
         s = self._shared
@@ -511,9 +512,10 @@ class DeviceModel:
         with _memory_of(stream):
             capturing = torch.cuda.is_current_stream_capturing()
             if s["replayed"] or (s["bound"] and s["steps"] + rows > capacity):
-                if not capturing:
-                    torch.cuda.synchronize()
-                    s["steps"], s["bound"] = int(s["pos"].max()), False
+                if capturing:
+                    return True
+                torch.cuda.synchronize()
+                s["steps"], s["bound"] = int(s["pos"].max()), False
         if s["steps"] + rows > capacity:
             raise ValueError(f"the requests hold their {s['steps']} rows already" if rows == 1 else
                              f"no room for {rows} rows behind {s['steps']} of a capacity of {capacity}")

@@ -1,5 +1,6 @@
 """GPU: drafted tokens where a request's rows end: a step that passes the capacity,
-verification within a limit, replays that reach it."""
+verification within a limit, replays that reach it, captures after rejected
+drafts."""
 import numpy as np
 import pytest
 
@@ -129,5 +130,35 @@ def test_replays_up_to_the_capacity(ctx, orc, fmt):
     for call in (lambda: m.verify_shared(tokens, u), lambda: m.step_shared([1] * n)):
         with pytest.raises(ValueError, match="no room for 4 rows behind 17 of|hold their 17 rows already"):
             call()
+    del graph
+    m.close()
+
+
+def test_captures_after_drafts_that_were_not_kept(ctx, orc):
+    """What eager calls did not keep is no reason to refuse a capture, which fetches nothing; one whose requests are
+    known to be full is refused."""
+    m = model(ctx, orc, 40)
+    n, k, cap = 2, 3, 12
+    m.share_prefix([1, 2, 3, 4, 5], n, cap, fmt="fp4")
+    u, cold = torch.full((n, k + 1), 0.5, device="cuda"), torch.zeros(n, device="cuda")
+    wrong = words([3, -1, -1, -1, 4, -1, -1, -1]).view(n, k + 1)
+    for _ in range(3):
+        _, counts = m.verify_shared(wrong, u, temperature=cold)  # an id of -1 is never kept: one row a call
+    assert m._shared["pos"].tolist() == [3, 3]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out, counts = m.verify_shared(wrong, u, temperature=cold, stream=torch.cuda.current_stream())
+    for at in range(4, 15):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert m._shared["pos"].tolist() == [min(at, cap)] * n and counts.tolist() == [int(at <= cap)] * n
+    with pytest.raises(ValueError, match="hold their 12 rows already"):
+        m.step_shared([1, 2])
+    m.share_prefix([1, 2, 3, 4, 5], n, 6, fmt="fp4")  # steps count what they hold exactly
+    for _ in range(5):
+        m.step_shared([1, 2])
+    with pytest.raises(ValueError, match="no room for 4 rows behind 5 of a capacity of 6"):
+        m.verify_shared(wrong, u, temperature=cold)
     del graph
     m.close()
