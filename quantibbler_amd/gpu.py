@@ -399,6 +399,16 @@ def verify_drafts_dev(ctx: GpuContext, logits, n: int, drafts: int, vocab: int, 
     advanced by as many.  drafts = 0 draws a token a request.  With ``pos_limit``
     (a cache's capacity) a request at pos[i] has at most pos_limit - pos[i] - 1
     drafts, and one at the limit emits nothing (a count of 0)."""
+    check(_lib.load().qbk_verify_drafts_within_dev(*_verify_drafts_args(
+        ctx, logits, n, drafts, vocab, ids, uniforms, tokens, counts, workspace, workspace_size, draft_logits, n_drafts,
+        temperature, pos, dtype, row_stride, draft_row_stride, stream, pos_limit)))
+
+
+def _verify_drafts_args(ctx, logits, n, drafts, vocab, ids, uniforms, tokens, counts, workspace, workspace_size,
+                        draft_logits=None, n_drafts=None, temperature=None, pos=None, dtype="float32", row_stride=None,
+                        draft_row_stride=None, stream=None, pos_limit=None):
+    """verify_drafts_dev's tensors looked at, as the library's arguments (addresses: the tensors are the caller's to
+    keep)."""
     code = _SERVING_DTYPES.get(dtype)
     if code is None:
         raise _lib.KernelError(f"verify_drafts takes 'float32' or 'bfloat16' logits, got {dtype!r}")
@@ -413,7 +423,7 @@ def verify_drafts_dev(ctx: GpuContext, logits, n: int, drafts: int, vocab: int, 
                        row_stride is not None)
     y = _device_values(draft_logits, dtype, (drows - 1) * dstride + vocab if drows else 0, ctx,
                        "verify_drafts: draft_logits", draft_row_stride is not None)
-    check(_lib.load().qbk_verify_drafts_within_dev(
+    return (
         ctx.handle, x, y, code, n, k, vocab, stride, dstride, _device_words(ids, drows, ctx, "ids"),
         _device_words(n_drafts, n, ctx, "n_drafts"), _device_values(uniforms, "float32", rows, ctx,
                                                                     "verify_drafts: uniforms"),
@@ -421,7 +431,7 @@ def verify_drafts_dev(ctx: GpuContext, logits, n: int, drafts: int, vocab: int, 
         _device_words(tokens, rows, ctx, "tokens"), _device_words(counts, n, ctx, "counts"),
         _device_words(pos, n, ctx, "positions"), limit,
         _device_bytes(workspace, workspace_size, ctx, "verify_drafts: workspace"), int(workspace_size),
-        _stream(stream)))
+        _stream(stream))
 
 
 class Rope:

@@ -538,7 +538,8 @@ class DeviceModel:
         requests hold (a synchronization each)."""
         import torch
 
-        from .gpu import embed_dev, rms_norm_dev, verify_drafts_dev, verify_drafts_workspace_size
+        from ._lib import check, load
+        from .gpu import _verify_drafts_args, embed_dev, rms_norm_dev, verify_drafts_workspace_size
 
         md, s = self.md, self._shared
         if s is None:
@@ -552,6 +553,8 @@ class DeviceModel:
             if n * per > 64:
                 raise ValueError(f"{n} requests of {per} tokens are more than the 64 rows of a step")
             k, rows, d = per - 1, n * per, md.d_model
+            if uniforms is None or (draft_logits is not None and k == 0):
+                raise ValueError("verify_shared needs uniforms" if uniforms is None else "draft logits without drafts")
             captured = self._room(per, stream)
             if per not in s["drafts"]:
                 need = max(b.decode_kv_workspace_size(c, n, prefix_len=s["len"], n_tokens=per)
@@ -566,16 +569,18 @@ class DeviceModel:
                                     "vws": torch.empty(vneed, dtype=torch.uint8, device="cuda"), "vneed": vneed}
             b = s["drafts"][per]
             ids = tokens[:, 1:].contiguous()
+            # looked at before a block has written a row
+            verify = _verify_drafts_args(self.ctx, b["logits"], n, k, md.vocab_size, ids, uniforms, b["tokens"],
+                                         b["counts"], b["vws"], b["vneed"], draft_logits=draft_logits,
+                                         n_drafts=n_drafts, temperature=temperature, pos=s["pos"], stream=stream,
+                                         pos_limit=s["own"][0].capacity)
             embed_dev(self.ctx, self.embedding, md.vocab_size, d, tokens, rows, b["h"], stream)
             for block, own, prefix in zip(self.blocks, s["own"], s["prefix"]):
                 block.decode_kv_dev(b["h"], s["pos"], n, own, b["ws"], b["need"], prefix=prefix, prefix_len=s["len"],
                                     stream=stream, n_tokens=per)
             rms_norm_dev(self.ctx, b["h"], rows, d, self.final_norm, md.rms_norm_eps, b["hn"], stream)
             self.head.logits_dev(b["hn"], rows, b["logits"], stream)
-            verify_drafts_dev(self.ctx, b["logits"], n, k, md.vocab_size, ids, uniforms, b["tokens"], b["counts"],
-                              b["vws"], b["vneed"], draft_logits=draft_logits, n_drafts=n_drafts,
-                              temperature=temperature, pos=s["pos"], stream=stream,
-                              pos_limit=s["own"][0].capacity)
+            check(load().qbk_verify_drafts_within_dev(*verify))
         s["steps"] += per
         s["bound"] = True
         s["replayed"] |= captured

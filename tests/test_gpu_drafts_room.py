@@ -162,3 +162,28 @@ def test_captures_after_drafts_that_were_not_kept(ctx, orc):
         m.verify_shared(wrong, u, temperature=cold)
     del graph
     m.close()
+
+
+def test_what_is_refused_runs_nothing(ctx, orc):
+    """Tensors that do not fit are refused before a block has written a row."""
+    m = model(ctx, orc, 40)
+    n, k, vocab = 2, 2, m.md.vocab_size
+    m.share_prefix([1, 2, 3], n, 20, fmt="fp4")
+    rows, u = [[1, 2, 3], [4, 5, 6]], torch.zeros((n, k + 1), device="cuda")
+    m.verify_shared(rows, u)
+    torch.cuda.synchronize()
+    before, steps = [c.buffer.clone() for c in m._shared["own"]], m._shared["steps"]
+    for kw in (dict(uniforms=u[:1]), dict(uniforms=u.double()), dict(uniforms=u.cpu()),
+               dict(draft_logits=torch.zeros((n, k, vocab - 1), device="cuda")),
+               dict(draft_logits=torch.zeros((n, k, vocab), dtype=torch.bfloat16, device="cuda")),
+               dict(n_drafts=torch.zeros(n, dtype=torch.int64, device="cuda")), dict(n_drafts=words([1])),
+               dict(temperature=torch.zeros(1, device="cuda")), dict(temperature=[1.0, 1.0]),
+               dict(tokens=torch.zeros((n, k + 1), dtype=torch.int64, device="cuda")),
+               dict(tokens=words(range(12)).view(n, 6)[:, ::2]), dict(uniforms=None),
+               dict(tokens=[[1], [2]], draft_logits=torch.zeros((n, 1, vocab), device="cuda"))):
+        with pytest.raises(ValueError):
+            m.verify_shared(**{"tokens": rows, "uniforms": u, **kw})
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c.buffer) for a, c in zip(before, m._shared["own"])), f"{sorted(kw)}"
+        assert m._shared["steps"] == steps
+    m.close()
