@@ -656,10 +656,14 @@ int qbk_rotate_heads_dev(qbk_ctx *ctx, const qbk_rope *rope, const void *q, cons
  * [n][k + 1] gets the drafts that were kept, the drawn one and -1 behind; counts
  * [n] how many that are; pos (may be NULL, device uint32) is advanced by it.  So
  * what is emitted is distributed as tokens drawn from p one by one; k = 0 draws
- * one token a request.  A draft outside the vocabulary is not kept; a target row
- * with a NaN or +inf or nothing above -inf ends its request without a drawn token
- * (-1, not counted), such a row of draft logits keeps no draft and draws from p.
- * Exponentials and sums are 64-bit.  workspace of at least
+ * one token a request.  A draft outside the vocabulary is not kept.  At a
+ * temperature above 0 a target row with a NaN or +inf or nothing above -inf ends
+ * its request without a drawn token (-1, not counted), and such a row of draft
+ * logits keeps no draft and draws from p.  At one that is not, a target row is
+ * what qbk_argmax_dev makes of it, whatever it holds: a NaN is passed over, +inf
+ * is the likeliest, and a row with nothing above -inf is id 0, kept where it was
+ * drafted, emitted and counted (a caller whose masks can leave nothing looks for
+ * that itself, as with qbk_argmax_dev).  Exponentials and sums are 64-bit.  workspace of at least
  * qbk_verify_drafts_workspace_size bytes (draft_logits: whether there are any),
  * 16-byte aligned. */
 size_t qbk_verify_drafts_workspace_size(size_t n, size_t k, size_t vocab, int draft_logits);

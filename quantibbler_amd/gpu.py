@@ -393,7 +393,9 @@ def verify_drafts_dev(ctx: GpuContext, logits, n: int, drafts: int, vocab: int, 
     "bfloat16"), rows ``row_stride`` / ``draft_row_stride`` values apart;
     ``uniforms`` [n][drafts + 1] f32 in [0, 1), of which a request's number
     n_drafts[i] draws; ``n_drafts`` device words (None: all have ``drafts``);
-    ``temperature`` device f32 a request (None: 1; 0: the likeliest id).
+    ``temperature`` device f32 a request (None: 1; 0: the likeliest id, which
+    is argmax_dev's whatever a row holds, 0 where a mask leaves nothing; above 0
+    a row without a distribution ends its request without a token).
     ``tokens`` [n][drafts + 1] int32 gets the kept drafts, the drawn token and -1
     behind, ``counts`` [n] how many there are, and ``pos``, where given, is
     advanced by as many.  drafts = 0 draws a token a request.  With ``pos_limit``
