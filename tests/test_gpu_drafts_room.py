@@ -1,6 +1,6 @@
 """GPU: drafted tokens where a request's rows end: a step that passes the capacity,
 verification within a limit, replays that reach it, captures after rejected
-drafts."""
+drafts, numbers of drafts of a request's own."""
 import numpy as np
 import pytest
 
@@ -162,6 +162,47 @@ def test_captures_after_drafts_that_were_not_kept(ctx, orc):
         m.verify_shared(wrong, u, temperature=cold)
     del graph
     m.close()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8", "fp4"])
+def test_numbers_of_drafts_of_a_requests_own(ctx, orc, fmt):
+    """Rows padded with -1, as the call's own output is: the same tokens, counts, logits and, in the steps after, rows as
+    with other ids there, which no request looks at; sampled and greedy, against the definition on the logits."""
+    rng = np.random.default_rng(9)
+    n, k, cap = 4, 3, 40
+    models = [model(ctx, orc, 80) for _ in range(2)]
+    vocab = models[0].md.vocab_size
+    prompt = rng.integers(0, vocab, 33).tolist()
+    for m in models:
+        m.share_prefix(prompt, n, cap, fmt=fmt)
+    heat = torch.tensor([0.9, 0.0, 1.3, 0.7], device="cuda")
+    for rep in range(5):
+        have = [[3, 0, 1, 2], [0, 0, 0, 0], [2, 3, 0, 1], [1, 1, 3, 3], [3, 2, 2, 0]][rep]
+        ids = rng.integers(0, vocab, (n, k + 1))
+        padded = ids.copy()
+        for i in range(n):
+            padded[i, 1 + have[i]:] = -1
+        u = torch.from_numpy(rng.random((n, k + 1)).astype(np.float32) * (0.05 if rep % 2 else 1.0)).cuda()
+        y = torch.randn((n, k, vocab), device="cuda") if rep in (2, 4) else None
+        got = []
+        for m, rows in zip(models, (ids, padded)):
+            tokens = words(rows.reshape(-1).tolist()).view(n, k + 1)
+            out = m.verify_shared(tokens, u, draft_logits=y, n_drafts=words(have), temperature=heat)
+            torch.cuda.synchronize()
+            logits = m._shared["drafts"][k + 1]["logits"].view(n, k + 1, vocab).clone()
+            got.append((out[0].clone(), out[1].clone(), logits, m._shared["pos"].clone()))
+        for a, b in zip(got[0], got[1]):
+            if a is got[0][2]:
+                assert all(torch.equal(a[i, :have[i] + 1], b[i, :have[i] + 1]) for i in range(n)), f"call {rep}"
+                assert all(bool(torch.isfinite(b[i, :have[i] + 1]).all()) for i in range(n))
+            else:
+                assert torch.equal(a, b), f"call {rep}"
+        out, counts, logits, _ = got[1]
+        ver.check(out, counts, logits, y, torch.from_numpy(ids[:, 1:].copy()), u, have, heat, f"call {rep}")
+        step = rng.integers(0, vocab, n).tolist()
+        assert torch.equal(models[0].step_shared(step), models[1].step_shared(step))
+    for m in models:
+        m.close()
 
 
 def test_what_is_refused_runs_nothing(ctx, orc):
