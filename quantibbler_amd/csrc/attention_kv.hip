@@ -76,12 +76,14 @@ struct KvAttArgs {
     float scale;                     // log2(e) / sqrt(hd)
 };
 
-// Own rows of sequence b that count, and the key tiles a split of them takes:
-// at least one a wave, so that short sequences use few splits.
-__device__ __forceinline__ uint32_t kva_len(const KvAttArgs &a, uint32_t b) {
+// Own rows of sequence b that count (end: as many as there would be, had its
+// last ones room), and the key tiles a split of them takes: at least one a wave,
+// so that short sequences use few splits.
+__device__ __forceinline__ uint32_t kva_end(const KvAttArgs &a, uint32_t b) {
     const uint32_t l = a.lens[b];
-    return l < a.max_len && a.plus < a.max_len - l ? l + a.plus : a.max_len;
+    return (l < a.max_len ? l : a.max_len) + a.plus;
 }
+__device__ __forceinline__ uint32_t kva_len(const KvAttArgs &a, uint32_t end) { return end < a.max_len ? end : a.max_len; }
 __device__ __forceinline__ uint32_t kva_run(const KvAttArgs &a, uint32_t len) {
     uint32_t rest;
     const uint32_t c = a.by_ss.split((len + 63) / 64 + a.ss - 1, rest);
@@ -468,13 +470,21 @@ struct KvaSlab {
     }
 };
 
+// A lane's scales of tile tt: of rows 16 i + 4 g .. 16 i + 4 g + 3.
+__device__ __forceinline__ void kva_scales(const float *of, uint32_t tt, int g, kva_f4_t (&s)[4]) {
+    const float *st = of + (size_t)tt * 64 + 4 * g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[i] = *(const kva_f4_t *)(st + 16 * i);
+}
+
 // A key tile's codes on their way to a wave, and its operands.
 template <int FMT, int DC>
 struct KvaTile {
     kva_u4_t kc[DC][4], vc[4 * DC];
-    __device__ __forceinline__ void load_k(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+    __device__ __forceinline__ void load_k(const KvaSlab &c, uint32_t tt, int hd, int col, int g, kva_f4_t (&ks)[4]) {
         const int nc = hd / 16;
         const uint8_t *kt = c.k + (size_t)tt * 64 * hd + col * 16;
+        kva_scales(c.ks, tt, g, ks);
 #pragma unroll
         for (int x = 0; x < DC; x++) {
             const int chunk = 4 * x + g < nc ? 4 * x + g : nc - 1;  // past the last chunk q is zero
@@ -482,9 +492,10 @@ struct KvaTile {
             for (int i = 0; i < 4; i++) kc[x][i] = *(const kva_u4_t *)(kt + (i * nc + chunk) * 256);
         }
     }
-    __device__ __forceinline__ void load_v(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+    __device__ __forceinline__ void load_v(const KvaSlab &c, uint32_t tt, int hd, int col, int g, kva_f4_t (&vs)[4]) {
         const int nc = hd / 16;
         const uint8_t *vt = c.v + (size_t)tt * 64 * hd + col * 64 + g * 16;
+        kva_scales(c.vs, tt, g, vs);
 #pragma unroll
         for (int ct = 0; ct < 4 * DC; ct++)
             vc[ct] = *(const kva_u4_t *)(vt + (ct < nc ? ct : nc - 1) * 1024);  // past the last tile: not stored
@@ -502,10 +513,11 @@ template <int DC>
 struct KvaTile<QBK_KV_FP4, DC> {
     kva_u4_t kc[DC][2], vc[2 * DC], vm[2 * DC];
     uint32_t km[DC];
-    __device__ __forceinline__ void load_k(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+    __device__ __forceinline__ void load_k(const KvaSlab &c, uint32_t tt, int hd, int col, int g, kva_f4_t (&ks)[4]) {
         const int nc = hd / 16, ng = (int)c.ng;
         const uint8_t *kt = c.k + (size_t)tt * 32 * hd + col * 16;
         const uint8_t *mt = c.km + (size_t)tt * 64 * ng + col * 4;
+        kva_scales(c.ks, tt, g, ks);
 #pragma unroll
         for (int x = 0; x < DC; x++) {
             const int chunk = 4 * x + g < nc ? 4 * x + g : nc - 1;  // past the last chunk q is zero
@@ -514,10 +526,11 @@ struct KvaTile<QBK_KV_FP4, DC> {
             for (int p = 0; p < 2; p++) kc[x][p] = *(const kva_u4_t *)(kt + (p * nc + chunk) * 256);
         }
     }
-    __device__ __forceinline__ void load_v(const KvaSlab &c, uint32_t tt, int hd, int col, int g) {
+    __device__ __forceinline__ void load_v(const KvaSlab &c, uint32_t tt, int hd, int col, int g, kva_f4_t (&vs)[4]) {
         const int ng = (int)c.ng;
         const uint8_t *vt = c.v + (size_t)tt * 1024 * ng + col * 64 + g * 16;
         const uint8_t *mt = c.vm + (size_t)tt * 64 * ng + g * 16;
+        kva_scales(c.vs, tt, g, vs);
 #pragma unroll
         for (int m = 0; m < 2 * DC; m++) {
             const int at = m < ng ? m : ng - 1;  // past the last tile: not stored
@@ -557,23 +570,14 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
     // A tile's codes and scales travel while the one before is worked on: keys
     // and their scales are asked for again as soon as the scores are formed,
     // values once they are added, the first of both before the queries are read.
-    // Codes before scales: in the other order the compiler holds four registers
-    // more, and heads of 64 lose one of three waves a SIMD (512 sequences of 500
-    // rows, fp8, f32 queries 41 / 52 us).
+    // The codes' address is formed before the scales are asked for, which come
+    // first all the same: formed behind them it takes four registers more, and
+    // heads of 64 lose one of three waves a SIMD (512 sequences of 500 rows, fp8,
+    // f32 queries 41 / 52 us); codes asked for first cost 2 to 3 % of most calls.
     KvaTile<FMT, DC> tile;
     kva_f4_t ks[4], vs[4];
-    auto load_k = [&](uint32_t tt) {
-        tile.load_k(slab, tt, hd, col, g);
-        const float *st = slab.ks + (size_t)tt * 64 + 4 * g;
-#pragma unroll
-        for (int i = 0; i < 4; i++) ks[i] = *(const kva_f4_t *)(st + 16 * i);
-    };
-    auto load_v = [&](uint32_t tt) {
-        tile.load_v(slab, tt, hd, col, g);
-        const float *st = slab.vs + (size_t)tt * 64 + 4 * g;
-#pragma unroll
-        for (int i = 0; i < 4; i++) vs[i] = *(const kva_f4_t *)(st + 16 * i);
-    };
+    auto load_k = [&](uint32_t tt) { tile.load_k(slab, tt, hd, col, g, ks); };
+    auto load_v = [&](uint32_t tt) { tile.load_v(slab, tt, hd, col, g, vs); };
     const uint32_t first = tile0 + wave;
     if (first < tile1) {
         load_k(first);
@@ -1110,11 +1114,11 @@ __global__ void __launch_bounds__(64 * KVA_WAVES, DC < 4 ? 2 : 1) kva_items(KvAt
     const uint32_t item = blockIdx.x - a.n_pre;
     uint32_t hk, rt, b;
     const uint32_t split = a.by_n.split(a.by_rts.split(a.by_hk.split(item, hk), rt), b);
-    const uint32_t len = kva_len(a, b), tiles = (len + 63) / 64, run = kva_run(a, len);
+    const uint32_t end = kva_end(a, b), len = kva_len(a, end), tiles = (len + 63) / 64, run = kva_run(a, len);
     if (split * run >= tiles && split > 0) return;  // split 0 is there for a sequence with no rows
     constexpr uint32_t R = OWN == KVA_ROWS64 ? 64 : 16;
     const uint32_t per = a.sq * a.G, r0 = rt * R, n_rows = per - r0 < R ? per - r0 : R;
-    const uint32_t sq = a.sq, l = a.lens[b], end = (l < a.max_len ? l : a.max_len) + a.plus;
+    const uint32_t sq = a.sq;
     const KvaRow rows(a, r0);
     // own rows seen by row r of the body: end - sq + t + 1, none where that is negative; end is past len where a step's
     // last tokens have no room, which does not move the others
@@ -1145,7 +1149,7 @@ __global__ void __launch_bounds__(256) kva_join(KvAttArgs a) {
     const uint32_t hk = a.by_rows.split(item, rho), query = a.by_g.split(rho, head);
     uint32_t splits = a.sp;
     if (a.ss) {
-        const uint32_t len = kva_len(a, a.by_sq.split(query, rest)), run = kva_run(a, len);
+        const uint32_t len = kva_len(a, kva_end(a, a.by_sq.split(query, rest))), run = kva_run(a, len);
         for (uint32_t at = 0; at == 0 || (at < len && splits < a.sp + a.ss); at += 64 * run) splits++;
     }
     splits = kva_scalar(splits);
