@@ -520,10 +520,13 @@ int qbk_kv_cache_read_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *c
  * scales, as fp16 numbers relative to the row's largest: two halves, 22 bits,
  * for QBK_F32, one, 11 bits, for QBK_BF16, whose outputs hold 8; a weight
  * times scale keeps them down to 2^-26 of the largest that the query sees,
- * and is off by 2^-36 of that at most below.  Rows that a query does not see
- * have no part in its result, and other calls neither.  workspace of at least
- * qbk_attention_kv_workspace_size bytes, 16-byte aligned; calls that share
- * one must not overlap. */
+ * and is off by 2^-36 of that at most below.  (fp4 with up to four query rows
+ * a kv head holds the product with the 32 channels' multiplier m over 448 so,
+ * off by 2^-35.8 of the same largest: a channel of a small m by 2^-27 / m of its
+ * size, 2^-18 at the smallest, where that is more than 2^-22.)  Rows that a
+ * query does not see have no part in its result, and other calls neither.
+ * workspace of at least qbk_attention_kv_workspace_size bytes, 16-byte aligned;
+ * calls that share one must not overlap. */
 size_t qbk_attention_kv_workspace_size(const qbk_kv_shape *shape, size_t n_heads, size_t n, size_t seq_q,
                                        size_t max_len, size_t prefix_len);
 int qbk_attention_kv_dev(qbk_ctx *ctx, const qbk_kv_shape *shape, const void *cache, size_t first_seq, size_t n,
