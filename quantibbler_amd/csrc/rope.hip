@@ -142,7 +142,9 @@ __global__ void __launch_bounds__(256) rot_quads(RotArgs a) {
         ss = rot_sum<LANES>(ss);
         if (!live) continue;
         if (w) {
-            const float inv = __builtin_amdgcn_rsqf(ss / (float)hd + a.eps);
+            const float mean = ss / (float)hd + a.eps;
+            const bool low = mean < 0x1p-126f;  // eps 0: the instruction takes a subnormal number for 0
+            const float inv = __builtin_amdgcn_rsqf(low ? mean * 0x1p64f : mean) * (low ? 0x1p32f : 1.0f);
             const Rot4<float> lo = *(const Rot4<float> *)(w + c0), hi = *(const Rot4<float> *)(w + c1);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
