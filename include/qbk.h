@@ -615,7 +615,8 @@ typedef struct {
  *           between them k f_i + (1 - k) f_i / factor, k = (t - low) / (high - low)
  *   YARN    the same by the pair's number, k = 1 up to floor of the number that
  *           makes `high` turns, 0 from ceil of that which makes `low` on, and
- *           size = 0.1 ln(factor) + 1 (Peng et al., 2023) */
+ *           size = 0.1 ln(factor) + 1, 1 for factors up to 1 (Peng et al.,
+ *           2023) */
 enum { QBK_ROPE_PLAIN = 0, QBK_ROPE_LINEAR = 1, QBK_ROPE_BASE = 2, QBK_ROPE_RAMP = 3, QBK_ROPE_YARN = 4 };
 typedef struct {
     int kind;

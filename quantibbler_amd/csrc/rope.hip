@@ -304,7 +304,7 @@ int qbk_rope_init(qbk_rope *rope, size_t head_dim, size_t rotary_dim, int interl
     r.head_dim = (uint32_t)head_dim;
     r.rotary_dim = (uint32_t)rotary_dim;
     r.interleaved = interleaved != 0;
-    r.size = kind == QBK_ROPE_YARN ? 0.1 * log(factor) + 1.0 : 1.0;
+    r.size = kind == QBK_ROPE_YARN && factor > 1.0 ? 0.1 * log(factor) + 1.0 : 1.0;
     for (size_t i = 0; i < rotary_dim / 2; i++) {
         long double f = powl(base, -2.0L * (long double)i / (long double)rotary_dim), keep = 1.0L;
         if (kind == QBK_ROPE_LINEAR) keep = 0.0L;
