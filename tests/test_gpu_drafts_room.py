@@ -228,3 +228,29 @@ def test_what_is_refused_runs_nothing(ctx, orc):
         assert all(torch.equal(a, c.buffer) for a, c in zip(before, m._shared["own"])), f"{sorted(kw)}"
         assert m._shared["steps"] == steps
     m.close()
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_the_returned_tokens_as_the_next_input(ctx, orc, n):
+    """The tensor that a call returned, filled with the next step's rows and handed back: as a tensor of its own."""
+    models = [model(ctx, orc, 80) for _ in range(2)]
+    k, vocab = 4, models[0].md.vocab_size
+    rng = np.random.default_rng(17)
+    for m in models:
+        m.share_prefix([5, 6, 7], n, 60, fmt="fp4")
+    held = [None, None]
+    for rep in range(6):
+        rows = words(rng.integers(0, vocab, n * (k + 1)).tolist()).view(n, k + 1)
+        u = torch.from_numpy((0.02 * rng.random((n, k + 1))).astype(np.float32)).cuda()
+        got = []
+        for i, m in enumerate(models):
+            tokens = rows.clone()
+            if i and held[1] is not None:
+                tokens = held[1].copy_(rows)
+            out, counts = m.verify_shared(tokens, u)
+            torch.cuda.synchronize()
+            held[i] = out
+            got.append((out.clone(), counts.clone()))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]), f"call {rep}"
+    for m in models:
+        m.close()
