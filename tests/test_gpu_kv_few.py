@@ -124,3 +124,31 @@ def test_channels_far_below_their_rows_largest(ctx, n, heads, kv, d, sq, rows, p
             off = (got[b] - want).abs()
             assert bool((off <= (2.0 ** -22 + lost.double() + 16 * EPS) * want.abs()).all()), \
                 f"row {where} of sequence {b}: off by {float((off / want.abs().clamp_min(1e-30)).max()):.3g} of a value"
+
+
+@BOTH
+@pytest.mark.parametrize("fmt", ["int8", "fp8", "fp4"])
+def test_calls_repeat_themselves(ctx, dtype, fmt):
+    """The same call again, on a workspace that holds something else, behind other work and on another stream: the same
+    bits, in every body and with splits."""
+    for n, heads, kv, d, sq, rows, plen in [(32, 32, 8, 128, 1, [1076 + 32 * i for i in range(32)], 0),
+                                            (16, 8, 8, 80, 5, [40 + 9 * i for i in range(16)], 4001),
+                                            (64, 32, 8, 128, 1, [200 + 9 * i for i in range(64)], 3000),
+                                            (1, 4, 1, 256, 1, [2000], 0), (2, 64, 64, 64, 70, [90, 200], 100)]:
+        cache = att.make(ctx, fmt, n, max(rows), kv, d)
+        att.fill(cache, 10, rows)
+        shared = None
+        if plen:
+            shared = att.make(ctx, fmt, 1, plen, kv, d)
+            att.fill(shared, 30, [plen])
+        q = (1.5 * normal(n + d, (n, sq, heads, d))).to(getattr(torch, dtype))
+        need = cache.attention_workspace_size(heads, n, seq_q=sq, prefix_len=plen)
+        first, s = att.attend(cache, q, words(rows), dtype, shared, plen), torch.cuda.Stream()
+        for rep in range(6):
+            ws = torch.full((max(need, 16),), 17 * rep, dtype=torch.uint8, device="cuda")
+            att.attend(cache, -q, words(rows), dtype, shared, plen)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s if rep % 2 else torch.cuda.current_stream()):
+                again = att.attend(cache, q, words(rows), dtype, shared, plen, ws=ws, stream=torch.cuda.current_stream())
+            torch.cuda.synchronize()
+            assert torch.equal(again, first), f"{(n, heads, kv, d, sq, plen)}, {rep}"
