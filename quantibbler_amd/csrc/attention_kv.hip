@@ -905,8 +905,8 @@ __device__ __forceinline__ void kva_few(const KvAttArgs &a, char *smem, uint32_t
 // at unlike places (one alone issues a vector operation every four cycles, two
 // of one workgroup stand at its barriers together); 32 rows a wave would halve
 // the widening but do not fit 256 registers.  64 requests of up to 2048 rows
-// behind 16384, 32/8 heads of 128: 244 MB in 54 to 55 us, 4.5 TB/s; fp4, bound by
-// the widening, 134 MB in 58.
+// behind 16384, 32/8 heads of 128: 244 MB in 60.6 us with the join, 4.0 TB/s; fp4,
+// half the bytes and no fewer operations, 134 MB in 56.7.
 template <int DC>
 struct KvaStage {
     static constexpr int KEYS = 4 * 2 * DC * 1024, BYTES = 2 * KEYS + 512, BUFS = DC < 4 ? 2 : 1;
@@ -1284,8 +1284,9 @@ static KvaPlan kva_plan(const qbk_kv_shape *s, size_t n_heads, size_t n, size_t 
     if (max_len) p.ss = splits(os >= 256 ? div_ceil(ts, 64) : div_ceil(512, os), ts);
     // a second launch takes longer than one more tile a wave (one sequence of 512 rows in one launch 7.9 us, split 9.2;
     // of 768 9.6 and 9.4, of 1024 11.1 and 9.4)
-    // (the body of four rows, heads of 64: 1024 rows 8.0 and 6.9, 1500 8.2 and 8.3; of 128: 768 9.2 and 8.4, 1024 9.2 and
-    // 9.5; of 256: 512 10.5, 600 11.4 and 12.5)
+    // (the body of four rows, f32, in one launch and split, heads of 64: 1024 rows 7.2 and 7.9, 1500 8.8 and 8.2; of 128:
+    // 768 9.0 and 9.3, 1024 10.2 and 9.5; of 256: 512 12.2 and 12.3, 600 14.7 and 12.5; bf16 6.7 and 8.1, 8.1 and 8.1;
+    // 8.1 and 9.2, 9.2 and 9.2; 11.0 and 11.6, 12.9 and 11.8)
     const size_t tiles = !p.few || dc == 4 ? 2 : dc == 2 ? 3 : 4;  // a wave's
     if (!prefix_len && ts <= tiles * KVA_WAVES) p.ss = 1;
     p.items = op * p.sp + os * p.ss;

@@ -379,10 +379,12 @@ __global__ void __launch_bounds__(256) kv_read_tiles(KvRows a, T *k, T *v) {
 //   1024 sequences, written: two rows each 31 / 47, four 57 / 49, sixteen 135 / 57; read 26 / 34, 49 / 35, 71 / 42
 //   4096 sequences, 2 heads of 64, written: four rows 20.5 / 37, eight 37.5 / 38, sixteen 69 / 39
 // fp4 has more to do a tile, and its rows go in twos: from eight rows a sequence
-// on
-//   one sequence, written: 1024 rows 8.7 / 6.4, 2048 15.3 / 7.8; read 5.4 / 5.9, 7.9 / 6.9
-//   1024 sequences, written: four rows each 55 / 78, eight 76 / 79, sixteen 123 / 81; read 30 / 28, 36 / 29, 48 / 32
-//   the same, 2 heads of 64: eight rows 13.8 / 20, sixteen 22.7 / 20; heads of 256: two 67 / 138, eight 207 / 134
+// on, one rule for both directions, which is early for rows written (they cross
+// near twelve) and late for rows read (near four)
+//   one sequence, written: 512 rows 5.9 / 5.1, 1024 8.3 / 5.7, 2048 15.0 / 6.1; read 4.0 / 5.6, 5.6 / 6.1, 8.2 / 7.3
+//   1024 sequences, written: four rows each 32 / 79, eight 52 / 79, sixteen 95 / 81; read 34 / 28, 37 / 30, 54 / 44
+//   the same, 2 heads of 64, written: eight 12.4 / 19.4, sixteen 20.8 / 19.9; read 7.9 / 9.5, 13.9 / 10.7
+//   the same, 8 heads of 256, written: four 58 / 132, eight 134 / 134; read 63 / 35, 72 / 49
 static bool kv_by_tiles(size_t n_rows, size_t n, const qbk_kv_shape *s) {
     return (unsigned __int128)n_rows * s->n_kv_heads > 4096 &&
            (s->format == QBK_KV_FP4 ? n_rows / 8 : n_rows * s->head_dim / 512) >= n;

@@ -24,9 +24,9 @@
 //      of exponentials by that, or, T = 0, the first of the largest
 //   2. (drafts with logits) which row ends the request, that row's units' sums of w
 //   3. the unit that holds the draw, the id in it, and the outputs
-// 32 requests of four drafts, 128256 ids, f32 (148 MB): 32 us, 4.6 TB/s, then 13
-// for two rows of each again (33 MB) and 7 to 8; four looked-up rows of 32003 3.2
-// and 5.1.  Two of three launches depend on the one before and are bound by
+// 32 requests of four drafts, 128256 ids, f32 (148 MB): 33 us, 4.5 TB/s, then 13
+// for two rows of each again and 8, traced launch by launch (the call 49); four
+// looked-up rows of 32003 3.2 and 5.3 (the call 8.1).  Two of three launches depend on the one before and are bound by
 // that; the last workgroup of 2 doing 3 took longer (its fences, 28 us).
 #include <math.h>
 
@@ -515,9 +515,14 @@ __global__ void __launch_bounds__(VF_THREADS) vf_choose(VfArgs a) {
     }
 }
 
-// Ids a lane: 32, fewer where that leaves SIMDs idle (units of 2048 ids of all
-// rows, us a call for 8, 16 and 32 a lane: 4500, bf16 22.5 / 20.7 / 23.8; 18144,
-// f32 77.7 / 57.8 / 54.6).
+// Ids a lane: 32, fewer where that leaves SIMDs idle, by the units of 2048 ids
+// of all rows (us a call for 8, 16 and 32 a lane, draft logits unless said):
+//   looked up, f32: 64 units 7.8 / 8.6 / 10.6, 256 8.0 / 8.8 / 10.9, 315 of one row of 128256 each 11.9 / 10.4 / 10.9
+//   448, f32 12.8 / 14.0 / 18.9; 1800, f32 17.9 / 17.6 / 21.2; 2268, bf16 22.4 / 19.6 / 21.1
+//   7200, rows of 50021, bf16 31.0 / 27.6 / 28.8; 7938, of 128256, bf16 37.4 / 29.6 / 28.1
+//   13600, of 50021, f32 44.2 / 39.1 / 42.4; 13608, of 128256, f32 49.4 / 41.2 / 41.3; 18144, of 128256, f32 77.7 / 57.8 / 54.6
+// Rows of 128256 gain from more ids a lane earlier than those of 50021: the
+// borders stand between.
 static int vf_per(size_t n, size_t k, size_t vocab, bool given) {
     const size_t units = n * (given ? 2 * k + 1 : k + 1) * div_ceil(vocab, 32 * 64);
     return units < 2048 ? 8 : units < 8192 ? 16 : 32;

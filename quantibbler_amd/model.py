@@ -535,7 +535,8 @@ class DeviceModel:
         token a request.  A captured call's replays keep to the capacity: a request
         takes as many drafts as it has rows for, and emits nothing (a count of 0)
         where it has none; the calls that are made behind a capture look up what
-        requests hold (a synchronization each)."""
+        requests hold (a synchronization each).  Each k has buffers of its own, its
+        rows' logits among them, until share_prefix() is called again."""
         import torch
 
         from ._lib import check, load
