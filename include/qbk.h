@@ -667,9 +667,9 @@ int qbk_rotate_heads_dev(qbk_ctx *ctx, const qbk_rope *rope, const void *q, cons
  * what qbk_argmax_dev makes of it, whatever it holds: a NaN is passed over, +inf
  * is the likeliest, and a row with nothing above -inf is id 0, kept where it was
  * drafted, emitted and counted (a caller whose masks can leave nothing looks for
- * that itself, as with qbk_argmax_dev).  Exponentials and sums are 64-bit.  workspace of at least
- * qbk_verify_drafts_workspace_size bytes (draft_logits: whether there are any),
- * 16-byte aligned. */
+ * that itself, as with qbk_argmax_dev).  Exponentials and sums are 64-bit.
+ * workspace of at least qbk_verify_drafts_workspace_size bytes (draft_logits:
+ * whether there are any), 16-byte aligned. */
 size_t qbk_verify_drafts_workspace_size(size_t n, size_t k, size_t vocab, int draft_logits);
 int qbk_verify_drafts_dev(qbk_ctx *ctx, const void *logits, const void *draft_logits, int dtype, size_t n, size_t k,
                           size_t vocab, size_t row_stride, size_t draft_row_stride, const int32_t *ids,

@@ -687,9 +687,10 @@ __device__ __forceinline__ void kva_body(const KvAttArgs &a, char *smem, uint32_
 // number: its second half (f32 queries) is a step of 2^-24 from x = 2^-3 on, so
 // that the row's largest weight, 2^11 m / 2^9 and more, is off by 2^-27 / m of
 // itself where that is more than 2^-22: channels of 2^-17 of their row's largest
-// keep 18 bits, those from 2^-14 on 22.  The cache holds two of them; multipliers
-// with the codes, as in kva_body, are 4 % slower (f32 queries, 700 rows 8.9 / 9.3
-// us, 32 sequences 21.2 / 22.0).  The columns of a row are joined as the waves are.
+// keep 18 bits, those from 2^-14 on 22, of values whose codes have two;
+// multipliers with the codes, as in kva_body, are 4 % slower (f32 queries, 700
+// rows 8.9 / 9.3 us, 32 sequences 21.2 / 22.0).  The columns of a row are joined as
+// the waves are.
 // 32 sequences of up to 2085 rows, 32/8 heads of 128: 59 MB in 18.0 us, by
 // kva_body 20.9, by eight waves a workgroup 17.8 (64 sequences of 600 18.2, by
 // four 11.6); 128 of up to 4000 446 MB in 85.5, 5.2 TB/s.

@@ -26,8 +26,9 @@
 //   3. the unit that holds the draw, the id in it, and the outputs
 // 32 requests of four drafts, 128256 ids, f32 (148 MB): 33 us, 4.5 TB/s, then 13
 // for two rows of each again and 8, traced launch by launch (the call 49); four
-// looked-up rows of 32003 3.2 and 5.3 (the call 8.1).  Two of three launches depend on the one before and are bound by
-// that; the last workgroup of 2 doing 3 took longer (its fences, 28 us).
+// looked-up rows of 32003 3.2 and 5.3 (the call 8.1).  Two of three launches
+// depend on the one before and are bound by that; the last workgroup of 2 doing 3
+// took longer (its fences, 28 us).
 #include <math.h>
 
 #include "qbk_internal.h"
@@ -521,8 +522,9 @@ __global__ void __launch_bounds__(VF_THREADS) vf_choose(VfArgs a) {
 //   448, f32 12.8 / 14.0 / 18.9; 1800, f32 17.9 / 17.6 / 21.2; 2268, bf16 22.4 / 19.6 / 21.1
 //   7200, rows of 50021, bf16 31.0 / 27.6 / 28.8; 7938, of 128256, bf16 37.4 / 29.6 / 28.1
 //   13600, of 50021, f32 44.2 / 39.1 / 42.4; 13608, of 128256, f32 49.4 / 41.2 / 41.3; 18144, of 128256, f32 77.7 / 57.8 / 54.6
-// Rows of 128256 gain from more ids a lane earlier than those of 50021: the
-// borders stand between.
+// Rows of 128256 gain from more ids a lane earlier than those of 50021 or 32003;
+// the borders stand where neither loses much of what it takes (the lower one is
+// late for looked-up rows: 1260 units of 128256 14.3 / 12.2 / 12.6).
 static int vf_per(size_t n, size_t k, size_t vocab, bool given) {
     const size_t units = n * (given ? 2 * k + 1 : k + 1) * div_ceil(vocab, 32 * 64);
     return units < 2048 ? 8 : units < 8192 ? 16 : 32;
