@@ -69,14 +69,18 @@ struct VfArgs {
     uint32_t n, k, rows, vocab, units;
 };
 
-// Rows that request i has left, and the drafts that are looked at.
+// Rows that request i has left where there is a limit, the drafts that it has,
+// and those that are looked at.
 __device__ __forceinline__ uint64_t vf_room(const VfArgs &a, uint32_t i) {
-    if (a.limit >> 32) return a.limit;
     const uint32_t at = a.pos[i];
     return a.limit > at ? a.limit - at : 0;
 }
+__device__ __forceinline__ uint32_t vf_given(const VfArgs &a, uint32_t i) {
+    return a.n_drafts ? (a.n_drafts[i] < a.k ? a.n_drafts[i] : a.k) : a.k;
+}
 __device__ __forceinline__ uint32_t vf_drafts(const VfArgs &a, uint32_t i) {
-    const uint32_t m = a.n_drafts ? (a.n_drafts[i] < a.k ? a.n_drafts[i] : a.k) : a.k;
+    const uint32_t m = vf_given(a, i);
+    if (a.limit >> 32) return m;
     const uint64_t room = vf_room(a, i);
     return m < room ? m : room ? (uint32_t)room - 1 : 0;
 }
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(VF_THREADS) vf_stats(VfArgs a) {
     const uint32_t groups = (a.units + VF_WAVES - 1) / VF_WAVES;
     const uint32_t unit = blockIdx.x % groups * VF_WAVES + wave, row = blockIdx.x / groups, i = row / a.rows, r = row % a.rows;
     const bool target = r <= a.k;
-    const uint32_t j = target ? r : r - a.k - 1, drafts = vf_drafts(a, i);
+    const uint32_t j = target ? r : r - a.k - 1, drafts = vf_given(a, i);  // no fewer than are looked at
     const double heat = vf_heat(a, i);
     if (unit >= a.units || j > drafts || (!target && (j == drafts || heat == 0.0))) return;
     const T *src = target ? (const T *)a.x + ((size_t)i * (a.k + 1) + j) * a.xs : (const T *)a.y + ((size_t)i * a.k + j) * a.ys;
